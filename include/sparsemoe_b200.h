@@ -223,6 +223,77 @@ int moe_stage_expert_ffn_planned(const struct MoEArgs* args, const MoeDims* dims
                                  int num_groups, int64_t rows_capacity, float* const* out_bases, int num_bases,
                                  cudaStream_t stream);
 
+// ---- expert routing from given logits (no reference counterpart: the
+//      reference's gate is the softmax of the top-k logits,
+//      kernels/capacity.cu:171-238, which is score softmax, renormalised, one group) ----
+// Element types of the stand-alone operators below.
+#define MOE_TYPE_F32  0
+#define MOE_TYPE_F16  1
+#define MOE_TYPE_BF16 2
+#define MOE_SCORE_SOFTMAX 0   // s_e = exp(x_e - max) / sum over all experts
+#define MOE_SCORE_SIGMOID 1   // s_e = 1 / (1 + exp(-x_e))
+typedef struct MoeRouting {
+    int score;         // MOE_SCORE_*
+    int num_groups;    // >= 1, divides the experts: groups of neighbours
+    int groups_kept;   // 1..num_groups: only experts of the best groups are chosen
+    int group_top;     // a group's score: its largest value (1) or the sum of its two largest (2)
+    int renormalise;   // non-zero: the weights of the chosen add up to `scale`
+    float scale;       // times every weight
+} MoeRouting;
+// Chooses top_k experts for each of `tokens` rows of num_experts logits (rows
+// row_stride elements apart).  An expert's value is its score + select_bias[e]
+// (device f32 [num_experts]; it moves the choice, never the weight), or
+// without a bias its logit.  Order: value descending, equal values by the
+// lower index, as f64 arithmetic on the logits orders them (group sums that
+// agree to 2^-49 are equal).  Weights: the scores of the chosen,
+// renormalised if asked, times scale.  An expert is masked by a logit that is
+// NaN, -infinity, <= -1e20 or f16's lowest value, or by such a bias; slots
+// that no expert fills hold index -1 and weight 0.  Writes indices and weights
+// [tokens, top_k]; num_experts <= 1024, top_k <= 32.
+int moe_route_experts(const void* logits, int logits_type, int64_t tokens, int num_experts, int64_t row_stride,
+                      int top_k, const MoeRouting* routing, const float* select_bias, int* indices, float* weights,
+                      cudaStream_t stream);
+
+// ---- dense int8 products (no reference counterpart; its int8 is per tensor) ----
+// An int8 matrix of K inputs and N outputs with one f32 scale per output.
+#define MOE_WEIGHT_KN 0   // w[k * row_stride + n], as the expert weights
+#define MOE_WEIGHT_NK 1   // w[n * row_stride + k]
+typedef struct MoeInt8Weight {
+    const int8_t* w;       // device, 16-byte aligned
+    int64_t row_stride;    // bytes between rows, a multiple of 16
+    const float* scale;    // device [N]
+    int order;             // MOE_WEIGHT_*
+} MoeInt8Weight;
+// Per-token quantiser: scale[t] = max |x_t| * f32(1/127) in f32 (1 where that is 0),
+// q = round-half-even(x / scale) of the exact quotient.  A row with a NaN or
+// an infinity gets a NaN scale (and so NaN outputs).  q: [tokens, q_stride],
+// q_stride a multiple of 16; bytes behind K are left as they are.
+int moe_int8_quantize_tokens(const void* x, int x_type, int64_t tokens, int K, int64_t row_stride, int8_t* q,
+                             int64_t q_stride, float* scale, cudaStream_t stream);
+// out[t, n] = (sum_k q[t, k] w[k, n]) * scale[t] * w->scale[n] + bias[n]
+// (bias: device f32 [N] or null), s32 sums, f32 after them, rounded once to
+// out_type.  K <= 131071.
+int moe_int8_matmul(const int8_t* q, int64_t q_stride, const float* scale, int64_t tokens, int K,
+                    const MoeInt8Weight* w, int N, const float* bias, void* out, int out_type, int64_t out_stride,
+                    cudaStream_t stream);
+// Both in one call: 16-bit or f32 activations times an int8 matrix.  scratch:
+// device, 256-byte aligned, moe_int8_linear_scratch_bytes(tokens, K).
+int moe_int8_linear(const void* x, int x_type, int64_t tokens, int K, int64_t row_stride, const MoeInt8Weight* w,
+                    int N, const float* bias, void* out, int out_type, int64_t out_stride, void* scratch,
+                    size_t scratch_bytes, cudaStream_t stream);
+size_t moe_int8_linear_scratch_bytes(int64_t tokens, int K);
+// The shared expert of an MoE layer, a SwiGLU FFN that every token takes:
+//   g = linear(x, gate), u = linear(x, up), h = u * g / (1 + exp(-g)) (f32),
+//   out = linear(h, down) + residual,
+// with x and h quantised per token.  residual: [tokens, d_model] of x_type, or
+// null; it may be `out` itself when the types are the same.  gate and up have
+// one order.
+int moe_int8_shared_expert(const void* x, int x_type, int64_t tokens, int d_model, int64_t row_stride,
+                           const MoeInt8Weight* gate, const MoeInt8Weight* up, const MoeInt8Weight* down, int d_ff,
+                           const void* residual, int64_t residual_stride, void* out, int out_type, int64_t out_stride,
+                           void* scratch, size_t scratch_bytes, cudaStream_t stream);
+size_t moe_int8_shared_expert_scratch_bytes(int64_t tokens, int d_model, int d_ff);
+
 // ---- expert weight files (.bin): a layer's router and expert weights in the
 //      formats the kernels read (no repacking on load).  The reference's
 //      driver names a cache file it never writes (drivers/main.cu:27-31).

@@ -40,6 +40,10 @@ DTYPE_INT4_PTX = 7   # the reference's capacity_int4_ptx format (packed-transpos
 DTYPE_FP8 = 8        # the reference's capacity_fp8_ptx format (per-tensor e4m3)
 ROUTER_SAME = 0
 ROUTER_F32 = 1
+# element types, scores and weight orders of the stand-alone operators
+MOE_TYPE_F32, MOE_TYPE_F16, MOE_TYPE_BF16 = 0, 1, 2
+MOE_SCORES = {"softmax": 0, "sigmoid": 1}
+MOE_WEIGHT_KN, MOE_WEIGHT_NK = 0, 1
 
 
 class MoeError(RuntimeError):
@@ -93,6 +97,19 @@ class MoeDims(ctypes.Structure):
         ("slot_base", _p), ("act_scale", _p), ("skip_gather", ctypes.c_int),
         ("norm_weight", _p), ("norm_eps", ctypes.c_float), ("norm_out", _p), ("residual", _p),
     ]
+
+
+class MoeRouting(ctypes.Structure):
+    """ctypes image of `MoeRouting` (include/sparsemoe_b200.h)."""
+
+    _fields_ = [("score", ctypes.c_int), ("num_groups", ctypes.c_int), ("groups_kept", ctypes.c_int),
+                ("group_top", ctypes.c_int), ("renormalise", ctypes.c_int), ("scale", ctypes.c_float)]
+
+
+class MoeInt8Weight(ctypes.Structure):
+    """ctypes image of `MoeInt8Weight` (include/sparsemoe_b200.h)."""
+
+    _fields_ = [("w", _p), ("row_stride", ctypes.c_int64), ("scale", _p), ("order", ctypes.c_int)]
 
 
 class MoeWeightArray(ctypes.Structure):

@@ -1,0 +1,962 @@
+// Dense int8 products with a scale per token and per output channel, the
+// per-token quantiser in front of them, and the shared expert built from both.
+//
+//   quantise   s_t = max_k |x_tk| * f32(1/127), one f32 product (1 for a zero row),
+//              q_tk = round-half-even(x_tk / s_t) of the exact quotient;
+//   product    y_tn = (sum_k q_tk w_kn) * s_t * s_n (+ bias_n) (+ residual_tn),
+//              the sum exact in s32 (K <= 131071), the rest in f32, one
+//              rounding to the output type;
+//   shared     g = product(x, Wg), u = product(x, Wu), h = u * g / (1 + exp(-g))
+//   expert     kept in f32, quantised per token, y = product(h, Wd) + residual.
+// A row holding a NaN or an infinity gets s_t = NaN, so its outputs are NaN.
+#include "moe_internal.h"
+#include "common.cuh"
+#include "sm100.cuh"
+
+#include <cudaTypedefs.h>
+#include <cuda.h>
+#include <algorithm>
+
+namespace moe {
+
+// expert_gemm.cu: [outer, inner] bytes, rows `stride` bytes apart, boxes of 128 bytes x box_outer rows, 128-byte swizzle
+bool make_map_u8_strided(CUtensorMap* map, const void* base, uint64_t inner, uint64_t outer, uint64_t stride,
+                         uint32_t box_outer);
+
+namespace {
+
+using namespace sm100;
+
+// Set by a wait that ran out; read and cleared by moe_check_device_status.
+__device__ int g_linear_status;
+
+// ---- per-token quantisation --------------------------------------------------------
+
+// Rows of up to TPR * 32 elements stay in registers (four vectors of eight a
+// thread); longer ones are read twice, the second time from L1 / L2.
+constexpr int kQVec = 4;
+
+template <typename T> struct In8;   // eight elements
+template <> struct In8<float> {
+    float v[8];
+    __device__ __forceinline__ void load(const float* p) {
+        const float4 a = __ldg(reinterpret_cast<const float4*>(p)), b = __ldg(reinterpret_cast<const float4*>(p) + 1);
+        v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+    }
+    __device__ __forceinline__ void load_part(const float* p, int n) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = i < n ? __ldg(p + i) : 0.0f;
+    }
+    __device__ __forceinline__ void zero() {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = 0.0f;
+    }
+    // largest magnitude as f32 bits: NaN > infinity > every finite value
+    __device__ __forceinline__ uint32_t amax_bits() const {
+        uint32_t m = 0;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) m = max(m, __float_as_uint(v[i]) & 0x7FFFFFFFu);
+        return m;
+    }
+    __device__ __forceinline__ void get(float (&f)[8]) const {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) f[i] = v[i];
+    }
+};
+template <typename T16> struct In8_16 {
+    uint4 raw;
+    __device__ __forceinline__ void load(const T16* p) { raw = __ldg(reinterpret_cast<const uint4*>(p)); }
+    __device__ __forceinline__ void load_part(const T16* p, int n) {
+        uint32_t u[4] = {0u, 0u, 0u, 0u};
+        const unsigned short* s = reinterpret_cast<const unsigned short*>(p);
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            if (i < n) u[i >> 1] |= (uint32_t)__ldg(s + i) << (16 * (i & 1));
+        raw = make_uint4(u[0], u[1], u[2], u[3]);
+    }
+    __device__ __forceinline__ void zero() { raw = make_uint4(0u, 0u, 0u, 0u); }
+    __device__ __forceinline__ uint32_t amax_bits() const {
+        const uint32_t m = __vmaxu2(__vmaxu2(raw.x & 0x7FFF7FFFu, raw.y & 0x7FFF7FFFu),
+                                    __vmaxu2(raw.z & 0x7FFF7FFFu, raw.w & 0x7FFF7FFFu));
+        const float2 f = F16Traits<T16>::unpack2(max(m & 0xFFFFu, m >> 16));
+        return __float_as_uint(f.x) & 0x7FFFFFFFu;
+    }
+    __device__ __forceinline__ void get(float (&f)[8]) const {
+        const uint32_t u[4] = {raw.x, raw.y, raw.z, raw.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float2 p = F16Traits<T16>::unpack2(u[i]);
+            f[2 * i] = p.x;
+            f[2 * i + 1] = p.y;
+        }
+    }
+};
+template <> struct In8<__half> : In8_16<__half> {};
+template <> struct In8<__nv_bfloat16> : In8_16<__nv_bfloat16> {};
+
+// round-half-even of the exact x / s.  x * (1/s) is within 127 * 2^-22 of the
+// quotient, so only values that close to a border n + 1/2 need more; there
+// the sign of x - (n + 1/2) s decides, which one fma gives exactly.
+__device__ __forceinline__ int quant1(float x, float s, float inv) {
+    const float r = x * inv;
+    float n = rintf(r);
+    if (fabsf(r - n) > 0.49995f) {
+        const float lo = floorf(r), e = fmaf(-(lo + 0.5f), s, x);
+        n = e > 0.0f ? lo + 1.0f : e < 0.0f ? lo : 2.0f * rintf(0.5f * (lo + 0.5f));
+    }
+    return (int)n;
+}
+
+// Rows whose scale is so small or large that 1/s or the border's fma leaves
+// the normal range are scaled by a power of two first (pre != 1), which changes
+// no quotient; a subnormal scale has few bits, so there the codes are clamped.
+__device__ __forceinline__ uint2 quant8(const float (&f)[8], float s, float inv, float pre) {
+    uint32_t w[2] = {0u, 0u};
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const int q = pre == 1.0f ? quant1(f[i], s, inv) : max(-127, min(127, quant1(f[i] * pre, s, inv)));
+        w[i >> 2] |= (uint32_t)(q & 0xFF) << (8 * (i & 3));
+    }
+    return make_uint2(w[0], w[1]);
+}
+
+__device__ __forceinline__ void store8(int8_t* q, uint2 w, int n, bool vec) {
+    if (vec && n >= 8) {
+        *reinterpret_cast<uint2*>(q) = w;
+        return;
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+        if (i < n) q[i] = (int8_t)((i < 4 ? w.x : w.y) >> (8 * (i & 3)));
+}
+
+// kPair (T = float): x holds gate values, the up values start `up` elements
+// behind them, and the row that is quantised is up * gate / (1 + exp(-gate)).
+template <typename T, int TPR, bool kPair>
+__global__ void __launch_bounds__(256) quantize_tokens_kernel(const T* __restrict__ x, int64_t rows, int K, int64_t ldx,
+                                                             int64_t up, int8_t* __restrict__ q, int64_t ldq,
+                                                             float* __restrict__ scale, int vec) {
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    constexpr int kRows = 256 / TPR;
+    __shared__ uint32_t red[8];
+    const int tr = threadIdx.x % TPR;
+    const int64_t t = (int64_t)blockIdx.x * kRows + threadIdx.x / TPR;
+    const bool live = t < rows;
+    const T* src = x + t * ldx;
+    const bool keep = K <= TPR * 8 * kQVec;
+    In8<T> v[kQVec];
+    uint32_t m = 0;
+    auto fetch = [&](In8<T>& d, int k) {
+        if (!live || k >= K) d.zero();
+        else if (vec && k + 8 <= K) d.load(src + k);
+        else d.load_part(src + k, K - k);
+        if constexpr (kPair) {
+            if (live && k < K) {
+                In8<T> u;
+                if (vec && k + 8 <= K) u.load(src + up + k);
+                else u.load_part(src + up + k, K - k);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) d.v[i] = u.v[i] * (d.v[i] / (1.0f + __expf(-d.v[i])));
+            }
+        }
+    };
+    if (keep) {
+#pragma unroll
+        for (int i = 0; i < kQVec; ++i) fetch(v[i], (i * TPR + tr) * 8);
+#pragma unroll
+        for (int i = 0; i < kQVec; ++i) m = max(m, v[i].amax_bits());
+    } else {
+        for (int k = tr * 8; k < K; k += TPR * 8) {
+            fetch(v[0], k);
+            m = max(m, v[0].amax_bits());
+        }
+    }
+    m = __reduce_max_sync(0xffffffffu, m);
+    if constexpr (TPR > 32) {
+        if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = m;
+        __syncthreads();
+        const int w0 = threadIdx.x / TPR * (TPR / 32);
+#pragma unroll
+        for (int i = 0; i < TPR / 32; ++i) m = max(m, red[w0 + i]);
+    }
+    if (!live) return;
+    const float amax = __uint_as_float(m);
+    const bool bad = m >= 0x7F800000u;
+    float s = bad ? __uint_as_float(0x7FFFFFFFu) : __fmul_rn(amax, 1.0f / 127.0f);
+    if (s == 0.0f) s = 1.0f;   // a zero row, or one whose scale rounds to zero
+    // 2^100 and 2^-100: the scale is rounded first, a subnormal one keeps its few bits
+    const float pre = amax < 5.4e-20f && s != 1.0f ? 1.2676506e30f : amax > 1.8e19f ? 7.8886091e-31f : 1.0f;
+    const float ss = s * pre, inv = bad ? 0.0f : __fdiv_rn(1.0f, ss);
+    if (tr == 0) scale[t] = s;
+    int8_t* dst = q + t * ldq;
+    auto put = [&](const In8<T>& d, int k) {
+        if (k >= K) return;
+        float f[8];
+        d.get(f);
+        uint2 w = bad ? make_uint2(0u, 0u) : quant8(f, ss, inv, pre);
+        store8(dst + k, w, K - k, true);
+    };
+    if (keep) {
+#pragma unroll
+        for (int i = 0; i < kQVec; ++i) put(v[i], (i * TPR + tr) * 8);
+    } else {
+        for (int k = tr * 8; k < K; k += TPR * 8) {
+            fetch(v[0], k);
+            put(v[0], k);
+        }
+    }
+}
+
+// ---- product -----------------------------------------------------------------------
+
+constexpr int kBM = 128;       // tokens of a tile
+constexpr int kBK = 128;       // K of a stage: one 128-byte swizzle span
+constexpr int kThreads = 192;  // TMA warp, MMA warp, four epilogue warps
+constexpr int kMaxSplit = 8;
+
+struct LinearParams {
+    int T, N, K;               // N: output columns
+    int m_tiles, n_tiles, kblocks;
+    int n0_tiles;              // column tiles of the first matrix; the others are of the second (plain product of two)
+    int64_t out1;              // elements from the first matrix's outputs to the second's
+    int split;                 // CTAs of a cluster that share a tile's K
+    int a_rows;                // rows of the A box
+    int b_nk;                  // weights [N, K] (K-contiguous) rather than [K, N]
+    int pdl;                   // launched while its predecessor may still run
+    const float* s_tok;
+    const float* s_ch0;        // channel scales (swiglu: gate)
+    const float* s_ch1;        // swiglu: up
+    const float* bias;
+    const void* residual;
+    int64_t ld_res;
+    int res_type;
+    void* out;
+    int64_t ld_out;
+    int out_type;
+    int vec_out, vec_res;      // rows allow 16-byte accesses of eight columns
+    uint32_t idesc;
+};
+
+template <int kBN>
+struct LinearCfg {
+    static constexpr int kStages = 4;
+    static constexpr int kABytes = kBM * kBK;
+    static constexpr int kBBytes = kBN * kBK;
+    static constexpr int kStageBytes = kABytes + kBBytes;
+    static constexpr int kRecvBytes = kBN == 128 ? kBM * kBN * 4 : 0;   // split sums (kBN = 128 only)
+    static constexpr size_t kSmem = 1024 + (size_t)kStages * kStageBytes + kRecvBytes + 256;
+};
+
+__device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ uint32_t cluster_rank() {
+    uint32_t r;
+    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+    return r;
+}
+__device__ __forceinline__ uint32_t mapa(uint32_t addr, uint32_t rank) {
+    uint32_t r;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
+    return r;
+}
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+__device__ __forceinline__ void st_cluster4(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+    asm volatile("st.shared::cluster.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d)
+                 : "memory");
+}
+__device__ __forceinline__ void tmem_ld_32x32b_x8(uint32_t taddr, uint32_t (&r)[8]) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
+                 : "r"(taddr));
+}
+
+__device__ __forceinline__ float load_as_f32(const void* p, int64_t i, int type) {
+    if (type == MOE_TYPE_F32) return static_cast<const float*>(p)[i];
+    if (type == MOE_TYPE_F16) return __half2float(static_cast<const __half*>(p)[i]);
+    return __bfloat162float(static_cast<const __nv_bfloat16*>(p)[i]);
+}
+
+// Eight consecutive outputs of row t from column n on (those below N) of the first or second matrix.
+__device__ __forceinline__ void emit8(const LinearParams& p, int64_t t, bool second, int n, float (&v)[8]) {
+    const int left = p.N - n;
+    if (p.residual) {   // plain loads: it may be the output itself
+        const int64_t at = t * p.ld_res + n;
+        if (p.vec_res && left >= 8) {
+            if (p.res_type == MOE_TYPE_F32) {
+                const float4* r = reinterpret_cast<const float4*>(static_cast<const float*>(p.residual) + at);
+                const float4 a = r[0], b = r[1];
+                v[0] += a.x; v[1] += a.y; v[2] += a.z; v[3] += a.w; v[4] += b.x; v[5] += b.y; v[6] += b.z; v[7] += b.w;
+            } else {
+                const uint4 r = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p.residual) + at);
+                const uint32_t u[4] = {r.x, r.y, r.z, r.w};
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const float2 f = p.res_type == MOE_TYPE_F16 ? F16Traits<__half>::unpack2(u[i])
+                                                                : F16Traits<__nv_bfloat16>::unpack2(u[i]);
+                    v[2 * i] += f.x;
+                    v[2 * i + 1] += f.y;
+                }
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                if (i < left) v[i] += load_as_f32(p.residual, at + i, p.res_type);
+        }
+    }
+    const int64_t at = t * p.ld_out + n + (second ? p.out1 : 0);
+    if (p.out_type == MOE_TYPE_F32) {
+        float* o = static_cast<float*>(p.out) + at;
+        if (p.vec_out && left >= 8) {
+            reinterpret_cast<float4*>(o)[0] = make_float4(v[0], v[1], v[2], v[3]);
+            reinterpret_cast<float4*>(o)[1] = make_float4(v[4], v[5], v[6], v[7]);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                if (i < left) o[i] = v[i];
+        }
+        return;
+    }
+    uint32_t u[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        u[i] = p.out_type == MOE_TYPE_F16 ? F16Traits<__half>::pack2(v[2 * i], v[2 * i + 1])
+                                          : F16Traits<__nv_bfloat16>::pack2(v[2 * i], v[2 * i + 1]);
+    uint16_t* o = static_cast<uint16_t*>(p.out) + at;
+    if (p.vec_out && left >= 8) {
+        *reinterpret_cast<uint4*>(o) = make_uint4(u[0], u[1], u[2], u[3]);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            if (i < left) o[i] = (uint16_t)(u[i >> 1] >> (16 * (i & 1)));
+    }
+}
+
+// Tiles of 128 tokens x kBN weight columns (kSwiglu, kBN = 256: 128 gate
+// columns, then the same 128 up columns, one output column each).
+// split == 1: every CTA walks the tiles with a double-buffered accumulator.
+// split > 1 (kBN = 128): a cluster shares one tile, each CTA a part of K; the
+// s32 parts meet in shared memory, where CTA r adds up the r-th slice of the
+// columns -- integer sums, so the split changes no bit of the result.
+template <int kBN, bool kSwiglu>
+__global__ void __launch_bounds__(kThreads, 1)
+    linear_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB0,
+                  const __grid_constant__ CUtensorMap tmB1, const LinearParams p) {
+    using C = LinearCfg<kBN>;
+    static_assert(!kSwiglu || kBN == 256, "the gate and up halves are whole 128-column boxes");
+    constexpr int kOutN = kSwiglu ? kBN / 2 : kBN;
+    constexpr int kTmemCols = 2 * kBN;
+    extern __shared__ uint8_t smem_raw[];
+    __shared__ float s_scale[2][kBN];
+    __shared__ float s_bias[2][kBN];
+
+    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    uint8_t* sA = smem;
+    uint8_t* sB = smem + C::kStages * C::kABytes;
+    uint8_t* recv = sB + C::kStages * C::kBBytes;
+    uint64_t* full = reinterpret_cast<uint64_t*>(recv + C::kRecvBytes);
+    uint64_t* empty = full + C::kStages;
+    uint64_t* tfull = empty + C::kStages;
+    uint64_t* tempty = tfull + 2;
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(tempty + 2);
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int rank = (int)cluster_rank();
+    int* status = &g_linear_status;
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < C::kStages; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], 1); }
+        for (int a = 0; a < 2; ++a) { mbar_init(&tfull[a], 1); mbar_init(&tempty[a], 128); }
+        fence_mbar_init();
+        tma_prefetch_desc(&tmA);
+        tma_prefetch_desc(&tmB0);
+        tma_prefetch_desc(&tmB1);
+    }
+    if (warp == 1) {
+        tmem_alloc(tmem_slot, kTmemCols);
+        tmem_relinquish();
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem_base = *tmem_slot;
+    // first phase of the cluster barrier: every CTA has started before anything is sent to it
+    if (p.split > 1) cluster_arrive();
+
+    const int total = p.m_tiles * p.n_tiles;
+    const int tile0 = (int)blockIdx.x / p.split, step = (int)gridDim.x / p.split;
+    // this CTA's part of K, in blocks (the host leaves no part empty)
+    const int kb0 = (int)((int64_t)p.kblocks * rank / p.split);
+    const int kb1 = (int)((int64_t)p.kblocks * (rank + 1) / p.split);
+    const uint32_t stage_bytes = (uint32_t)(p.a_rows * kBK + C::kBBytes);
+
+    if (warp == 0) {
+        if (lane == 0) {
+            // ---------------- TMA producer ----------------
+            auto load_b = [&](int s, int n, int kb) {
+                uint8_t* dst = sB + s * C::kBBytes;
+                const int k0 = kb * kBK;
+                const bool second = !kSwiglu && n >= p.n0_tiles;
+                const CUtensorMap* b0 = second ? &tmB1 : &tmB0;
+                const CUtensorMap* b1 = kSwiglu || second ? &tmB1 : &tmB0;
+                const int col = (second ? n - p.n0_tiles : n) * kOutN;
+                if (p.b_nk) {   // a box is kBN / 2 rows of N x 128 of K
+                    tma_load_2d(dst, b0, &full[s], k0, col);
+                    tma_load_2d(dst + C::kBBytes / 2, b1, &full[s], k0, kSwiglu ? col : col + kBN / 2);
+                } else {        // a box is 128 rows of K x 128 of N
+                    tma_load_2d(dst, b0, &full[s], col, k0);
+                    if (kBN == 256) tma_load_2d(dst + C::kBBytes / 2, b1, &full[s], kSwiglu ? col : col + 128, k0);
+                }
+            };
+            // the weights of the first stages do not depend on the kernel before this one
+            int ahead = 0;
+            if (p.pdl) {
+                for (int kb = kb0; tile0 < total && kb < kb1 && ahead < C::kStages; ++kb, ++ahead) {
+                    mbar_arrive_expect_tx(&full[ahead], stage_bytes);
+                    load_b(ahead, tile0 / p.m_tiles, kb);
+                }
+                pdl_wait();
+            }
+            int s = 0;
+            uint32_t ph = 0;
+            for (int t = tile0; t < total; t += step) {
+                const int n = t / p.m_tiles, m = t - n * p.m_tiles;
+                for (int kb = kb0; kb < kb1; ++kb) {
+                    if (ahead > 0) {
+                        --ahead;
+                    } else {
+                        if (!mbar_wait(&empty[s], ph ^ 1u, status, kDevErrTimeout)) goto producer_done;
+                        mbar_arrive_expect_tx(&full[s], stage_bytes);
+                        load_b(s, n, kb);
+                    }
+                    tma_load_2d(sA + s * C::kABytes, &tmA, &full[s], kb * kBK, m * kBM);
+                    if (++s == C::kStages) { s = 0; ph ^= 1u; }
+                }
+            }
+        producer_done:;
+        }
+    } else if (warp == 1) {
+        if (lane == 0) {
+            // ---------------- MMA issuer ----------------
+            int s = 0;
+            uint32_t ph = 0;
+            int acc = 0;
+            uint32_t aph = 0;
+            for (int t = tile0; t < total; t += step) {
+                if (!mbar_wait(&tempty[acc], aph ^ 1u, status, kDevErrTimeout)) break;
+                tc_fence_after();
+                const uint32_t d_tmem = tmem_base + acc * kBN;
+                bool ok = true;
+                for (int kb = kb0; kb < kb1; ++kb) {
+                    if (!mbar_wait(&full[s], ph, status, kDevErrTimeout)) { ok = false; break; }
+                    tc_fence_after();
+                    const uint32_t a_base = smem_u32(sA + s * C::kABytes);
+                    const uint32_t b_base = smem_u32(sB + s * C::kBBytes);
+#pragma unroll
+                    for (int kk = 0; kk < kBK / 32; ++kk) {
+                        // A, and B of [N, K] weights: K-major, 8-row groups 1 KB apart, K step 32 bytes.
+                        // B of [K, N] weights: MN-major, 128-column chunks 16 KB apart, K step 32 rows.
+                        const uint64_t adesc = smem_desc_sw128(a_base + kk * 32, 16, 1024);
+                        const uint64_t bdesc = p.b_nk ? smem_desc_sw128(b_base + kk * 32, 16, 1024)
+                                                      : smem_desc_sw128(b_base + kk * 32 * 128, kBK * 128, 1024);
+                        mma_i8_ss(d_tmem, adesc, bdesc, p.idesc, (kb != kb0 || kk != 0) ? 1u : 0u);
+                    }
+                    mma_commit(&empty[s]);
+                    if (++s == C::kStages) { s = 0; ph ^= 1u; }
+                }
+                if (!ok) break;
+                mma_commit(&tfull[acc]);
+                acc ^= 1;
+                if (acc == 0) aph ^= 1u;
+            }
+        }
+    } else {
+        // ---------------- epilogue (warps 2..5) ----------------
+        if (p.pdl) pdl_wait();
+        if (p.split > 1) cluster_wait();
+        const int q = warp & 3;
+        const int etid = threadIdx.x - 64;
+        int acc = 0;
+        uint32_t aph = 0;
+        bool ok = true;   // a wait that ran out: the warp keeps to its barriers and writes nothing more
+        for (int t = tile0; t < total; t += step) {
+            const int n = t / p.m_tiles, m = t - n * p.m_tiles;
+            const bool second = !kSwiglu && n >= p.n0_tiles;
+            const int col0 = (second ? n - p.n0_tiles : n) * kOutN;
+            // channel scales of the tile, in the order of the accumulator's columns
+            float* sc = s_scale[acc];
+            float* sb = s_bias[acc];
+            for (int c = etid; c < kBN; c += 128) {
+                const int col = col0 + (kSwiglu ? c % kOutN : c);
+                const float* src = second || (kSwiglu && c >= kOutN) ? p.s_ch1 : p.s_ch0;
+                sc[c] = col < p.N ? __ldg(src + col) : 0.0f;
+                sb[c] = !kSwiglu && p.bias && col < p.N ? __ldg(p.bias + col) : 0.0f;
+            }
+            asm volatile("bar.sync 1, 128;" ::: "memory");
+            if (ok) ok = mbar_wait_warp(&tfull[acc], aph, status, kDevErrTimeout);
+            if (ok) {
+                tc_fence_after();
+                const int row = m * kBM + q * 32 + lane;
+                const bool valid = row < p.T;
+                const uint32_t taddr = tmem_base + ((uint32_t)(q * 32) << 16) + acc * kBN;
+                if (p.split == 1) {
+                    const float st = valid ? p.s_tok[row] : 0.0f;
+#pragma unroll 1
+                    for (int c = 0; c < kOutN; c += 16) {
+                        uint32_t a[16], b[16];
+                        tmem_ld_32x32b_x16(taddr + c, a);
+                        if (kSwiglu) tmem_ld_32x32b_x16(taddr + kOutN + c, b);
+                        tmem_wait_ld();
+                        if (c + 16 == kOutN) { tc_fence_before(); mbar_arrive(&tempty[acc]); }
+                        if (!valid) continue;
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) {
+                            float v[8];
+#pragma unroll
+                            for (int i = 0; i < 8; ++i) {
+                                const int cc = c + 8 * h + i;
+                                v[i] = (float)(int)a[8 * h + i] * st * sc[cc];
+                                if (kSwiglu) {
+                                    const float u = (float)(int)b[8 * h + i] * st * sc[kOutN + cc];
+                                    v[i] = u * (v[i] / (1.0f + __expf(-v[i])));
+                                } else {
+                                    v[i] += sb[cc];
+                                }
+                            }
+                            if (col0 + c + 8 * h < p.N) emit8(p, row, second, col0 + c + 8 * h, v);
+                        }
+                    }
+                } else if constexpr (kBN == 128) {
+                    // send the parts in units of eight columns: [source][unit of the slice][row][8]
+                    if (m * kBM + q * 32 < p.T) {   // a warp without a token has nothing to send
+                        const int units = kBN / 8 / p.split;
+#pragma unroll 1
+                        for (int u = 0; u < kBN / 8; ++u) {
+                            uint32_t a[8];
+                            tmem_ld_32x32b_x8(taddr + 8 * u, a);
+                            tmem_wait_ld();
+                            const uint32_t dst = mapa(
+                                smem_u32(recv) + (uint32_t)(((rank * units + u % units) * kBM + q * 32 + lane) * 32),
+                                u / units);
+                            st_cluster4(dst, a[0], a[1], a[2], a[3]);
+                            st_cluster4(dst + 16, a[4], a[5], a[6], a[7]);
+                        }
+                    }
+                }
+            }
+            acc ^= 1;
+            if (acc == 0) aph ^= 1u;
+        }
+    }
+    if (p.split > 1) {
+        __syncwarp();
+        if (warp < 2) cluster_wait();   // the first phase, which the epilogue warps have waited for above
+        cluster_arrive();               // second phase: every part has been sent
+        cluster_wait();
+        if constexpr (kBN == 128 && !kSwiglu) {
+            const int n = tile0 / p.m_tiles, m = tile0 - n * p.m_tiles;   // one tile a cluster
+            const bool second = n >= p.n0_tiles;
+            const int col0 = (second ? n - p.n0_tiles : n) * kOutN;
+            const int q = warp & 3;
+            const int row = m * kBM + q * 32 + lane;
+            if (warp >= 2 && row < p.T) {
+                const float st = p.s_tok[row];
+                const int units = kBN / 8 / p.split;
+                for (int u = 0; u < units; ++u) {
+                    int sum[8] = {};
+                    for (int src = 0; src < p.split; ++src) {
+                        const int4* a = reinterpret_cast<const int4*>(
+                            recv + (size_t)((src * units + u) * kBM + q * 32 + lane) * 32);
+                        const int4 x = a[0], y = a[1];
+                        sum[0] += x.x; sum[1] += x.y; sum[2] += x.z; sum[3] += x.w;
+                        sum[4] += y.x; sum[5] += y.y; sum[6] += y.z; sum[7] += y.w;
+                    }
+                    const int c = (rank * units + u) * 8;
+                    float v[8];
+#pragma unroll
+                    for (int i = 0; i < 8; ++i)
+                        v[i] = (float)sum[i] * st * s_scale[0][c + i] + s_bias[0][c + i];
+                    if (col0 + c < p.N) emit8(p, row, second, col0 + c, v);
+                }
+            }
+        }
+    }
+    __syncthreads();
+    if (warp == 1) {
+        tc_fence_after();
+        tmem_dealloc(tmem_base, kTmemCols);
+    }
+}
+
+// ---- host side -----------------------------------------------------------------------
+
+// SMs the tile rules count on (B200).
+constexpr int kRuleSms = 148;
+constexpr int kMaxK = 131071;   // 128 * 128 * K stays below 2^31
+
+int elem_bytes(int type) { return type == MOE_TYPE_F32 ? 4 : 2; }
+bool is_type(int t) { return t == MOE_TYPE_F32 || t == MOE_TYPE_F16 || t == MOE_TYPE_BF16; }
+bool aligned(const void* p, size_t n) { return reinterpret_cast<uintptr_t>(p) % n == 0; }
+int64_t up16(int64_t v) { return (v + 15) / 16 * 16; }
+size_t up256(size_t v) { return (v + 255) & ~size_t(255); }
+
+template <typename... P, typename... A>
+cudaError_t launch_ex(void (*kern)(P...), unsigned grid, unsigned threads, size_t smem, int cluster, bool pdl,
+                      cudaStream_t st, A... args) {
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(grid);
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cudaLaunchAttribute at[2];
+    int n = 0;
+    if (cluster > 1) {
+        at[n].id = cudaLaunchAttributeClusterDimension;
+        at[n].val.clusterDim = {(unsigned)cluster, 1, 1};
+        ++n;
+    }
+    if (pdl) {
+        at[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        at[n].val.programmaticStreamSerializationAllowed = 1;
+        ++n;
+    }
+    cfg.attrs = at;
+    cfg.numAttrs = n;
+    return cudaLaunchKernelEx(&cfg, kern, P(args)...);
+}
+
+template <typename T, bool kPair>
+cudaError_t launch_quantize_typed(const T* x, int64_t rows, int K, int64_t ldx, int64_t up, int8_t* q, int64_t ldq,
+                                  float* s, bool pdl, cudaStream_t st) {
+    const int vec = aligned(x, 16) && (ldx * (int64_t)sizeof(T)) % 16 == 0;
+    // a warp a row up to 1024 elements, else as many threads as hold the row in registers
+    const int tpr = K <= 1024 ? 32 : K <= 4096 ? 128 : 256;
+    const int64_t blocks = (rows * tpr + 255) / 256;
+    auto kern = tpr == 32    ? quantize_tokens_kernel<T, 32, kPair>
+                : tpr == 128 ? quantize_tokens_kernel<T, 128, kPair>
+                             : quantize_tokens_kernel<T, 256, kPair>;
+    return launch_ex(kern, (unsigned)blocks, 256u, 0, 1, pdl, st, x, rows, K, ldx, up, q, ldq, s, vec);
+}
+
+// up != 0: x holds f32 gate values with the up values `up` elements behind.
+cudaError_t launch_quantize(const void* x, int type, int64_t rows, int K, int64_t ldx, int64_t up, int8_t* q,
+                            int64_t ldq, float* s, bool pdl, cudaStream_t st) {
+    if (up != 0)
+        return launch_quantize_typed<float, true>(static_cast<const float*>(x), rows, K, ldx, up, q, ldq, s, pdl, st);
+    switch (type) {
+        case MOE_TYPE_F32:
+            return launch_quantize_typed<float, false>(static_cast<const float*>(x), rows, K, ldx, 0, q, ldq, s, pdl, st);
+        case MOE_TYPE_F16:
+            return launch_quantize_typed<__half, false>(static_cast<const __half*>(x), rows, K, ldx, 0, q, ldq, s, pdl,
+                                                        st);
+        default:
+            return launch_quantize_typed<__nv_bfloat16, false>(static_cast<const __nv_bfloat16*>(x), rows, K, ldx, 0, q,
+                                                               ldq, s, pdl, st);
+    }
+}
+
+template <int kBN, bool kSwiglu>
+cudaError_t launch_linear_cfg(const CUtensorMap& a, const CUtensorMap& b0, const CUtensorMap& b1,
+                              const LinearParams& p, int clusters, cudaStream_t st) {
+    auto kern = linear_kernel<kBN, kSwiglu>;
+    static SmemAttr attr;
+    const size_t smem = LinearCfg<kBN>::kSmem;
+    cudaError_t err = ensure_smem(kern, smem, attr);
+    if (err != cudaSuccess) return err;
+    return launch_ex(kern, (unsigned)(clusters * p.split), (unsigned)kThreads, smem, p.split, p.pdl != 0, st, a, b0, b1,
+                     p);
+}
+
+struct Matrix {
+    const int8_t* w;
+    int64_t ld;
+    const float* scale;
+};
+
+// One product over one matrix, two of the same shape side by side (w1: the
+// second's outputs start out1 elements behind the first's), or (swiglu) the
+// gate and up matrices of h.
+cudaError_t launch_linear(const int8_t* q, int64_t ldq, LinearParams p, const Matrix& w0, const Matrix* w1, bool swiglu,
+                          int num_sms, cudaStream_t st) {
+    p.m_tiles = (p.T + kBM - 1) / kBM;
+    p.kblocks = (p.K + kBK - 1) / kBK;
+    p.a_rows = p.T >= kBM ? kBM : (p.T + 7) / 8 * 8;
+    p.split = 1;
+    const int mats = w1 && !swiglu ? 2 : 1;
+    const int64_t tiles128 = (int64_t)p.m_tiles * ((p.N + 127) / 128) * mats;
+    const int64_t tiles256 = (int64_t)p.m_tiles * ((p.N + 255) / 256) * mats;
+    bool wide = swiglu;
+    if (!swiglu) {
+        // few tiles: K is shared by as many CTAs as there are SMs for; many:
+        // 256 columns a tile, which halves the reads of A per product
+        wide = tiles256 >= num_sms;
+        if (!wide)
+            while (p.split < kMaxSplit && tiles128 * p.split * 2 <= num_sms && p.kblocks >= p.split * 2) p.split *= 2;
+    }
+    const int bn = wide ? 256 : 128;
+    const int out_n = swiglu ? bn / 2 : bn;
+    p.n0_tiles = (p.N + out_n - 1) / out_n;
+    p.n_tiles = p.n0_tiles * mats;
+    p.s_ch0 = w0.scale;
+    p.s_ch1 = w1 ? w1->scale : w0.scale;
+    p.idesc = idesc_i8(kBM, bn, !p.b_nk);
+    CUtensorMap ta, tb[2];
+    if (!make_map_u8_strided(&ta, q, p.K, p.T, ldq, p.a_rows)) return cudaErrorInvalidValue;
+    const Matrix* ws[2] = {&w0, w1 ? w1 : &w0};
+    for (int i = 0; i < 2; ++i) {
+        const bool ok = p.b_nk ? make_map_u8_strided(&tb[i], ws[i]->w, p.K, p.N, ws[i]->ld, bn / 2)
+                               : make_map_u8_strided(&tb[i], ws[i]->w, p.N, p.K, ws[i]->ld, kBK);
+        if (!ok) return cudaErrorInvalidValue;
+    }
+    const int64_t tiles = (int64_t)p.m_tiles * p.n_tiles;
+    const int clusters = (int)(p.split > 1 ? tiles : std::min<int64_t>(tiles, num_sms));
+    if (swiglu) return launch_linear_cfg<256, true>(ta, tb[0], tb[1], p, clusters, st);
+    if (wide) return launch_linear_cfg<256, false>(ta, tb[0], tb[1], p, clusters, st);
+    return launch_linear_cfg<128, false>(ta, tb[0], tb[1], p, clusters, st);
+}
+
+int bad(const char* who, const char* what) {
+    set_error("%s: %s", who, what);
+    return MOE_ERR_INVALID_ARG;
+}
+
+// Shape checks that every entry point here shares.
+int check_dims(const char* who, int64_t T, int64_t K, int64_t N) {
+    if (T < 0 || K < 1 || N < 1) return bad(who, "tokens must be >= 0, dimensions >= 1");
+    if (K > kMaxK) {
+        set_error("%s: K = %lld, s32 sums are exact up to %d", who, (long long)K, kMaxK);
+        return MOE_ERR_UNSUPPORTED;
+    }
+    if (T > 0x7FFFFF00ll || N > 0x7FFFFF00ll || ((T + 127) / 128) * ((N + 127) / 128) * 2 > 0x7FFFFFFFll) {
+        set_error("%s: %lld x %lld outputs are too many for one call", who, (long long)T, (long long)N);
+        return MOE_ERR_UNSUPPORTED;
+    }
+    return MOE_OK;
+}
+
+int check_matrix(const char* who, const MoeInt8Weight* w, int64_t K, int64_t N) {
+    if (!w || !w->w || !w->scale) return bad(who, "a weight matrix or its scales are null");
+    if (w->order != MOE_WEIGHT_KN && w->order != MOE_WEIGHT_NK) return bad(who, "weight order unknown");
+    if (!aligned(w->w, 16) || w->row_stride % 16 != 0 || w->row_stride < (w->order == MOE_WEIGHT_KN ? N : K))
+        return bad(who, "weight rows must start on 16-byte boundaries and hold a whole row (row_stride % 16 == 0)");
+    if (!aligned(w->scale, 4)) return bad(who, "weight scales are not aligned to f32");
+    return MOE_OK;
+}
+
+int check_x(const char* who, const void* x, int type, int64_t T, int64_t K, int64_t ldx) {
+    if (!is_type(type)) return bad(who, "activation type unknown");
+    if (ldx < K) return bad(who, "activation row stride is smaller than a row");
+    if (T > 0 && (!x || !aligned(x, elem_bytes(type)))) return bad(who, "activations are null or not aligned to their type");
+    return MOE_OK;
+}
+
+int check_out(const char* who, const void* out, int type, int64_t T, int64_t N, int64_t ldo) {
+    if (!is_type(type)) return bad(who, "output type unknown");
+    if (ldo < N) return bad(who, "output row stride is smaller than a row");
+    if (T > 0 && (!out || !aligned(out, elem_bytes(type)))) return bad(who, "output is null or not aligned to its type");
+    return MOE_OK;
+}
+
+int check_scratch(const char* who, const void* scratch, size_t have, size_t need) {
+    if (!scratch || !aligned(scratch, 256)) return bad(who, "scratch is null or not 256-byte aligned");
+    if (have < need) {
+        set_error("%s: scratch of %zu bytes is smaller than the %zu this call needs", who, have, need);
+        return MOE_ERR_INVALID_ARG;
+    }
+    return MOE_OK;
+}
+
+int cuda_error(const char* who, cudaError_t e) {
+    set_error("%s: %s", who, cudaGetErrorString(e));
+    return MOE_ERR_CUDA;
+}
+
+LinearParams out_params(int64_t T, int K, int N, const float* s_tok, const float* bias, void* out, int out_type,
+                        int64_t ldo, int order, bool pdl) {
+    LinearParams p{};
+    p.T = (int)T;
+    p.K = K;
+    p.N = N;
+    p.b_nk = order == MOE_WEIGHT_NK;
+    p.pdl = pdl;
+    p.s_tok = s_tok;
+    p.bias = bias;
+    p.out = out;
+    p.out_type = out_type;
+    p.ld_out = ldo;
+    p.vec_out = aligned(out, 16) && (ldo * elem_bytes(out_type)) % 16 == 0;
+    return p;
+}
+
+// Whether the gate and up products run as one fused launch (h written), or as
+// two plain products whose SwiGLU the quantiser of h applies: fused tiles are
+// 128 tokens x 128 features, and too few of them leave SMs idle that the plain
+// product's split of K fills.
+bool fused_swiglu(int64_t T, int64_t f) { return (T + 127) / 128 * ((f + 127) / 128) * 4 >= kRuleSms * 3; }
+
+size_t linear_scratch(int64_t T, int64_t K) {
+    return up256((size_t)T * up16(K)) + up256((size_t)T * sizeof(float));
+}
+
+struct SharedScratch {
+    size_t qx, sx, h, qh, sh, total;
+    int64_t ldh;
+};
+SharedScratch shared_scratch(int64_t T, int64_t d, int64_t f) {
+    SharedScratch s;
+    s.ldh = (f + 3) / 4 * 4;
+    size_t at = 0;
+    s.qx = at; at += up256((size_t)T * up16(d));
+    s.sx = at; at += up256((size_t)T * sizeof(float));
+    s.h = at;  at += up256((size_t)T * s.ldh * sizeof(float)) * (fused_swiglu(T, f) ? 1 : 2);
+    s.qh = at; at += up256((size_t)T * up16(f));
+    s.sh = at; at += up256((size_t)T * sizeof(float));
+    s.total = at;
+    return s;
+}
+
+}  // namespace
+
+// Devices on which a product has run (only there is the status word read).
+std::atomic<bool> g_linear_used[64];
+
+int linear_status_collect(int dev) {
+    if (dev < 0 || dev >= 64 || !g_linear_used[dev].load()) return MOE_OK;
+    int host = 0;
+    cudaError_t e = cudaMemcpyFromSymbol(&host, g_linear_status, sizeof(int));
+    if (e != cudaSuccess) return cuda_error("moe_check_device_status", e);
+    if (host == 0) return MOE_OK;
+    const int zero = 0;
+    e = cudaMemcpyToSymbol(g_linear_status, &zero, sizeof(int));
+    if (e != cudaSuccess) return cuda_error("moe_check_device_status", e);
+    set_error("device-side wait timed out (int8 product, status %d)", host);
+    return MOE_ERR_TIMEOUT;
+}
+
+}  // namespace moe
+
+using namespace moe;
+
+extern "C" size_t moe_int8_linear_scratch_bytes(int64_t tokens, int K) {
+    return tokens < 0 || K < 1 ? 0 : linear_scratch(tokens, K);
+}
+
+extern "C" size_t moe_int8_shared_expert_scratch_bytes(int64_t tokens, int d_model, int d_ff) {
+    return tokens < 0 || d_model < 1 || d_ff < 1 ? 0 : shared_scratch(tokens, d_model, d_ff).total;
+}
+
+extern "C" int moe_int8_quantize_tokens(const void* x, int x_type, int64_t tokens, int K, int64_t row_stride, int8_t* q,
+                                        int64_t q_stride, float* scale, cudaStream_t stream) {
+    const char* who = "moe_int8_quantize_tokens";
+    int rc = check_dims(who, tokens, K, 1);
+    if (rc == MOE_OK) rc = check_x(who, x, x_type, tokens, K, row_stride);
+    if (rc != MOE_OK) return rc;
+    if (tokens == 0) return MOE_OK;
+    if (!q || !scale || !aligned(q, 16) || q_stride % 16 != 0 || q_stride < K || !aligned(scale, 4))
+        return bad(who, "codes must be rows on 16-byte boundaries (q_stride % 16 == 0, >= K) and scales f32");
+    int dev = 0, num_sms = 0;
+    rc = current_device(&dev, &num_sms);
+    if (rc != MOE_OK) return rc;
+    const cudaError_t e = launch_quantize(x, x_type, tokens, K, row_stride, 0, q, q_stride, scale, false, stream);
+    return e == cudaSuccess ? MOE_OK : cuda_error(who, e);
+}
+
+extern "C" int moe_int8_matmul(const int8_t* q, int64_t q_stride, const float* scale, int64_t tokens, int K,
+                               const MoeInt8Weight* w, int N, const float* bias, void* out, int out_type,
+                               int64_t out_stride, cudaStream_t stream) {
+    const char* who = "moe_int8_matmul";
+    int rc = check_dims(who, tokens, K, N);
+    if (rc == MOE_OK) rc = check_matrix(who, w, K, N);
+    if (rc == MOE_OK) rc = check_out(who, out, out_type, tokens, N, out_stride);
+    if (rc != MOE_OK) return rc;
+    if (tokens == 0) return MOE_OK;
+    if (!q || !scale || !aligned(q, 16) || q_stride % 16 != 0 || q_stride < K || !aligned(scale, 4))
+        return bad(who, "codes must be rows on 16-byte boundaries (q_stride % 16 == 0, >= K) and scales f32");
+    if (!aligned(bias, 4)) return bad(who, "bias is not aligned to f32");
+    int dev = 0, num_sms = 0;
+    rc = current_device(&dev, &num_sms);
+    if (rc != MOE_OK) return rc;
+    g_linear_used[dev] = true;
+    const cudaError_t e =
+        launch_linear(q, q_stride, out_params(tokens, K, N, scale, bias, out, out_type, out_stride, w->order, false),
+                      Matrix{w->w, w->row_stride, w->scale}, nullptr, false, num_sms, stream);
+    return e == cudaSuccess ? MOE_OK : cuda_error(who, e);
+}
+
+extern "C" int moe_int8_linear(const void* x, int x_type, int64_t tokens, int K, int64_t row_stride,
+                               const MoeInt8Weight* w, int N, const float* bias, void* out, int out_type,
+                               int64_t out_stride, void* scratch, size_t scratch_bytes, cudaStream_t stream) {
+    const char* who = "moe_int8_linear";
+    int rc = check_dims(who, tokens, K, N);
+    if (rc == MOE_OK) rc = check_x(who, x, x_type, tokens, K, row_stride);
+    if (rc == MOE_OK) rc = check_matrix(who, w, K, N);
+    if (rc == MOE_OK) rc = check_out(who, out, out_type, tokens, N, out_stride);
+    if (rc != MOE_OK) return rc;
+    if (!aligned(bias, 4)) return bad(who, "bias is not aligned to f32");
+    if (tokens == 0) return MOE_OK;
+    rc = check_scratch(who, scratch, scratch_bytes, linear_scratch(tokens, K));
+    if (rc != MOE_OK) return rc;
+    int dev = 0, num_sms = 0;
+    rc = current_device(&dev, &num_sms);
+    if (rc != MOE_OK) return rc;
+    g_linear_used[dev] = true;
+    int8_t* q = static_cast<int8_t*>(scratch);
+    float* s = reinterpret_cast<float*>(q + up256((size_t)tokens * up16(K)));
+    cudaError_t e = launch_quantize(x, x_type, tokens, K, row_stride, 0, q, up16(K), s, false, stream);
+    if (e == cudaSuccess)
+        e = launch_linear(q, up16(K), out_params(tokens, K, N, s, bias, out, out_type, out_stride, w->order, true),
+                          Matrix{w->w, w->row_stride, w->scale}, nullptr, false, num_sms, stream);
+    return e == cudaSuccess ? MOE_OK : cuda_error(who, e);
+}
+
+extern "C" int moe_int8_shared_expert(const void* x, int x_type, int64_t tokens, int d_model, int64_t row_stride,
+                                      const MoeInt8Weight* gate, const MoeInt8Weight* up, const MoeInt8Weight* down,
+                                      int d_ff, const void* residual, int64_t residual_stride, void* out, int out_type,
+                                      int64_t out_stride, void* scratch, size_t scratch_bytes, cudaStream_t stream) {
+    const char* who = "moe_int8_shared_expert";
+    int rc = check_dims(who, tokens, d_model, d_ff);
+    if (rc == MOE_OK) rc = check_dims(who, tokens, d_ff, d_model);
+    if (rc == MOE_OK) rc = check_x(who, x, x_type, tokens, d_model, row_stride);
+    if (rc == MOE_OK) rc = check_matrix(who, gate, d_model, d_ff);
+    if (rc == MOE_OK) rc = check_matrix(who, up, d_model, d_ff);
+    if (rc == MOE_OK) rc = check_matrix(who, down, d_ff, d_model);
+    if (rc == MOE_OK) rc = check_out(who, out, out_type, tokens, d_model, out_stride);
+    if (rc != MOE_OK) return rc;
+    if (gate->order != up->order) return bad(who, "gate and up weights must have the same order");
+    if (residual && (residual_stride < d_model || !aligned(residual, elem_bytes(x_type))))
+        return bad(who, "residual rows are shorter than d_model or not aligned to their type");
+    if (tokens == 0) return MOE_OK;
+    const SharedScratch sc = shared_scratch(tokens, d_model, d_ff);
+    rc = check_scratch(who, scratch, scratch_bytes, sc.total);
+    if (rc != MOE_OK) return rc;
+    int dev = 0, num_sms = 0;
+    rc = current_device(&dev, &num_sms);
+    if (rc != MOE_OK) return rc;
+    g_linear_used[dev] = true;
+    uint8_t* base = static_cast<uint8_t*>(scratch);
+    int8_t *qx = reinterpret_cast<int8_t*>(base + sc.qx), *qh = reinterpret_cast<int8_t*>(base + sc.qh);
+    float *sx = reinterpret_cast<float*>(base + sc.sx), *sh = reinterpret_cast<float*>(base + sc.sh);
+    float* h = reinterpret_cast<float*>(base + sc.h);
+    const bool fused = fused_swiglu(tokens, d_ff);
+    const int64_t behind = (int64_t)(up256((size_t)tokens * sc.ldh * sizeof(float)) / sizeof(float));
+    cudaError_t e = launch_quantize(x, x_type, tokens, d_model, row_stride, 0, qx, up16(d_model), sx, false, stream);
+    if (e == cudaSuccess) {
+        LinearParams p = out_params(tokens, d_model, d_ff, sx, nullptr, h, MOE_TYPE_F32, sc.ldh, gate->order, true);
+        p.out1 = behind;
+        const Matrix u{up->w, up->row_stride, up->scale};
+        e = launch_linear(qx, up16(d_model), p, Matrix{gate->w, gate->row_stride, gate->scale}, &u, fused, num_sms,
+                          stream);
+    }
+    if (e == cudaSuccess)
+        e = launch_quantize(h, MOE_TYPE_F32, tokens, d_ff, sc.ldh, fused ? 0 : behind, qh, up16(d_ff), sh, true, stream);
+    if (e == cudaSuccess) {
+        LinearParams p = out_params(tokens, d_ff, d_model, sh, nullptr, out, out_type, out_stride, down->order, true);
+        p.residual = residual;
+        p.ld_res = residual_stride;
+        p.res_type = x_type;
+        p.vec_res = aligned(residual, 16) && (residual_stride * elem_bytes(x_type)) % 16 == 0;
+        e = launch_linear(qh, up16(d_ff), p, Matrix{down->w, down->row_stride, down->scale}, nullptr, false, num_sms,
+                          stream);
+    }
+    return e == cudaSuccess ? MOE_OK : cuda_error(who, e);
+}

@@ -878,6 +878,8 @@ extern "C" int moe_check_device_status(cudaStream_t stream) {
     int dev = 0;
     e = cudaGetDevice(&dev);
     if (e != cudaSuccess) return cuda_fail(e, "cudaGetDevice");
+    const int lrc = linear_status_collect(dev);
+    if (lrc != MOE_OK) return lrc;
     if (dev >= kMaxDevices || !g_dev[dev].status) return MOE_OK;
     int host = 0;
     e = cudaMemcpy(&host, g_dev[dev].status, sizeof(int), cudaMemcpyDeviceToHost);

@@ -184,6 +184,15 @@ cudaError_t launch_combine(const float* y_rows, const int* idx, const float* w, 
 // norm.cu: RMSNorm of the [T, d] input rows into out (MoeDims.norm_* semantics).
 cudaError_t launch_rmsnorm(const void* x, const void* g, const Shape& s, float eps, void* out, cudaStream_t st);
 
+// route.cu: expert routing from given logits (MoeRouting).
+constexpr int kRouteMaxExperts = 1024;
+int check_routing(const MoeRouting* r, int E, int k);
+cudaError_t launch_route(const void* logits, int type, int64_t T, int E, int64_t ld, int k, const MoeRouting& r,
+                         const float* bias, int* idx, float* w, cudaStream_t st);
+
+// int8_linear.cu: reads and clears the status word of the int8 products on `dev`.
+int linear_status_collect(int dev);
+
 void set_error(const char* fmt, ...);
 
 // moe.cu: shared pieces of the layer entry points.
