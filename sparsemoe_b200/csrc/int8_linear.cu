@@ -94,30 +94,42 @@ template <typename T16> struct In8_16 {
 template <> struct In8<__half> : In8_16<__half> {};
 template <> struct In8<__nv_bfloat16> : In8_16<__nv_bfloat16> {};
 
-// round-half-even of the exact x / s.  x * (1/s) is within 127 * 2^-22 of the
-// quotient, so only values that close to a border n + 1/2 need more; there
-// the sign of x - (n + 1/2) s decides, which one fma gives exactly.
-__device__ __forceinline__ int quant1(float x, float s, float inv) {
-    const float r = x * inv;
-    float n = rintf(r);
-    if (fabsf(r - n) > 0.49995f) {
-        const float lo = floorf(r), e = fmaf(-(lo + 0.5f), s, x);
-        n = e > 0.0f ? lo + 1.0f : e < 0.0f ? lo : 2.0f * rintf(0.5f * (lo + 0.5f));
-    }
-    return (int)n;
+// round-half-even of the exact x / s next to a border n + 1/2: the sign of
+// x - (n + 1/2) s decides, which one fma gives exactly.
+__device__ __noinline__ int quant_border(float x, float s, float inv) {
+    const float r = x * inv, n = rintf(r);
+    if (fabsf(r - n) <= 0.4999f) return (int)n;
+    const float lo = floorf(r), e = fmaf(-(lo + 0.5f), s, x);
+    return (int)(e > 0.0f ? lo + 1.0f : e < 0.0f ? lo : 2.0f * rintf(0.5f * (lo + 0.5f)));
 }
 
-// Rows whose scale is so small or large that 1/s or the border's fma leaves
-// the normal range are scaled by a power of two first (pre != 1), which changes
-// no quotient; a subnormal scale has few bits, so there the codes are clamped.
+// Codes of eight values.  x * (1/s) is within 127 * 2^-23 of the quotient, so
+// only values that close to a border need more than its nearest integer, which
+// one fma leaves in the low bits of 1.5 * 2^23 + n.  Rows whose scale is so
+// small or large that 1/s or the border's fma leaves the normal range are
+// scaled by a power of two first (pre != 1), which changes no quotient; a
+// subnormal scale has few bits, so there the codes are clamped.
 __device__ __forceinline__ uint2 quant8(const float (&f)[8], float s, float inv, float pre) {
-    uint32_t w[2] = {0u, 0u};
+    constexpr float kMagic = 12582912.0f;
+    uint32_t t[8];
+    float off = 0.0f;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-        const int q = pre == 1.0f ? quant1(f[i], s, inv) : max(-127, min(127, quant1(f[i] * pre, s, inv)));
-        w[i >> 2] |= (uint32_t)(q & 0xFF) << (8 * (i & 3));
+        const float m = fmaf(f[i], inv, kMagic);
+        off = fmaxf(off, fabsf(fmaf(f[i], inv, kMagic - m)));
+        t[i] = __float_as_uint(m);
     }
-    return make_uint2(w[0], w[1]);
+    if (pre != 1.0f || off > 0.49995f) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const int q = quant_border(f[i] * pre, s, pre == 1.0f ? inv : __fdiv_rn(1.0f, s));
+            t[i] = (uint32_t)(pre == 1.0f ? q : max(-127, min(127, q)));
+        }
+    }
+    uint2 w;
+    w.x = __byte_perm(__byte_perm(t[0], t[1], 0x0040), __byte_perm(t[2], t[3], 0x0040), 0x5410);
+    w.y = __byte_perm(__byte_perm(t[4], t[5], 0x0040), __byte_perm(t[6], t[7], 0x0040), 0x5410);
+    return w;
 }
 
 __device__ __forceinline__ void store8(int8_t* q, uint2 w, int n, bool vec) {

@@ -12,15 +12,19 @@
 // Masked experts (NaN, logits <= -1e20 or f16's lowest value, a bias that is
 // NaN or <= -1e20) are never chosen; slots that stay empty hold (-1, 0).
 //
-// The order is that of exact arithmetic: the f32 scores carry an error bound,
-// and a row in which two values that follow each other in the order (or the
-// last kept and the first left group) are closer than twice that is selected
-// again in f64, where group sums that agree to 2^-49 are ties.  Rows that need
-// it are about 1 in 10^4 for continuous logits.
+// The order is that of f64 arithmetic.  The selection runs on 32-bit keys, the
+// value's order-preserving bits with the expert's index in the low ones, which
+// makes every key unique and a tie fall to the lower index.  f32 scores carry an
+// error bound and the index takes low bits of the value, so where two neighbours
+// of the order are closer than both, the candidates (the chosen and what is that
+// close behind them) are ranked again, one a lane, by their f64 values; where the
+// last kept and the first left group are, the whole row is selected in f64, and
+// group sums that agree to 2^-49 are ties (sigmoid(x) + sigmoid(-x) is 1 for every
+// x).  16-bit logits without a bias give up only zeros and need neither.
 //
-// One warp per token, lane l holding experts l*NV .. l*NV + NV - 1, so the
-// lowest lane of a ballot is the lowest index of a tie.  A round of the
-// selection is one redux.sync over the lanes' best keys and a ballot.
+// One warp per token, lane l holding experts l*NV .. l*NV + NV - 1.  Each lane
+// sorts its keys once; a round of the selection is one redux.sync over the
+// lanes' first keys and a pop in the lane that has it.
 #include "moe_internal.h"
 #include "common.cuh"
 
@@ -36,13 +40,14 @@ struct RouteParams {
     int E, k;
     int sigmoid;            // else softmax
     int G, per, kept, group_top;
-    int sub;                // lanes that share one group of the fast group pass (0: G > 32, f64 path)
+    int lanes;              // > 0: a group is this many whole lanes (a power of two)
+    int sub;                // else: lanes that share the pass over one group (0: G > 32, left to the f64 path)
     int renorm;
     float scale;
     const float* bias;
     int* idx;
     float* w;
-    int vec;                // rows allow the vector loads
+    int vec, vec_bias;      // rows / the bias allow the vector loads
 };
 
 template <typename T> __device__ __forceinline__ float to_f32(T v);
@@ -62,10 +67,20 @@ __device__ __forceinline__ uint32_t order_key(float v) {
 __device__ __forceinline__ float key_value(uint32_t key) {
     return __uint_as_float((key & 0x80000000u) ? (key & 0x7FFFFFFFu) : ~key);
 }
-__device__ __forceinline__ float warp_max(float v) {
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(kFull, v, o));
-    return v;
+__device__ __forceinline__ unsigned long long order_key(double v) {
+    const unsigned long long u = __double_as_longlong(v + 0.0);
+    return (u >> 63) ? ~u : (u | 0x8000000000000000ull);
+}
+__device__ __forceinline__ double key_value(unsigned long long key) {
+    return __longlong_as_double((key >> 63) ? (key & 0x7FFFFFFFFFFFFFFFull) : ~key);
+}
+
+__device__ __forceinline__ float warp_max(float v) { return key_value(__reduce_max_sync(kFull, order_key(v))); }
+__device__ __forceinline__ double warp_max(double v) {
+    const unsigned long long k = order_key(v);
+    const uint32_t hi = __reduce_max_sync(kFull, (uint32_t)(k >> 32));
+    const uint32_t lo = __reduce_max_sync(kFull, (uint32_t)(k >> 32) == hi ? (uint32_t)k : 0u);
+    return key_value((unsigned long long)hi << 32 | lo);
 }
 template <typename V> __device__ __forceinline__ V warp_sum(V v) {
 #pragma unroll
@@ -78,6 +93,23 @@ template <typename V> __device__ __forceinline__ void merge2(V& a, V& b, V c, V 
     const V lo = fmin(a, c);
     a = fmax(a, c);
     b = fmax(lo, fmax(b, d));
+}
+
+// Descending in-register sort (odd-even merge network, NV a power of two).
+template <int NV> __device__ __forceinline__ void sort_desc(uint32_t (&k)[NV]) {
+#pragma unroll
+    for (int p = 1; p < NV; p *= 2)
+#pragma unroll
+        for (int q = p; q >= 1; q /= 2)
+#pragma unroll
+            for (int j = q % p; j + q < NV; j += 2 * q)
+#pragma unroll
+                for (int i = 0; i < q; ++i)
+                    if (i + j + q < NV && (i + j) / (2 * p) == (i + j + q) / (2 * p)) {
+                        const uint32_t hi = max(k[i + j], k[i + j + q]);
+                        k[i + j + q] = min(k[i + j], k[i + j + q]);
+                        k[i + j] = hi;
+                    }
 }
 
 template <typename T, int NV>
@@ -104,102 +136,173 @@ __device__ __forceinline__ void load_row(const T* row, int e0, int E, bool vec, 
     for (int i = 0; i < NV; ++i) x[i] = e0 + i < E ? to_f32<T>(row[e0 + i]) : -INFINITY;
 }
 
-// The whole selection of one row in f64: lane l looks at experts l, l + 32, ..
-// (E <= 1024).  Returns the lane's choice (lane l: the l-th) or -1.
-template <typename T>
-__device__ __noinline__ int route_row_f64(const RouteParams& p, const T* row, int lane) {
-    const int n = (p.E + 31) / 32;
-    double v[32], s[32];
+// The whole selection of one row in f64.  Returns the lane's choice (lane l: the
+// l-th) or -1.  buf: 32 * NV doubles of shared memory of this warp.
+template <typename T, int NV>
+__device__ __noinline__ int route_row_f64(const RouteParams& p, const T* row, double* buf, int lane) {
+    const int e0 = lane * NV;
+    float x[NV];
+    load_row<T, NV>(row, e0, p.E, p.vec != 0, x);
+    double v[NV];
     double top = -INFINITY;
-    for (int i = 0; i < n; ++i) {
-        const int e = lane + 32 * i;
-        const float x = e < p.E ? to_f32<T>(row[e]) : -INFINITY;
-        v[i] = selectable<T>(x) ? (double)x : -INFINITY;
-        top = fmax(top, v[i]);
-    }
-    if (p.bias || p.group_top == 2) {
-        double sum = 0.0;
-        if (!p.sigmoid)
 #pragma unroll
-            for (int o = 16; o > 0; o >>= 1) top = fmax(top, __shfl_xor_sync(kFull, top, o));
-        for (int i = 0; i < n; ++i) {
-            if (p.sigmoid) s[i] = 1.0 / (1.0 + exp(-v[i]));
-            else s[i] = v[i] == -INFINITY ? 0.0 : v[i] == top ? 1.0 : exp(v[i] - top);
-            sum += s[i];
+    for (int q = 0; q < NV; ++q) {
+        v[q] = selectable<T>(x[q]) ? (double)x[q] : -INFINITY;
+        top = fmax(top, v[q]);
+    }
+    const bool pair = p.group_top == 2;
+    if (p.bias || pair) {
+        double s[NV], sum = 0.0;
+        top = warp_max(top);
+#pragma unroll
+        for (int q = 0; q < NV; ++q) {
+            if (p.sigmoid) s[q] = 1.0 / (1.0 + exp(-v[q]));
+            else s[q] = v[q] == -INFINITY ? 0.0 : v[q] == top ? 1.0 : exp(v[q] - top);
+            sum += s[q];
         }
         sum = p.sigmoid ? 1.0 : warp_sum(sum);
-        for (int i = 0; i < n; ++i) {
-            const int e = lane + 32 * i;
-            s[i] = p.sigmoid ? s[i] : s[i] / sum;
-            if (v[i] == -INFINITY) s[i] = -INFINITY;
-            if (p.bias && e < p.E) {
-                const float b = __ldg(p.bias + e);
-                v[i] = b > kMasked ? s[i] + (double)b : -INFINITY;
-                s[i] = v[i];
+#pragma unroll
+        for (int q = 0; q < NV; ++q) {
+            s[q] = v[q] == -INFINITY ? -INFINITY : p.sigmoid ? s[q] : s[q] / sum;
+            if (p.bias) {
+                const float b = e0 + q < p.E ? __ldg(p.bias + e0 + q) : -INFINITY;
+                v[q] = s[q] = b > kMasked ? s[q] + (double)b : -INFINITY;
             }
+            buf[e0 + q] = pair ? s[q] : v[q];
         }
+    } else if (p.G > 1) {
+#pragma unroll
+        for (int q = 0; q < NV; ++q) buf[e0 + q] = v[q];
     }
-    // a round over d[0..m): the largest value, then the lowest index of those
-    // that reach it (within `tie` of it, relative to 1 + |value|)
-    auto best_of = [&](const double* d, int m, double tie) {
-        double a = -INFINITY;
-        for (int i = 0; i < m; ++i) a = fmax(a, d[i]);
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) a = fmax(a, __shfl_xor_sync(kFull, a, o));
-        if (a == -INFINITY) return -1;
-        const double from = isinf(a) ? a : a - tie * (1.0 + fabs(a));
-        uint32_t at = 0xFFFFFFFFu;
-        for (int i = m - 1; i >= 0; --i)
-            if (d[i] >= from) at = lane + 32 * i;
-        return (int)__reduce_min_sync(kFull, at);
-    };
     if (p.G > 1) {
-        double gs[32];   // lane l: groups l, l + 32, ..
-        const int gn = (p.G + 31) / 32;
-        for (int i = 0; i < gn; ++i) gs[i] = -INFINITY;
-        for (int g = 0; g < p.G; ++g) {
-            double a = -INFINITY, b = -INFINITY;
-            for (int i = 0; i < n; ++i) {
-                const int e = lane + 32 * i;
-                if (e < p.E && e / p.per == g) merge2(a, b, p.group_top == 2 ? s[i] : v[i], (double)-INFINITY);
-            }
+        __syncwarp();
+        // scores of the groups into the first G places once every lane has read its members:
+        // lane l holds groups l, l + 32, .. (at most NV of them)
+        double gs[NV];
 #pragma unroll
-            for (int o = 16; o > 0; o >>= 1) {
+        for (int i = 0; i < NV; ++i) gs[i] = -INFINITY;
+        if (p.G <= 32) {
+            int sub = 32;
+            while (32 / sub < p.G) sub >>= 1;
+            const int g = lane / sub;
+            double a = -INFINITY, b = -INFINITY;
+            if (g < p.G)
+                for (int i = lane % sub; i < p.per; i += sub) merge2(a, b, buf[g * p.per + i], (double)-INFINITY);
+            for (int o = sub >> 1; o > 0; o >>= 1) {
                 const double c = __shfl_xor_sync(kFull, a, o), d = __shfl_xor_sync(kFull, b, o);
                 merge2(a, b, c, d);
             }
-            if (p.group_top == 2 && b != -INFINITY) a += b;
-            if ((g & 31) == lane) gs[g >> 5] = a;
-        }
-        uint32_t keep = 0;
-        // sums that agree to 2^-49 are ties: sigmoid(x) + sigmoid(-x) is 1 for every x
-        const double tie = p.group_top == 2 ? 0x1p-49 : 0.0;
-        for (int r = 0; r < p.kept; ++r) {
-            const int g = best_of(gs, gn, tie);
-            if (g < 0) break;
-            if ((g & 31) == lane) {
-                keep |= 1u << (g >> 5);
-                gs[g >> 5] = -INFINITY;
+            if (pair && b != -INFINITY) a += b;
+            a = __shfl_sync(kFull, a, (lane * sub) & 31);
+            if (lane < p.G) gs[0] = a;
+        } else {
+#pragma unroll
+            for (int i = 0; i < NV; ++i) {
+                const int g = lane + 32 * i;
+                if (g >= p.G) break;
+                double a = -INFINITY, b = -INFINITY;
+                for (int j = 0; j < p.per; ++j) merge2(a, b, buf[g * p.per + j], (double)-INFINITY);
+                gs[i] = pair && b != -INFINITY ? a + b : a;
             }
         }
-        for (int i = 0; i < n; ++i) {
-            const int e = lane + 32 * i, g = e < p.E ? e / p.per : 0;
-            if (!((__shfl_sync(kFull, keep, g & 31) >> (g >> 5)) & 1)) v[i] = -INFINITY;
+        uint32_t keep = 0;
+        const double tie = pair ? 0x1p-49 : 0.0;
+        for (int r = 0; r < p.kept; ++r) {
+            double a = gs[0];
+#pragma unroll
+            for (int i = 1; i < NV; ++i) a = fmax(a, gs[i]);
+            a = warp_max(a);
+            if (a == -INFINITY) break;
+            const double from = isinf(a) ? a : a - tie * (1.0 + fabs(a));
+            uint32_t at = 0xFFFFFFFFu;
+#pragma unroll
+            for (int i = NV - 1; i >= 0; --i)
+                if (gs[i] >= from) at = lane + 32 * i;
+            at = __reduce_min_sync(kFull, at);
+            if ((at & 31) == lane) {
+                keep |= 1u << (at >> 5);
+#pragma unroll
+                for (int i = 0; i < NV; ++i)
+                    if (i == (int)(at >> 5)) gs[i] = -INFINITY;
+            }
+        }
+#pragma unroll
+        for (int q = 0; q < NV; ++q) {
+            const int g = min(e0 + q, p.E - 1) / p.per;
+            if (!((__shfl_sync(kFull, keep, g & 31) >> (g >> 5)) & 1)) v[q] = -INFINITY;
         }
     }
     int mine = -1;
     for (int l = 0; l < p.k; ++l) {
-        const int e = best_of(v, n, 0.0);
-        if (e < 0) break;
-        if (lane == l) mine = e;
-        if ((e & 31) == lane) v[e >> 5] = -INFINITY;
+        double a = v[0];
+#pragma unroll
+        for (int q = 1; q < NV; ++q) a = fmax(a, v[q]);
+        const double m = warp_max(a);
+        if (m == -INFINITY) break;
+        const int wl = __ffs(__ballot_sync(kFull, a == m)) - 1;
+        int at = 0;
+#pragma unroll
+        for (int q = NV - 1; q >= 0; --q) at = v[q] == m ? q : at;
+        at = __shfl_sync(kFull, at, wl);
+        if (lane == l) mine = wl * NV + at;
+#pragma unroll
+        for (int q = 0; q < NV; ++q)
+            if (lane == wl && q == at) v[q] = -INFINITY;
     }
     return mine;
 }
 
+// exp(x): ex2.approx of the rounded x log2(e), (2 + 1.2 |x|) 2^-23 relative
+// (results below 2^-126 become 0).
+__device__ __forceinline__ float exp_fast(float x) {
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x * 1.4426950408889634f));
+    return r;
+}
+__device__ __forceinline__ float rcp_fast(float x) {   // 1 ulp
+    float r;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+
+// The candidates in lanes 0 .. n-1 (n >= k, or fewer where nothing else is
+// left) ranked by f64 value, equal values by the lower index: lane l gets the
+// l-th.  `top`: largest unmasked logit, where the softmax needs it.
 template <typename T, int NV>
-__global__ void __launch_bounds__(kRouteWarps * 32) route_kernel(const RouteParams p) {
-    __shared__ float sv[kRouteWarps][NV * 32];
+__device__ __noinline__ int rank_candidates(const RouteParams& p, const T* row, float top, int cand, int n, int* buf,
+                                            int lane) {
+    const float x = lane < n ? to_f32<T>(row[cand]) : 0.0f;
+    double v = x;
+    if (p.bias) {
+        const double b = lane < n ? __ldg(p.bias + cand) : 0.0f;
+        if (p.sigmoid) {
+            v = 1.0 / (1.0 + exp(-(double)x)) + b;
+        } else {
+            float xs[NV];
+            load_row<T, NV>(row, lane * NV, p.E, p.vec != 0, xs);
+            double sum = 0.0;
+#pragma unroll
+            for (int q = 0; q < NV; ++q)
+                if (selectable<T>(xs[q])) sum += xs[q] == top ? 1.0 : exp((double)xs[q] - (double)top);
+            sum = warp_sum(sum);
+            v = (x == top ? 1.0 : exp((double)x - (double)top)) / sum + b;
+        }
+    }
+    int rank = 0;
+    for (int j = 0; j < n; ++j) {
+        const double o = __shfl_sync(kFull, v, j);
+        const int e = __shfl_sync(kFull, cand, j);
+        rank += o > v || (o == v && e < cand) ? 1 : 0;
+    }
+    if (lane < n) buf[rank] = cand;
+    __syncwarp();
+    return lane < n ? buf[lane] : -1;
+}
+
+template <typename T, int NV>
+__global__ void __launch_bounds__(kRouteWarps * 32) route_kernel(const __grid_constant__ RouteParams p) {
+    constexpr uint32_t kIdx = 32 * NV - 1;      // the key bits that hold the index
+    __shared__ double sv[kRouteWarps][NV * 32];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int64_t t = (int64_t)blockIdx.x * kRouteWarps + warp;
     if (t >= p.T) return;
@@ -207,137 +310,180 @@ __global__ void __launch_bounds__(kRouteWarps * 32) route_kernel(const RoutePara
     const int e0 = lane * NV;
     float v[NV];
     load_row<T, NV>(row, e0, p.E, p.vec != 0, v);
-    uint32_t seen = 0;
 #pragma unroll
-    for (int q = 0; q < NV; ++q)
-        if (selectable<T>(v[q])) seen |= 1u << q;
-        else v[q] = -INFINITY;
+    for (int q = 0; q < NV; ++q) v[q] = selectable<T>(v[q]) ? v[q] : -INFINITY;
 
-    // softmax statistics, where a score or an unnormalised weight needs them
-    const bool pair = p.G > 1 && p.group_top == 2;
-    const bool scores = p.bias != nullptr || pair;
+    const bool pair = p.group_top == 2;         // (one group has group_top 1)
+    // 16-bit logits without a bias: at most 10 of 13 zero bits are given up
+    const bool exact = p.bias == nullptr && sizeof(T) == 2;
     float top = 0.0f, inv_sum = 1.0f;
     float s[NV];
-    if (!p.sigmoid && (scores || !p.renorm)) {
-        top = -INFINITY;
+    if (p.sigmoid) {
+        if (p.bias || pair)
 #pragma unroll
-        for (int q = 0; q < NV; ++q) top = fmaxf(top, v[q]);
+            for (int q = 0; q < NV; ++q) s[q] = rcp_fast(1.0f + exp_fast(-v[q]));
+    } else if (p.bias || pair || !p.renorm) {
+        top = v[0];
+#pragma unroll
+        for (int q = 1; q < NV; ++q) top = fmaxf(top, v[q]);
         top = warp_max(top);
         float sum = 0.0f;
 #pragma unroll
         for (int q = 0; q < NV; ++q) {
-            s[q] = !((seen >> q) & 1) ? 0.0f : v[q] == top ? 1.0f : __expf(v[q] - top);
+            s[q] = v[q] == top ? 1.0f : exp_fast(v[q] - top);
             sum += s[q];
         }
         sum = warp_sum(sum);
-        inv_sum = sum > 0.0f ? 1.0f / sum : 0.0f;
+        inv_sum = 1.0f / sum;
 #pragma unroll
         for (int q = 0; q < NV; ++q) s[q] *= inv_sum;
-    } else if (p.sigmoid && scores) {
-#pragma unroll
-        for (int q = 0; q < NV; ++q) s[q] = __fdividef(1.0f, 1.0f + __expf(-v[q]));
     }
     if (p.bias) {
+        float b[NV];
+        load_row<float, NV>(p.bias, e0, p.E, p.vec_bias != 0, b);
 #pragma unroll
-        for (int q = 0; q < NV; ++q) {
-            const float b = e0 + q < p.E ? __ldg(p.bias + e0 + q) : -INFINITY;
-            v[q] = ((seen >> q) & 1) && b > kMasked ? s[q] + b : -INFINITY;
-        }
+        for (int q = 0; q < NV; ++q) v[q] = v[q] > -INFINITY && b[q] > kMasked ? s[q] + b[q] : -INFINITY;
     }
-    // Error bounds: |s - exact| <= 4e-7 for the sigmoid (__expf: (2 + 1.2|x|)
-    // 2^-23 relative, times s(1-s); __fdividef 2 ulp) and <= 2e-6 for the
-    // softmax (the sum's relative error times s); two values compared, each of
-    // one or (groups) two scores, plus the roundings of the sums.
-    const float err = p.sigmoid ? 4e-7f : 2e-6f;
-    bool near = p.sub == 0 && p.G > 1;   // more than 32 groups: the f64 pass does them
+    // Twice the error of a score: the sigmoid's is at most 0.65 2^-23 (of exp,
+    // times s (1 - s)) + 2^-24 + 2^-23 (of 1 + e and rcp), the softmax's at most
+    // 17 2^-23 of its largest score (the sum's relative error times s).
+    const float err2 = p.sigmoid ? 6e-7f : 4.2e-6f * inv_sum;
 
-    if (p.G > 1 && !near) {
-        float* buf = sv[warp];
-        const bool from_scores = pair && !p.bias;
+    bool redo = false;                          // the whole row in f64
+    if (p.G > 1) {
+        const bool scored = p.bias || pair;
+        float m[NV];
 #pragma unroll
-        for (int q = 0; q < NV; ++q) buf[e0 + q] = !from_scores ? v[q] : ((seen >> q) & 1) ? s[q] : -INFINITY;
-        __syncwarp();
-        const int g = lane / p.sub, j = lane % p.sub;
+        for (int q = 0; q < NV; ++q) m[q] = v[q];
+        if (pair && !p.bias)
+#pragma unroll
+            for (int q = 0; q < NV; ++q) m[q] = v[q] == -INFINITY ? v[q] : s[q];
         float a = -INFINITY, b = -INFINITY;
-        if (g < p.G)
-            for (int i = j; i < p.per; i += p.sub) merge2(a, b, buf[g * p.per + i], -INFINITY);
-        for (int o = p.sub >> 1; o > 0; o >>= 1) {
-            const float c = __shfl_xor_sync(kFull, a, o), d = __shfl_xor_sync(kFull, b, o);
-            merge2(a, b, c, d);
+        int g;
+        if (p.lanes > 0) {
+            g = lane / p.lanes;
+#pragma unroll
+            for (int q = 0; q < NV; ++q) {
+                b = fmaxf(b, fminf(a, m[q]));
+                a = fmaxf(a, m[q]);
+            }
+            for (int o = p.lanes >> 1; o > 0; o >>= 1) {
+                const float c = __shfl_xor_sync(kFull, a, o), d = __shfl_xor_sync(kFull, b, o);
+                merge2(a, b, c, d);
+            }
+        } else {
+            float* buf = reinterpret_cast<float*>(sv[warp]);
+#pragma unroll
+            for (int q = 0; q < NV; ++q) buf[e0 + q] = m[q];
+            __syncwarp();
+            const int sub = max(p.sub, 1);
+            g = lane / sub;
+            if (p.sub > 0 && g < p.G)
+                for (int i = lane % sub; i < p.per; i += sub) merge2(a, b, buf[g * p.per + i], -INFINITY);
+            for (int o = sub >> 1; o > 0; o >>= 1) {
+                const float c = __shfl_xor_sync(kFull, a, o), d = __shfl_xor_sync(kFull, b, o);
+                merge2(a, b, c, d);
+            }
+            redo = p.sub == 0;
+            __syncwarp();
         }
         if (pair && b != -INFINITY) a += b;
-        const uint32_t key = g < p.G && a != -INFINITY ? order_key(a) : 0u;
-        int rank = 0;
-        for (int h = 0; h < p.G; ++h) {
-            const uint32_t other = __shfl_sync(kFull, key, h * p.sub);
-            rank += other > key || (other == key && h < g) ? 1 : 0;
+        if (g >= p.G) a = -INFINITY;
+        const uint32_t gk = a != -INFINITY ? (order_key(a) & ~31u) | (31 - g) : 0u;
+        uint32_t cur = gk, last = 0;
+        for (int r = 0; r < p.kept; ++r) {
+            const uint32_t best = __reduce_max_sync(kFull, cur);
+            if (best == 0) break;
+            last = best;
+            if (cur == best) cur = 0;
         }
-        const bool stay = key != 0 && rank < p.kept;
-        if (scores) {
-            const uint32_t last = __reduce_min_sync(kFull, stay ? key : 0xFFFFFFFFu);
-            const uint32_t out = __reduce_max_sync(kFull, stay ? 0u : key);
-            if (out != 0) {
-                const float lo = key_value(last), hi = key_value(out);
-                near = !(lo - hi > 4.0f * err + 6e-7f * fmaxf(fabsf(lo), fabsf(hi)));
+        const bool stay = gk != 0 && cur == 0;
+        const uint32_t out = __reduce_max_sync(kFull, cur);
+        if (out != 0 && (scored || !exact)) {
+            // close with the index in the low bits: the scores themselves decide
+            const float lo = key_value(last & ~31u), hi = key_value(out & ~31u);
+            if (!(lo - hi > 1.2e-5f * fmaxf(fabsf(lo), fabsf(hi)) + 2.0f * err2)) {
+                const float worst = key_value(__reduce_min_sync(kFull, stay ? order_key(a) : 0xFFFFFFFFu));
+                const float other = key_value(__reduce_max_sync(kFull, stay || gk == 0 ? 0u : order_key(a)));
+                redo |= scored ? !(worst - other > 2.0f * err2 + 6e-7f * fmaxf(fabsf(worst), fabsf(other)))
+                               : !(worst > other);
             }
         }
-        const uint32_t kept = __ballot_sync(kFull, stay);
-        int gg = e0 / p.per, r = e0 - gg * p.per;
+        if (p.lanes > 0) {
 #pragma unroll
-        for (int q = 0; q < NV; ++q) {
-            if (e0 + q >= p.E || !((kept >> (gg * p.sub & 31)) & 1)) v[q] = -INFINITY;
-            if (++r == p.per) { r = 0; ++gg; }
+            for (int q = 0; q < NV; ++q) v[q] = stay ? v[q] : -INFINITY;
+        } else {
+            const uint32_t kept = __ballot_sync(kFull, stay);
+            int gg = e0 / p.per, r = e0 - gg * p.per;
+#pragma unroll
+            for (int q = 0; q < NV; ++q) {
+                if (e0 + q >= p.E || !((kept >> (gg * p.sub & 31)) & 1)) v[q] = -INFINITY;
+                if (++r == p.per) { r = 0; ++gg; }
+            }
         }
     }
 
-    int my_i = -1;
-    if (!near) {
-        uint32_t key[NV], bk = 0;
+    uint32_t key[NV];
 #pragma unroll
-        for (int q = 0; q < NV; ++q) {
-            key[q] = v[q] == -INFINITY ? 0u : order_key(v[q]);
-            bk = max(bk, key[q]);
+    for (int q = 0; q < NV; ++q) key[q] = v[q] == -INFINITY ? 0u : (order_key(v[q]) & ~kIdx) | (kIdx - (e0 + q));
+    sort_desc<NV>(key);
+    uint32_t mine = 0;
+    int n = 0;
+    auto pop = [&](uint32_t best) {
+        if (key[0] == best) {
+#pragma unroll
+            for (int q = 0; q + 1 < NV; ++q) key[q] = key[q + 1];
+            key[NV - 1] = 0;
         }
-        float prev = INFINITY;
-        for (int l = 0; l <= p.k; ++l) {
-            const uint32_t m = __reduce_max_sync(kFull, bk);
-            if (m == 0) break;
-            if (p.bias) {
-                const float val = key_value(m);
-                if (l > 0) near |= !(prev - val > 2.0f * err + 3e-7f * fmaxf(fabsf(prev), fabsf(val)));
-                prev = val;
+        if (lane == n) mine = best;
+    };
+    uint32_t best = __reduce_max_sync(kFull, key[0]);
+    for (; n < p.k && best != 0; ++n) {
+        pop(best);
+        best = __reduce_max_sync(kFull, key[0]);
+    }
+    int my_i = mine != 0 ? (int)(kIdx - (mine & kIdx)) : -1;
+    if (!exact && !redo) {
+        auto close = [&](uint32_t a, uint32_t b) {   // a >= b, keys that follow each other
+            const float hi = key_value(a & ~kIdx), lo = key_value(b & ~kIdx);
+            return p.bias ? !(hi - lo > err2 + (32 * NV * 1.2e-7f + 3e-7f) * fmaxf(fabsf(hi), fabsf(lo))) : !(hi > lo);
+        };
+        uint32_t next = __shfl_down_sync(kFull, mine, 1);
+        if (lane == n - 1) next = best;
+        if (__any_sync(kFull, lane < n && next != 0 && close(mine, next))) {
+            // all that is close behind the last chosen is a candidate too
+            uint32_t last = __shfl_sync(kFull, mine, n - 1);
+            while (best != 0 && close(last, best) && n < 32) {
+                pop(best);
+                ++n;
+                last = best;
+                best = __reduce_max_sync(kFull, key[0]);
             }
-            if (l == p.k) break;
-            const int wl = __ffs(__ballot_sync(kFull, bk == m)) - 1;
-            int bq = 0;
-            if (lane == wl) {
-#pragma unroll
-                for (int q = NV - 1; q >= 0; --q) bq = key[q] == m ? q : bq;
-                bk = 0;
-#pragma unroll
-                for (int q = 0; q < NV; ++q) {
-                    if (q == bq) key[q] = 0;
-                    bk = max(bk, key[q]);
-                }
-            }
-            bq = __shfl_sync(kFull, bq, wl);
-            if (lane == l) my_i = wl * NV + bq;
+            redo = best != 0 && close(last, best);
+            if (!redo)
+                my_i = rank_candidates<T, NV>(p, row, top, mine != 0 ? (int)(kIdx - (mine & kIdx)) : -1, n,
+                                              reinterpret_cast<int*>(sv[warp]), lane);
         }
     }
-    if (near) my_i = route_row_f64<T>(p, row, lane);
+    if (redo) my_i = route_row_f64<T, NV>(p, row, sv[warp], lane);
+    if (lane >= p.k) my_i = -1;
 
     const float xs = my_i >= 0 ? to_f32<T>(row[my_i]) : -INFINITY;
-    float e;
-    if (p.renorm) {
-        const float mx = warp_max(xs);
-        if (p.sigmoid && mx > -80.0f) e = my_i >= 0 ? 1.0f / (1.0f + expf(-xs)) : 0.0f;
-        else e = my_i < 0 ? 0.0f : xs == mx ? 1.0f : expf(xs - mx);
-        const float sum = warp_sum(e);
-        e = sum > 0.0f ? e / sum : 0.0f;
-    } else if (p.sigmoid) {
-        e = my_i >= 0 ? 1.0f / (1.0f + expf(-xs)) : 0.0f;
-    } else {
+    float e = 0.0f;
+    if (p.sigmoid) {
+        e = rcp_fast(1.0f + expf(-xs));
+    } else if (!p.renorm) {
         e = my_i < 0 ? 0.0f : (xs == top ? 1.0f : expf(xs - top)) * inv_sum;
+    }
+    if (p.renorm) {
+        float sum = 0.0f;
+        if (p.sigmoid) sum = warp_sum(e);
+        if (!(sum > 1e-30f)) {   // softmax, or sigmoids so small that only their ratios, exp of the differences, are left
+            const float mx = warp_max(xs);
+            e = my_i < 0 ? 0.0f : xs == mx ? 1.0f : expf(xs - mx);
+            sum = warp_sum(e);
+        }
+        e = sum > 0.0f ? e * rcp_fast(sum) : 0.0f;
     }
     if (lane < p.k) {
         p.idx[t * p.k + lane] = my_i;
@@ -350,6 +496,10 @@ cudaError_t launch_nv(RouteParams p, cudaStream_t st) {
     constexpr int kBytes = NV * (int)sizeof(T);
     constexpr int kVec = kBytes % 16 == 0 ? 16 : kBytes % 8 == 0 ? 8 : kBytes % 4 == 0 ? 4 : 2;
     p.vec = reinterpret_cast<uintptr_t>(p.x) % kVec == 0 && (p.ld * (int64_t)sizeof(T)) % kVec == 0;
+    constexpr int kVecB = NV >= 4 ? 16 : NV * 4;
+    p.vec_bias = reinterpret_cast<uintptr_t>(p.bias) % kVecB == 0;
+    const int whole = p.per % NV == 0 ? p.per / NV : 0;
+    p.lanes = p.G > 1 && (whole & (whole - 1)) == 0 ? whole : 0;
     const int64_t blocks = (p.T + kRouteWarps - 1) / kRouteWarps;
     route_kernel<T, NV><<<(unsigned)blocks, kRouteWarps * 32, 0, st>>>(p);
     return cudaGetLastError();
