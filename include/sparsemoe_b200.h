@@ -294,6 +294,37 @@ int moe_int8_shared_expert(const void* x, int x_type, int64_t tokens, int d_mode
                            void* scratch, size_t scratch_bytes, cudaStream_t stream);
 size_t moe_int8_shared_expert_scratch_bytes(int64_t tokens, int d_model, int d_ff);
 
+// The layer with its own choice of experts and a shared expert (DeepSeek-style
+// layers).  moe_solve_v2 is this with null options.
+typedef struct MoeSharedExpert {
+    MoeInt8Weight gate, up, down;   // [d_model, d_ff] twice, [d_ff, d_model]
+    int d_ff;
+    void* out;                      // device [B, N, d_model], activation dtype: the shared expert's output (+ residual)
+    void* scratch;                  // device, 256-byte aligned, moe_int8_shared_expert_scratch_bytes(B * N, d_model, d_ff)
+    size_t scratch_bytes;
+} MoeSharedExpert;
+typedef struct MoeLayerOptions {
+    const MoeRouting* routing;      // null: the layer's own gate (softmax over the top-k logits)
+    const float* select_bias;       // device [E] or null (needs routing)
+    const MoeSharedExpert* shared;  // null: none
+} MoeLayerOptions;
+// moe_solve_v2 with options.  routing: the experts are chosen from the router's
+// logits as moe_route_experts does (MoEArgs.expert_logits is then required);
+// slots without an expert (index -1) take no capacity.  shared: the shared
+// expert runs on the rows the router reads (the normalised ones with
+// norm_weight), adds MoeDims.residual, rounds once to the activation dtype into
+// shared->out, and the combine starts from that row.
+int moe_solve_v2_ex(const struct MoEArgs* args, const MoeDims* dims, const MoeLayerOptions* options,
+                    cudaStream_t stream);
+// moe_stage_route / moe_stage_route_counts with options->routing and
+// select_bias (options->shared must be null: an expert-parallel caller runs
+// moe_int8_shared_expert on its own tokens and passes the result as
+// MoeDims.residual of moe_stage_combine).
+int moe_stage_route_ex(const struct MoEArgs* args, const MoeDims* dims, const MoeLayerOptions* options,
+                       cudaStream_t stream);
+int moe_stage_route_counts_ex(const struct MoEArgs* args, const MoeDims* dims, const MoeLayerOptions* options,
+                              int* raw_counts, cudaStream_t stream);
+
 // ---- expert weight files (.bin): a layer's router and expert weights in the
 //      formats the kernels read (no repacking on load).  The reference's
 //      driver names a cache file it never writes (drivers/main.cu:27-31).

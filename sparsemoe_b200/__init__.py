@@ -23,7 +23,7 @@ from .config import (  # noqa: F401  (re-exported)
     MOE_OK, MOE_ERR_INVALID_ARG, MOE_ERR_UNSUPPORTED, MOE_ERR_CUDA, MOE_ERR_TIMEOUT, MOE_ERR_NO_KERNEL,
     DTYPE_F16, DTYPE_BF16, DTYPE_INT8, DTYPE_FP8_BLOCK, DTYPE_W4A16, DTYPE_INT8_CHANNEL, DTYPE_NVFP4,
     DTYPE_INT4_PTX, DTYPE_FP8, ROUTER_SAME, ROUTER_F32, MoeError, MoEArgs, MoeDims, MoeWeightArray,
-    MoeWeightFile, MoeRouting, MoeInt8Weight, LayerConfig, _p)
+    MoeWeightFile, MoeRouting, MoeInt8Weight, MoeSharedExpert, MoeLayerOptions, LayerConfig, _p)
 from . import config as _config
 
 
@@ -87,6 +87,12 @@ def _load() -> ctypes.CDLL:
                                                           _p, _p, _p, _p]),
         "moe_quantize_nvfp4_device": (ctypes.c_int, [_p, ctypes.c_int, ctypes.c_int, ctypes.c_int, ctypes.c_int,
                                                       _p, _p, _p, _p]),
+        "moe_solve_v2_ex": (ctypes.c_int, [ctypes.POINTER(MoEArgs), ctypes.POINTER(MoeDims),
+                                           ctypes.POINTER(MoeLayerOptions), _p]),
+        "moe_stage_route_ex": (ctypes.c_int, [ctypes.POINTER(MoEArgs), ctypes.POINTER(MoeDims),
+                                              ctypes.POINTER(MoeLayerOptions), _p]),
+        "moe_stage_route_counts_ex": (ctypes.c_int, [ctypes.POINTER(MoEArgs), ctypes.POINTER(MoeDims),
+                                                     ctypes.POINTER(MoeLayerOptions), _p, _p]),
         "moe_route_experts": (ctypes.c_int, [_p, ctypes.c_int, ctypes.c_int64, ctypes.c_int, ctypes.c_int64,
                                              ctypes.c_int, ctypes.POINTER(MoeRouting), _p, _p, _p, _p]),
         "moe_int8_quantize_tokens": (ctypes.c_int, [_p, ctypes.c_int, ctypes.c_int64, ctypes.c_int, ctypes.c_int64, _p,
@@ -321,9 +327,9 @@ def quantize_per_tensor(w16: np.ndarray, qmax: float = 127.0):
     return q.reshape(w16.shape), float(scale)
 
 
-from .layer import MoeLayer  # noqa: E402  (needs `lib` above)
-from .operators import (  # noqa: E402
+from .operators import (  # noqa: E402  (needs `lib` above)
     Routing, int8_linear, int8_matmul, int8_shared_expert, int8_weight, quantize_int8_tokens, route_experts)
+from .layer import MoeLayer  # noqa: E402
 
 __all__ = ["MoEArgs", "MoeDims", "LayerConfig", "MoeLayer", "make_inputs", "capacity", "lib", "check",
            "MoeError", "normal16", "normal_f32", "zipf_bias", "quantize_per_tensor", "DTYPE_F16", "DTYPE_BF16",
@@ -331,4 +337,4 @@ __all__ = ["MoEArgs", "MoeDims", "LayerConfig", "MoeLayer", "make_inputs", "capa
            "DTYPE_W4A16", "quantize_int4_g128", "DTYPE_INT8_CHANNEL", "quantize_int8_channel",
            "DTYPE_NVFP4", "quantize_nvfp4", "DTYPE_INT4_PTX", "DTYPE_FP8", "save_weights", "load_weights", "MoeWeightFile", "MoeWeightArray",
            "Routing", "route_experts", "quantize_int8_tokens", "int8_matmul", "int8_linear", "int8_weight",
-           "int8_shared_expert", "MoeRouting", "MoeInt8Weight"]
+           "int8_shared_expert", "MoeRouting", "MoeInt8Weight", "MoeSharedExpert", "MoeLayerOptions"]

@@ -112,6 +112,20 @@ class MoeInt8Weight(ctypes.Structure):
     _fields_ = [("w", _p), ("row_stride", ctypes.c_int64), ("scale", _p), ("order", ctypes.c_int)]
 
 
+class MoeSharedExpert(ctypes.Structure):
+    """ctypes image of `MoeSharedExpert` (include/sparsemoe_b200.h)."""
+
+    _fields_ = [("gate", MoeInt8Weight), ("up", MoeInt8Weight), ("down", MoeInt8Weight), ("d_ff", ctypes.c_int),
+                ("out", _p), ("scratch", _p), ("scratch_bytes", ctypes.c_size_t)]
+
+
+class MoeLayerOptions(ctypes.Structure):
+    """ctypes image of `MoeLayerOptions` (include/sparsemoe_b200.h)."""
+
+    _fields_ = [("routing", ctypes.POINTER(MoeRouting)), ("select_bias", _p),
+                ("shared", ctypes.POINTER(MoeSharedExpert))]
+
+
 class MoeWeightArray(ctypes.Structure):
     """ctypes image of `MoeWeightArray` (include/sparsemoe_b200.h)."""
 

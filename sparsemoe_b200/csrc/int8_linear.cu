@@ -845,6 +845,57 @@ int linear_status_collect(int dev) {
     return MOE_ERR_TIMEOUT;
 }
 
+int run_shared_expert(const char* who, const void* x, int x_type, int64_t tokens, int d_model, int64_t row_stride,
+                      const MoeInt8Weight* gate, const MoeInt8Weight* up, const MoeInt8Weight* down, int d_ff,
+                      const void* residual, int64_t residual_stride, void* out, int out_type, int64_t out_stride,
+                      void* scratch, size_t scratch_bytes, bool check_only, cudaStream_t stream) {
+    int rc = check_dims(who, tokens, d_model, d_ff);
+    if (rc == MOE_OK) rc = check_dims(who, tokens, d_ff, d_model);
+    if (rc == MOE_OK) rc = check_x(who, x, x_type, tokens, d_model, row_stride);
+    if (rc == MOE_OK) rc = check_matrix(who, gate, d_model, d_ff);
+    if (rc == MOE_OK) rc = check_matrix(who, up, d_model, d_ff);
+    if (rc == MOE_OK) rc = check_matrix(who, down, d_ff, d_model);
+    if (rc == MOE_OK) rc = check_out(who, out, out_type, tokens, d_model, out_stride);
+    if (rc != MOE_OK) return rc;
+    if (gate->order != up->order) return bad(who, "gate and up weights must have the same order");
+    if (residual && (residual_stride < d_model || !aligned(residual, elem_bytes(x_type))))
+        return bad(who, "residual rows are shorter than d_model or not aligned to their type");
+    if (tokens == 0) return MOE_OK;
+    const SharedScratch sc = shared_scratch(tokens, d_model, d_ff);
+    rc = check_scratch(who, scratch, scratch_bytes, sc.total);
+    if (rc != MOE_OK || check_only) return rc;
+    int dev = 0, num_sms = 0;
+    rc = current_device(&dev, &num_sms);
+    if (rc != MOE_OK) return rc;
+    g_linear_used[dev] = true;
+    uint8_t* base = static_cast<uint8_t*>(scratch);
+    int8_t *qx = reinterpret_cast<int8_t*>(base + sc.qx), *qh = reinterpret_cast<int8_t*>(base + sc.qh);
+    float *sx = reinterpret_cast<float*>(base + sc.sx), *sh = reinterpret_cast<float*>(base + sc.sh);
+    float* h = reinterpret_cast<float*>(base + sc.h);
+    const bool fused = fused_swiglu(tokens, d_ff);
+    const int64_t behind = (int64_t)(up256((size_t)tokens * sc.ldh * sizeof(float)) / sizeof(float));
+    cudaError_t e = launch_quantize(x, x_type, tokens, d_model, row_stride, 0, qx, up16(d_model), sx, false, stream);
+    if (e == cudaSuccess) {
+        LinearParams p = out_params(tokens, d_model, d_ff, sx, nullptr, h, MOE_TYPE_F32, sc.ldh, gate->order, true);
+        p.out1 = behind;
+        const Matrix u{up->w, up->row_stride, up->scale};
+        e = launch_linear(qx, up16(d_model), p, Matrix{gate->w, gate->row_stride, gate->scale}, &u, fused, num_sms,
+                          stream);
+    }
+    if (e == cudaSuccess)
+        e = launch_quantize(h, MOE_TYPE_F32, tokens, d_ff, sc.ldh, fused ? 0 : behind, qh, up16(d_ff), sh, true, stream);
+    if (e == cudaSuccess) {
+        LinearParams p = out_params(tokens, d_ff, d_model, sh, nullptr, out, out_type, out_stride, down->order, true);
+        p.residual = residual;
+        p.ld_res = residual_stride;
+        p.res_type = x_type;
+        p.vec_res = aligned(residual, 16) && (residual_stride * elem_bytes(x_type)) % 16 == 0;
+        e = launch_linear(qh, up16(d_ff), p, Matrix{down->w, down->row_stride, down->scale}, nullptr, false, num_sms,
+                          stream);
+    }
+    return e == cudaSuccess ? MOE_OK : cuda_error(who, e);
+}
+
 }  // namespace moe
 
 using namespace moe;
@@ -925,50 +976,6 @@ extern "C" int moe_int8_shared_expert(const void* x, int x_type, int64_t tokens,
                                       const MoeInt8Weight* gate, const MoeInt8Weight* up, const MoeInt8Weight* down,
                                       int d_ff, const void* residual, int64_t residual_stride, void* out, int out_type,
                                       int64_t out_stride, void* scratch, size_t scratch_bytes, cudaStream_t stream) {
-    const char* who = "moe_int8_shared_expert";
-    int rc = check_dims(who, tokens, d_model, d_ff);
-    if (rc == MOE_OK) rc = check_dims(who, tokens, d_ff, d_model);
-    if (rc == MOE_OK) rc = check_x(who, x, x_type, tokens, d_model, row_stride);
-    if (rc == MOE_OK) rc = check_matrix(who, gate, d_model, d_ff);
-    if (rc == MOE_OK) rc = check_matrix(who, up, d_model, d_ff);
-    if (rc == MOE_OK) rc = check_matrix(who, down, d_ff, d_model);
-    if (rc == MOE_OK) rc = check_out(who, out, out_type, tokens, d_model, out_stride);
-    if (rc != MOE_OK) return rc;
-    if (gate->order != up->order) return bad(who, "gate and up weights must have the same order");
-    if (residual && (residual_stride < d_model || !aligned(residual, elem_bytes(x_type))))
-        return bad(who, "residual rows are shorter than d_model or not aligned to their type");
-    if (tokens == 0) return MOE_OK;
-    const SharedScratch sc = shared_scratch(tokens, d_model, d_ff);
-    rc = check_scratch(who, scratch, scratch_bytes, sc.total);
-    if (rc != MOE_OK) return rc;
-    int dev = 0, num_sms = 0;
-    rc = current_device(&dev, &num_sms);
-    if (rc != MOE_OK) return rc;
-    g_linear_used[dev] = true;
-    uint8_t* base = static_cast<uint8_t*>(scratch);
-    int8_t *qx = reinterpret_cast<int8_t*>(base + sc.qx), *qh = reinterpret_cast<int8_t*>(base + sc.qh);
-    float *sx = reinterpret_cast<float*>(base + sc.sx), *sh = reinterpret_cast<float*>(base + sc.sh);
-    float* h = reinterpret_cast<float*>(base + sc.h);
-    const bool fused = fused_swiglu(tokens, d_ff);
-    const int64_t behind = (int64_t)(up256((size_t)tokens * sc.ldh * sizeof(float)) / sizeof(float));
-    cudaError_t e = launch_quantize(x, x_type, tokens, d_model, row_stride, 0, qx, up16(d_model), sx, false, stream);
-    if (e == cudaSuccess) {
-        LinearParams p = out_params(tokens, d_model, d_ff, sx, nullptr, h, MOE_TYPE_F32, sc.ldh, gate->order, true);
-        p.out1 = behind;
-        const Matrix u{up->w, up->row_stride, up->scale};
-        e = launch_linear(qx, up16(d_model), p, Matrix{gate->w, gate->row_stride, gate->scale}, &u, fused, num_sms,
-                          stream);
-    }
-    if (e == cudaSuccess)
-        e = launch_quantize(h, MOE_TYPE_F32, tokens, d_ff, sc.ldh, fused ? 0 : behind, qh, up16(d_ff), sh, true, stream);
-    if (e == cudaSuccess) {
-        LinearParams p = out_params(tokens, d_ff, d_model, sh, nullptr, out, out_type, out_stride, down->order, true);
-        p.residual = residual;
-        p.ld_res = residual_stride;
-        p.res_type = x_type;
-        p.vec_res = aligned(residual, 16) && (residual_stride * elem_bytes(x_type)) % 16 == 0;
-        e = launch_linear(qh, up16(d_ff), p, Matrix{down->w, down->row_stride, down->scale}, nullptr, false, num_sms,
-                          stream);
-    }
-    return e == cudaSuccess ? MOE_OK : cuda_error(who, e);
+    return run_shared_expert("moe_int8_shared_expert", x, x_type, tokens, d_model, row_stride, gate, up, down, d_ff,
+                             residual, residual_stride, out, out_type, out_stride, scratch, scratch_bytes, false, stream);
 }

@@ -440,15 +440,60 @@ int enqueue_norm(const MoEArgs* a, const MoeDims* dims, const Shape& s, cudaStre
     return MOE_OK;
 }
 
+int check_options(const MoEArgs* a, const MoeDims* dims, const Shape& s, const MoeLayerOptions* o) {
+    if (!o) return MOE_OK;
+    if (o->routing) {
+        const int rc = check_routing(o->routing, s.E, s.k);
+        if (rc != MOE_OK) return rc;
+        if (!a->expert_logits) {
+            set_error("MoeLayerOptions.routing needs MoEArgs.expert_logits (the logits it chooses from)");
+            return MOE_ERR_INVALID_ARG;
+        }
+        if (reinterpret_cast<uintptr_t>(o->select_bias) % 4 != 0) {
+            set_error("MoeLayerOptions.select_bias is not aligned to f32");
+            return MOE_ERR_INVALID_ARG;
+        }
+    } else if (o->select_bias) {
+        set_error("MoeLayerOptions.select_bias needs routing");
+        return MOE_ERR_INVALID_ARG;
+    }
+    return MOE_OK;
+}
+
+// The shared expert of the routed rows: its output starts the combine.
+int shared_expert(const MoEArgs* a, const MoeDims* dims, const Shape& s, const MoeSharedExpert& e, bool check_only,
+                  cudaStream_t stream) {
+    const int type = s.act_bf16 ? MOE_TYPE_BF16 : MOE_TYPE_F16;
+    return run_shared_expert("MoeLayerOptions.shared", routed_args(a, dims).input, type, s.T(), s.d, s.d, &e.gate, &e.up,
+                             &e.down, e.d_ff, dims->residual, s.d, e.out, type, s.d, e.scratch, e.scratch_bytes,
+                             check_only, stream);
+}
+
+// Router, then the experts of every token: the gate fused into the router
+// kernels, or (options) the routing operator on the logits they write.
+int enqueue_choice(const MoEArgs* a, const MoeDims* dims, const Shape& s, const Workspace& ws,
+                   const MoeLayerOptions* o, cudaStream_t stream) {
+    Shape rs = s;
+    if (o && o->routing) rs.k = 0;   // logits only
+    MOE_TRY(launch_router_topk(a->input, a->router_weights, dims->router_bias, rs, ws.router_logits, a->expert_logits,
+                               a->selected_expert_indices, a->selected_expert_weights, stream),
+            "router_topk");
+    if (o && o->routing)
+        MOE_TRY(launch_route(a->expert_logits, MOE_TYPE_F32, s.T(), s.E, s.E, s.k, *o->routing, o->select_bias,
+                             a->selected_expert_indices, a->selected_expert_weights, stream),
+                "route_experts");
+    return MOE_OK;
+}
+
 // Stages 1-3: router + top-k, slots, gather into the dense expert-major rows.
-int enqueue_route(const MoEArgs* a_in, const MoeDims* dims, const Shape& s, const Workspace& ws, cudaStream_t stream) {
+int enqueue_route(const MoEArgs* a_in, const MoeDims* dims, const Shape& s, const Workspace& ws, cudaStream_t stream,
+                  const MoeLayerOptions* options = nullptr) {
     int rc = enqueue_norm(a_in, dims, s, stream);
     if (rc != MOE_OK) return rc;
     const MoEArgs ra = routed_args(a_in, dims);
     const MoEArgs* a = &ra;
-    MOE_TRY(launch_router_topk(a->input, a->router_weights, dims->router_bias, s, ws.router_logits, a->expert_logits,
-                               a->selected_expert_indices, a->selected_expert_weights, stream),
-            "router_topk");
+    rc = enqueue_choice(a, dims, s, ws, options, stream);
+    if (rc != MOE_OK) return rc;
     MOE_TRY(mark_stage(1, stream), "cudaEventRecord(stage event)");
     const FfnBuffers fb = ffn_buffers(a, s);
     MOE_TRY(launch_dispatch_count(a->selected_expert_indices, s, ws, a->expert_counts, nullptr, stream),
@@ -526,12 +571,18 @@ int enqueue_ffn(const MoEArgs* a, const MoeDims* dims, const Shape& s, const Gro
 
 // The stage sequence of one layer call on `stream`, given its scratch.
 int enqueue_layer(const MoEArgs* a, const MoeDims* dims, const Shape& s, const Workspace& ws, int num_sms,
-                  cudaStream_t stream) {
+                  cudaStream_t stream, const MoeLayerOptions* options) {
     MOE_TRY(cudaMemsetAsync(ws.status, 0, sizeof(int), stream), "cudaMemsetAsync(status)");
     MOE_TRY(mark_stage(0, stream), "cudaEventRecord(stage event)");
-    int rc = enqueue_route(a, dims, s, ws, stream);
+    int rc = enqueue_route(a, dims, s, ws, stream, options);
     if (rc != MOE_OK) return rc;
     MOE_TRY(mark_stage(2, stream), "cudaEventRecord(stage event)");
+    const void* start = dims->residual;   // the rows the combine starts from
+    if (options && options->shared) {
+        rc = shared_expert(a, dims, s, *options->shared, false, stream);
+        if (rc != MOE_OK) return rc;
+        start = options->shared->out;
+    }
     if (s.T() > 0 && s.cap > 0) {
         const GroupTable gt{ws.expert_rows, ws.expert_start, nullptr, s.E, s.rows_capacity()};
         rc = enqueue_ffn(a, dims, s, gt, ws.status, ws.a_scale, ws.h_scale, num_sms, stream);
@@ -541,7 +592,7 @@ int enqueue_layer(const MoEArgs* a, const MoeDims* dims, const Shape& s, const W
     }
     MOE_TRY(mark_stage(4, stream), "cudaEventRecord(stage event)");
     MOE_TRY(launch_combine(a->hidden_mlp_layer_2_out, a->selected_expert_indices, a->selected_expert_weights, s, ws,
-                           a->final_output, dims->output_16, stream, dims->residual),
+                           a->final_output, dims->output_16, stream, start),
             "combine");
     MOE_TRY(mark_stage(5, stream), "cudaEventRecord(stage event)");
     return MOE_OK;
@@ -550,6 +601,11 @@ int enqueue_layer(const MoEArgs* a, const MoeDims* dims, const Shape& s, const W
 }  // namespace moe
 
 extern "C" int moe_solve_v2(const MoEArgs* a, const MoeDims* dims, cudaStream_t stream) {
+    return moe_solve_v2_ex(a, dims, nullptr, stream);
+}
+
+extern "C" int moe_solve_v2_ex(const MoEArgs* a, const MoeDims* dims, const MoeLayerOptions* options,
+                               cudaStream_t stream) {
     Shape s;
     int rc = make_shape(dims, &s);
     if (rc != MOE_OK) return rc;
@@ -557,6 +613,12 @@ extern "C" int moe_solve_v2(const MoEArgs* a, const MoeDims* dims, cudaStream_t 
     if (rc != MOE_OK) return rc;
     rc = check_norm(dims);
     if (rc != MOE_OK) return rc;
+    rc = check_options(a, dims, s, options);
+    if (rc != MOE_OK) return rc;
+    if (options && options->shared) {
+        rc = shared_expert(a, dims, s, *options->shared, true, stream);
+        if (rc != MOE_OK) return rc;
+    }
     DeviceState* st = nullptr;
     int dev = 0;
     rc = device_state(&st, &dev);
@@ -564,12 +626,13 @@ extern "C" int moe_solve_v2(const MoEArgs* a, const MoeDims* dims, cudaStream_t 
     Workspace ws;
     rc = resolve_workspace(*st, dev, dims, s, &ws);
     if (rc != MOE_OK) return rc;
-    return enqueue_layer(a, dims, s, ws, st->num_sms, stream);
+    return enqueue_layer(a, dims, s, ws, st->num_sms, stream, options);
 }
 
 // ---- expert-parallel building blocks ---------------------------------------
 namespace {
-int route_stage_setup(const MoEArgs* a, const MoeDims* dims, const char* who, Shape* s, Workspace* ws) {
+int route_stage_setup(const MoEArgs* a, const MoeDims* dims, const char* who, Shape* s, Workspace* ws,
+                      const MoeLayerOptions* options = nullptr) {
     int rc = make_shape(dims, s, /*bind_check=*/false);   // routing needs no weights
     if (rc != MOE_OK) return rc;
     if (!a || !a->input || !a->router_weights || !a->selected_expert_indices || !a->selected_expert_weights ||
@@ -579,6 +642,12 @@ int route_stage_setup(const MoEArgs* a, const MoeDims* dims, const char* who, Sh
     }
     rc = check_norm(dims);
     if (rc != MOE_OK) return rc;
+    rc = check_options(a, dims, *s, options);
+    if (rc != MOE_OK) return rc;
+    if (options && options->shared) {
+        set_error("%s: the routing stages run no shared expert (MoeLayerOptions.shared must be null)", who);
+        return MOE_ERR_INVALID_ARG;
+    }
     DeviceState* st = nullptr;
     int dev = 0;
     rc = device_state(&st, &dev);
@@ -588,27 +657,36 @@ int route_stage_setup(const MoEArgs* a, const MoeDims* dims, const char* who, Sh
 }  // namespace
 
 extern "C" int moe_stage_route(const MoEArgs* a, const MoeDims* dims, cudaStream_t stream) {
+    return moe_stage_route_ex(a, dims, nullptr, stream);
+}
+
+extern "C" int moe_stage_route_ex(const MoEArgs* a, const MoeDims* dims, const MoeLayerOptions* options,
+                                  cudaStream_t stream) {
     Shape s;
     Workspace ws;
-    const int rc = route_stage_setup(a, dims, "moe_stage_route", &s, &ws);
+    const int rc = route_stage_setup(a, dims, "moe_stage_route", &s, &ws, options);
     if (rc != MOE_OK) return rc;
     MOE_TRY(cudaMemsetAsync(ws.status, 0, sizeof(int), stream), "cudaMemsetAsync(status)");
-    return enqueue_route(a, dims, s, ws, stream);
+    return enqueue_route(a, dims, s, ws, stream, options);
 }
 
 extern "C" int moe_stage_route_counts(const MoEArgs* a, const MoeDims* dims, int* raw_counts, cudaStream_t stream) {
+    return moe_stage_route_counts_ex(a, dims, nullptr, raw_counts, stream);
+}
+
+extern "C" int moe_stage_route_counts_ex(const MoEArgs* a, const MoeDims* dims, const MoeLayerOptions* options,
+                                         int* raw_counts, cudaStream_t stream) {
     Shape s;
     Workspace ws;
-    const int rc = route_stage_setup(a, dims, "moe_stage_route_counts", &s, &ws);
+    const int rc = route_stage_setup(a, dims, "moe_stage_route_counts", &s, &ws, options);
     if (rc != MOE_OK) return rc;
     if (!raw_counts) { set_error("moe_stage_route_counts: raw_counts is null"); return MOE_ERR_INVALID_ARG; }
     MOE_TRY(cudaMemsetAsync(ws.status, 0, sizeof(int), stream), "cudaMemsetAsync(status)");
     const int nrc = enqueue_norm(a, dims, s, stream);
     if (nrc != MOE_OK) return nrc;
     const MoEArgs ra = routed_args(a, dims);
-    MOE_TRY(launch_router_topk(ra.input, a->router_weights, dims->router_bias, s, ws.router_logits, a->expert_logits,
-                               a->selected_expert_indices, a->selected_expert_weights, stream),
-            "router_topk");
+    const int crc = enqueue_choice(&ra, dims, s, ws, options, stream);
+    if (crc != MOE_OK) return crc;
     MOE_TRY(launch_dispatch_count(a->selected_expert_indices, s, ws, a->expert_counts, raw_counts, stream),
             "dispatch (count)");
     return MOE_OK;

@@ -190,6 +190,11 @@ int check_routing(const MoeRouting* r, int E, int k);
 cudaError_t launch_route(const void* logits, int type, int64_t T, int E, int64_t ld, int k, const MoeRouting& r,
                          const float* bias, int* idx, float* w, cudaStream_t st);
 
+// int8_linear.cu: checks and (unless check_only) enqueues the shared expert of T rows.
+int run_shared_expert(const char* who, const void* x, int x_type, int64_t tokens, int d_model, int64_t row_stride,
+                      const MoeInt8Weight* gate, const MoeInt8Weight* up, const MoeInt8Weight* down, int d_ff,
+                      const void* residual, int64_t residual_stride, void* out, int out_type, int64_t out_stride,
+                      void* scratch, size_t scratch_bytes, bool check_only, cudaStream_t stream);
 // int8_linear.cu: reads and clears the status word of the int8 products on `dev`.
 int linear_status_collect(int dev);
 
@@ -203,6 +208,6 @@ int check_norm(const MoeDims* dims);
 int current_device(int* dev, int* num_sms);           // sm_100 check, cached SM count
 void note_status_word(int dev, int* status);            // read by moe_check_device_status
 int enqueue_layer(const MoEArgs* a, const MoeDims* dims, const Shape& s, const Workspace& ws, int num_sms,
-                  cudaStream_t stream);
+                  cudaStream_t stream, const MoeLayerOptions* options = nullptr);
 
 }  // namespace moe

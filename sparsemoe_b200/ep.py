@@ -51,6 +51,8 @@ import ctypes
 import numpy as np
 
 from . import LayerConfig, MoEArgs, MoeDims, capacity, check, lib
+from .config import MoeLayerOptions
+from .operators import int8_shared_expert
 
 
 # ---- planner ---------------------------------------------------------------------
@@ -161,10 +163,13 @@ class ExpertParallelLayer:
 
     def __init__(self, cfg: LayerConfig, device, group=None, chunks: int | None = None,
                  global_batch: bool = False, transport: str = "nccl", placement: str = "contiguous",
-                 health_timeout: float | None = None, store=None):
+                 health_timeout: float | None = None, store=None, routing=None):
         import torch
         import torch.distributed as dist
         self.torch, self.dist = torch, dist
+        # routing (a Routing) replaces the layer's own gate on every rank, as in MoeLayer
+        self.routing = routing
+        self.select_bias = self.shared = None
         self.group = group
         self.world = dist.get_world_size(group)
         self.rank = dist.get_rank(group)
@@ -361,7 +366,34 @@ class ExpertParallelLayer:
                                         for k in ("wg_g", "wu_g", "wd_g")]
         if inputs.get("bias") is not None:
             self.bias = torch.from_numpy(inputs["bias"]).to(self.device)
+        if inputs.get("select_bias") is not None:
+            if self.routing is None:
+                raise ValueError("select_bias needs a routing (ExpertParallelLayer(..., routing=Routing(...)))")
+            if np.shape(inputs["select_bias"]) != (cfg.num_experts,):
+                raise ValueError(f"select_bias must have {cfg.num_experts} values")
+            self.select_bias = torch.from_numpy(np.ascontiguousarray(inputs["select_bias"], np.float32)).to(self.device)
+        if inputs.get("shared_wg") is not None:
+            # replicated on every rank, each running it on its own tokens
+            from .layer import SharedExpert
+            self.shared = SharedExpert(inputs, cfg.d_model, self.device)
+            self.shared_out = torch.empty_like(self.x)
         return self
+
+    def _options(self):
+        """The routing options of the routing stages (None: the layer's own gate)."""
+        if self.routing is None:
+            return None
+        o = MoeLayerOptions()
+        o.routing = ctypes.pointer(self.routing.struct())
+        o.select_bias = None if self.select_bias is None else self.select_bias.data_ptr()
+        return ctypes.byref(o)
+
+    def _enqueue_shared(self, ch):
+        """The shared expert of a chunk's tokens on the current stream; the combine starts from its rows."""
+        if self.shared is not None and ch.x.shape[0] > 0:
+            out = self.shared_out[ch.x.storage_offset() // self.cfg.d_model:][: ch.x.shape[0]]
+            int8_shared_expert(ch.x, *self.shared.weights(), out=out)
+            ch.dims.residual = out.data_ptr()
 
     @property
     def wg(self):
@@ -531,15 +563,16 @@ class ExpertParallelLayer:
             ch.ra = self._route_args(ch)
             if self.global_batch:
                 # phase 1, then every rank's totals; slot_base = sum over the lower ranks
-                check(lib.moe_stage_route_counts(ctypes.byref(ch.ra), ctypes.byref(ch.dims),
-                                                 self.raw.data_ptr(), sp))
+                check(lib.moe_stage_route_counts_ex(ctypes.byref(ch.ra), ctypes.byref(ch.dims), self._options(),
+                                                    self.raw.data_ptr(), sp))
                 allraw = torch.empty(self.world, *self.raw.shape, dtype=torch.int32, device=self.device)
                 dist.all_gather_into_tensor(allraw, self.raw, group=self.group)
                 torch.sum(allraw[: self.rank], dim=0, dtype=torch.int32, out=self.slot_base)
                 ch.dims.slot_base = self.slot_base.data_ptr()
                 check(lib.moe_stage_route_finish(ctypes.byref(ch.ra), ctypes.byref(ch.dims), sp))
             else:
-                check(lib.moe_stage_route(ctypes.byref(ch.ra), ctypes.byref(ch.dims), sp))
+                check(lib.moe_stage_route_ex(ctypes.byref(ch.ra), ctypes.byref(ch.dims), self._options(), sp))
+            self._enqueue_shared(ch)
         ev("routed")
         if self.transport == "peer":
             ch = self.chunks[0]

@@ -11,17 +11,44 @@ import numpy as np
 import torch
 
 from . import LayerConfig, MoEArgs, check, lib
+from .config import MoeLayerOptions, MoeSharedExpert
+from .operators import Routing, int8_weight, _weight
 
 
 def _t16(cfg: LayerConfig):
     return torch.bfloat16 if cfg.act_bf16 else torch.float16
 
 
+class SharedExpert:
+    """Weights of the shared expert on one device, from a load() dict: "shared_wg", "shared_wu" [d, f] and
+    "shared_wd" [f, d] int8 with f32 scales "shared_sg", "shared_su" [f] and "shared_sd" [d]."""
+
+    KEYS = ("shared_wg", "shared_sg", "shared_wu", "shared_su", "shared_wd", "shared_sd")
+
+    def __init__(self, inputs: dict, d_model: int, device: torch.device):
+        dev = lambda a: torch.from_numpy(np.ascontiguousarray(a)).to(device)  # noqa: E731
+        self.wg, self.wu, self.wd = (int8_weight(dev(inputs[k])) for k in ("shared_wg", "shared_wu", "shared_wd"))
+        self.sg, self.su, self.sd = (dev(inputs[k]) for k in ("shared_sg", "shared_su", "shared_sd"))
+        self.d_ff = self.wg.shape[1]
+        if self.wu.shape != (d_model, self.d_ff) or self.wd.shape != (self.d_ff, d_model):
+            raise ValueError(f"shared_wu must be [{d_model}, {self.d_ff}] and shared_wd [{self.d_ff}, {d_model}]")
+
+    def weights(self) -> tuple:
+        return self.wg, self.sg, self.wu, self.su, self.wd, self.sd
+
+
 class MoeLayer:
+    """`routing` (a Routing) replaces the layer's own gate; "select_bias" [E] f32 in load()'s inputs then moves the
+    choice, and the SharedExpert keys there add a shared expert to every token."""
+
     def __init__(self, cfg: LayerConfig, device: str | torch.device = "cuda", want_logits: bool = True,
-                 want_out16: bool = True):
+                 want_out16: bool = True, routing: Routing | None = None):
         self.cfg = cfg
         self.device = torch.device(device)
+        self.routing = routing
+        self.select_bias = self.shared = None
+        if routing is not None and not want_logits:
+            raise ValueError("routing chooses from the logits: want_logits must be True")
         B, N, d, f, E, k = cfg.num_batches, cfg.tokens, cfg.d_model, cfg.d_ff, cfg.num_experts, cfg.top_k
         cap = cfg.capacity()
         self.cap = cap
@@ -96,6 +123,17 @@ class MoeLayer:
                            for k in ("sg", "su", "sd")]
         if inputs.get("bias") is not None:
             self.bias = torch.from_numpy(inputs["bias"]).to(self.device)
+        if inputs.get("select_bias") is not None:
+            if self.routing is None:
+                raise ValueError("select_bias needs a routing (MoeLayer(cfg, routing=Routing(...)))")
+            if np.shape(inputs["select_bias"]) != (self.cfg.num_experts,):
+                raise ValueError(f"select_bias must have {self.cfg.num_experts} values")
+            self.select_bias = torch.from_numpy(np.ascontiguousarray(inputs["select_bias"], np.float32)).to(self.device)
+        if inputs.get("shared_wg") is not None:
+            self.shared = SharedExpert(inputs, self.cfg.d_model, self.device)
+            self.shared_out = torch.empty_like(self.x)
+            n = lib.moe_int8_shared_expert_scratch_bytes(self.cfg.T, self.cfg.d_model, self.shared.d_ff)
+            self.shared_scratch = torch.empty(max(n, 256), dtype=torch.uint8, device=self.device)
         if inputs.get("norm_w") is not None:       # pre-MoE RMSNorm of x (gamma [d], 16-bit)
             self.norm_w = torch.empty(self.cfg.d_model, dtype=self.x.dtype, device=self.device)
             put(self.norm_w, inputs["norm_w"])
@@ -186,12 +224,31 @@ class MoeLayer:
             dm.residual = self.residual.data_ptr()
         return dm
 
+    def options(self) -> MoeLayerOptions | None:
+        """The routing and shared expert of the call (None: neither)."""
+        if self.routing is None and self.shared is None:
+            return None
+        o = MoeLayerOptions()
+        if self.routing is not None:
+            o.routing = ctypes.pointer(self.routing.struct())
+            o.select_bias = None if self.select_bias is None else self.select_bias.data_ptr()
+        if self.shared is not None:
+            sh, d, i = self.shared, self.cfg.d_model, self.shared.wg.get_device()
+            o.shared = ctypes.pointer(MoeSharedExpert(
+                _weight(sh.wg, sh.sg, "shared_wg", d, i)[0], _weight(sh.wu, sh.su, "shared_wu", d, i)[0],
+                _weight(sh.wd, sh.sd, "shared_wd", sh.d_ff, i)[0], sh.d_ff, self.shared_out.data_ptr(),
+                self.shared_scratch.data_ptr(), self.shared_scratch.numel()))
+        return o
+
     def forward(self, stream: torch.cuda.Stream | None = None) -> torch.Tensor:
         """Enqueues one layer call on `stream` (default: torch's current stream)."""
         s = stream if stream is not None else torch.cuda.current_stream(self.device)
-        a, dm = self.args(), self.dims()
-        self._keep = (a, dm)
-        check(lib.moe_solve_v2(ctypes.byref(a), ctypes.byref(dm), ctypes.c_void_p(s.cuda_stream)))
+        a, dm, o = self.args(), self.dims(), self.options()
+        self._keep = (a, dm, o)
+        if o is None:
+            check(lib.moe_solve_v2(ctypes.byref(a), ctypes.byref(dm), ctypes.c_void_p(s.cuda_stream)))
+        else:
+            check(lib.moe_solve_v2_ex(ctypes.byref(a), ctypes.byref(dm), ctypes.byref(o), ctypes.c_void_p(s.cuda_stream)))
         return self.out
 
     def capture(self, stream: torch.cuda.Stream | None = None) -> "torch.cuda.CUDAGraph":
