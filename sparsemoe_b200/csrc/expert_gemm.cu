@@ -500,21 +500,23 @@ bool make_map_box(CUtensorMap* map, const void* base, CUtensorMapDataType dt, in
     return true;
 }
 
-// [outer, inner] bytes with rows `stride` bytes apart (a multiple of 16), boxes of 128 bytes x box_outer rows.
+// [outer, inner] bytes with rows `stride` bytes apart (a multiple of 16), boxes of
+// box_inner (64 or 128) bytes x box_outer rows, swizzled over box_inner.
 bool make_map_u8_strided(CUtensorMap* map, const void* base, uint64_t inner, uint64_t outer, uint64_t stride,
-                         uint32_t box_outer) {
+                         uint32_t box_inner, uint32_t box_outer) {
     auto fn = encode_fn();
     if (!fn) { set_error("cuTensorMapEncodeTiled unavailable"); return false; }
     cuuint64_t dims[2] = {inner, outer};
     cuuint64_t strides[1] = {stride};
-    cuuint32_t box[2] = {128, box_outer};
+    cuuint32_t box[2] = {box_inner, box_outer};
     cuuint32_t estr[2] = {1, 1};
     CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides, box, estr,
-                    CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                    CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+                    CU_TENSOR_MAP_INTERLEAVE_NONE,
+                    box_inner == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B,
+                    CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     if (r != CUDA_SUCCESS) {
-        set_error("cuTensorMapEncodeTiled failed (%d) for [%llu, %llu] stride %llu box [%u, 128]", (int)r,
-                  (unsigned long long)outer, (unsigned long long)inner, (unsigned long long)stride, box_outer);
+        set_error("cuTensorMapEncodeTiled failed (%d) for [%llu, %llu] stride %llu box [%u, %u]", (int)r,
+                  (unsigned long long)outer, (unsigned long long)inner, (unsigned long long)stride, box_outer, box_inner);
         return false;
     }
     return true;

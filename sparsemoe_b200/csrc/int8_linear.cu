@@ -19,9 +19,10 @@
 
 namespace moe {
 
-// expert_gemm.cu: [outer, inner] bytes, rows `stride` bytes apart, boxes of 128 bytes x box_outer rows, 128-byte swizzle
+// expert_gemm.cu: [outer, inner] bytes, rows `stride` bytes apart, boxes of box_inner (64 or 128, the swizzle span)
+// bytes x box_outer rows
 bool make_map_u8_strided(CUtensorMap* map, const void* base, uint64_t inner, uint64_t outer, uint64_t stride,
-                         uint32_t box_outer);
+                         uint32_t box_inner, uint32_t box_outer);
 
 namespace {
 
@@ -247,6 +248,8 @@ struct LinearParams {
     int64_t ld_out;
     int out_type;
     int vec_out, vec_res;      // rows allow 16-byte accesses of eight columns
+    int row_end16;             // a row of outputs is a whole number of 16-byte units
+    int staged;                // outputs leave through shared memory and TMA stores (rows on 16-byte boundaries)
     uint32_t idesc;
 };
 
@@ -256,7 +259,8 @@ struct LinearCfg {
     static constexpr int kABytes = kBM * kBK;
     static constexpr int kBBytes = kBN * kBK;
     static constexpr int kStageBytes = kABytes + kBBytes;
-    static constexpr int kRecvBytes = kBN == 128 ? kBM * kBN * 4 : 0;   // split sums (kBN = 128 only)
+    // split sums (kBN = 128 only), or two staged chunks of 32 rows x 64 bytes for each epilogue warp
+    static constexpr int kRecvBytes = kBN == 128 ? kBM * kBN * 4 : 4 * 2 * 2048;
     static constexpr size_t kSmem = 1024 + (size_t)kStages * kStageBytes + kRecvBytes + 256;
 };
 
@@ -282,6 +286,19 @@ __device__ __forceinline__ void tmem_ld_32x32b_x8(uint32_t taddr, uint32_t (&r)[
                  : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
                  : "r"(taddr));
 }
+
+// 2-D tiled store from shared memory, and the bulk groups that track its reads.
+__device__ __forceinline__ void tma_store_2d(const void* tmap, const void* src, int x, int y) {
+    asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%2, %3}], [%1];" ::"l"(
+                     reinterpret_cast<uint64_t>(tmap)),
+                 "r"(smem_u32(src)), "r"(x), "r"(y)
+                 : "memory");
+}
+__device__ __forceinline__ void bulk_commit() { asm volatile("cp.async.bulk.commit_group;" ::: "memory"); }
+template <int kPending> __device__ __forceinline__ void bulk_wait_read() {
+    asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(kPending) : "memory");
+}
+__device__ __forceinline__ void fence_async_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
 __device__ __forceinline__ float load_as_f32(const void* p, int64_t i, int type) {
     if (type == MOE_TYPE_F32) return static_cast<const float*>(p)[i];
@@ -344,6 +361,126 @@ __device__ __forceinline__ void emit8(const LinearParams& p, int64_t t, bool sec
     }
 }
 
+template <int kC> __device__ __forceinline__ void tmem_ld(uint32_t taddr, uint32_t (&r)[kC]) {
+    if constexpr (kC == 32) tmem_ld_32x32b_x32(taddr, r);
+    else tmem_ld_32x32b_x16(taddr, r);
+}
+
+// One epilogue warp's 32 rows of a tile, staged: chunks of kC columns (64 bytes
+// a row) go from TMEM through the arithmetic into a shared-memory buffer
+// (64-byte swizzle: 16-byte unit j of row r at j ^ ((r >> 1) & 3)) and from
+// there by a TMA store, which leaves out rows and columns outside the tensor.
+// Direct stores of one row a thread touched 32 rows an instruction; with the
+// residual's loads between, a tile of 128 x 256 took 20 us (8192 x 2048 x 7168:
+// 247 us in all, 96 us staged).  A 16-bit residual is fetched coalesced into
+// registers before the accumulator is waited for, and meets its row's thread in
+// the same buffer.
+template <int kOutN, bool kSwiglu, bool kF32>
+struct StagedEpilogue {
+    static constexpr int kC = kF32 ? 16 : 32;
+    static constexpr int kChunks = kOutN / kC;
+    uint4 res[kF32 || kSwiglu ? 1 : kChunks][4];
+
+    // rows (lane / 4) + 8 i, 16-byte unit lane % 4 of every chunk
+    __device__ __forceinline__ void fetch_residual(const LinearParams& p, int row0, int col0, int lane) {
+        if constexpr (!kF32 && !kSwiglu) {
+#pragma unroll
+            for (int c = 0; c < kChunks; ++c)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int row = row0 + lane / 4 + 8 * i, col = col0 + c * kC + 8 * (lane % 4);
+                    res[c][i] = make_uint4(0u, 0u, 0u, 0u);
+                    if (row >= p.T || col >= p.N) continue;
+                    const uint16_t* src = static_cast<const uint16_t*>(p.residual) + (int64_t)row * p.ld_res + col;
+                    if (p.vec_res && col + 8 <= p.N) {
+                        res[c][i] = *reinterpret_cast<const uint4*>(src);
+                    } else {
+                        uint32_t u[4] = {0u, 0u, 0u, 0u};
+#pragma unroll
+                        for (int j = 0; j < 8; ++j)
+                            if (col + j < p.N) u[j >> 1] |= (uint32_t)src[j] << (16 * (j & 1));
+                        res[c][i] = make_uint4(u[0], u[1], u[2], u[3]);
+                    }
+                }
+        }
+    }
+
+    __device__ __forceinline__ void run(const LinearParams& p, const CUtensorMap* map, uint8_t* buf, uint32_t& turn,
+                                        uint32_t taddr, float st, const float* sc, const float* sb, int row0, int col0,
+                                        uint64_t* release, int lane) {
+#pragma unroll
+        for (int c = 0; c < kChunks; ++c) {
+            const int n = c * kC;
+            uint32_t a[kC], b[kSwiglu ? kC : 1];
+            tmem_ld<kC>(taddr + n, a);
+            if constexpr (kSwiglu) tmem_ld<kC>(taddr + kOutN + n, b);
+            tmem_wait_ld();
+            if (c == kChunks - 1) { tc_fence_before(); mbar_arrive(release); }
+            if (row0 >= p.T || col0 + n >= p.N) continue;   // the same for the whole warp
+            uint8_t* const stage = buf + (turn & 1) * 2048;
+            turn ^= 1;
+            if (lane == 0) bulk_wait_read<1>();             // the store before the last has read this buffer
+            __syncwarp();
+            uint4* const mine = reinterpret_cast<uint4*>(stage + lane * 64);
+            const int sw = (lane >> 1) & 3;
+            const bool add = !kF32 && !kSwiglu && p.residual != nullptr;
+            if constexpr (!kF32 && !kSwiglu)
+                if (add) {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const int r = lane / 4 + 8 * i;
+                        reinterpret_cast<uint4*>(stage + r * 64)[(lane % 4) ^ ((r >> 1) & 3)] = res[c][i];
+                    }
+                    __syncwarp();
+                }
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                constexpr int kU = kC / 4;                  // columns of a 16-byte unit
+                float v[kU];
+#pragma unroll
+                for (int i = 0; i < kU; ++i) {
+                    const int k = j * kU + i;
+                    v[i] = (float)(int)a[k] * st * sc[n + k];
+                    if constexpr (kSwiglu) {
+                        const float u = (float)(int)b[k] * st * sc[kOutN + n + k];
+                        v[i] = u * (v[i] / (1.0f + __expf(-v[i])));
+                    } else {
+                        v[i] += sb[n + k];
+                    }
+                }
+                if constexpr (kF32) {
+                    mine[j ^ sw] = make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]),
+                                              __float_as_uint(v[3]));
+                } else {
+                    const bool half = p.out_type == MOE_TYPE_F16;
+                    if (add) {
+                        const uint4 r = mine[j ^ sw];
+                        const uint32_t u[4] = {r.x, r.y, r.z, r.w};
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            const float2 f = half ? F16Traits<__half>::unpack2(u[i]) : F16Traits<__nv_bfloat16>::unpack2(u[i]);
+                            v[2 * i] += f.x;
+                            v[2 * i + 1] += f.y;
+                        }
+                    }
+                    uint32_t o[4];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        o[i] = half ? F16Traits<__half>::pack2(v[2 * i], v[2 * i + 1])
+                                    : F16Traits<__nv_bfloat16>::pack2(v[2 * i], v[2 * i + 1]);
+                    mine[j ^ sw] = make_uint4(o[0], o[1], o[2], o[3]);
+                }
+            }
+            fence_async_smem();
+            __syncwarp();
+            if (lane == 0) {
+                tma_store_2d(map, stage, (col0 + n) * (64 / kC), row0);
+                bulk_commit();
+            }
+        }
+    }
+};
+
 // Tiles of 128 tokens x kBN weight columns (kSwiglu, kBN = 256: 128 gate
 // columns, then the same 128 up columns, one output column each).
 // split == 1: every CTA walks the tiles with a double-buffered accumulator.
@@ -353,7 +490,8 @@ __device__ __forceinline__ void emit8(const LinearParams& p, int64_t t, bool sec
 template <int kBN, bool kSwiglu>
 __global__ void __launch_bounds__(kThreads, 1)
     linear_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB0,
-                  const __grid_constant__ CUtensorMap tmB1, const LinearParams p) {
+                  const __grid_constant__ CUtensorMap tmB1, const __grid_constant__ CUtensorMap tmO0,
+                  const __grid_constant__ CUtensorMap tmO1, const __grid_constant__ LinearParams p) {
     using C = LinearCfg<kBN>;
     static_assert(!kSwiglu || kBN == 256, "the gate and up halves are whole 128-column boxes");
     constexpr int kOutN = kSwiglu ? kBN / 2 : kBN;
@@ -490,6 +628,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int etid = threadIdx.x - 64;
         int acc = 0;
         uint32_t aph = 0;
+        uint32_t turn = 0;
         bool ok = true;   // a wait that ran out: the warp keeps to its barriers and writes nothing more
         for (int t = tile0; t < total; t += step) {
             const int n = t / p.m_tiles, m = t - n * p.m_tiles;
@@ -505,12 +644,33 @@ __global__ void __launch_bounds__(kThreads, 1)
                 sb[c] = !kSwiglu && p.bias && col < p.N ? __ldg(p.bias + col) : 0.0f;
             }
             asm volatile("bar.sync 1, 128;" ::: "memory");
+            const int row0 = m * kBM + q * 32, row = row0 + lane;
+            const bool valid = row < p.T;
+            const uint32_t taddr = tmem_base + ((uint32_t)(q * 32) << 16) + acc * kBN;
+            // (TMA stores clip rows at 16-byte units: a row that ends inside one leaves its last tile to emit8)
+            if (p.staged && (p.row_end16 || col0 + kOutN <= p.N)) {
+                const float st = valid ? p.s_tok[row] : 0.0f;
+                uint8_t* const buf = recv + q * 4096;
+                const CUtensorMap* map = second ? &tmO1 : &tmO0;
+                if (!kSwiglu && p.out_type != MOE_TYPE_F32) {
+                    StagedEpilogue<kOutN, kSwiglu, kSwiglu> e;   // (h of the fused pass is f32)
+                    if (p.residual) e.fetch_residual(p, row0, col0, lane);
+                    if (ok) ok = mbar_wait_warp(&tfull[acc], aph, status, kDevErrTimeout);
+                    tc_fence_after();
+                    if (ok) e.run(p, map, buf, turn, taddr, st, sc, sb, row0, col0, &tempty[acc], lane);
+                } else {
+                    StagedEpilogue<kOutN, kSwiglu, true> e;
+                    if (ok) ok = mbar_wait_warp(&tfull[acc], aph, status, kDevErrTimeout);
+                    tc_fence_after();
+                    if (ok) e.run(p, map, buf, turn, taddr, st, sc, sb, row0, col0, &tempty[acc], lane);
+                }
+                acc ^= 1;
+                if (acc == 0) aph ^= 1u;
+                continue;
+            }
             if (ok) ok = mbar_wait_warp(&tfull[acc], aph, status, kDevErrTimeout);
             if (ok) {
                 tc_fence_after();
-                const int row = m * kBM + q * 32 + lane;
-                const bool valid = row < p.T;
-                const uint32_t taddr = tmem_base + ((uint32_t)(q * 32) << 16) + acc * kBN;
                 if (p.split == 1) {
                     const float st = valid ? p.s_tok[row] : 0.0f;
 #pragma unroll 1
@@ -559,6 +719,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             acc ^= 1;
             if (acc == 0) aph ^= 1u;
         }
+        if (lane == 0) bulk_wait_read<0>();   // the staged chunks are read before the CTA's memory goes
     }
     if (p.split > 1) {
         __syncwarp();
@@ -668,15 +829,15 @@ cudaError_t launch_quantize(const void* x, int type, int64_t rows, int K, int64_
 }
 
 template <int kBN, bool kSwiglu>
-cudaError_t launch_linear_cfg(const CUtensorMap& a, const CUtensorMap& b0, const CUtensorMap& b1,
+cudaError_t launch_linear_cfg(const CUtensorMap& a, const CUtensorMap (&b)[2], const CUtensorMap (&o)[2],
                               const LinearParams& p, int clusters, cudaStream_t st) {
     auto kern = linear_kernel<kBN, kSwiglu>;
     static SmemAttr attr;
     const size_t smem = LinearCfg<kBN>::kSmem;
     cudaError_t err = ensure_smem(kern, smem, attr);
     if (err != cudaSuccess) return err;
-    return launch_ex(kern, (unsigned)(clusters * p.split), (unsigned)kThreads, smem, p.split, p.pdl != 0, st, a, b0, b1,
-                     p);
+    return launch_ex(kern, (unsigned)(clusters * p.split), (unsigned)kThreads, smem, p.split, p.pdl != 0, st, a, b[0], b[1],
+                     o[0], o[1], p);
 }
 
 struct Matrix {
@@ -712,19 +873,27 @@ cudaError_t launch_linear(const int8_t* q, int64_t ldq, LinearParams p, const Ma
     p.s_ch0 = w0.scale;
     p.s_ch1 = w1 ? w1->scale : w0.scale;
     p.idesc = idesc_i8(kBM, bn, !p.b_nk);
-    CUtensorMap ta, tb[2];
-    if (!make_map_u8_strided(&ta, q, p.K, p.T, ldq, p.a_rows)) return cudaErrorInvalidValue;
+    CUtensorMap ta, tb[2], to[2] = {};
+    if (!make_map_u8_strided(&ta, q, p.K, p.T, ldq, 128, p.a_rows)) return cudaErrorInvalidValue;
     const Matrix* ws[2] = {&w0, w1 ? w1 : &w0};
     for (int i = 0; i < 2; ++i) {
-        const bool ok = p.b_nk ? make_map_u8_strided(&tb[i], ws[i]->w, p.K, p.N, ws[i]->ld, bn / 2)
-                               : make_map_u8_strided(&tb[i], ws[i]->w, p.N, p.K, ws[i]->ld, kBK);
+        const bool ok = p.b_nk ? make_map_u8_strided(&tb[i], ws[i]->w, p.K, p.N, ws[i]->ld, 128, bn / 2)
+                               : make_map_u8_strided(&tb[i], ws[i]->w, p.N, p.K, ws[i]->ld, 128, kBK);
         if (!ok) return cudaErrorInvalidValue;
     }
+    // staged outputs need rows on 16-byte boundaries, and a residual of the output's 16-bit type
+    const int size = elem_bytes(p.out_type);
+    p.row_end16 = (int64_t)p.N * size % 16 == 0;
+    p.staged = p.split == 1 && p.vec_out && (!p.residual || (size == 2 && p.res_type == p.out_type));
+    for (int i = 0; p.staged && i < mats; ++i)
+        if (!make_map_u8_strided(&to[i], static_cast<uint8_t*>(p.out) + i * p.out1 * size, (uint64_t)p.N * size, p.T,
+                                 (uint64_t)p.ld_out * size, 64, 32))
+            return cudaErrorInvalidValue;
     const int64_t tiles = (int64_t)p.m_tiles * p.n_tiles;
     const int clusters = (int)(p.split > 1 ? tiles : std::min<int64_t>(tiles, num_sms));
-    if (swiglu) return launch_linear_cfg<256, true>(ta, tb[0], tb[1], p, clusters, st);
-    if (wide) return launch_linear_cfg<256, false>(ta, tb[0], tb[1], p, clusters, st);
-    return launch_linear_cfg<128, false>(ta, tb[0], tb[1], p, clusters, st);
+    if (swiglu) return launch_linear_cfg<256, true>(ta, tb, to, p, clusters, st);
+    if (wide) return launch_linear_cfg<256, false>(ta, tb, to, p, clusters, st);
+    return launch_linear_cfg<128, false>(ta, tb, to, p, clusters, st);
 }
 
 int bad(const char* who, const char* what) {
@@ -739,7 +908,7 @@ int check_dims(const char* who, int64_t T, int64_t K, int64_t N) {
         set_error("%s: K = %lld, s32 sums are exact up to %d", who, (long long)K, kMaxK);
         return MOE_ERR_UNSUPPORTED;
     }
-    if (T > 0x7FFFFF00ll || N > 0x7FFFFF00ll || ((T + 127) / 128) * ((N + 127) / 128) * 2 > 0x7FFFFFFFll) {
+    if (T > 0x7FFFFF00ll || N > (1ll << 28) || ((T + 127) / 128) * ((N + 127) / 128) * 2 > 0x7FFFFFFFll) {
         set_error("%s: %lld x %lld outputs are too many for one call", who, (long long)T, (long long)N);
         return MOE_ERR_UNSUPPORTED;
     }
