@@ -225,7 +225,8 @@ __global__ void __launch_bounds__(256) quantize_tokens_kernel(const T* __restric
 
 constexpr int kBM = 128;       // tokens of a tile
 constexpr int kBK = 128;       // K of a stage: one 128-byte swizzle span
-constexpr int kThreads = 192;  // TMA warp, MMA warp, four epilogue warps
+constexpr int kEpiThreads = 256;  // eight epilogue warps: two for each quarter of the TMEM lanes
+constexpr int kThreads = 64 + kEpiThreads;  // behind the TMA and the MMA warp
 constexpr int kMaxSplit = 8;
 
 struct LinearParams {
@@ -259,8 +260,8 @@ struct LinearCfg {
     static constexpr int kABytes = kBM * kBK;
     static constexpr int kBBytes = kBN * kBK;
     static constexpr int kStageBytes = kABytes + kBBytes;
-    // split sums (kBN = 128 only), or two staged chunks of 32 rows x 64 bytes for each epilogue warp
-    static constexpr int kRecvBytes = kBN == 128 ? kBM * kBN * 4 : 4 * 2 * 2048;
+    // split sums (kBN = 128 only), or a staged chunk of 32 rows x 64 bytes for each epilogue warp
+    static constexpr int kRecvBytes = kBN == 128 ? kBM * kBN * 4 : 8 * 2048;
     static constexpr size_t kSmem = 1024 + (size_t)kStages * kStageBytes + kRecvBytes + 256;
 };
 
@@ -361,116 +362,135 @@ __device__ __forceinline__ void emit8(const LinearParams& p, int64_t t, bool sec
     }
 }
 
+__device__ __forceinline__ float silu(float g) { return g / (1.0f + __expf(-g)); }
+
 template <int kC> __device__ __forceinline__ void tmem_ld(uint32_t taddr, uint32_t (&r)[kC]) {
     if constexpr (kC == 32) tmem_ld_32x32b_x32(taddr, r);
     else tmem_ld_32x32b_x16(taddr, r);
 }
 
-// One epilogue warp's 32 rows of a tile, staged: chunks of kC columns (64 bytes
-// a row) go from TMEM through the arithmetic into a shared-memory buffer
-// (64-byte swizzle: 16-byte unit j of row r at j ^ ((r >> 1) & 3)) and from
-// there by a TMA store, which leaves out rows and columns outside the tensor.
-// Direct stores of one row a thread touched 32 rows an instruction; with the
-// residual's loads between, a tile of 128 x 256 took 20 us (8192 x 2048 x 7168:
-// 247 us in all, 96 us staged).  A 16-bit residual is fetched coalesced into
-// registers before the accumulator is waited for, and meets its row's thread in
-// the same buffer.
-template <int kOutN, bool kSwiglu, bool kF32>
+// One epilogue warp's 32 rows and kCols output columns of a tile, staged: chunks
+// of kC columns (64 bytes a row) go from TMEM through the arithmetic into the
+// warp's 2 KB of shared memory (64-byte swizzle: 16-byte unit j of row r at
+// j ^ ((r >> 1) & 3)) and from there by a TMA store, which leaves out rows and
+// columns outside the tensor.  Storing one row a thread instead touched 32 rows
+// an instruction.  A 16-bit residual is read coalesced, a chunk ahead (its lines
+// are asked into L2 before the accumulator is waited for), and meets its row's
+// thread in the same buffer.
+template <int kCols, int kOutN, bool kSwiglu, bool kF32>
 struct StagedEpilogue {
     static constexpr int kC = kF32 ? 16 : 32;
-    static constexpr int kChunks = kOutN / kC;
-    uint4 res[kF32 || kSwiglu ? 1 : kChunks][4];
+    static constexpr bool kRes = !kF32 && !kSwiglu;
 
-    // rows (lane / 4) + 8 i, 16-byte unit lane % 4 of every chunk
-    __device__ __forceinline__ void fetch_residual(const LinearParams& p, int row0, int col0, int lane) {
-        if constexpr (!kF32 && !kSwiglu) {
+    static __device__ __forceinline__ void prefetch_residual(const LinearParams& p, int row, int col0) {
+        if (row >= p.T) return;
+        const uint16_t* src = static_cast<const uint16_t*>(p.residual) + (int64_t)row * p.ld_res;
 #pragma unroll
-            for (int c = 0; c < kChunks; ++c)
+        for (int c = 0; c < kCols; c += 64)
+            if (col0 + c < p.N) asm volatile("prefetch.global.L2 [%0];" ::"l"(src + col0 + c));
+    }
+    // rows (lane / 4) + 8 i, 16-byte unit lane % 4 of a chunk
+    static __device__ __forceinline__ void fetch(const LinearParams& p, int row0, int col0, int lane, uint4 (&res)[4]) {
+        const int col = col0 + 8 * (lane % 4);
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const int row = row0 + lane / 4 + 8 * i, col = col0 + c * kC + 8 * (lane % 4);
-                    res[c][i] = make_uint4(0u, 0u, 0u, 0u);
-                    if (row >= p.T || col >= p.N) continue;
-                    const uint16_t* src = static_cast<const uint16_t*>(p.residual) + (int64_t)row * p.ld_res + col;
-                    if (p.vec_res && col + 8 <= p.N) {
-                        res[c][i] = *reinterpret_cast<const uint4*>(src);
-                    } else {
-                        uint32_t u[4] = {0u, 0u, 0u, 0u};
+        for (int i = 0; i < 4; ++i) {
+            const int row = row0 + lane / 4 + 8 * i;
+            res[i] = make_uint4(0u, 0u, 0u, 0u);
+            if (row >= p.T || col >= p.N) continue;
+            const uint16_t* src = static_cast<const uint16_t*>(p.residual) + (int64_t)row * p.ld_res + col;
+            if (p.vec_res && col + 8 <= p.N) {
+                res[i] = *reinterpret_cast<const uint4*>(src);
+            } else {
+                uint32_t u[4] = {0u, 0u, 0u, 0u};
 #pragma unroll
-                        for (int j = 0; j < 8; ++j)
-                            if (col + j < p.N) u[j >> 1] |= (uint32_t)src[j] << (16 * (j & 1));
-                        res[c][i] = make_uint4(u[0], u[1], u[2], u[3]);
-                    }
-                }
+                for (int j = 0; j < 8; ++j)
+                    if (col + j < p.N) u[j >> 1] |= (uint32_t)src[j] << (16 * (j & 1));
+                res[i] = make_uint4(u[0], u[1], u[2], u[3]);
+            }
         }
     }
 
-    __device__ __forceinline__ void run(const LinearParams& p, const CUtensorMap* map, uint8_t* buf, uint32_t& turn,
-                                        uint32_t taddr, float st, const float* sc, const float* sb, int row0, int col0,
-                                        uint64_t* release, int lane) {
-#pragma unroll
-        for (int c = 0; c < kChunks; ++c) {
-            const int n = c * kC;
+    template <bool kHalf>
+    static __device__ __forceinline__ void run(const LinearParams& p, const CUtensorMap* map, uint8_t* stage,
+                                               uint32_t taddr, float st, const float* sc, const float* sb, int row0,
+                                               int col0, uint64_t* release, int lane) {
+        using T16 = typename std::conditional<kHalf, __half, __nv_bfloat16>::type;
+        uint4* const mine = reinterpret_cast<uint4*>(stage + lane * 64);
+        const int sw = (lane >> 1) & 3;
+        const bool add = kRes && p.residual != nullptr;
+        const bool biased = !kSwiglu && p.bias != nullptr;
+        uint4 next[4];
+        if (add) fetch(p, row0, col0, lane, next);
+#pragma unroll 1
+        for (int n = 0; n < kCols; n += kC) {
             uint32_t a[kC], b[kSwiglu ? kC : 1];
             tmem_ld<kC>(taddr + n, a);
             if constexpr (kSwiglu) tmem_ld<kC>(taddr + kOutN + n, b);
             tmem_wait_ld();
-            if (c == kChunks - 1) { tc_fence_before(); mbar_arrive(release); }
+            if (n + kC == kCols) { tc_fence_before(); mbar_arrive(release); }
             if (row0 >= p.T || col0 + n >= p.N) continue;   // the same for the whole warp
-            uint8_t* const stage = buf + (turn & 1) * 2048;
-            turn ^= 1;
-            if (lane == 0) bulk_wait_read<1>();             // the store before the last has read this buffer
-            __syncwarp();
-            uint4* const mine = reinterpret_cast<uint4*>(stage + lane * 64);
-            const int sw = (lane >> 1) & 3;
-            const bool add = !kF32 && !kSwiglu && p.residual != nullptr;
-            if constexpr (!kF32 && !kSwiglu)
-                if (add) {
+            uint4 r[4];
+            if (add) {
+                if (lane == 0) bulk_wait_read<0>();         // the last chunk has been read
+                __syncwarp();
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const int r = lane / 4 + 8 * i;
-                        reinterpret_cast<uint4*>(stage + r * 64)[(lane % 4) ^ ((r >> 1) & 3)] = res[c][i];
-                    }
-                    __syncwarp();
+                for (int i = 0; i < 4; ++i) {
+                    const int q = lane / 4 + 8 * i;
+                    reinterpret_cast<uint4*>(stage + q * 64)[(lane % 4) ^ ((q >> 1) & 3)] = next[i];
                 }
+                if (n + kC < kCols) fetch(p, row0, col0 + n + kC, lane, next);
+                __syncwarp();
+#pragma unroll
+                for (int j = 0; j < 4; ++j) r[j] = mine[j ^ sw];
+            }
+            uint4 out[4];
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
                 constexpr int kU = kC / 4;                  // columns of a 16-byte unit
                 float v[kU];
 #pragma unroll
-                for (int i = 0; i < kU; ++i) {
+                for (int i = 0; i < kU; i += 4) {
                     const int k = j * kU + i;
-                    v[i] = (float)(int)a[k] * st * sc[n + k];
+                    const float4 w = *reinterpret_cast<const float4*>(sc + n + k);
+                    v[i] = (float)(int)a[k] * st * w.x;
+                    v[i + 1] = (float)(int)a[k + 1] * st * w.y;
+                    v[i + 2] = (float)(int)a[k + 2] * st * w.z;
+                    v[i + 3] = (float)(int)a[k + 3] * st * w.w;
                     if constexpr (kSwiglu) {
-                        const float u = (float)(int)b[k] * st * sc[kOutN + n + k];
-                        v[i] = u * (v[i] / (1.0f + __expf(-v[i])));
-                    } else {
-                        v[i] += sb[n + k];
+                        const float4 g = *reinterpret_cast<const float4*>(sc + kOutN + n + k);
+                        const float u[4] = {(float)(int)b[k] * st * g.x, (float)(int)b[k + 1] * st * g.y,
+                                            (float)(int)b[k + 2] * st * g.z, (float)(int)b[k + 3] * st * g.w};
+#pragma unroll
+                        for (int h = 0; h < 4; ++h) v[i + h] = u[h] * silu(v[i + h]);
                     }
                 }
+                if (biased) {
+#pragma unroll
+                    for (int i = 0; i < kU; ++i) v[i] += sb[n + j * kU + i];
+                }
                 if constexpr (kF32) {
-                    mine[j ^ sw] = make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]),
-                                              __float_as_uint(v[3]));
+                    out[j] = make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]),
+                                        __float_as_uint(v[3]));
                 } else {
-                    const bool half = p.out_type == MOE_TYPE_F16;
                     if (add) {
-                        const uint4 r = mine[j ^ sw];
-                        const uint32_t u[4] = {r.x, r.y, r.z, r.w};
+                        const uint32_t u[4] = {r[j].x, r[j].y, r[j].z, r[j].w};
 #pragma unroll
                         for (int i = 0; i < 4; ++i) {
-                            const float2 f = half ? F16Traits<__half>::unpack2(u[i]) : F16Traits<__nv_bfloat16>::unpack2(u[i]);
+                            const float2 f = F16Traits<T16>::unpack2(u[i]);
                             v[2 * i] += f.x;
                             v[2 * i + 1] += f.y;
                         }
                     }
-                    uint32_t o[4];
-#pragma unroll
-                    for (int i = 0; i < 4; ++i)
-                        o[i] = half ? F16Traits<__half>::pack2(v[2 * i], v[2 * i + 1])
-                                    : F16Traits<__nv_bfloat16>::pack2(v[2 * i], v[2 * i + 1]);
-                    mine[j ^ sw] = make_uint4(o[0], o[1], o[2], o[3]);
+                    out[j] = make_uint4(F16Traits<T16>::pack2(v[0], v[1]), F16Traits<T16>::pack2(v[2], v[3]),
+                                        F16Traits<T16>::pack2(v[4], v[5]), F16Traits<T16>::pack2(v[6], v[7]));
                 }
             }
+            if (!add) {
+                if (lane == 0) bulk_wait_read<0>();
+                __syncwarp();
+            }
+#pragma unroll
+            for (int j = 0; j < 4; ++j) mine[j ^ sw] = out[j];
             fence_async_smem();
             __syncwarp();
             if (lane == 0) {
@@ -516,7 +536,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < C::kStages; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], 1); }
-        for (int a = 0; a < 2; ++a) { mbar_init(&tfull[a], 1); mbar_init(&tempty[a], 128); }
+        for (int a = 0; a < 2; ++a) { mbar_init(&tfull[a], 1); mbar_init(&tempty[a], kEpiThreads); }
         fence_mbar_init();
         tma_prefetch_desc(&tmA);
         tma_prefetch_desc(&tmB0);
@@ -621,97 +641,93 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
         }
     } else {
-        // ---------------- epilogue (warps 2..5) ----------------
+        // ---------------- epilogue (warps 2..9) ----------------
         if (p.pdl) pdl_wait();
         if (p.split > 1) cluster_wait();
-        const int q = warp & 3;
+        constexpr int kCols = kOutN / 2;          // output columns of a warp
+        const int q = warp & 3, half = (warp - 2) >> 2;
         const int etid = threadIdx.x - 64;
+        uint8_t* const stage = recv + (warp - 2) * 2048;
         int acc = 0;
         uint32_t aph = 0;
-        uint32_t turn = 0;
         bool ok = true;   // a wait that ran out: the warp keeps to its barriers and writes nothing more
         for (int t = tile0; t < total; t += step) {
             const int n = t / p.m_tiles, m = t - n * p.m_tiles;
             const bool second = !kSwiglu && n >= p.n0_tiles;
-            const int col0 = (second ? n - p.n0_tiles : n) * kOutN;
+            const int tile_col = (second ? n - p.n0_tiles : n) * kOutN, col0 = tile_col + half * kCols;
             // channel scales of the tile, in the order of the accumulator's columns
-            float* sc = s_scale[acc];
-            float* sb = s_bias[acc];
-            for (int c = etid; c < kBN; c += 128) {
-                const int col = col0 + (kSwiglu ? c % kOutN : c);
+            float* const scales = s_scale[acc];
+            float* const biases = s_bias[acc];
+            for (int c = etid; c < kBN; c += kEpiThreads) {
+                const int col = tile_col + (kSwiglu ? c % kOutN : c);
                 const float* src = second || (kSwiglu && c >= kOutN) ? p.s_ch1 : p.s_ch0;
-                sc[c] = col < p.N ? __ldg(src + col) : 0.0f;
-                sb[c] = !kSwiglu && p.bias && col < p.N ? __ldg(p.bias + col) : 0.0f;
+                scales[c] = col < p.N ? __ldg(src + col) : 0.0f;
+                biases[c] = !kSwiglu && p.bias && col < p.N ? __ldg(p.bias + col) : 0.0f;
             }
-            asm volatile("bar.sync 1, 128;" ::: "memory");
+            asm volatile("bar.sync 1, 256;" ::: "memory");
+            const float* const sc = scales + half * kCols;
+            const float* const sb = biases + half * kCols;
             const int row0 = m * kBM + q * 32, row = row0 + lane;
             const bool valid = row < p.T;
-            const uint32_t taddr = tmem_base + ((uint32_t)(q * 32) << 16) + acc * kBN;
-            // (TMA stores clip rows at 16-byte units: a row that ends inside one leaves its last tile to emit8)
-            if (p.staged && (p.row_end16 || col0 + kOutN <= p.N)) {
-                const float st = valid ? p.s_tok[row] : 0.0f;
-                uint8_t* const buf = recv + q * 4096;
-                const CUtensorMap* map = second ? &tmO1 : &tmO0;
-                if (!kSwiglu && p.out_type != MOE_TYPE_F32) {
-                    StagedEpilogue<kOutN, kSwiglu, kSwiglu> e;   // (h of the fused pass is f32)
-                    if (p.residual) e.fetch_residual(p, row0, col0, lane);
-                    if (ok) ok = mbar_wait_warp(&tfull[acc], aph, status, kDevErrTimeout);
-                    tc_fence_after();
-                    if (ok) e.run(p, map, buf, turn, taddr, st, sc, sb, row0, col0, &tempty[acc], lane);
-                } else {
-                    StagedEpilogue<kOutN, kSwiglu, true> e;
-                    if (ok) ok = mbar_wait_warp(&tfull[acc], aph, status, kDevErrTimeout);
-                    tc_fence_after();
-                    if (ok) e.run(p, map, buf, turn, taddr, st, sc, sb, row0, col0, &tempty[acc], lane);
-                }
-                acc ^= 1;
-                if (acc == 0) aph ^= 1u;
-                continue;
-            }
+            const float st = valid ? p.s_tok[row] : 0.0f;
+            const uint32_t taddr = tmem_base + ((uint32_t)(q * 32) << 16) + acc * kBN + half * kCols;
+            // TMA stores clip rows at 16-byte units: a row of outputs that ends inside one leaves its last tile to emit8
+            const bool staged = p.staged && (p.row_end16 || tile_col + kOutN <= p.N);
+            if (staged && p.residual) StagedEpilogue<kCols, kOutN, false, false>::prefetch_residual(p, row, col0);
             if (ok) ok = mbar_wait_warp(&tfull[acc], aph, status, kDevErrTimeout);
-            if (ok) {
-                tc_fence_after();
-                if (p.split == 1) {
-                    const float st = valid ? p.s_tok[row] : 0.0f;
+            tc_fence_after();
+            if (ok && staged) {
+                const CUtensorMap* map = second ? &tmO1 : &tmO0;
+                if (kSwiglu || p.out_type == MOE_TYPE_F32)
+                    StagedEpilogue<kCols, kOutN, kSwiglu, true>::template run<false>(p, map, stage, taddr, st, sc, sb,
+                                                                                     row0, col0, &tempty[acc], lane);
+                else if (p.out_type == MOE_TYPE_F16)
+                    StagedEpilogue<kCols, kOutN, false, kSwiglu>::template run<true>(p, map, stage, taddr, st, sc, sb,
+                                                                                     row0, col0, &tempty[acc], lane);
+                else
+                    StagedEpilogue<kCols, kOutN, false, kSwiglu>::template run<false>(p, map, stage, taddr, st, sc, sb,
+                                                                                      row0, col0, &tempty[acc], lane);
+            } else if (ok && p.split == 1) {
 #pragma unroll 1
-                    for (int c = 0; c < kOutN; c += 16) {
-                        uint32_t a[16], b[16];
-                        tmem_ld_32x32b_x16(taddr + c, a);
-                        if (kSwiglu) tmem_ld_32x32b_x16(taddr + kOutN + c, b);
-                        tmem_wait_ld();
-                        if (c + 16 == kOutN) { tc_fence_before(); mbar_arrive(&tempty[acc]); }
-                        if (!valid) continue;
+                for (int c = 0; c < kCols; c += 16) {
+                    uint32_t a[16], b[16];
+                    tmem_ld_32x32b_x16(taddr + c, a);
+                    if (kSwiglu) tmem_ld_32x32b_x16(taddr + kOutN + c, b);
+                    tmem_wait_ld();
+                    if (c + 16 == kCols) { tc_fence_before(); mbar_arrive(&tempty[acc]); }
+                    if (!valid) continue;
 #pragma unroll
-                        for (int h = 0; h < 2; ++h) {
-                            float v[8];
+                    for (int h = 0; h < 16; h += 8) {
+                        float v[8];
 #pragma unroll
-                            for (int i = 0; i < 8; ++i) {
-                                const int cc = c + 8 * h + i;
-                                v[i] = (float)(int)a[8 * h + i] * st * sc[cc];
-                                if (kSwiglu) {
-                                    const float u = (float)(int)b[8 * h + i] * st * sc[kOutN + cc];
-                                    v[i] = u * (v[i] / (1.0f + __expf(-v[i])));
-                                } else {
-                                    v[i] += sb[cc];
-                                }
-                            }
-                            if (col0 + c + 8 * h < p.N) emit8(p, row, second, col0 + c + 8 * h, v);
+                        for (int i = 0; i < 8; ++i) {
+                            v[i] = (float)(int)a[h + i] * st * sc[c + h + i];
+                            if (kSwiglu) v[i] = (float)(int)b[h + i] * st * sc[kOutN + c + h + i] * silu(v[i]);
+                            else v[i] += sb[c + h + i];
                         }
+                        if (col0 + c + h < p.N) emit8(p, row, second, col0 + c + h, v);
                     }
-                } else if constexpr (kBN == 128) {
+                }
+            } else if (ok) {
+                if constexpr (kBN == 128) {
                     // send the parts in units of eight columns: [source][unit of the slice][row][8]
-                    if (m * kBM + q * 32 < p.T) {   // a warp without a token has nothing to send
+                    if (row0 < p.T) {   // a warp without a token has nothing to send
                         const int units = kBN / 8 / p.split;
 #pragma unroll 1
-                        for (int u = 0; u < kBN / 8; ++u) {
-                            uint32_t a[8];
-                            tmem_ld_32x32b_x8(taddr + 8 * u, a);
+                        for (int u = half * 8; u < half * 8 + 8; u += 4) {
+                            uint32_t a[32];
+                            tmem_ld_32x32b_x32(taddr + 8 * (u - half * 8), a);
                             tmem_wait_ld();
-                            const uint32_t dst = mapa(
-                                smem_u32(recv) + (uint32_t)(((rank * units + u % units) * kBM + q * 32 + lane) * 32),
-                                u / units);
-                            st_cluster4(dst, a[0], a[1], a[2], a[3]);
-                            st_cluster4(dst + 16, a[4], a[5], a[6], a[7]);
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) {
+                                const int at = u + i;
+                                const uint32_t dst = mapa(
+                                    smem_u32(recv) +
+                                        (uint32_t)(((rank * units + at % units) * kBM + q * 32 + lane) * 32),
+                                    at / units);
+                                st_cluster4(dst, a[8 * i], a[8 * i + 1], a[8 * i + 2], a[8 * i + 3]);
+                                st_cluster4(dst + 16, a[8 * i + 4], a[8 * i + 5], a[8 * i + 6], a[8 * i + 7]);
+                            }
                         }
                     }
                 }
@@ -735,7 +751,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (warp >= 2 && row < p.T) {
                 const float st = p.s_tok[row];
                 const int units = kBN / 8 / p.split;
-                for (int u = 0; u < units; ++u) {
+                for (int u = (warp - 2) >> 2; u < units; u += 2) {
                     int sum[8] = {};
                     for (int src = 0; src < p.split; ++src) {
                         const int4* a = reinterpret_cast<const int4*>(
