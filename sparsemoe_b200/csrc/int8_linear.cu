@@ -250,7 +250,8 @@ struct LinearParams {
     int out_type;
     int vec_out, vec_res;      // rows allow 16-byte accesses of eight columns
     int row_end16;             // a row of outputs is a whole number of 16-byte units
-    int staged;                // outputs leave through shared memory and TMA stores (rows on 16-byte boundaries)
+    int staged;                // outputs leave through shared memory (all but split tiles and unlike residuals)
+    int tma_out;               // and from there by TMA (rows on 16-byte boundaries)
     uint32_t idesc;
 };
 
@@ -410,9 +411,25 @@ struct StagedEpilogue {
         }
     }
 
+    // Rows that TMA cannot store (not on 16-byte boundaries, or a last tile that
+    // ends inside 16 bytes): consecutive lanes write consecutive columns.
+    static __device__ __forceinline__ void store_rows(const LinearParams& p, const uint8_t* stage, int64_t base, int row0,
+                                                      int col0, int lane) {
+        const int c = lane % kC;
+        if (col0 + c >= p.N) return;
+        const int unit = c / (kC / 4), in = c % (kC / 4);
+#pragma unroll 4
+        for (int r = lane / kC; r < 32 && row0 + r < p.T; r += 32 / kC) {
+            const uint8_t* src = stage + r * 64 + ((unit ^ ((r >> 1) & 3)) * 16) + in * (64 / kC);
+            const int64_t at = base + (int64_t)(row0 + r) * p.ld_out + col0 + c;
+            if (kF32) static_cast<float*>(p.out)[at] = *reinterpret_cast<const float*>(src);
+            else static_cast<uint16_t*>(p.out)[at] = *reinterpret_cast<const uint16_t*>(src);
+        }
+    }
+
     template <bool kHalf>
-    static __device__ __forceinline__ void run(const LinearParams& p, const CUtensorMap* map, uint8_t* stage,
-                                               uint32_t taddr, float st, const float* sc, const float* sb, int row0,
+    static __device__ __forceinline__ void run(const LinearParams& p, const CUtensorMap* map, int64_t base,
+                                               uint8_t* stage, uint32_t taddr, float st, const float* sc, const float* sb, int row0,
                                                int col0, uint64_t* release, int lane) {
         using T16 = typename std::conditional<kHalf, __half, __nv_bfloat16>::type;
         uint4* const mine = reinterpret_cast<uint4*>(stage + lane * 64);
@@ -491,11 +508,17 @@ struct StagedEpilogue {
             }
 #pragma unroll
             for (int j = 0; j < 4; ++j) mine[j ^ sw] = out[j];
-            fence_async_smem();
-            __syncwarp();
-            if (lane == 0) {
-                tma_store_2d(map, stage, (col0 + n) * (64 / kC), row0);
-                bulk_commit();
+            if (map) {
+                fence_async_smem();
+                __syncwarp();
+                if (lane == 0) {
+                    tma_store_2d(map, stage, (col0 + n) * (64 / kC), row0);
+                    bulk_commit();
+                }
+            } else {
+                __syncwarp();
+                store_rows(p, stage, base, row0, col0 + n, lane);
+                __syncwarp();
             }
         }
     }
@@ -671,21 +694,22 @@ __global__ void __launch_bounds__(kThreads, 1)
             const bool valid = row < p.T;
             const float st = valid ? p.s_tok[row] : 0.0f;
             const uint32_t taddr = tmem_base + ((uint32_t)(q * 32) << 16) + acc * kBN + half * kCols;
-            // TMA stores clip rows at 16-byte units: a row of outputs that ends inside one leaves its last tile to emit8
-            const bool staged = p.staged && (p.row_end16 || tile_col + kOutN <= p.N);
-            if (staged && p.residual) StagedEpilogue<kCols, kOutN, false, false>::prefetch_residual(p, row, col0);
+            if (p.staged && p.residual) StagedEpilogue<kCols, kOutN, false, false>::prefetch_residual(p, row, col0);
             if (ok) ok = mbar_wait_warp(&tfull[acc], aph, status, kDevErrTimeout);
             tc_fence_after();
-            if (ok && staged) {
-                const CUtensorMap* map = second ? &tmO1 : &tmO0;
+            if (ok && p.staged) {
+                // TMA stores clip rows at 16-byte units: not for a last tile that ends inside one
+                const CUtensorMap* map =
+                    !p.tma_out || !(p.row_end16 || tile_col + kOutN <= p.N) ? nullptr : second ? &tmO1 : &tmO0;
+                const int64_t base = second ? p.out1 : 0;
                 if (kSwiglu || p.out_type == MOE_TYPE_F32)
-                    StagedEpilogue<kCols, kOutN, kSwiglu, true>::template run<false>(p, map, stage, taddr, st, sc, sb,
+                    StagedEpilogue<kCols, kOutN, kSwiglu, true>::template run<false>(p, map, base, stage, taddr, st, sc, sb,
                                                                                      row0, col0, &tempty[acc], lane);
                 else if (p.out_type == MOE_TYPE_F16)
-                    StagedEpilogue<kCols, kOutN, false, kSwiglu>::template run<true>(p, map, stage, taddr, st, sc, sb,
+                    StagedEpilogue<kCols, kOutN, false, kSwiglu>::template run<true>(p, map, base, stage, taddr, st, sc, sb,
                                                                                      row0, col0, &tempty[acc], lane);
                 else
-                    StagedEpilogue<kCols, kOutN, false, kSwiglu>::template run<false>(p, map, stage, taddr, st, sc, sb,
+                    StagedEpilogue<kCols, kOutN, false, kSwiglu>::template run<false>(p, map, base, stage, taddr, st, sc, sb,
                                                                                       row0, col0, &tempty[acc], lane);
             } else if (ok && p.split == 1) {
 #pragma unroll 1
@@ -746,26 +770,23 @@ __global__ void __launch_bounds__(kThreads, 1)
             const int n = tile0 / p.m_tiles, m = tile0 - n * p.m_tiles;   // one tile a cluster
             const bool second = n >= p.n0_tiles;
             const int col0 = (second ? n - p.n0_tiles : n) * kOutN;
-            const int q = warp & 3;
-            const int row = m * kBM + q * 32 + lane;
-            if (warp >= 2 && row < p.T) {
+            // this CTA's 128 / split columns: consecutive lanes take consecutive columns of a row
+            const int w = kBN / p.split, per = 32 / min(w, 32), rows = min(kBM, p.T - m * kBM);
+            for (int r = (warp - 2) * per + lane / w; warp >= 2 && r < rows; r += 8 * per) {
+                const int64_t row = (int64_t)m * kBM + r;
                 const float st = p.s_tok[row];
-                const int units = kBN / 8 / p.split;
-                for (int u = (warp - 2) >> 2; u < units; u += 2) {
-                    int sum[8] = {};
-                    for (int src = 0; src < p.split; ++src) {
-                        const int4* a = reinterpret_cast<const int4*>(
-                            recv + (size_t)((src * units + u) * kBM + q * 32 + lane) * 32);
-                        const int4 x = a[0], y = a[1];
-                        sum[0] += x.x; sum[1] += x.y; sum[2] += x.z; sum[3] += x.w;
-                        sum[4] += y.x; sum[5] += y.y; sum[6] += y.z; sum[7] += y.w;
-                    }
-                    const int c = (rank * units + u) * 8;
-                    float v[8];
-#pragma unroll
-                    for (int i = 0; i < 8; ++i)
-                        v[i] = (float)sum[i] * st * s_scale[0][c + i] + s_bias[0][c + i];
-                    if (col0 + c < p.N) emit8(p, row, second, col0 + c, v);
+                for (int c = lane % w; c < w; c += 32) {
+                    const int* part = reinterpret_cast<const int*>(recv) + ((c / 8) * kBM + r) * 8 + c % 8;
+                    int sum = 0;
+                    for (int src = 0; src < p.split; ++src) sum += part[src * (w / 8) * kBM * 8];
+                    const int tc = rank * w + c, col = col0 + tc;
+                    if (col >= p.N) break;
+                    float v = (float)sum * st * s_scale[0][tc] + s_bias[0][tc];
+                    if (p.residual) v += load_as_f32(p.residual, row * p.ld_res + col, p.res_type);
+                    const int64_t at = row * p.ld_out + col + (second ? p.out1 : 0);
+                    if (p.out_type == MOE_TYPE_F32) static_cast<float*>(p.out)[at] = v;
+                    else if (p.out_type == MOE_TYPE_F16) static_cast<__half*>(p.out)[at] = __float2half_rn(v);
+                    else static_cast<__nv_bfloat16*>(p.out)[at] = __float2bfloat16_rn(v);
                 }
             }
         }
@@ -856,6 +877,35 @@ cudaError_t launch_linear_cfg(const CUtensorMap& a, const CUtensorMap (&b)[2], c
                      o[0], o[1], p);
 }
 
+// Tile width and split of K, by the estimated time of a launch: rounds of tiles
+// over the SMs x K blocks of a tile x the time of a block, plus what a launch
+// costs besides.  A block takes 0.34 us at 128 columns and 0.43 at 256 (bound by
+// what an SM takes in, 64 B/clk: 32 and 48 KB); a launch 3.5 us, a split one
+// 5.2 us and up to 2.5 more for sending the parts of 128 tokens.  Clusters of 4
+// and 8 CTAs of this size fit 33 and 15 times at once.  Measured (us, T x K x N,
+// 128 columns split 1 / 2 / 4 / 8, 256 columns): 1x7168x2048 18.6 / 12.7 / 9.4 /
+// 13.9, 20.8; 512x7168x2048 19.6 / 15.9 / 27.2 / 57.6, 23.1; 512x2048x7168 14.2 /
+// 37.3 / 71.5 / 155, 10.8; 512x7168x4096 21.7 / 32.3 / 54.6 / 107, 24.7.
+void pick_tiles(const LinearParams& p, int mats, int num_sms, bool* wide, int* split) {
+    auto rounds = [](int64_t n, int64_t at_once) { return (double)((n + at_once - 1) / at_once); };
+    const int64_t tiles128 = (int64_t)p.m_tiles * ((p.N + 127) / 128) * mats;
+    const int64_t tiles256 = (int64_t)p.m_tiles * ((p.N + 255) / 256) * mats;
+    double best = 3.5 + rounds(tiles256, num_sms) * p.kblocks * 0.43;
+    *wide = true;
+    *split = 1;
+    for (int s = 1; s <= kMaxSplit && s <= p.kblocks; s *= 2) {
+        const int64_t at_once = s == 1 ? num_sms : s == 2 ? num_sms / 2 : s == 4 ? num_sms * 33 / 148 : num_sms * 15 / 148;
+        if (at_once < 1 || (s > 1 && tiles128 > at_once)) break;   // a split tile's CTAs run one tile each
+        const double t = (s == 1 ? 3.5 : 5.2 + 2.5 * std::min(p.T, kBM) / kBM) +
+                         rounds(tiles128, at_once) * ((p.kblocks + s - 1) / s) * 0.34;
+        if (t < best) {
+            best = t;
+            *wide = false;
+            *split = s;
+        }
+    }
+}
+
 struct Matrix {
     const int8_t* w;
     int64_t ld;
@@ -870,18 +920,10 @@ cudaError_t launch_linear(const int8_t* q, int64_t ldq, LinearParams p, const Ma
     p.m_tiles = (p.T + kBM - 1) / kBM;
     p.kblocks = (p.K + kBK - 1) / kBK;
     p.a_rows = p.T >= kBM ? kBM : (p.T + 7) / 8 * 8;
-    p.split = 1;
     const int mats = w1 && !swiglu ? 2 : 1;
-    const int64_t tiles128 = (int64_t)p.m_tiles * ((p.N + 127) / 128) * mats;
-    const int64_t tiles256 = (int64_t)p.m_tiles * ((p.N + 255) / 256) * mats;
     bool wide = swiglu;
-    if (!swiglu) {
-        // few tiles: K is shared by as many CTAs as there are SMs for; many:
-        // 256 columns a tile, which halves the reads of A per product
-        wide = tiles256 >= num_sms;
-        if (!wide)
-            while (p.split < kMaxSplit && tiles128 * p.split * 2 <= num_sms && p.kblocks >= p.split * 2) p.split *= 2;
-    }
+    p.split = 1;
+    if (!swiglu) pick_tiles(p, mats, num_sms, &wide, &p.split);
     const int bn = wide ? 256 : 128;
     const int out_n = swiglu ? bn / 2 : bn;
     p.n0_tiles = (p.N + out_n - 1) / out_n;
@@ -897,11 +939,11 @@ cudaError_t launch_linear(const int8_t* q, int64_t ldq, LinearParams p, const Ma
                                : make_map_u8_strided(&tb[i], ws[i]->w, p.N, p.K, ws[i]->ld, 128, kBK);
         if (!ok) return cudaErrorInvalidValue;
     }
-    // staged outputs need rows on 16-byte boundaries, and a residual of the output's 16-bit type
     const int size = elem_bytes(p.out_type);
     p.row_end16 = (int64_t)p.N * size % 16 == 0;
-    p.staged = p.split == 1 && p.vec_out && (!p.residual || (size == 2 && p.res_type == p.out_type));
-    for (int i = 0; p.staged && i < mats; ++i)
+    p.staged = p.split == 1 && (!p.residual || (size == 2 && p.res_type == p.out_type));
+    p.tma_out = p.staged && p.vec_out;
+    for (int i = 0; p.tma_out && i < mats; ++i)
         if (!make_map_u8_strided(&to[i], static_cast<uint8_t*>(p.out) + i * p.out1 * size, (uint64_t)p.N * size, p.T,
                                  (uint64_t)p.ld_out * size, 64, 32))
             return cudaErrorInvalidValue;
