@@ -133,6 +133,26 @@ __device__ __forceinline__ uint2 quant8(const float (&f)[8], float s, float inv,
     return w;
 }
 
+// Scale of a row from the bits of its largest magnitude, and what quant8 needs.
+struct RowScale {
+    float s;          // the scale as it is handed out: NaN for a row with a NaN or an infinity
+    float ss, inv;    // scale x pre, its reciprocal
+    float pre;        // 2^100 or 2^-100 for tiny and huge rows (s is rounded before: a subnormal one keeps its few bits)
+    bool bad;
+    __device__ __forceinline__ explicit RowScale(uint32_t m) {
+        const float amax = __uint_as_float(m);
+        bad = m >= 0x7F800000u;
+        s = bad ? __uint_as_float(0x7FFFFFFFu) : __fmul_rn(amax, 1.0f / 127.0f);
+        if (s == 0.0f) s = 1.0f;   // a zero row, or one whose scale rounds to zero
+        pre = amax < 5.4e-20f && s != 1.0f ? 1.2676506e30f : amax > 1.8e19f ? 7.8886091e-31f : 1.0f;
+        ss = s * pre;
+        inv = bad ? 0.0f : __fdiv_rn(1.0f, ss);
+    }
+    __device__ __forceinline__ uint2 codes(const float (&f)[8]) const {
+        return bad ? make_uint2(0u, 0u) : quant8(f, ss, inv, pre);
+    }
+};
+
 __device__ __forceinline__ void store8(int8_t* q, uint2 w, int n, bool vec) {
     if (vec && n >= 8) {
         *reinterpret_cast<uint2*>(q) = w;
@@ -142,6 +162,8 @@ __device__ __forceinline__ void store8(int8_t* q, uint2 w, int n, bool vec) {
     for (int i = 0; i < 8; ++i)
         if (i < n) q[i] = (int8_t)((i < 4 ? w.x : w.y) >> (8 * (i & 3)));
 }
+
+__device__ __forceinline__ float silu(float g) { return g / (1.0f + __expf(-g)); }
 
 // kPair (T = float): x holds gate values, the up values start `up` elements
 // behind them, and the row that is quantised is up * gate / (1 + exp(-gate)).
@@ -170,7 +192,7 @@ __global__ void __launch_bounds__(256) quantize_tokens_kernel(const T* __restric
                 if (vec && k + 8 <= K) u.load(src + up + k);
                 else u.load_part(src + up + k, K - k);
 #pragma unroll
-                for (int i = 0; i < 8; ++i) d.v[i] = u.v[i] * (d.v[i] / (1.0f + __expf(-d.v[i])));
+                for (int i = 0; i < 8; ++i) d.v[i] = u.v[i] * silu(d.v[i]);
             }
         }
     };
@@ -194,21 +216,14 @@ __global__ void __launch_bounds__(256) quantize_tokens_kernel(const T* __restric
         for (int i = 0; i < TPR / 32; ++i) m = max(m, red[w0 + i]);
     }
     if (!live) return;
-    const float amax = __uint_as_float(m);
-    const bool bad = m >= 0x7F800000u;
-    float s = bad ? __uint_as_float(0x7FFFFFFFu) : __fmul_rn(amax, 1.0f / 127.0f);
-    if (s == 0.0f) s = 1.0f;   // a zero row, or one whose scale rounds to zero
-    // 2^100 and 2^-100: the scale is rounded first, a subnormal one keeps its few bits
-    const float pre = amax < 5.4e-20f && s != 1.0f ? 1.2676506e30f : amax > 1.8e19f ? 7.8886091e-31f : 1.0f;
-    const float ss = s * pre, inv = bad ? 0.0f : __fdiv_rn(1.0f, ss);
-    if (tr == 0) scale[t] = s;
+    const RowScale rs(m);
+    if (tr == 0) scale[t] = rs.s;
     int8_t* dst = q + t * ldq;
     auto put = [&](const In8<T>& d, int k) {
         if (k >= K) return;
         float f[8];
         d.get(f);
-        uint2 w = bad ? make_uint2(0u, 0u) : quant8(f, ss, inv, pre);
-        store8(dst + k, w, K - k, true);
+        store8(dst + k, rs.codes(f), K - k, true);
     };
     if (keep) {
 #pragma unroll
@@ -362,8 +377,6 @@ __device__ __forceinline__ void emit8(const LinearParams& p, int64_t t, bool sec
             if (i < left) o[i] = (uint16_t)(u[i >> 1] >> (16 * (i & 1)));
     }
 }
-
-__device__ __forceinline__ float silu(float g) { return g / (1.0f + __expf(-g)); }
 
 template <int kC> __device__ __forceinline__ void tmem_ld(uint32_t taddr, uint32_t (&r)[kC]) {
     if constexpr (kC == 32) tmem_ld_32x32b_x32(taddr, r);
@@ -798,6 +811,347 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
 }
 
+// ---- product of a few tokens ---------------------------------------------------------
+
+// Up to kNT tokens in one launch, quantiser included.  The product is turned
+// round: the 128 weight columns of a tile are the rows of the MMA (M = 128) and
+// the tokens its columns (N = kNT), so a thread of the epilogue holds one
+// channel's sums of all tokens and consecutive lanes write consecutive columns.
+// A cluster of `split` CTAs shares a tile, each a part of K.  Each CTA asks for
+// its weights at once, reads its part of the tokens twice (amax, which the
+// cluster exchanges through shared memory, then the codes, written where the MMA
+// reads them) and hands the s32 sums of each slice of the channels to the CTA
+// that adds them up.  What bounds it is latency: of the 6 us that 1 x 7168 x 2048
+// takes the 14.7 MB of weights are 2.2 at the HBM's rate.
+struct SmallParams {
+    const void* x;             // tokens, rows ld_x elements apart (pair: gate values, up values `up` elements behind)
+    int64_t ld_x, up;
+    const float* s_tok;        // codes given: their scales
+    int T, K, N;
+    int kblocks, split, stages;
+    int tiles0;                // tiles of the first matrix; the others are of the second
+    int64_t out1;
+    int b_nk, pdl, vec_x;
+    const float* s_ch0;
+    const float* s_ch1;
+    const float* bias;
+    const void* residual;
+    int64_t ld_res;
+    int res_type;
+    void* out;
+    int64_t ld_out;
+    int out_type;
+    uint32_t idesc;
+};
+
+enum SmallInput { kInF32, kInF16, kInBF16, kInPair, kInCodes };
+template <int kIn> struct SmallIn { using T = float; };
+template <> struct SmallIn<kInF16> { using T = __half; };
+template <> struct SmallIn<kInBF16> { using T = __nv_bfloat16; };
+template <> struct SmallIn<kInCodes> { using T = int8_t; };
+
+constexpr int kSmallWorkers = 256;
+constexpr int kSmallThreads = 64 + kSmallWorkers;
+constexpr int kSmallStageBytes = 128 * kBK;
+
+// Shared memory behind the aligned base: weight stages, code blocks, parts, barriers.
+template <int kNT> __host__ __device__ constexpr size_t small_smem(int stages, int blocks, int split) {
+    return 1024 + (size_t)stages * kSmallStageBytes + (size_t)blocks * kNT * kBK + (split > 1 ? 128 * kNT * 4 : 0) + 256;
+}
+
+template <int kNT, int kIn>
+__global__ void __launch_bounds__(kSmallThreads, 2)
+    small_linear_kernel(const __grid_constant__ CUtensorMap tmW0, const __grid_constant__ CUtensorMap tmW1,
+                        const __grid_constant__ SmallParams p) {
+    using T = typename SmallIn<kIn>::T;
+    constexpr int kTmemCols = kNT < 32 ? 32 : kNT;
+    extern __shared__ uint8_t smem_raw[];
+    __shared__ uint32_t s_amax[kMaxSplit][kNT];   // [source CTA][token]: bits of the largest magnitude
+    __shared__ float s_tok[kNT];
+
+    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    const int rank = p.split > 1 ? (int)cluster_rank() : 0;
+    const int kb0 = (int)((int64_t)p.kblocks * rank / p.split);
+    const int kb1 = (int)((int64_t)p.kblocks * (rank + 1) / p.split);
+    const int max_blocks = (p.kblocks + p.split - 1) / p.split;
+    uint8_t* const sW = smem;
+    uint8_t* const sQ = sW + p.stages * kSmallStageBytes;
+    uint8_t* const recv = sQ + (size_t)max_blocks * kNT * kBK;
+    uint64_t* const full = reinterpret_cast<uint64_t*>(recv + (p.split > 1 ? 128 * kNT * 4 : 0));
+    uint64_t* const empty = full + 8;
+    uint64_t* const ready = empty + 8;   // the codes are written
+    uint64_t* const tfull = ready + 1;
+    uint32_t* const tmem_slot = reinterpret_cast<uint32_t*>(tfull + 1);
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    int* status = &g_linear_status;
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < p.stages; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], 1); }
+        mbar_init(ready, kSmallWorkers);
+        mbar_init(tfull, 1);
+        fence_mbar_init();
+        tma_prefetch_desc(&tmW0);
+        tma_prefetch_desc(&tmW1);
+    }
+    if (warp == 1) {
+        tmem_alloc(tmem_slot, kTmemCols);
+        tmem_relinquish();
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    const uint32_t tmem_base = *tmem_slot;
+    const bool split = p.split > 1;
+    if (split) cluster_arrive();   // phase 1: every CTA has started
+
+    const int tile = (int)blockIdx.x / p.split;
+    const bool second = tile >= p.tiles0;
+    const int col0 = (second ? tile - p.tiles0 : tile) * 128;
+
+    if (warp == 0) {
+        // ---------------- TMA producer ----------------
+        const CUtensorMap* map = second ? &tmW1 : &tmW0;
+        auto load = [&](int s, int kb) {
+            mbar_arrive_expect_tx(&full[s], kSmallStageBytes);
+            if (p.b_nk) tma_load_2d(sW + s * kSmallStageBytes, map, &full[s], kb * kBK, col0);
+            else tma_load_2d(sW + s * kSmallStageBytes, map, &full[s], col0, kb * kBK);
+        };
+        const int first = min(p.stages, kb1 - kb0);
+        if (lane == 0)
+            for (int i = 0; i < first; ++i) load(i, kb0 + i);
+        __syncwarp();
+        if (split) {   // phases 1 and 2, before any wait that the other warps' progress ends
+            cluster_wait();
+            cluster_arrive();
+            cluster_wait();
+        }
+        if (lane == 0) {
+            int s = 0;
+            uint32_t ph = 0;
+            for (int kb = kb0 + first; kb < kb1; ++kb) {
+                if (!mbar_wait(&empty[s], ph, status, kDevErrTimeout)) break;
+                load(s, kb);
+                if (++s == p.stages) { s = 0; ph ^= 1u; }
+            }
+        }
+    } else if (warp == 1) {
+        // ---------------- MMA issuer ----------------
+        if (split) {
+            cluster_wait();
+            cluster_arrive();
+            cluster_wait();
+        }
+        if (lane == 0) {
+            bool ok = mbar_wait(ready, 0, status, kDevErrTimeout);
+            int s = 0;
+            uint32_t ph = 0;
+            for (int kb = kb0; ok && kb < kb1; ++kb) {
+                if (!mbar_wait(&full[s], ph, status, kDevErrTimeout)) { ok = false; break; }
+                tc_fence_after();
+                const uint32_t w_base = smem_u32(sW + s * kSmallStageBytes);
+                const uint32_t q_base = smem_u32(sQ + (size_t)(kb - kb0) * kNT * kBK);
+#pragma unroll
+                for (int kk = 0; kk < kBK / 32; ++kk) {
+                    // weights [N, K]: K-major rows; [K, N]: MN-major, a K step is 32 rows of 128 bytes
+                    const uint64_t wdesc = p.b_nk ? smem_desc_sw128(w_base + kk * 32, 16, 1024)
+                                                  : smem_desc_sw128(w_base + kk * 32 * 128, kBK * 128, 1024);
+                    mma_i8_ss(tmem_base, wdesc, smem_desc_sw128(q_base + kk * 32, 16, 1024), p.idesc,
+                              (kb != kb0 || kk != 0) ? 1u : 0u);
+                }
+                mma_commit(&empty[s]);
+                if (++s == p.stages) { s = 0; ph ^= 1u; }
+            }
+            if (ok) mma_commit(tfull);
+        }
+    } else {
+        // ---------------- quantiser, then epilogue (warps 2..9) ----------------
+        if (p.pdl) pdl_wait();
+        const int w = warp - 2;
+        const int k0 = kb0 * kBK, k1 = min(p.K, kb1 * kBK);
+        const T* const x = static_cast<const T*>(p.x);
+        if constexpr (kIn != kInCodes) {
+            // a warp takes tokens w, w + 8; with up to 4 the warps share a token's units of eight
+            const int share = p.T > 4 ? 1 : p.T > 2 ? 2 : p.T > 1 ? 4 : 8;   // warps of a token
+            const int tok0 = w / share, tstep = 8 / share;
+            const int u0 = (w % share) * 32 + lane, ustep = 32 * share * 8;
+            constexpr int kBatch = 4;
+            const bool whole = p.vec_x && (k1 - k0) % 8 == 0;
+            // units k, k + ustep, .. of token t, all asked for before any is used
+            auto fetch = [&](In8<T> (&d)[kBatch], int t, int k) {
+                const T* src = x + t * p.ld_x;
+                if (whole) {
+#pragma unroll
+                    for (int i = 0; i < kBatch; ++i) {
+                        d[i].zero();
+                        if (t < p.T && k + i * ustep < k1) d[i].load(src + k + i * ustep);
+                    }
+                } else {
+#pragma unroll
+                    for (int i = 0; i < kBatch; ++i) {
+                        d[i].zero();
+                        if (t < p.T && k + i * ustep < k1) d[i].load_part(src + k + i * ustep, k1 - k - i * ustep);
+                    }
+                }
+                if constexpr (kIn == kInPair) {
+                    In8<T> u[kBatch];
+#pragma unroll
+                    for (int i = 0; i < kBatch; ++i) {
+                        u[i].zero();
+                        if (t >= p.T || k + i * ustep >= k1) continue;
+                        if (whole) u[i].load(src + p.up + k + i * ustep);
+                        else u[i].load_part(src + p.up + k + i * ustep, k1 - k - i * ustep);
+                    }
+#pragma unroll
+                    for (int i = 0; i < kBatch; ++i)
+#pragma unroll
+                        for (int j = 0; j < 8; ++j) d[i].v[j] = u[i].v[j] * silu(d[i].v[j]);
+                }
+            };
+            if (threadIdx.x - 64 < kNT) s_amax[rank][threadIdx.x - 64] = 0u;
+            asm volatile("bar.sync 1, 256;" ::: "memory");
+            for (int t = tok0; t < p.T; t += 2 * tstep) {
+                uint32_t m[2] = {0u, 0u};
+                for (int k = k0 + u0 * 8; k - u0 * 8 < k1; k += kBatch * ustep) {
+                    In8<T> d[2][kBatch];
+                    fetch(d[0], t, k);
+                    fetch(d[1], t + tstep, k);
+#pragma unroll
+                    for (int i = 0; i < kBatch; ++i) {
+                        m[0] = max(m[0], d[0][i].amax_bits());
+                        m[1] = max(m[1], d[1][i].amax_bits());
+                    }
+                }
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    m[h] = __reduce_max_sync(0xffffffffu, m[h]);
+                    if (lane == 0 && t + h * tstep < p.T) atomicMax(&s_amax[rank][t + h * tstep], m[h]);
+                }
+            }
+            asm volatile("bar.sync 1, 256;" ::: "memory");
+            if (split) {
+                cluster_wait();   // phase 1
+                for (int i = threadIdx.x - 64; i < p.T * p.split; i += kSmallWorkers) {
+                    const int to = i / p.T, t = i % p.T;
+                    if (to != rank)
+                        asm volatile("st.shared::cluster.b32 [%0], %1;" ::"r"(mapa(smem_u32(&s_amax[rank][t]), to)),
+                                     "r"(s_amax[rank][t])
+                                     : "memory");
+                }
+                __syncwarp();
+                cluster_arrive();   // phase 2: every part's amax is here
+                cluster_wait();
+            }
+            for (int t = tok0; t < p.T; t += tstep) {
+                uint32_t m = s_amax[0][t];
+                for (int r = 1; r < p.split; ++r) m = max(m, s_amax[r][t]);
+                const RowScale rs(m);
+                if (u0 == 0) s_tok[t] = rs.s;
+                for (int k = k0 + u0 * 8; k - u0 * 8 < k1; k += kBatch * ustep) {
+                    In8<T> d[kBatch];
+                    fetch(d, t, k);
+#pragma unroll
+                    for (int i = 0; i < kBatch; ++i) {
+                        const int kk = k + i * ustep - k0;
+                        if (kk >= k1 - k0) continue;
+                        float f[8];
+                        d[i].get(f);
+                        // K-major, 128-byte swizzle: 16-byte unit j of row t at j ^ (t & 7)
+                        uint8_t* dst = sQ + (size_t)(kk / kBK) * kNT * kBK + t * 128 +
+                                       ((((kk & 127) >> 4) ^ (t & 7)) << 4) + (kk & 8);
+                        *reinterpret_cast<uint2*>(dst) = rs.codes(f);
+                    }
+                }
+            }
+        } else {
+            if (split) {
+                cluster_wait();
+                cluster_arrive();
+                cluster_wait();
+            }
+            if (threadIdx.x - 64 < p.T) s_tok[threadIdx.x - 64] = p.s_tok[threadIdx.x - 64];
+            const int units = (k1 - k0 + 15) / 16;   // rows start on 16-byte boundaries
+            for (int i = threadIdx.x - 64; i < units * p.T; i += kSmallWorkers) {
+                const int t = i / units, kk = (i - t * units) * 16;
+                const int8_t* src = x + t * p.ld_x + k0 + kk;
+                union { uint4 v; int8_t b[16]; } q;
+                if (k0 + kk + 16 <= k1) {
+                    q.v = __ldg(reinterpret_cast<const uint4*>(src));
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) q.b[j] = k0 + kk + j < k1 ? __ldg(src + j) : (int8_t)0;
+                }
+                *reinterpret_cast<uint4*>(sQ + (size_t)(kk / kBK) * kNT * kBK + t * 128 +
+                                          ((((kk & 127) >> 4) ^ (t & 7)) << 4)) = q.v;
+            }
+        }
+        fence_async_smem();
+        mbar_arrive(ready);
+        asm volatile("bar.sync 1, 256;" ::: "memory");   // s_tok
+
+        // a thread: channel c, half of the tokens
+        constexpr int kHalfTok = kNT / 2;
+        const int q = warp & 3, half = w >> 2, c = q * 32 + lane, tok = half * kHalfTok;
+        const bool ok = mbar_wait_warp(tfull, 0, status, kDevErrTimeout);
+        tc_fence_after();
+        const uint32_t taddr = tmem_base + ((uint32_t)(q * 32) << 16) + tok;
+        auto put = [&](int sum, int t, int ch) {   // channel ch of the tile
+            const int col = col0 + ch;
+            if (col >= p.N) return;
+            float v = (float)sum * s_tok[t] * __ldg((second ? p.s_ch1 : p.s_ch0) + col);
+            if (p.bias) v += __ldg(p.bias + col);
+            if (p.residual) v += load_as_f32(p.residual, t * p.ld_res + col, p.res_type);
+            const int64_t at = t * p.ld_out + col + (second ? p.out1 : 0);
+            if (p.out_type == MOE_TYPE_F32) static_cast<float*>(p.out)[at] = v;
+            else if (p.out_type == MOE_TYPE_F16) static_cast<__half*>(p.out)[at] = __float2half_rn(v);
+            else static_cast<__nv_bfloat16*>(p.out)[at] = __float2bfloat16_rn(v);
+        };
+        const int wch = 128 / p.split;              // channels of a slice
+#pragma unroll
+        for (int g = 0; g < kHalfTok; g += 8) {
+            if (!ok || tok + g >= p.T) break;       // the same for the whole warp
+            uint32_t a[8];
+            tmem_ld_32x32b_x8(taddr + g, a);
+            tmem_wait_ld();
+            if (!split) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+                    if (tok + g + i < p.T) put((int)a[i], tok + g + i, c);
+            } else {
+                // parts: [source][token / 4][channel of the slice][4 tokens]
+#pragma unroll
+                for (int i = 0; i < 8; i += 4) {
+                    if (tok + g + i >= p.T) break;
+                    const uint32_t at = (uint32_t)(((rank * (kNT / 4) + (tok + g + i) / 4) * wch + c % wch) * 16);
+                    st_cluster4(mapa(smem_u32(recv) + at, c / wch), a[i], a[i + 1], a[i + 2], a[i + 3]);
+                }
+            }
+        }
+        if (split) {
+            __syncwarp();
+            cluster_arrive();   // phase 3: every part has been sent
+            cluster_wait();
+            const int* part = reinterpret_cast<const int*>(recv);
+            for (int i = threadIdx.x - 64; ok && i < wch * p.T; i += kSmallWorkers) {
+                const int t = i / wch, ch = i % wch;
+                int sum = 0;
+                for (int r = 0; r < p.split; ++r) sum += part[((r * (kNT / 4) + t / 4) * wch + ch) * 4 + t % 4];
+                put(sum, t, rank * wch + ch);
+            }
+        }
+    }
+    if (split && warp < 2) {
+        __syncwarp();
+        cluster_arrive();       // phase 3
+        cluster_wait();
+    }
+    __syncthreads();
+    if (warp == 1) {
+        tc_fence_after();
+        tmem_dealloc(tmem_base, kTmemCols);
+    }
+}
+
 // ---- host side -----------------------------------------------------------------------
 
 // SMs the tile rules count on (B200).
@@ -954,6 +1308,102 @@ cudaError_t launch_linear(const int8_t* q, int64_t ldq, LinearParams p, const Ma
     return launch_linear_cfg<128, false>(ta, tb, to, p, clusters, st);
 }
 
+// Up to this many tokens small_linear_kernel is used (its MMA has 16 columns).
+// Measured (us in a graph, 7168 x 2048, quantiser included; small kernel, and
+// quantiser + tiles): 1 token 10.9, 11.8; 4 tokens 11.8, 11.8; 8 tokens 13.4,
+// 12.1; 16 tokens 17.5, 14.0.  One launch instead of two costs the host 4.9 us
+// instead of 7.5, which decides at 8.
+constexpr int kSmallTokens = 8;
+constexpr int kSmallN = 16;
+constexpr int kSmallStages = 5;
+constexpr size_t kSmallSmem = 112 * 1024;   // two CTAs an SM
+
+template <int kNT, int kIn>
+cudaError_t launch_small_typed(const CUtensorMap (&w)[2], const SmallParams& p, int tiles, size_t smem, cudaStream_t st) {
+    auto kern = small_linear_kernel<kNT, kIn>;
+    static SmemAttr attr;
+    cudaError_t err = ensure_smem(kern, smem, attr);
+    if (err != cudaSuccess) return err;
+    return launch_ex(kern, (unsigned)(tiles * p.split), (unsigned)kSmallThreads, smem, p.split, p.pdl != 0, st, w[0], w[1],
+                     p);
+}
+
+// Whether a call's codes fit beside the weight stages at some split; the split
+// with the most CTAs that are resident at once (two an SM).
+bool plan_small(int64_t T, int K, int N, int mats, int num_sms, int* split, int* stages, size_t* smem) {
+    if (T > kSmallTokens) return false;
+    const int kblocks = (K + kBK - 1) / kBK, tiles = (N + 127) / 128 * mats;
+    *split = 0;
+    for (int s = 1; s <= kMaxSplit && s <= kblocks; s *= 2) {
+        const int blocks = (kblocks + s - 1) / s, st = std::min(kSmallStages, blocks);
+        const size_t need = small_smem<kSmallN>(st, blocks, s);
+        if (need > kSmallSmem) continue;
+        // clusters of 1, 2, 4 and 8 CTAs of up to half an SM's memory fit 296, 148, 71 and 33 times
+        const int at_once = s == 1 ? 2 * num_sms : s == 2 ? num_sms : s == 4 ? num_sms * 71 / 148 : num_sms * 33 / 148;
+        if (*split != 0 && tiles > at_once) break;
+        *split = s;
+        *stages = st;
+        *smem = need;
+    }
+    return *split != 0;
+}
+
+// A product of few tokens in one launch; x_type: MOE_TYPE_* of x, or -1 for
+// codes.  up != 0: gate and up values.  False where the shape needs the tiles.
+bool try_small(const void* x, int x_type, int64_t ld_x, int64_t up, const LinearParams& l, const Matrix& w0,
+               const Matrix* w1, int num_sms, cudaStream_t st, cudaError_t* err) {
+    int split, stages;
+    size_t smem;
+    const int mats = w1 ? 2 : 1;
+    if (!plan_small(l.T, l.K, l.N, mats, num_sms, &split, &stages, &smem)) return false;
+    SmallParams p{};
+    p.x = x;
+    p.ld_x = ld_x;
+    p.up = up;
+    p.s_tok = l.s_tok;
+    p.T = l.T;
+    p.K = l.K;
+    p.N = l.N;
+    p.kblocks = (l.K + kBK - 1) / kBK;
+    p.split = split;
+    p.stages = stages;
+    p.tiles0 = (l.N + 127) / 128;
+    p.out1 = l.out1;
+    p.b_nk = l.b_nk;
+    p.pdl = l.pdl;
+    p.s_ch0 = w0.scale;
+    p.s_ch1 = w1 ? w1->scale : w0.scale;
+    p.bias = l.bias;
+    p.residual = l.residual;
+    p.ld_res = l.ld_res;
+    p.res_type = l.res_type;
+    p.out = l.out;
+    p.ld_out = l.ld_out;
+    p.out_type = l.out_type;
+    const int size = x_type < 0 ? 1 : elem_bytes(x_type);
+    p.vec_x = aligned(x, 16) && (ld_x * size) % 16 == 0;
+    // weights are the A operand (M = 128 channels): MN-major for [K, N]
+    p.idesc = idesc_i8(128, kSmallN, false) | (p.b_nk ? 0u : 1u << 15);
+    CUtensorMap w[2];
+    const Matrix* ws[2] = {&w0, w1 ? w1 : &w0};
+    for (int i = 0; i < mats; ++i) {
+        const bool ok = p.b_nk ? make_map_u8_strided(&w[i], ws[i]->w, p.K, p.N, ws[i]->ld, 128, 128)
+                               : make_map_u8_strided(&w[i], ws[i]->w, p.N, p.K, ws[i]->ld, 128, kBK);
+        if (!ok) {
+            *err = cudaErrorInvalidValue;
+            return true;
+        }
+    }
+    if (mats == 1) w[1] = w[0];
+    const int tiles = p.tiles0 * mats;
+    if (x_type < 0) *err = launch_small_typed<kSmallN, kInCodes>(w, p, tiles, smem, st);
+    else if (up != 0) *err = launch_small_typed<kSmallN, kInPair>(w, p, tiles, smem, st);
+    else if (x_type == MOE_TYPE_F32) *err = launch_small_typed<kSmallN, kInF32>(w, p, tiles, smem, st);
+    else if (x_type == MOE_TYPE_F16) *err = launch_small_typed<kSmallN, kInF16>(w, p, tiles, smem, st);
+    else *err = launch_small_typed<kSmallN, kInBF16>(w, p, tiles, smem, st);
+    return true;
+}
+
 int bad(const char* who, const char* what) {
     set_error("%s: %s", who, what);
     return MOE_ERR_INVALID_ARG;
@@ -997,6 +1447,7 @@ int check_out(const char* who, const void* out, int type, int64_t T, int64_t N, 
 }
 
 int check_scratch(const char* who, const void* scratch, size_t have, size_t need) {
+    if (need == 0) return MOE_OK;
     if (!scratch || !aligned(scratch, 256)) return bad(who, "scratch is null or not 256-byte aligned");
     if (have < need) {
         set_error("%s: scratch of %zu bytes is smaller than the %zu this call needs", who, have, need);
@@ -1033,8 +1484,15 @@ LinearParams out_params(int64_t T, int K, int N, const float* s_tok, const float
 // product's split of K fills.
 bool fused_swiglu(int64_t T, int64_t f) { return (T + 127) / 128 * ((f + 127) / 128) * 4 >= kRuleSms * 3; }
 
-size_t linear_scratch(int64_t T, int64_t K) {
-    return up256((size_t)T * up16(K)) + up256((size_t)T * sizeof(float));
+// Whether the small kernel takes a call (its shared memory depends on K alone).
+bool is_small(int64_t T, int K) {
+    int split, stages;
+    size_t smem;
+    return plan_small(T, K, 1, 1, kRuleSms, &split, &stages, &smem);
+}
+
+size_t linear_scratch(int64_t T, int K) {
+    return is_small(T, K) ? 0 : up256((size_t)T * up16(K)) + up256((size_t)T * sizeof(float));
 }
 
 struct SharedScratch {
@@ -1101,24 +1559,26 @@ int run_shared_expert(const char* who, const void* x, int x_type, int64_t tokens
     float* h = reinterpret_cast<float*>(base + sc.h);
     const bool fused = fused_swiglu(tokens, d_ff);
     const int64_t behind = (int64_t)(up256((size_t)tokens * sc.ldh * sizeof(float)) / sizeof(float));
-    cudaError_t e = launch_quantize(x, x_type, tokens, d_model, row_stride, 0, qx, up16(d_model), sx, false, stream);
-    if (e == cudaSuccess) {
-        LinearParams p = out_params(tokens, d_model, d_ff, sx, nullptr, h, MOE_TYPE_F32, sc.ldh, gate->order, true);
-        p.out1 = behind;
-        const Matrix u{up->w, up->row_stride, up->scale};
-        e = launch_linear(qx, up16(d_model), p, Matrix{gate->w, gate->row_stride, gate->scale}, &u, fused, num_sms,
-                          stream);
+    const Matrix mg{gate->w, gate->row_stride, gate->scale}, mu{up->w, up->row_stride, up->scale},
+        md{down->w, down->row_stride, down->scale};
+    LinearParams ph = out_params(tokens, d_model, d_ff, sx, nullptr, h, MOE_TYPE_F32, sc.ldh, gate->order, false);
+    ph.out1 = behind;
+    LinearParams py = out_params(tokens, d_ff, d_model, sh, nullptr, out, out_type, out_stride, down->order, true);
+    py.residual = residual;
+    py.ld_res = residual_stride;
+    py.res_type = x_type;
+    py.vec_res = aligned(residual, 16) && (residual_stride * elem_bytes(x_type)) % 16 == 0;
+    cudaError_t e = cudaSuccess;
+    // gate and up: g and u (few tokens, or too few tiles to fuse), or h
+    if (fused || !try_small(x, x_type, row_stride, 0, ph, mg, &mu, num_sms, stream, &e)) {
+        ph.pdl = 1;
+        e = launch_quantize(x, x_type, tokens, d_model, row_stride, 0, qx, up16(d_model), sx, false, stream);
+        if (e == cudaSuccess) e = launch_linear(qx, up16(d_model), ph, mg, &mu, fused, num_sms, stream);
     }
-    if (e == cudaSuccess)
+    if (e != cudaSuccess) return cuda_error(who, e);
+    if (fused || !try_small(h, MOE_TYPE_F32, sc.ldh, behind, py, md, nullptr, num_sms, stream, &e)) {
         e = launch_quantize(h, MOE_TYPE_F32, tokens, d_ff, sc.ldh, fused ? 0 : behind, qh, up16(d_ff), sh, true, stream);
-    if (e == cudaSuccess) {
-        LinearParams p = out_params(tokens, d_ff, d_model, sh, nullptr, out, out_type, out_stride, down->order, true);
-        p.residual = residual;
-        p.ld_res = residual_stride;
-        p.res_type = x_type;
-        p.vec_res = aligned(residual, 16) && (residual_stride * elem_bytes(x_type)) % 16 == 0;
-        e = launch_linear(qh, up16(d_ff), p, Matrix{down->w, down->row_stride, down->scale}, nullptr, false, num_sms,
-                          stream);
+        if (e == cudaSuccess) e = launch_linear(qh, up16(d_ff), py, md, nullptr, false, num_sms, stream);
     }
     return e == cudaSuccess ? MOE_OK : cuda_error(who, e);
 }
@@ -1167,9 +1627,11 @@ extern "C" int moe_int8_matmul(const int8_t* q, int64_t q_stride, const float* s
     rc = current_device(&dev, &num_sms);
     if (rc != MOE_OK) return rc;
     g_linear_used[dev] = true;
-    const cudaError_t e =
-        launch_linear(q, q_stride, out_params(tokens, K, N, scale, bias, out, out_type, out_stride, w->order, false),
-                      Matrix{w->w, w->row_stride, w->scale}, nullptr, false, num_sms, stream);
+    const LinearParams p = out_params(tokens, K, N, scale, bias, out, out_type, out_stride, w->order, false);
+    const Matrix m{w->w, w->row_stride, w->scale};
+    cudaError_t e;
+    if (!try_small(q, -1, q_stride, 0, p, m, nullptr, num_sms, stream, &e))
+        e = launch_linear(q, q_stride, p, m, nullptr, false, num_sms, stream);
     return e == cudaSuccess ? MOE_OK : cuda_error(who, e);
 }
 
@@ -1190,12 +1652,16 @@ extern "C" int moe_int8_linear(const void* x, int x_type, int64_t tokens, int K,
     rc = current_device(&dev, &num_sms);
     if (rc != MOE_OK) return rc;
     g_linear_used[dev] = true;
-    int8_t* q = static_cast<int8_t*>(scratch);
-    float* s = reinterpret_cast<float*>(q + up256((size_t)tokens * up16(K)));
-    cudaError_t e = launch_quantize(x, x_type, tokens, K, row_stride, 0, q, up16(K), s, false, stream);
-    if (e == cudaSuccess)
-        e = launch_linear(q, up16(K), out_params(tokens, K, N, s, bias, out, out_type, out_stride, w->order, true),
-                          Matrix{w->w, w->row_stride, w->scale}, nullptr, false, num_sms, stream);
+    int8_t* q = static_cast<int8_t*>(scratch);   // (null where the small kernel needs none)
+    float* s = q ? reinterpret_cast<float*>(q + up256((size_t)tokens * up16(K))) : nullptr;
+    LinearParams p = out_params(tokens, K, N, s, bias, out, out_type, out_stride, w->order, false);
+    const Matrix m{w->w, w->row_stride, w->scale};
+    cudaError_t e;
+    if (!try_small(x, x_type, row_stride, 0, p, m, nullptr, num_sms, stream, &e)) {
+        p.pdl = 1;
+        e = launch_quantize(x, x_type, tokens, K, row_stride, 0, q, up16(K), s, false, stream);
+        if (e == cudaSuccess) e = launch_linear(q, up16(K), p, m, nullptr, false, num_sms, stream);
+    }
     return e == cudaSuccess ? MOE_OK : cuda_error(who, e);
 }
 

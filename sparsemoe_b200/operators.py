@@ -21,25 +21,28 @@ from .config import (MOE_SCORES, MOE_TYPE_BF16, MOE_TYPE_F16, MOE_TYPE_F32, MOE_
 
 _TYPE = {torch.float32: MOE_TYPE_F32, torch.float16: MOE_TYPE_F16, torch.bfloat16: MOE_TYPE_BF16}
 _ref = ctypes.byref
-_empty = torch.empty
+_empty = torch.empty        # (sizes are given one by one: a tuple of them takes torch's parser longer)
+_i32, _f32, _i8, _u8 = torch.int32, torch.float32, torch.int8, torch.uint8
 _device = torch.cuda.current_device
 _raw_stream = torch._C._cuda_getCurrentRawStream   # the handle alone: current_stream() builds an object first
+_route_fn, _linear_fn, _shared_fn = lib.moe_route_experts, lib.moe_int8_linear, lib.moe_int8_shared_expert
+_linear_scratch = functools.lru_cache(maxsize=4096)(lib.moe_int8_linear_scratch_bytes)
+_shared_scratch = functools.lru_cache(maxsize=4096)(lib.moe_int8_shared_expert_scratch_bytes)
 
 
-def _run(t: torch.Tensor, fn, *args) -> None:
-    """fn(*args, stream) with the device of `t` current, on torch's current stream there."""
-    index = t.get_device()
-    prev = _device()
-    if prev == index:
+def _call(index: int, fn, *args) -> None:
+    """fn(*args, stream) on device `index` and torch's current stream there."""
+    if _device() == index:
         rc = fn(*args, _raw_stream(index))
-    else:
-        torch.cuda.set_device(index)
-        try:
-            rc = fn(*args, _raw_stream(index))
-        finally:
-            torch.cuda.set_device(prev)
-    if rc:
-        check(rc)
+        if rc:
+            check(rc)
+        return
+    prev = _device()
+    torch.cuda.set_device(index)
+    try:
+        check(fn(*args, _raw_stream(index)))
+    finally:
+        torch.cuda.set_device(prev)
 
 
 def _rows(t: torch.Tensor, name: str) -> tuple[int, int, int]:
@@ -71,7 +74,7 @@ def _output(out, rows: int, cols: int, dtype, like: torch.Tensor):
         kind = _TYPE.get(dtype)
         if kind is None:
             raise ValueError(f"the output must be f32, f16 or bf16, not {dtype}")
-        return _empty((rows, cols), dtype=dtype, device=like.device), kind, cols
+        return _empty(rows, cols, dtype=dtype, device=like.device), kind, cols
     kind = _TYPE.get(out.dtype)
     if kind is None or out.shape != (rows, cols) or out.get_device() != like.get_device() or \
             (dtype is not None and out.dtype != dtype):
@@ -112,6 +115,11 @@ def _routing(score, groups, kept_groups, group_top, renormalise, scale) -> MoeRo
     return MoeRouting(MOE_SCORES[score], groups, kept_groups, group_top, 1 if renormalise else 0, scale)
 
 
+@functools.lru_cache(maxsize=512)
+def _routing_ref(*spec):
+    return _ref(_routing(*spec))
+
+
 def route_experts(logits: torch.Tensor, top_k: int, *, score: str = "softmax", bias: torch.Tensor | None = None,
                   groups: int = 1, kept_groups: int = 1, group_top: int = 1, renormalise: bool = True,
                   scale: float = 1.0, out: tuple[torch.Tensor, torch.Tensor] | None = None):
@@ -131,18 +139,18 @@ def route_experts(logits: torch.Tensor, top_k: int, *, score: str = "softmax", b
     if kind is None or index < 0:
         raise ValueError("logits must be f32, f16 or bf16 on a GPU")
     T, E, ld = _rows(logits, "logits")
-    r = _routing(score, groups, kept_groups, group_top, renormalise, scale)
+    r = _routing_ref(score, groups, kept_groups, group_top, renormalise, scale)
     b = _vector(bias, E, "bias", index)
     if out is None:
-        idx = _empty((T, top_k), dtype=torch.int32, device=logits.device)
-        w = _empty((T, top_k), dtype=torch.float32, device=logits.device)
+        dev = logits.device
+        idx = _empty(T, top_k, dtype=_i32, device=dev)
+        w = _empty(T, top_k, dtype=_f32, device=dev)
     else:
         idx, w = out
         for t, dt in ((idx, torch.int32), (w, torch.float32)):
             if t.shape != (T, top_k) or t.dtype != dt or not t.is_contiguous() or t.get_device() != index:
                 raise ValueError(f"out must be contiguous int32 and f32 tensors of shape {(T, top_k)} on cuda:{index}")
-    _run(logits, lib.moe_route_experts, logits.data_ptr(), kind, T, E, ld, top_k, _ref(r), b, idx.data_ptr(),
-         w.data_ptr())
+    _call(index, _route_fn, logits.data_ptr(), kind, T, E, ld, top_k, r, b, idx.data_ptr(), w.data_ptr())
     return idx, w
 
 
@@ -193,11 +201,11 @@ def quantize_int8_tokens(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     boundaries, scale [T] f32 = max|x| / 127 -- times f32(1/127) -- or 1 where
     that is zero; q = round-half-even of the exact x / scale).  A row with a NaN
     or an infinity gets a NaN scale."""
-    kind, _, T, K, ld = _x(x)
+    kind, index, T, K, ld = _x(x)
     kp = (K + 15) // 16 * 16
-    q = _empty((T, kp), dtype=torch.int8, device=x.device)
-    s = _empty(T, dtype=torch.float32, device=x.device)
-    _run(x, lib.moe_int8_quantize_tokens, x.data_ptr(), kind, T, K, ld, q.data_ptr(), kp, s.data_ptr())
+    q = _empty(T, kp, dtype=_i8, device=x.device)
+    s = _empty(T, dtype=_f32, device=x.device)
+    _call(index, lib.moe_int8_quantize_tokens, x.data_ptr(), kind, T, K, ld, q.data_ptr(), kp, s.data_ptr())
     return q[:, :K], s
 
 
@@ -218,7 +226,7 @@ def int8_matmul(q: torch.Tensor, scale: torch.Tensor, w: torch.Tensor, w_scale: 
     b = _vector(bias, N, "bias", index)
     s = _vector(scale, T, "scale", index)
     out, kind, ldo = _output(out, T, N, out_dtype if out is not None or out_dtype is not None else torch.bfloat16, q)
-    _run(q, lib.moe_int8_matmul, q.data_ptr(), ld, s, T, K, _ref(wt), N, b, out.data_ptr(), kind, ldo)
+    _call(index, lib.moe_int8_matmul, q.data_ptr(), ld, s, T, K, _ref(wt), N, b, out.data_ptr(), kind, ldo)
     return out
 
 
@@ -231,10 +239,10 @@ def int8_linear(x: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, *, bias
     wt, N = _weight(w, w_scale, "w", K, index)
     b = _vector(bias, N, "bias", index)
     out, okind, ldo = _output(out, T, N, x.dtype if out is None and out_dtype is None else out_dtype, x)
-    n = lib.moe_int8_linear_scratch_bytes(T, K)
-    scratch = _empty(n, dtype=torch.uint8, device=x.device)
-    _run(x, lib.moe_int8_linear, x.data_ptr(), kind, T, K, ld, _ref(wt), N, b, out.data_ptr(), okind, ldo,
-         scratch.data_ptr(), n)
+    n = _linear_scratch(T, K)
+    scratch = _empty(n, dtype=_u8, device=x.device) if n else None
+    _call(index, _linear_fn, x.data_ptr(), kind, T, K, ld, _ref(wt), N, b, out.data_ptr(), okind, ldo,
+          scratch.data_ptr() if n else None, n)
     return out
 
 
@@ -259,8 +267,8 @@ def int8_shared_expert(x: torch.Tensor, w_gate: torch.Tensor, s_gate: torch.Tens
         ld_res = _rows(residual, "residual")[2]
         res = residual.data_ptr()
     out, okind, ldo = _output(out, T, d, x.dtype if out is None else None, x)
-    n = lib.moe_int8_shared_expert_scratch_bytes(T, d, f)
-    scratch = _empty(n, dtype=torch.uint8, device=x.device)
-    _run(x, lib.moe_int8_shared_expert, x.data_ptr(), kind, T, d, ld, _ref(g), _ref(u), _ref(dn), f, res, ld_res,
-         out.data_ptr(), okind, ldo, scratch.data_ptr(), n)
+    n = _shared_scratch(T, d, f)
+    scratch = _empty(n, dtype=_u8, device=x.device)
+    _call(index, _shared_fn, x.data_ptr(), kind, T, d, ld, _ref(g), _ref(u), _ref(dn), f, res, ld_res, out.data_ptr(),
+          okind, ldo, scratch.data_ptr(), n)
     return out

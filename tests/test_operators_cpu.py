@@ -43,7 +43,7 @@ def weight(w=FAKE, ld=64, scale=FAKE, order=0):
     return sm.MoeInt8Weight(w, ld, scale, order)
 
 
-def linear(T=4, K=64, N=64, x=FAKE, typ=2, ldx=64, wt=None, bias=None, out=FAKE, otyp=2, ldo=64, scratch=FAKE,
+def linear(T=32, K=64, N=64, x=FAKE, typ=2, ldx=64, wt=None, bias=None, out=FAKE, otyp=2, ldo=64, scratch=FAKE,
            n=1 << 20):
     wt = weight() if wt is None else wt
     return sm.lib.moe_int8_linear(x, typ, T, K, ldx, ctypes.byref(wt), N, bias, out, otyp, ldo, scratch, n, None)
@@ -67,7 +67,9 @@ def test_linear_limits():
     assert linear(K=131072, ldx=131072) == sm.MOE_ERR_UNSUPPORTED
     assert linear(T=1 << 31) == sm.MOE_ERR_UNSUPPORTED
     assert linear(T=0, x=None, out=None, scratch=None, n=0) == sm.MOE_OK
-    assert sm.lib.moe_int8_linear_scratch_bytes(5, 100) >= 5 * 112 + 5 * 4
+    assert sm.lib.moe_int8_linear_scratch_bytes(50, 100) >= 50 * 112 + 50 * 4
+    assert sm.lib.moe_int8_linear_scratch_bytes(1, 7168) == 0   # a few tokens: one kernel, no scratch
+    assert sm.lib.moe_int8_linear_scratch_bytes(1, 131071) > 0  # whose codes do not fit its shared memory
     assert sm.lib.moe_int8_linear_scratch_bytes(-1, 100) == 0
 
 
