@@ -136,74 +136,110 @@ __device__ __forceinline__ void load_row(const T* row, int e0, int E, bool vec, 
     for (int i = 0; i < NV; ++i) x[i] = e0 + i < E ? to_f32<T>(row[e0 + i]) : -INFINITY;
 }
 
+// f64 values of a row's experts lane*NV .. lane*NV + NV - 1: v orders the
+// experts (their logits without a bias), m the members of groups.
+template <typename T, int NV>
+__device__ __forceinline__ void values_f64(const RouteParams& p, const T* row, int lane, double (&v)[NV],
+                                           double (&m)[NV]) {
+    const int e0 = lane * NV;
+    float x[NV];
+    load_row<T, NV>(row, e0, p.E, p.vec != 0, x);
+    double top = -INFINITY, sum = 1.0;
+#pragma unroll
+    for (int q = 0; q < NV; ++q) {
+        v[q] = m[q] = selectable<T>(x[q]) ? (double)x[q] : -INFINITY;
+        top = fmax(top, v[q]);
+    }
+    if (!p.bias && p.group_top == 1) return;
+    if (p.sigmoid) {
+#pragma unroll
+        for (int q = 0; q < NV; ++q) m[q] = exp(-v[q]);
+#pragma unroll
+        for (int q = 0; q < NV; ++q) m[q] = 1.0 / (1.0 + m[q]);
+    } else {
+        top = warp_max(top);
+        sum = 0.0;
+#pragma unroll
+        for (int q = 0; q < NV; ++q) {
+            m[q] = v[q] == -INFINITY ? 0.0 : v[q] == top ? 1.0 : exp(v[q] - top);
+            sum += m[q];
+        }
+        sum = warp_sum(sum);
+    }
+#pragma unroll
+    for (int q = 0; q < NV; ++q) {
+        m[q] = v[q] == -INFINITY ? -INFINITY : p.sigmoid ? m[q] : m[q] / sum;
+        if (p.bias) {
+            const float b = e0 + q < p.E ? __ldg(p.bias + e0 + q) : -INFINITY;
+            v[q] = m[q] = b > kMasked ? m[q] + (double)b : -INFINITY;
+        }
+    }
+}
+
+// Which of up to 32 groups of a row stay, in f64: bit g.  buf: 32 * NV doubles of
+// this warp's shared memory.  Sums of two that agree to 2^-49 are ties
+// (sigmoid(x) + sigmoid(-x) is 1 for every x).
+template <typename T, int NV>
+__device__ __noinline__ uint32_t groups_f64(const RouteParams& p, const T* row, double* buf, int lane) {
+    double v[NV], m[NV];
+    values_f64<T, NV>(p, row, lane, v, m);
+    __syncwarp();
+#pragma unroll
+    for (int q = 0; q < NV; ++q) buf[lane * NV + q] = m[q];
+    __syncwarp();
+    const bool pair = p.group_top == 2;
+    int sub = 32;
+    while (32 / sub < p.G) sub >>= 1;
+    const int g = lane / sub;
+    double a = -INFINITY, b = -INFINITY;
+    if (g < p.G)
+        for (int i = lane % sub; i < p.per; i += sub) merge2(a, b, buf[g * p.per + i], (double)-INFINITY);
+    for (int o = sub >> 1; o > 0; o >>= 1) {
+        const double c = __shfl_xor_sync(kFull, a, o), d = __shfl_xor_sync(kFull, b, o);
+        merge2(a, b, c, d);
+    }
+    if (pair && b != -INFINITY) a += b;
+    a = __shfl_sync(kFull, a, (lane * sub) & 31);   // lane g: group g
+    if (lane >= p.G) a = -INFINITY;
+    const double tie = pair && !isinf(a) ? 0x1p-49 * (1.0 + fabs(a)) : 0.0;
+    int rank = 0;
+    for (int h = 0; h < p.G; ++h) {
+        const double other = __shfl_sync(kFull, a, h);
+        rank += other > a + tie || (other >= a - tie && h < lane) ? 1 : 0;
+    }
+    __syncwarp();
+    return __ballot_sync(kFull, a != -INFINITY && rank < p.kept);
+}
+
 // The whole selection of one row in f64.  Returns the lane's choice (lane l: the
 // l-th) or -1.  buf: 32 * NV doubles of shared memory of this warp.
 template <typename T, int NV>
 __device__ __noinline__ int route_row_f64(const RouteParams& p, const T* row, double* buf, int lane) {
+    double v[NV], m[NV];
+    values_f64<T, NV>(p, row, lane, v, m);
     const int e0 = lane * NV;
-    float x[NV];
-    load_row<T, NV>(row, e0, p.E, p.vec != 0, x);
-    double v[NV];
-    double top = -INFINITY;
-#pragma unroll
-    for (int q = 0; q < NV; ++q) {
-        v[q] = selectable<T>(x[q]) ? (double)x[q] : -INFINITY;
-        top = fmax(top, v[q]);
-    }
     const bool pair = p.group_top == 2;
-    if (p.bias || pair) {
-        double s[NV], sum = 0.0;
-        top = warp_max(top);
+    if (p.G > 1 && p.G <= 32) {
+        const uint32_t stay = groups_f64<T, NV>(p, row, buf, lane);
 #pragma unroll
-        for (int q = 0; q < NV; ++q) {
-            if (p.sigmoid) s[q] = 1.0 / (1.0 + exp(-v[q]));
-            else s[q] = v[q] == -INFINITY ? 0.0 : v[q] == top ? 1.0 : exp(v[q] - top);
-            sum += s[q];
-        }
-        sum = p.sigmoid ? 1.0 : warp_sum(sum);
-#pragma unroll
-        for (int q = 0; q < NV; ++q) {
-            s[q] = v[q] == -INFINITY ? -INFINITY : p.sigmoid ? s[q] : s[q] / sum;
-            if (p.bias) {
-                const float b = e0 + q < p.E ? __ldg(p.bias + e0 + q) : -INFINITY;
-                v[q] = s[q] = b > kMasked ? s[q] + (double)b : -INFINITY;
-            }
-            buf[e0 + q] = pair ? s[q] : v[q];
-        }
-    } else if (p.G > 1) {
-#pragma unroll
-        for (int q = 0; q < NV; ++q) buf[e0 + q] = v[q];
-    }
-    if (p.G > 1) {
+        for (int q = 0; q < NV; ++q)
+            if (!(stay >> (min(e0 + q, p.E - 1) / p.per) & 1)) v[q] = -INFINITY;
+    } else if (p.G > 32) {
         __syncwarp();
-        // scores of the groups into the first G places once every lane has read its members:
+#pragma unroll
+        for (int q = 0; q < NV; ++q) buf[e0 + q] = m[q];
+        __syncwarp();
         // lane l holds groups l, l + 32, .. (at most NV of them)
         double gs[NV];
 #pragma unroll
         for (int i = 0; i < NV; ++i) gs[i] = -INFINITY;
-        if (p.G <= 32) {
-            int sub = 32;
-            while (32 / sub < p.G) sub >>= 1;
-            const int g = lane / sub;
-            double a = -INFINITY, b = -INFINITY;
-            if (g < p.G)
-                for (int i = lane % sub; i < p.per; i += sub) merge2(a, b, buf[g * p.per + i], (double)-INFINITY);
-            for (int o = sub >> 1; o > 0; o >>= 1) {
-                const double c = __shfl_xor_sync(kFull, a, o), d = __shfl_xor_sync(kFull, b, o);
-                merge2(a, b, c, d);
-            }
-            if (pair && b != -INFINITY) a += b;
-            a = __shfl_sync(kFull, a, (lane * sub) & 31);
-            if (lane < p.G) gs[0] = a;
-        } else {
 #pragma unroll
-            for (int i = 0; i < NV; ++i) {
-                const int g = lane + 32 * i;
-                if (g >= p.G) break;
-                double a = -INFINITY, b = -INFINITY;
-                for (int j = 0; j < p.per; ++j) merge2(a, b, buf[g * p.per + j], (double)-INFINITY);
-                gs[i] = pair && b != -INFINITY ? a + b : a;
-            }
+        for (int i = 0; i < NV; ++i) {
+            const int g = lane + 32 * i;
+            if (g >= p.G) break;
+            double a = -INFINITY, b = -INFINITY;
+            for (int j = 0; j < p.per; ++j) merge2(a, b, buf[g * p.per + j], (double)-INFINITY);
+            gs[i] = pair && b != -INFINITY ? a + b : a;
         }
         uint32_t keep = 0;
         const double tie = pair ? 0x1p-49 : 0.0;
@@ -387,6 +423,7 @@ __global__ void __launch_bounds__(kRouteWarps * 32) route_kernel(const __grid_co
             redo = p.sub == 0;
             __syncwarp();
         }
+        bool near = false;
         if (pair && b != -INFINITY) a += b;
         if (g >= p.G) a = -INFINITY;
         const uint32_t gk = a != -INFINITY ? (order_key(a) & ~31u) | (31 - g) : 0u;
@@ -397,7 +434,7 @@ __global__ void __launch_bounds__(kRouteWarps * 32) route_kernel(const __grid_co
             last = best;
             if (cur == best) cur = 0;
         }
-        const bool stay = gk != 0 && cur == 0;
+        bool stay = gk != 0 && cur == 0;
         const uint32_t out = __reduce_max_sync(kFull, cur);
         if (out != 0 && (scored || !exact)) {
             // close with the index in the low bits: the scores themselves decide
@@ -405,9 +442,13 @@ __global__ void __launch_bounds__(kRouteWarps * 32) route_kernel(const __grid_co
             if (!(lo - hi > 1.2e-5f * fmaxf(fabsf(lo), fabsf(hi)) + 2.0f * err2)) {
                 const float worst = key_value(__reduce_min_sync(kFull, stay ? order_key(a) : 0xFFFFFFFFu));
                 const float other = key_value(__reduce_max_sync(kFull, stay || gk == 0 ? 0u : order_key(a)));
-                redo |= scored ? !(worst - other > 2.0f * err2 + 6e-7f * fmaxf(fabsf(worst), fabsf(other)))
-                               : !(worst > other);
+                near = scored ? !(worst - other > 2.0f * err2 + 6e-7f * fmaxf(fabsf(worst), fabsf(other)))
+                              : !(worst > other);
             }
+        }
+        if (near && !redo) {
+            const uint32_t mask = groups_f64<T, NV>(p, row, sv[warp], lane);
+            stay = g < p.G && (mask >> g & 1);
         }
         if (p.lanes > 0) {
 #pragma unroll
@@ -491,6 +532,277 @@ __global__ void __launch_bounds__(kRouteWarps * 32) route_kernel(const __grid_co
     }
 }
 
+// Many tokens: four to a warp, eight lanes each, lane l of a token holding its
+// experts l*per .. l*per + per - 1 (per = E / 8: one group, where there are
+// eight).  Everything that a round costs a warp is then paid for four tokens, and
+// a group's score needs no shuffle.  A lane keeps the eight best of its experts
+// in order (sorting networks of eight, merged); k <= 8.  Rows in which neighbours
+// are too close for f32 are done again by the whole warp.  32768 x 256, sigmoid,
+// bias, 4 of 8 groups: 883 warp instructions a token and 35 us with a warp a
+// token, 300 and 16 us so; below about 4000 tokens the warp a token is faster,
+// its chain of dependent instructions being a third as long.
+__device__ __forceinline__ uint32_t max8(uint32_t v) {   // over a token's eight lanes
+#pragma unroll
+    for (int o = 4; o > 0; o >>= 1) v = max(v, __shfl_xor_sync(kFull, v, o));
+    return v;
+}
+__device__ __forceinline__ float fmax8(float v) {
+#pragma unroll
+    for (int o = 4; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(kFull, v, o));
+    return v;
+}
+__device__ __forceinline__ float sum8(float v) {
+#pragma unroll
+    for (int o = 4; o > 0; o >>= 1) v += __shfl_xor_sync(kFull, v, o);
+    return v;
+}
+
+// Four consecutive elements (rows allow it: the host checks).
+__device__ __forceinline__ void load4(const float* p, float* x) {
+    const float4 a = __ldg(reinterpret_cast<const float4*>(p));
+    x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w;
+}
+template <typename T16> __device__ __forceinline__ void load4(const T16* p, float* x) {
+    const uint2 a = __ldg(reinterpret_cast<const uint2*>(p));
+    const float2 lo = F16Traits<T16>::unpack2(a.x), hi = F16Traits<T16>::unpack2(a.y);
+    x[0] = lo.x; x[1] = lo.y; x[2] = hi.x; x[3] = hi.y;
+}
+
+// The eight largest of NV keys, descending, in key[0..8).
+template <int NV> __device__ __forceinline__ void top8(uint32_t (&key)[NV]) {
+#pragma unroll
+    for (int b = 0; b < NV; b += 8) {
+        uint32_t t[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) t[i] = key[b + i];
+        sort_desc<8>(t);
+        if (b == 0) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) key[i] = t[i];
+        } else {
+            // the larger of a_i and b_(7-i) are the eight largest, in bitonic order
+#pragma unroll
+            for (int i = 0; i < 8; ++i) key[i] = max(key[i], t[7 - i]);
+#pragma unroll
+            for (int q = 4; q > 0; q >>= 1)
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+                    if (!(i & q)) {
+                        const uint32_t hi = max(key[i], key[i + q]);
+                        key[i + q] = min(key[i], key[i + q]);
+                        key[i] = hi;
+                    }
+        }
+    }
+}
+
+template <typename T, int NV>
+__global__ void __launch_bounds__(kRouteWarps * 32) route_many_kernel(const __grid_constant__ RouteParams p) {
+    constexpr uint32_t kIdx = NV - 1;           // the key bits that hold the place in the lane
+    __shared__ double sv[kRouteWarps][NV / 4 * 32];   // for the whole warp on one row
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, sub = lane & 7;
+    const int64_t t = ((int64_t)blockIdx.x * kRouteWarps + warp) * 4 + (lane >> 3);
+    const int64_t tw = ((int64_t)blockIdx.x * kRouteWarps + warp) * 4;
+    if (tw >= p.T) return;
+    const bool live = t < p.T;                  // the last warp's lanes without a token work on its last one
+    const T* row = static_cast<const T*>(p.x) + (live ? t : p.T - 1) * p.ld;
+    const int per = p.E / 8, e0 = sub * per;
+    float v[NV];
+#pragma unroll
+    for (int q = 0; q < NV; q += 4) {
+        if (q < per) {
+            load4(row + e0 + q, v + q);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) v[q + i] = -INFINITY;
+        }
+    }
+#pragma unroll
+    for (int q = 0; q < NV; ++q) v[q] = selectable<T>(v[q]) ? v[q] : -INFINITY;
+
+    const bool pair = p.group_top == 2;
+    const bool exact = p.bias == nullptr && sizeof(T) == 2;
+    float top = 0.0f, inv_sum = 1.0f;
+    float a = -INFINITY, b = -INFINITY;         // the lane's two best members (the group's, where there are eight)
+    auto member = [&](float m) {
+        b = fmaxf(b, fminf(a, m));
+        a = fmaxf(a, m);
+    };
+    if (!p.sigmoid && (p.bias || pair || !p.renorm)) {
+        top = v[0];
+#pragma unroll
+        for (int q = 1; q < NV; ++q) top = fmaxf(top, v[q]);
+        top = fmax8(top);
+        float sum = 0.0f;
+#pragma unroll
+        for (int q = 0; q < NV; ++q) sum += v[q] == top ? 1.0f : exp_fast(v[q] - top);
+        inv_sum = 1.0f / sum8(sum);
+    }
+    auto score = [&](float x) {
+        return p.sigmoid ? rcp_fast(1.0f + exp_fast(-x)) : (x == top ? 1.0f : exp_fast(x - top)) * inv_sum;
+    };
+    if (p.bias) {
+#pragma unroll
+        for (int q = 0; q < NV; q += 4) {
+            if (q >= per) continue;
+            float bias[4];
+            load4(p.bias + e0 + q, bias);
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                v[q + i] = v[q + i] > -INFINITY && bias[i] > kMasked ? score(v[q + i]) + bias[i] : -INFINITY;
+        }
+    }
+    const float err2 = p.sigmoid ? 6e-7f : 4.2e-6f * inv_sum;   // as above
+    if (p.G > 1) {
+        if (pair && !p.bias) {
+#pragma unroll
+            for (int q = 0; q < NV; ++q) member(v[q] == -INFINITY ? v[q] : score(v[q]));
+        } else {
+#pragma unroll
+            for (int q = 0; q < NV; ++q) member(v[q]);
+        }
+        if (pair && b != -INFINITY) a += b;
+        const uint32_t mine = a != -INFINITY ? order_key(a) : 0u;
+        int rank = 0;
+        bool near = false;
+#pragma unroll
+        for (int h = 1; h < 8; ++h) {
+            const uint32_t other = __shfl_xor_sync(kFull, mine, h);
+            rank += other > mine || (other == mine && (sub ^ h) < sub) ? 1 : 0;
+        }
+        bool stay = mine != 0 && rank < p.kept;
+        const uint32_t worst = ~max8(stay ? ~mine : 0u), other = max8(stay ? 0u : mine);
+        if (other != 0) {
+            const float lo = key_value(worst), hi = key_value(other);
+            near = (p.bias || pair) && !(lo - hi > 2.0f * err2 + 6e-7f * fmaxf(fabsf(lo), fabsf(hi)));
+        }
+        const unsigned bad = __ballot_sync(kFull, near);
+        if (bad != 0)
+            for (int r = 0; r < 4; ++r) {
+                if ((bad >> (8 * r) & 255) == 0 || tw + r >= p.T) continue;
+                const uint32_t mask = groups_f64<T, NV / 4>(p, static_cast<const T*>(p.x) + (tw + r) * p.ld, sv[warp], lane);
+                if (lane >> 3 == r) stay = mask >> sub & 1;
+            }
+#pragma unroll
+        for (int q = 0; q < NV; ++q) v[q] = stay ? v[q] : -INFINITY;
+    }
+
+    uint32_t key[NV];
+#pragma unroll
+    for (int q = 0; q < NV; ++q) key[q] = v[q] == -INFINITY ? 0u : (order_key(v[q]) & ~kIdx) | (kIdx - q);
+    top8<NV>(key);
+    // rounds: the largest value, then the lowest lane (in the bits of the place), whose first key is popped
+    uint32_t val = 0;                           // lane l: the value bits of the l-th choice
+    int my_i = -1, extra = -1, n = 0;
+    auto best = [&]() { return max8(key[0] != 0 ? (key[0] & ~kIdx) | (7 - sub) : 0u); };
+    auto pop = [&](uint32_t m) {                // the expert of the winner
+        const int wl = 7 - (int)(m & kIdx);
+        const int e = __shfl_sync(kFull, e0 + (int)(kIdx - (key[0] & kIdx)), (lane & 24) | wl);
+        if (m != 0 && sub == wl) {
+#pragma unroll
+            for (int q = 0; q < 7; ++q) key[q] = key[q + 1];
+            key[7] = 0;
+        }
+        return e;
+    };
+    for (int l = 0; l < p.k; ++l) {             // (no early end: the four tokens go together)
+        const uint32_t m = best();
+        const int e = pop(m);
+        n += m != 0 ? 1 : 0;
+        if (sub == l && m != 0) {
+            val = m & ~kIdx;
+            my_i = e;
+        }
+    }
+    if (!exact) {
+        auto close = [&](uint32_t x, uint32_t y) {   // value bits that follow each other
+            const float hi = key_value(x), lo = key_value(y);
+            return p.bias ? !(hi - lo > err2 + (NV * 1.2e-7f + 3e-7f) * fmaxf(fabsf(hi), fabsf(lo))) : !(hi > lo);
+        };
+        const uint32_t out = best();            // the first that was left
+        uint32_t next = __shfl_down_sync(kFull, val, 1, 8);
+        if (sub == n - 1) next = out & ~kIdx;
+        const bool near = sub < n && next != 0 && close(val, next);
+        const unsigned bad = __ballot_sync(kFull, near);
+        if (bad != 0) {
+            // the last choice and the first left are close: the latter is a candidate too, if the one behind it is not
+            const bool border = near && sub == n - 1;
+            const bool grow = (__ballot_sync(kFull, border) >> (lane & 24) & 255) != 0;
+            const int e = pop(grow ? out : 0u);
+            const uint32_t after = best() & ~kIdx;
+            bool redo = false;                  // of the token: the whole row in f64
+            if (grow) {
+                extra = e;
+                redo = after != 0 && close(out & ~kIdx, after);
+            }
+            const unsigned again = __ballot_sync(kFull, redo);
+            for (int r = 0; r < 4; ++r) {
+                if ((bad >> (8 * r) & 255) == 0 || tw + r >= p.T) continue;
+                const T* rr = static_cast<const T*>(p.x) + (tw + r) * p.ld;
+                int got;
+                if ((again >> (8 * r) & 255) != 0) {
+                    got = route_row_f64<T, NV / 4>(p, rr, sv[warp], lane);
+                } else {
+                    const int count = __shfl_sync(kFull, n, 8 * r), ex = __shfl_sync(kFull, extra, 8 * r);
+                    const int c = __shfl_sync(kFull, my_i, 8 * r + (lane & 7));
+                    const float tp = __shfl_sync(kFull, top, 8 * r);
+                    got = rank_candidates<T, NV / 4>(p, rr, tp, lane < count ? c : ex, count + (ex >= 0 ? 1 : 0),
+                                                     reinterpret_cast<int*>(sv[warp]), lane);
+                    __syncwarp();
+                }
+                got = __shfl_sync(kFull, got, sub);
+                if (lane >> 3 == r) my_i = got;
+            }
+        }
+    }
+    if (sub >= p.k) my_i = -1;
+
+    const float xs = my_i >= 0 ? to_f32<T>(row[my_i]) : -INFINITY;
+    float e = 0.0f;
+    if (p.sigmoid) e = rcp_fast(1.0f + expf(-xs));
+    else if (!p.renorm) e = my_i < 0 ? 0.0f : (xs == top ? 1.0f : expf(xs - top)) * inv_sum;
+    if (p.renorm) {
+        float sum = p.sigmoid ? sum8(e) : 0.0f;
+        if (!__all_sync(kFull, sum > 1e-30f)) {   // as above; a token whose sum stands keeps it
+            const float mx = fmax8(xs);
+            const float f = my_i < 0 ? 0.0f : xs == mx ? 1.0f : expf(xs - mx);
+            const float g = sum8(f);
+            if (!(sum > 1e-30f)) {
+                e = f;
+                sum = g;
+            }
+        }
+        e = sum > 0.0f ? e * rcp_fast(sum) : 0.0f;
+    }
+    if (live && sub < p.k) {
+        p.idx[t * p.k + sub] = my_i;
+        p.w[t * p.k + sub] = e * p.scale;
+    }
+}
+
+// Tokens from which four share a warp.
+constexpr int64_t kManyTokens = 4096;
+
+template <typename T, int NV>
+cudaError_t launch_many(const RouteParams& p, cudaStream_t st) {
+    route_many_kernel<T, NV><<<(unsigned)((p.T + 4 * kRouteWarps - 1) / (4 * kRouteWarps)), kRouteWarps * 32, 0, st>>>(p);
+    return cudaGetLastError();
+}
+
+// True (and launched) where the shape fits: 8 parts of a multiple of 4 experts,
+// at most 256 in all, no groups or eight, rows that allow loads of four.
+template <typename T>
+bool try_many(RouteParams p, cudaStream_t st, cudaError_t* err) {
+    const int per = p.E / 8;
+    if (p.T < kManyTokens || p.E % 32 != 0 || p.E > 256 || p.k > 8 || (p.G != 1 && p.G != 8) ||
+        reinterpret_cast<uintptr_t>(p.x) % (4 * sizeof(T)) != 0 || p.ld % 4 != 0 ||
+        reinterpret_cast<uintptr_t>(p.bias) % 16 != 0)
+        return false;
+    p.vec = p.vec_bias = 0;   // (for the whole-warp pass)
+    *err = per <= 8 ? launch_many<T, 8>(p, st) : per <= 16 ? launch_many<T, 16>(p, st) : launch_many<T, 32>(p, st);
+    return true;
+}
+
 template <typename T, int NV>
 cudaError_t launch_nv(RouteParams p, cudaStream_t st) {
     constexpr int kBytes = NV * (int)sizeof(T);
@@ -507,6 +819,8 @@ cudaError_t launch_nv(RouteParams p, cudaStream_t st) {
 
 template <typename T>
 cudaError_t launch_typed(const RouteParams& p, cudaStream_t st) {
+    cudaError_t err;
+    if (try_many<T>(p, st, &err)) return err;
     if (p.E <= 32) return launch_nv<T, 1>(p, st);
     if (p.E <= 64) return launch_nv<T, 2>(p, st);
     if (p.E <= 128) return launch_nv<T, 4>(p, st);

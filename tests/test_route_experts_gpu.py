@@ -193,6 +193,50 @@ def test_default_is_the_layers_gate(gpu):
     torch.testing.assert_close(w, layer.w[: cfg.T], rtol=2e-6, atol=0)
 
 
+def special_rows(E, dtype):
+    """Ties, close neighbours, masked and infinite logits, and ordinary rows between them."""
+    x = logits_of(4105, E, torch.float32, E, spread=2.0)
+    g = torch.Generator().manual_seed(E)
+    x[10:200] = torch.randint(-2, 3, (190, E), generator=g).float().cuda()
+    x[200:230] = 0.0
+    x[230:260] = (torch.randint(0, 40, (30, E), generator=g).float() * 2.0 ** -22 + 1.0).cuda()
+    x[260:300, ::2] = -math.inf
+    x[300:320] = math.nan
+    x[320:330, 1:] = -1e20
+    x[330] = torch.finfo(torch.float32).min
+    x[331, 3] = math.inf
+    x[332, [3, E - 1]] = math.inf
+    x[333] = -300.0 + torch.arange(E).cuda() * 0.25
+    x[4096:] = x[230:239]
+    return x.to(dtype)
+
+
+@pytest.mark.parametrize("E, groups, kept", [(8, 1, 1), (32, 1, 1), (64, 1, 1), (64, 8, 2), (96, 8, 5), (128, 1, 1), (160, 8, 3),
+                                             (256, 1, 1), (256, 8, 4)])
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
+def test_large_batches_equal_small_ones(gpu, E, groups, kept, score, dtype):
+    """Batches large enough for four tokens a warp choose as the small ones do (which the tests above hold to the definition)."""
+    x = special_rows(E, dtype)
+    tied = torch.round(torch.randn(E, generator=torch.Generator().manual_seed(9)) * 2) / 16
+    for bias in (None, tied.cuda(), (0.1 * torch.randn(E, generator=torch.Generator().manual_seed(1))).cuda()):
+        for top in (1, 2):
+            for k in (1, min(E, 6), 8):
+                kw = dict(score=score, bias=bias, groups=groups, kept_groups=kept, group_top=top, renormalise=top == 1,
+                          scale=2.5)
+                idx, w = sm.route_experts(x, k, **kw)
+                parts = [sm.route_experts(x[i: i + 1500], k, **kw) for i in range(0, x.shape[0], 1500)]
+                assert torch.equal(idx, torch.cat([p[0] for p in parts]))
+                torch.testing.assert_close(w, torch.cat([p[1] for p in parts]), rtol=2 * REL[top == 1], atol=1e-37)
+    # and a sample of the rows against the definition
+    rows = torch.tensor([0, 1, 10, 50, 200, 230, 231, 259, 260, 300, 320, 330, 331, 332, 333, 4095, 4100, 4104])
+    bias = (0.1 * torch.randn(E, generator=torch.Generator().manual_seed(1))).cuda()
+    idx, w = sm.route_experts(x, min(E, 8), score=score, bias=bias, groups=groups, kept_groups=kept, group_top=2)
+    ri, rw = route_ref(x[rows.cuda()], min(E, 8), score, bias, groups, kept, 2, True, 1.0)
+    np.testing.assert_array_equal(idx[rows.cuda()].cpu().numpy(), ri)
+    np.testing.assert_allclose(w[rows.cuda()].cpu().double().numpy(), rw, rtol=REL[True], atol=1e-37)
+
+
 def test_streams_and_graphs(gpu):
     x = logits_of(500, 256, torch.float32, 11)
     kw = dict(score="sigmoid", groups=8, kept_groups=4, group_top=2, bias=torch.zeros(256, device=gpu), scale=2.5)
