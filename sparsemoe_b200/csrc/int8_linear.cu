@@ -95,38 +95,42 @@ template <typename T16> struct In8_16 {
 template <> struct In8<__half> : In8_16<__half> {};
 template <> struct In8<__nv_bfloat16> : In8_16<__nv_bfloat16> {};
 
-// round-half-even of the exact x / s next to a border n + 1/2: the sign of
-// x - (n + 1/2) s decides, which one fma gives exactly.
-__device__ __noinline__ int quant_border(float x, float s, float inv) {
-    const float r = x * inv, n = rintf(r);
-    if (fabsf(r - n) <= 0.4999f) return (int)n;
-    const float lo = floorf(r), e = fmaf(-(lo + 0.5f), s, x);
-    return (int)(e > 0.0f ? lo + 1.0f : e < 0.0f ? lo : 2.0f * rintf(0.5f * (lo + 0.5f)));
-}
-
-// Codes of eight values.  x * (1/s) is within 127 * 2^-23 of the quotient, so
-// only values that close to a border need more than its nearest integer, which
-// one fma leaves in the low bits of 1.5 * 2^23 + n.  Rows whose scale is so
-// small or large that 1/s or the border's fma leaves the normal range are
-// scaled by a power of two first (pre != 1), which changes no quotient; a
+// Codes of eight values: round-half-even of the exact x / s.  x * (1/s) is within
+// 127 * 2^-23 of the quotient, so its nearest integer n (which one fma leaves in
+// the low bits of 1.5 * 2^23 + n) is right or the other neighbour of a border.
+// e = x - n s, exact in one fma (both are multiples of the smaller of their last
+// places, and |e| <= s), tells: past s / 2 the neighbour is nearer, at s / 2 the
+// even one is taken.  bf16 rows meet a border in most warps (x / s is 127 times a
+// quotient of two 8-bit numbers), so the correction is a few instructions, not a
+// division.  Tiny and huge rows are scaled by a power of two first (pre != 1),
+// which changes no quotient and keeps the arithmetic in the normal range; a
 // subnormal scale has few bits, so there the codes are clamped.
-__device__ __forceinline__ uint2 quant8(const float (&f)[8], float s, float inv, float pre) {
+__device__ __forceinline__ uint2 quant8(float (&f)[8], float s, float inv, float pre) {
     constexpr float kMagic = 12582912.0f;
     uint32_t t[8];
-    float off = 0.0f;
+    float e[8], far = 0.0f;
+    if (pre != 1.0f)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) f[i] *= pre;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
         const float m = fmaf(f[i], inv, kMagic);
-        off = fmaxf(off, fabsf(fmaf(f[i], inv, kMagic - m)));
+        e[i] = fmaf(kMagic - m, s, f[i]);
+        far = fmaxf(far, fabsf(e[i]));
         t[i] = __float_as_uint(m);
     }
-    if (pre != 1.0f || off > 0.49995f) {
+    const float half = 0.5f * s;
+    if (far >= half) {
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-            const int q = quant_border(f[i] * pre, s, pre == 1.0f ? inv : __fdiv_rn(1.0f, s));
-            t[i] = (uint32_t)(pre == 1.0f ? q : max(-127, min(127, q)));
+            const float ae = fabsf(e[i]);
+            if (ae > half || (ae == half && (t[i] & 1u))) t[i] += e[i] > 0.0f ? 1u : 0xFFFFFFFFu;
         }
     }
+    if (pre != 1.0f)
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            t[i] = (uint32_t)max(-127, min(127, (int)(t[i] - __float_as_uint(kMagic))));
     uint2 w;
     w.x = __byte_perm(__byte_perm(t[0], t[1], 0x0040), __byte_perm(t[2], t[3], 0x0040), 0x5410);
     w.y = __byte_perm(__byte_perm(t[4], t[5], 0x0040), __byte_perm(t[6], t[7], 0x0040), 0x5410);
@@ -148,7 +152,7 @@ struct RowScale {
         ss = s * pre;
         inv = bad ? 0.0f : __fdiv_rn(1.0f, ss);
     }
-    __device__ __forceinline__ uint2 codes(const float (&f)[8]) const {
+    __device__ __forceinline__ uint2 codes(float (&f)[8]) const {
         return bad ? make_uint2(0u, 0u) : quant8(f, ss, inv, pre);
     }
 };
