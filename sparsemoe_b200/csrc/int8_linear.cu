@@ -172,7 +172,7 @@ __device__ __forceinline__ float silu(float g) { return g / (1.0f + __expf(-g));
 // kPair (T = float): x holds gate values, the up values start `up` elements
 // behind them, and the row that is quantised is up * gate / (1 + exp(-gate)).
 template <typename T, int TPR, bool kPair>
-__global__ void __launch_bounds__(256) quantize_tokens_kernel(const T* __restrict__ x, int64_t rows, int K, int64_t ldx,
+__global__ void __launch_bounds__(256, sizeof(T) == 2 ? 8 : 5) quantize_tokens_kernel(const T* __restrict__ x, int64_t rows, int K, int64_t ldx,
                                                              int64_t up, int8_t* __restrict__ q, int64_t ldq,
                                                              float* __restrict__ scale, int vec) {
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
@@ -1197,10 +1197,11 @@ template <typename T, bool kPair>
 cudaError_t launch_quantize_typed(const T* x, int64_t rows, int K, int64_t ldx, int64_t up, int8_t* q, int64_t ldq,
                                   float* s, bool pdl, cudaStream_t st) {
     const int vec = aligned(x, 16) && (ldx * (int64_t)sizeof(T)) % 16 == 0;
-    // a warp a row up to 1024 elements, else as many threads as hold the row in registers
-    const int tpr = K <= 1024 ? 32 : K <= 4096 ? 128 : 256;
+    // as many threads a row as hold it in registers, four vectors of eight each
+    const int tpr = K <= 1024 ? 32 : K <= 2048 ? 64 : K <= 4096 ? 128 : 256;
     const int64_t blocks = (rows * tpr + 255) / 256;
     auto kern = tpr == 32    ? quantize_tokens_kernel<T, 32, kPair>
+                : tpr == 64  ? quantize_tokens_kernel<T, 64, kPair>
                 : tpr == 128 ? quantize_tokens_kernel<T, 128, kPair>
                              : quantize_tokens_kernel<T, 256, kPair>;
     return launch_ex(kern, (unsigned)blocks, 256u, 0, 1, pdl, st, x, rows, K, ldx, up, q, ldq, s, vec);
