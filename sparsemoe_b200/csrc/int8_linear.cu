@@ -274,14 +274,18 @@ struct LinearParams {
     uint32_t idesc;
 };
 
-template <int kBN>
+// Eight columns of the parts of a split tile: 128 rows x 8 s32, and 16 bytes that
+// put consecutive units into different banks.
+constexpr int kUnitBytes = kBM * 32 + 16;
+
+template <int kBN, bool kPair>
 struct LinearCfg {
-    static constexpr int kStages = 4;
+    static constexpr int kStages = kPair ? 6 : 4;
     static constexpr int kABytes = kBM * kBK;
-    static constexpr int kBBytes = kBN * kBK;
+    static constexpr int kBBytes = (kPair ? kBN / 2 : kBN) * kBK;   // a pair's CTAs hold half of the columns each
     static constexpr int kStageBytes = kABytes + kBBytes;
     // split sums (kBN = 128 only), or a staged chunk of 32 rows x 64 bytes for each epilogue warp
-    static constexpr int kRecvBytes = kBN == 128 ? kBM * kBN * 4 : 8 * 2048;
+    static constexpr int kRecvBytes = kBN == 128 ? kBN / 8 * kUnitBytes : 8 * 2048;
     static constexpr size_t kSmem = 1024 + (size_t)kStages * kStageBytes + kRecvBytes + 256;
 };
 
@@ -320,6 +324,50 @@ template <int kPending> __device__ __forceinline__ void bulk_wait_read() {
     asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(kPending) : "memory");
 }
 __device__ __forceinline__ void fence_async_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+
+// ---- CTA pairs (tcgen05 cta_group::2) ----
+__device__ __forceinline__ void tmem_alloc2(uint32_t* dst_smem, uint32_t ncols) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(dst_smem)), "r"(ncols)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void tmem_dealloc2(uint32_t taddr, uint32_t ncols) {
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(taddr), "r"(ncols) : "memory");
+}
+__device__ __forceinline__ void mma_i8_ss2(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
+                                           uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::i8 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
+        "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+// Arrives on this barrier of both CTAs when the tcgen05 operations issued so far are done.
+__device__ __forceinline__ void mma_commit2(uint64_t* bar) {
+    asm volatile(
+        "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(
+            smem_u32(bar)),
+        "h"((uint16_t)3)
+        : "memory");
+}
+// A load into this CTA whose bytes count on a barrier of either CTA of the pair.
+__device__ __forceinline__ void tma_load_2d_pair(void* dst, const void* tmap, uint32_t bar, int x, int y) {
+    asm volatile(
+        "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes.cta_group::2"
+        " [%0], [%1, {%3, %4}], [%2];" ::"r"(smem_u32(dst)),
+        "l"(reinterpret_cast<uint64_t>(tmap)), "r"(bar), "r"(x), "r"(y)
+        : "memory");
+}
+__device__ __forceinline__ void arrive_cluster(uint32_t bar) {
+    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+// As mbar_wait, for arrivals from the cluster.
+__device__ __forceinline__ bool mbar_wait_cluster(uint64_t* bar, uint32_t parity, int* status, int code) {
+    const bool ok = mbar_wait(bar, parity, status, code);
+    asm volatile("fence.acq_rel.cluster;" ::: "memory");
+    return ok;
+}
 
 __device__ __forceinline__ float load_as_f32(const void* p, int64_t i, int type) {
     if (type == MOE_TYPE_F32) return static_cast<const float*>(p)[i];
@@ -380,6 +428,13 @@ __device__ __forceinline__ void emit8(const LinearParams& p, int64_t t, bool sec
         for (int i = 0; i < 8; ++i)
             if (i < left) o[i] = (uint16_t)(u[i >> 1] >> (16 * (i & 1)));
     }
+}
+
+// One arrival a warp: its reads of the accumulator are done.
+__device__ __forceinline__ void release_acc(uint32_t bar, int lane) {
+    tc_fence_before();
+    __syncwarp();
+    if (lane == 0) arrive_cluster(bar);
 }
 
 template <int kC> __device__ __forceinline__ void tmem_ld(uint32_t taddr, uint32_t (&r)[kC]) {
@@ -447,7 +502,7 @@ struct StagedEpilogue {
     template <bool kHalf>
     static __device__ __forceinline__ void run(const LinearParams& p, const CUtensorMap* map, int64_t base,
                                                uint8_t* stage, uint32_t taddr, float st, const float* sc, const float* sb, int row0,
-                                               int col0, uint64_t* release, int lane) {
+                                               int col0, uint32_t release, int lane) {
         using T16 = typename std::conditional<kHalf, __half, __nv_bfloat16>::type;
         uint4* const mine = reinterpret_cast<uint4*>(stage + lane * 64);
         const int sw = (lane >> 1) & 3;
@@ -461,7 +516,7 @@ struct StagedEpilogue {
             tmem_ld<kC>(taddr + n, a);
             if constexpr (kSwiglu) tmem_ld<kC>(taddr + kOutN + n, b);
             tmem_wait_ld();
-            if (n + kC == kCols) { tc_fence_before(); mbar_arrive(release); }
+            if (n + kC == kCols) release_acc(release, lane);
             if (row0 >= p.T || col0 + n >= p.N) continue;   // the same for the whole warp
             uint4 r[4];
             if (add) {
@@ -547,12 +602,18 @@ struct StagedEpilogue {
 // split > 1 (kBN = 128): a cluster shares one tile, each CTA a part of K; the
 // s32 parts meet in shared memory, where CTA r adds up the r-th slice of the
 // columns -- integer sums, so the split changes no bit of the result.
-template <int kBN, bool kSwiglu>
+// kPair (kBN = 256): two CTAs on a tile of 256 tokens, each with its 128 tokens
+// and half of the columns in shared memory; the first one issues the MMAs
+// (cta_group::2, M = 256) and every CTA drains its own 128 rows.  A K block then
+// brings 32 KB into an SM for the 48 KB of a CTA alone, which is what bounds the
+// latter: an SM takes in 64 B/clk, 768 clocks for 512 clocks of MMA.
+template <int kBN, bool kSwiglu, bool kPair>
 __global__ void __launch_bounds__(kThreads, 1)
     linear_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB0,
                   const __grid_constant__ CUtensorMap tmB1, const __grid_constant__ CUtensorMap tmO0,
                   const __grid_constant__ CUtensorMap tmO1, const __grid_constant__ LinearParams p) {
-    using C = LinearCfg<kBN>;
+    using C = LinearCfg<kBN, kPair>;
+    static_assert(!kPair || kBN == 256, "a pair shares 256 columns");
     static_assert(!kSwiglu || kBN == 256, "the gate and up halves are whole 128-column boxes");
     constexpr int kOutN = kSwiglu ? kBN / 2 : kBN;
     constexpr int kTmemCols = 2 * kBN;
@@ -576,33 +637,53 @@ __global__ void __launch_bounds__(kThreads, 1)
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < C::kStages; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], 1); }
-        for (int a = 0; a < 2; ++a) { mbar_init(&tfull[a], 1); mbar_init(&tempty[a], kEpiThreads); }
+        for (int a = 0; a < 2; ++a) { mbar_init(&tfull[a], 1); mbar_init(&tempty[a], (kPair ? 2 : 1) * kEpiThreads / 32); }
         fence_mbar_init();
         tma_prefetch_desc(&tmA);
         tma_prefetch_desc(&tmB0);
         tma_prefetch_desc(&tmB1);
     }
     if (warp == 1) {
-        tmem_alloc(tmem_slot, kTmemCols);
-        tmem_relinquish();
+        if (kPair) {
+            tmem_alloc2(tmem_slot, kTmemCols);
+        } else {
+            tmem_alloc(tmem_slot, kTmemCols);
+            tmem_relinquish();
+        }
     }
     tc_fence_before();
     __syncthreads();
+    if (kPair) {   // the barriers of both CTAs stand before anything arrives on them
+        cluster_arrive();
+        cluster_wait();
+    }
     tc_fence_after();
     const uint32_t tmem_base = *tmem_slot;
     // first phase of the cluster barrier: every CTA has started before anything is sent to it
     if (p.split > 1) cluster_arrive();
 
     const int total = p.m_tiles * p.n_tiles;
-    const int tile0 = (int)blockIdx.x / p.split, step = (int)gridDim.x / p.split;
+    const int ctas = kPair ? 2 : p.split;   // of a tile
+    const int tile0 = (int)blockIdx.x / ctas, step = (int)gridDim.x / ctas;
     // this CTA's part of K, in blocks (the host leaves no part empty)
-    const int kb0 = (int)((int64_t)p.kblocks * rank / p.split);
-    const int kb1 = (int)((int64_t)p.kblocks * (rank + 1) / p.split);
-    const uint32_t stage_bytes = (uint32_t)(p.a_rows * kBK + C::kBBytes);
+    const int part = kPair ? 0 : rank;
+    const int kb0 = (int)((int64_t)p.kblocks * part / p.split);
+    const int kb1 = (int)((int64_t)p.kblocks * (part + 1) / p.split);
+    const uint32_t stage_bytes = (kPair ? 2u : 1u) * (uint32_t)(p.a_rows * kBK + C::kBBytes);
+    const bool leads = !kPair || rank == 0;
+    // tile row m of the tokens: this CTA's 128
+    auto token_row = [&](int m) { return (kPair ? 2 * m + rank : m) * kBM; };
 
     if (warp == 0) {
         if (lane == 0) {
             // ---------------- TMA producer ----------------
+            auto expect = [&](int s) {
+                if (leads) mbar_arrive_expect_tx(&full[s], stage_bytes);   // the loads of both CTAs
+            };
+            auto load = [&](void* dst, const CUtensorMap* map, int s, int x, int y) {
+                if (kPair) tma_load_2d_pair(dst, map, mapa(smem_u32(&full[s]), 0), x, y);
+                else tma_load_2d(dst, map, &full[s], x, y);
+            };
             auto load_b = [&](int s, int n, int kb) {
                 uint8_t* dst = sB + s * C::kBBytes;
                 const int k0 = kb * kBK;
@@ -610,19 +691,22 @@ __global__ void __launch_bounds__(kThreads, 1)
                 const CUtensorMap* b0 = second ? &tmB1 : &tmB0;
                 const CUtensorMap* b1 = kSwiglu || second ? &tmB1 : &tmB0;
                 const int col = (second ? n - p.n0_tiles : n) * kOutN;
-                if (p.b_nk) {   // a box is kBN / 2 rows of N x 128 of K
-                    tma_load_2d(dst, b0, &full[s], k0, col);
-                    tma_load_2d(dst + C::kBBytes / 2, b1, &full[s], k0, kSwiglu ? col : col + kBN / 2);
-                } else {        // a box is 128 rows of K x 128 of N
-                    tma_load_2d(dst, b0, &full[s], col, k0);
-                    if (kBN == 256) tma_load_2d(dst + C::kBBytes / 2, b1, &full[s], kSwiglu ? col : col + 128, k0);
+                if (kPair) {    // this CTA's half, one box (gate or up columns of the fused pass)
+                    const int mine = kSwiglu ? col : col + rank * 128;
+                    load(dst, rank == 0 ? b0 : b1, s, p.b_nk ? k0 : mine, p.b_nk ? mine : k0);
+                } else if (p.b_nk) {   // a box is kBN / 2 rows of N x 128 of K
+                    load(dst, b0, s, k0, col);
+                    load(dst + C::kBBytes / 2, b1, s, k0, kSwiglu ? col : col + kBN / 2);
+                } else {               // a box is 128 rows of K x 128 of N
+                    load(dst, b0, s, col, k0);
+                    if (kBN == 256) load(dst + C::kBBytes / 2, b1, s, kSwiglu ? col : col + 128, k0);
                 }
             };
             // the weights of the first stages do not depend on the kernel before this one
             int ahead = 0;
             if (p.pdl) {
                 for (int kb = kb0; tile0 < total && kb < kb1 && ahead < C::kStages; ++kb, ++ahead) {
-                    mbar_arrive_expect_tx(&full[ahead], stage_bytes);
+                    expect(ahead);
                     load_b(ahead, tile0 / p.m_tiles, kb);
                 }
                 pdl_wait();
@@ -636,24 +720,24 @@ __global__ void __launch_bounds__(kThreads, 1)
                         --ahead;
                     } else {
                         if (!mbar_wait(&empty[s], ph ^ 1u, status, kDevErrTimeout)) goto producer_done;
-                        mbar_arrive_expect_tx(&full[s], stage_bytes);
+                        expect(s);
                         load_b(s, n, kb);
                     }
-                    tma_load_2d(sA + s * C::kABytes, &tmA, &full[s], kb * kBK, m * kBM);
+                    load(sA + s * C::kABytes, &tmA, s, kb * kBK, token_row(m));
                     if (++s == C::kStages) { s = 0; ph ^= 1u; }
                 }
             }
         producer_done:;
         }
     } else if (warp == 1) {
-        if (lane == 0) {
-            // ---------------- MMA issuer ----------------
+        if (lane == 0 && leads) {
+            // ---------------- MMA issuer (of a pair, its first CTA's) ----------------
             int s = 0;
             uint32_t ph = 0;
             int acc = 0;
             uint32_t aph = 0;
             for (int t = tile0; t < total; t += step) {
-                if (!mbar_wait(&tempty[acc], aph ^ 1u, status, kDevErrTimeout)) break;
+                if (!mbar_wait_cluster(&tempty[acc], aph ^ 1u, status, kDevErrTimeout)) break;
                 tc_fence_after();
                 const uint32_t d_tmem = tmem_base + acc * kBN;
                 bool ok = true;
@@ -669,13 +753,16 @@ __global__ void __launch_bounds__(kThreads, 1)
                         const uint64_t adesc = smem_desc_sw128(a_base + kk * 32, 16, 1024);
                         const uint64_t bdesc = p.b_nk ? smem_desc_sw128(b_base + kk * 32, 16, 1024)
                                                       : smem_desc_sw128(b_base + kk * 32 * 128, kBK * 128, 1024);
-                        mma_i8_ss(d_tmem, adesc, bdesc, p.idesc, (kb != kb0 || kk != 0) ? 1u : 0u);
+                        if (kPair) mma_i8_ss2(d_tmem, adesc, bdesc, p.idesc, (kb != kb0 || kk != 0) ? 1u : 0u);
+                        else mma_i8_ss(d_tmem, adesc, bdesc, p.idesc, (kb != kb0 || kk != 0) ? 1u : 0u);
                     }
-                    mma_commit(&empty[s]);
+                    if (kPair) mma_commit2(&empty[s]);
+                    else mma_commit(&empty[s]);
                     if (++s == C::kStages) { s = 0; ph ^= 1u; }
                 }
                 if (!ok) break;
-                mma_commit(&tfull[acc]);
+                if (kPair) mma_commit2(&tfull[acc]);
+                else mma_commit(&tfull[acc]);
                 acc ^= 1;
                 if (acc == 0) aph ^= 1u;
             }
@@ -707,8 +794,9 @@ __global__ void __launch_bounds__(kThreads, 1)
             asm volatile("bar.sync 1, 256;" ::: "memory");
             const float* const sc = scales + half * kCols;
             const float* const sb = biases + half * kCols;
-            const int row0 = m * kBM + q * 32, row = row0 + lane;
+            const int row0 = token_row(m) + q * 32, row = row0 + lane;
             const bool valid = row < p.T;
+            const uint32_t release = mapa(smem_u32(&tempty[acc]), kPair ? 0 : rank);
             const float st = valid ? p.s_tok[row] : 0.0f;
             const uint32_t taddr = tmem_base + ((uint32_t)(q * 32) << 16) + acc * kBN + half * kCols;
             if (p.staged && p.residual) StagedEpilogue<kCols, kOutN, false, false>::prefetch_residual(p, row, col0);
@@ -721,13 +809,13 @@ __global__ void __launch_bounds__(kThreads, 1)
                 const int64_t base = second ? p.out1 : 0;
                 if (kSwiglu || p.out_type == MOE_TYPE_F32)
                     StagedEpilogue<kCols, kOutN, kSwiglu, true>::template run<false>(p, map, base, stage, taddr, st, sc, sb,
-                                                                                     row0, col0, &tempty[acc], lane);
+                                                                                     row0, col0, release, lane);
                 else if (p.out_type == MOE_TYPE_F16)
                     StagedEpilogue<kCols, kOutN, false, kSwiglu>::template run<true>(p, map, base, stage, taddr, st, sc, sb,
-                                                                                     row0, col0, &tempty[acc], lane);
+                                                                                     row0, col0, release, lane);
                 else
                     StagedEpilogue<kCols, kOutN, false, kSwiglu>::template run<false>(p, map, base, stage, taddr, st, sc, sb,
-                                                                                      row0, col0, &tempty[acc], lane);
+                                                                                      row0, col0, release, lane);
             } else if (ok && p.split == 1) {
 #pragma unroll 1
                 for (int c = 0; c < kCols; c += 16) {
@@ -735,7 +823,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                     tmem_ld_32x32b_x16(taddr + c, a);
                     if (kSwiglu) tmem_ld_32x32b_x16(taddr + kOutN + c, b);
                     tmem_wait_ld();
-                    if (c + 16 == kCols) { tc_fence_before(); mbar_arrive(&tempty[acc]); }
+                    if (c + 16 == kCols) release_acc(release, lane);
                     if (!valid) continue;
 #pragma unroll
                     for (int h = 0; h < 16; h += 8) {
@@ -764,7 +852,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                                 const int at = u + i;
                                 const uint32_t dst = mapa(
                                     smem_u32(recv) +
-                                        (uint32_t)(((rank * units + at % units) * kBM + q * 32 + lane) * 32),
+                                        (uint32_t)((rank * units + at % units) * kUnitBytes + (q * 32 + lane) * 32),
                                     at / units);
                                 st_cluster4(dst, a[8 * i], a[8 * i + 1], a[8 * i + 2], a[8 * i + 3]);
                                 st_cluster4(dst + 16, a[8 * i + 4], a[8 * i + 5], a[8 * i + 6], a[8 * i + 7]);
@@ -787,31 +875,37 @@ __global__ void __launch_bounds__(kThreads, 1)
             const int n = tile0 / p.m_tiles, m = tile0 - n * p.m_tiles;   // one tile a cluster
             const bool second = n >= p.n0_tiles;
             const int col0 = (second ? n - p.n0_tiles : n) * kOutN;
-            // this CTA's 128 / split columns: consecutive lanes take consecutive columns of a row
-            const int w = kBN / p.split, per = 32 / min(w, 32), rows = min(kBM, p.T - m * kBM);
-            for (int r = (warp - 2) * per + lane / w; warp >= 2 && r < rows; r += 8 * per) {
+            // this CTA's 128 / split columns: consecutive lanes take consecutive units of a row
+            const int units = kBN / 8 / p.split, rows = min(kBM, p.T - m * kBM);
+            for (int i = threadIdx.x - 64; i >= 0 && i < units * rows; i += kEpiThreads) {
+                const int u = i % units, r = i / units, c = (rank * units + u) * 8;
+                if (col0 + c >= p.N) continue;
+                int sum[8] = {};
+                for (int src = 0; src < p.split; ++src) {
+                    const int4* a = reinterpret_cast<const int4*>(recv + (src * units + u) * kUnitBytes + r * 32);
+                    const int4 x = a[0], y = a[1];
+                    sum[0] += x.x; sum[1] += x.y; sum[2] += x.z; sum[3] += x.w;
+                    sum[4] += y.x; sum[5] += y.y; sum[6] += y.z; sum[7] += y.w;
+                }
                 const int64_t row = (int64_t)m * kBM + r;
                 const float st = p.s_tok[row];
-                for (int c = lane % w; c < w; c += 32) {
-                    const int* part = reinterpret_cast<const int*>(recv) + ((c / 8) * kBM + r) * 8 + c % 8;
-                    int sum = 0;
-                    for (int src = 0; src < p.split; ++src) sum += part[src * (w / 8) * kBM * 8];
-                    const int tc = rank * w + c, col = col0 + tc;
-                    if (col >= p.N) break;
-                    float v = (float)sum * st * s_scale[0][tc] + s_bias[0][tc];
-                    if (p.residual) v += load_as_f32(p.residual, row * p.ld_res + col, p.res_type);
-                    const int64_t at = row * p.ld_out + col + (second ? p.out1 : 0);
-                    if (p.out_type == MOE_TYPE_F32) static_cast<float*>(p.out)[at] = v;
-                    else if (p.out_type == MOE_TYPE_F16) static_cast<__half*>(p.out)[at] = __float2half_rn(v);
-                    else static_cast<__nv_bfloat16*>(p.out)[at] = __float2bfloat16_rn(v);
-                }
+                float v[8];
+#pragma unroll
+                for (int j = 0; j < 8; ++j) v[j] = (float)sum[j] * st * s_scale[0][c + j] + s_bias[0][c + j];
+                emit8(p, row, second, col0 + c, v);
             }
         }
+    }
+    if (kPair) {   // the first CTA's MMAs read both CTAs' memory, and both release into the first's barriers
+        __syncwarp();
+        cluster_arrive();
+        cluster_wait();
     }
     __syncthreads();
     if (warp == 1) {
         tc_fence_after();
-        tmem_dealloc(tmem_base, kTmemCols);
+        if (kPair) tmem_dealloc2(tmem_base, kTmemCols);
+        else tmem_dealloc(tmem_base, kTmemCols);
     }
 }
 
@@ -1224,45 +1318,57 @@ cudaError_t launch_quantize(const void* x, int type, int64_t rows, int K, int64_
     }
 }
 
-template <int kBN, bool kSwiglu>
+template <int kBN, bool kSwiglu, bool kPair>
 cudaError_t launch_linear_cfg(const CUtensorMap& a, const CUtensorMap (&b)[2], const CUtensorMap (&o)[2],
                               const LinearParams& p, int clusters, cudaStream_t st) {
-    auto kern = linear_kernel<kBN, kSwiglu>;
+    auto kern = linear_kernel<kBN, kSwiglu, kPair>;
     static SmemAttr attr;
-    const size_t smem = LinearCfg<kBN>::kSmem;
+    const size_t smem = LinearCfg<kBN, kPair>::kSmem;
+    const int ctas = kPair ? 2 : p.split;
     cudaError_t err = ensure_smem(kern, smem, attr);
     if (err != cudaSuccess) return err;
-    return launch_ex(kern, (unsigned)(clusters * p.split), (unsigned)kThreads, smem, p.split, p.pdl != 0, st, a, b[0], b[1],
+    return launch_ex(kern, (unsigned)(clusters * ctas), (unsigned)kThreads, smem, ctas, p.pdl != 0, st, a, b[0], b[1],
                      o[0], o[1], p);
 }
 
-// Tile width and split of K, by the estimated time of a launch: rounds of tiles
-// over the SMs x K blocks of a tile x the time of a block, plus what a launch
-// costs besides.  A block takes 0.34 us at 128 columns and 0.43 at 256 (bound by
-// what an SM takes in, 64 B/clk: 32 and 48 KB); a launch 3.5 us, a split one
-// 5.2 us and up to 2.5 more for sending the parts of 128 tokens.  Clusters of 4
-// and 8 CTAs of this size fit 33 and 15 times at once.  Measured (us, T x K x N,
-// 128 columns split 1 / 2 / 4 / 8, 256 columns): 1x7168x2048 18.6 / 12.7 / 9.4 /
-// 13.9, 20.8; 512x7168x2048 19.6 / 15.9 / 27.2 / 57.6, 23.1; 512x2048x7168 14.2 /
-// 37.3 / 71.5 / 155, 10.8; 512x7168x4096 21.7 / 32.3 / 54.6 / 107, 24.7.
-void pick_tiles(const LinearParams& p, int mats, int num_sms, bool* wide, int* split) {
+// Tiles and split of K, by the estimated time of a launch: rounds of tiles over
+// the SMs x K blocks of a tile x the time of a block, plus what a launch costs
+// besides.  A block takes 0.34 us at 128 x 128, 0.43 at 128 x 256 and 0.36 at 256 x
+// 256 on two SMs (a CTA alone is bound by what an SM takes in, 64 B/clk: 32 and 48
+// KB); a launch 3.5 us, a pair's 4.5, a split one 4.8 and up to 4 more for sending
+// the parts of 128 tokens.  Clusters of 4 and 8 CTAs of this size fit 33 and 15
+// times at once.  Measured (us; T x K x N: pair, 128 x 256, 128 x 128 with K split
+// 1 / 2 / 4 / 8 times): 16x7168x2048 21.5, 21.2, 19.3 / 13.0 / 9.8 / 15.2;
+// 128x7168x2048 22.5, 22.2, 20.3 / 16.3 / 13.6 / 22.5; 512x7168x2048 22.8, 22.8,
+// 20.9 / 17.6 / 28.7 / 59; 512x2048x7168 12.5, 12.1, 16.0 / 41.6 / 75.6 / 155;
+// 1024x2048x2048 12.1, 11.7, 10.8 / 22.4 / 44.5 / 92; 2048x7168x2048 25.0, 26.6,
+// 39.4 / 66 / 109 / 205; 8192x7168x4096 159, 201, 270 / 455 / 791 / 1577.
+struct Tiles {
+    bool wide, pair;
+    int split;
+};
+Tiles pick_tiles(int T, int N, int kblocks, int mats, bool swiglu, int num_sms) {
     auto rounds = [](int64_t n, int64_t at_once) { return (double)((n + at_once - 1) / at_once); };
-    const int64_t tiles128 = (int64_t)p.m_tiles * ((p.N + 127) / 128) * mats;
-    const int64_t tiles256 = (int64_t)p.m_tiles * ((p.N + 255) / 256) * mats;
-    double best = 3.5 + rounds(tiles256, num_sms) * p.kblocks * 0.43;
-    *wide = true;
-    *split = 1;
-    for (int s = 1; s <= kMaxSplit && s <= p.kblocks; s *= 2) {
+    const int64_t m128 = (T + 127) / 128, m256 = (T + 255) / 256;
+    const int64_t n128 = (int64_t)((N + 127) / 128) * mats, n256 = swiglu ? n128 : (int64_t)((N + 255) / 256) * mats;
+    double best = 3.5 + rounds(m128 * n256, num_sms) * kblocks * 0.43;
+    Tiles pick{true, false, 1};
+    const double pair = 4.5 + rounds(m256 * n256, num_sms / 2) * kblocks * 0.36;
+    if (num_sms >= 2 && pair < best) {
+        best = pair;
+        pick.pair = true;
+    }
+    for (int s = 1; !swiglu && s <= kMaxSplit && s <= kblocks; s *= 2) {
         const int64_t at_once = s == 1 ? num_sms : s == 2 ? num_sms / 2 : s == 4 ? num_sms * 33 / 148 : num_sms * 15 / 148;
-        if (at_once < 1 || (s > 1 && tiles128 > at_once)) break;   // a split tile's CTAs run one tile each
-        const double t = (s == 1 ? 3.5 : 5.2 + 2.5 * std::min(p.T, kBM) / kBM) +
-                         rounds(tiles128, at_once) * ((p.kblocks + s - 1) / s) * 0.34;
+        if (at_once < 1 || (s > 1 && m128 * n128 > at_once)) break;   // a split tile's CTAs run one tile each
+        const double t = (s == 1 ? 3.5 : 4.8 + 4.0 * std::min(T, kBM) / kBM) +
+                         rounds(m128 * n128, at_once) * ((kblocks + s - 1) / s) * 0.34;
         if (t < best) {
             best = t;
-            *wide = false;
-            *split = s;
+            pick = Tiles{false, false, s};
         }
     }
+    return pick;
 }
 
 struct Matrix {
@@ -1276,20 +1382,20 @@ struct Matrix {
 // gate and up matrices of h.
 cudaError_t launch_linear(const int8_t* q, int64_t ldq, LinearParams p, const Matrix& w0, const Matrix* w1, bool swiglu,
                           int num_sms, cudaStream_t st) {
-    p.m_tiles = (p.T + kBM - 1) / kBM;
     p.kblocks = (p.K + kBK - 1) / kBK;
-    p.a_rows = p.T >= kBM ? kBM : (p.T + 7) / 8 * 8;
     const int mats = w1 && !swiglu ? 2 : 1;
-    bool wide = swiglu;
-    p.split = 1;
-    if (!swiglu) pick_tiles(p, mats, num_sms, &wide, &p.split);
-    const int bn = wide ? 256 : 128;
+    const Tiles tiles = pick_tiles(p.T, p.N, p.kblocks, mats, swiglu, num_sms);
+    const bool pair = tiles.pair;
+    p.split = tiles.split;
+    p.m_tiles = pair ? (p.T + 2 * kBM - 1) / (2 * kBM) : (p.T + kBM - 1) / kBM;
+    p.a_rows = pair || p.T >= kBM ? kBM : (p.T + 7) / 8 * 8;
+    const int bn = tiles.wide ? 256 : 128;
     const int out_n = swiglu ? bn / 2 : bn;
     p.n0_tiles = (p.N + out_n - 1) / out_n;
     p.n_tiles = p.n0_tiles * mats;
     p.s_ch0 = w0.scale;
     p.s_ch1 = w1 ? w1->scale : w0.scale;
-    p.idesc = idesc_i8(kBM, bn, !p.b_nk);
+    p.idesc = idesc_i8(pair ? 2 * kBM : kBM, bn, !p.b_nk);
     CUtensorMap ta, tb[2], to[2] = {};
     if (!make_map_u8_strided(&ta, q, p.K, p.T, ldq, 128, p.a_rows)) return cudaErrorInvalidValue;
     const Matrix* ws[2] = {&w0, w1 ? w1 : &w0};
@@ -1306,11 +1412,14 @@ cudaError_t launch_linear(const int8_t* q, int64_t ldq, LinearParams p, const Ma
         if (!make_map_u8_strided(&to[i], static_cast<uint8_t*>(p.out) + i * p.out1 * size, (uint64_t)p.N * size, p.T,
                                  (uint64_t)p.ld_out * size, 64, 32))
             return cudaErrorInvalidValue;
-    const int64_t tiles = (int64_t)p.m_tiles * p.n_tiles;
-    const int clusters = (int)(p.split > 1 ? tiles : std::min<int64_t>(tiles, num_sms));
-    if (swiglu) return launch_linear_cfg<256, true>(ta, tb, to, p, clusters, st);
-    if (wide) return launch_linear_cfg<256, false>(ta, tb, to, p, clusters, st);
-    return launch_linear_cfg<128, false>(ta, tb, to, p, clusters, st);
+    const int64_t count = (int64_t)p.m_tiles * p.n_tiles;
+    const int clusters = (int)(p.split > 1 ? count : std::min<int64_t>(count, pair ? num_sms / 2 : num_sms));
+    if (pair)
+        return swiglu ? launch_linear_cfg<256, true, true>(ta, tb, to, p, clusters, st)
+                      : launch_linear_cfg<256, false, true>(ta, tb, to, p, clusters, st);
+    if (swiglu) return launch_linear_cfg<256, true, false>(ta, tb, to, p, clusters, st);
+    if (tiles.wide) return launch_linear_cfg<256, false, false>(ta, tb, to, p, clusters, st);
+    return launch_linear_cfg<128, false, false>(ta, tb, to, p, clusters, st);
 }
 
 // Up to this many tokens small_linear_kernel is used (its MMA has 16 columns).
