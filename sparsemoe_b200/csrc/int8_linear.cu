@@ -919,16 +919,21 @@ __global__ void __launch_bounds__(kThreads, 1)
 // its weights at once, reads its part of the tokens twice (amax, which the
 // cluster exchanges through shared memory, then the codes, written where the MMA
 // reads them) and hands the s32 sums of each slice of the channels to the CTA
-// that adds them up.  What bounds it is latency: of the 6 us that 1 x 7168 x 2048
-// takes the 14.7 MB of weights are 2.2 at the HBM's rate.
+// that adds them up.
+// kSwiglu: the tile is 128 features, their gate and up columns are multiplied in
+// turn (two accumulators), and h = up * silu(gate) is written.
+// What bounds it is latency: an empty launch of it takes 4 us, the exchanges of a
+// cluster 2.5, and the MMAs, 128 clocks each whatever their columns, 0.27 us for
+// each block of K; the 14.7 MB of weights of 1 x 7168 x 2048 (10.2 us) are 2.2 us at
+// the HBM's rate.  Kept short for one reason more: a code path that a CTA runs
+// once is fetched as slowly as it is long (the quantiser of gate / up pairs, 96
+// times silu in line, cost the down product 17 us).
 struct SmallParams {
-    const void* x;             // tokens, rows ld_x elements apart (pair: gate values, up values `up` elements behind)
-    int64_t ld_x, up;
+    const void* x;             // tokens, rows ld_x elements apart
+    int64_t ld_x;
     const float* s_tok;        // codes given: their scales
     int T, K, N;
     int kblocks, split, stages;
-    int tiles0;                // tiles of the first matrix; the others are of the second
-    int64_t out1;
     int b_nk, pdl, vec_x;
     const float* s_ch0;
     const float* s_ch1;
@@ -942,7 +947,7 @@ struct SmallParams {
     uint32_t idesc;
 };
 
-enum SmallInput { kInF32, kInF16, kInBF16, kInPair, kInCodes };
+enum SmallInput { kInF32, kInF16, kInBF16, kInCodes };
 template <int kIn> struct SmallIn { using T = float; };
 template <> struct SmallIn<kInF16> { using T = __half; };
 template <> struct SmallIn<kInBF16> { using T = __nv_bfloat16; };
@@ -953,16 +958,19 @@ constexpr int kSmallThreads = 64 + kSmallWorkers;
 constexpr int kSmallStageBytes = 128 * kBK;
 
 // Shared memory behind the aligned base: weight stages, code blocks, parts, barriers.
-template <int kNT> __host__ __device__ constexpr size_t small_smem(int stages, int blocks, int split) {
-    return 1024 + (size_t)stages * kSmallStageBytes + (size_t)blocks * kNT * kBK + (split > 1 ? 128 * kNT * 4 : 0) + 256;
+template <int kNT> __host__ __device__ constexpr size_t small_smem(int stages, int blocks, int split, int mats) {
+    return 1024 + (size_t)stages * kSmallStageBytes + (size_t)blocks * kNT * kBK +
+           (split > 1 ? (size_t)mats * 128 * kNT * 4 : 0) + 256;
 }
 
-template <int kNT, int kIn>
+template <int kNT, int kIn, bool kSwiglu>
 __global__ void __launch_bounds__(kSmallThreads, 2)
     small_linear_kernel(const __grid_constant__ CUtensorMap tmW0, const __grid_constant__ CUtensorMap tmW1,
                         const __grid_constant__ SmallParams p) {
     using T = typename SmallIn<kIn>::T;
-    constexpr int kTmemCols = kNT < 32 ? 32 : kNT;
+    constexpr int kMats = kSwiglu ? 2 : 1;
+    constexpr int kTmemCols = 32;
+    static_assert(kMats * kNT <= kTmemCols, "one accumulator for each matrix");
     extern __shared__ uint8_t smem_raw[];
     __shared__ uint32_t s_amax[kMaxSplit][kNT];   // [source CTA][token]: bits of the largest magnitude
     __shared__ float s_tok[kNT];
@@ -975,7 +983,7 @@ __global__ void __launch_bounds__(kSmallThreads, 2)
     uint8_t* const sW = smem;
     uint8_t* const sQ = sW + p.stages * kSmallStageBytes;
     uint8_t* const recv = sQ + (size_t)max_blocks * kNT * kBK;
-    uint64_t* const full = reinterpret_cast<uint64_t*>(recv + (p.split > 1 ? 128 * kNT * 4 : 0));
+    uint64_t* const full = reinterpret_cast<uint64_t*>(recv + (p.split > 1 ? kMats * 128 * kNT * 4 : 0));
     uint64_t* const empty = full + 8;
     uint64_t* const ready = empty + 8;   // the codes are written
     uint64_t* const tfull = ready + 1;
@@ -1003,21 +1011,21 @@ __global__ void __launch_bounds__(kSmallThreads, 2)
     const bool split = p.split > 1;
     if (split) cluster_arrive();   // phase 1: every CTA has started
 
-    const int tile = (int)blockIdx.x / p.split;
-    const bool second = tile >= p.tiles0;
-    const int col0 = (second ? tile - p.tiles0 : tile) * 128;
+    const int col0 = (int)blockIdx.x / p.split * 128;
+    const int loads = (kb1 - kb0) * kMats;   // weight boxes of this CTA: block by block, gate before up
 
     if (warp == 0) {
         // ---------------- TMA producer ----------------
-        const CUtensorMap* map = second ? &tmW1 : &tmW0;
-        auto load = [&](int s, int kb) {
+        auto load = [&](int s, int i) {
+            const CUtensorMap* map = kSwiglu && (i & 1) ? &tmW1 : &tmW0;
+            const int k = (kb0 + i / kMats) * kBK;
             mbar_arrive_expect_tx(&full[s], kSmallStageBytes);
-            if (p.b_nk) tma_load_2d(sW + s * kSmallStageBytes, map, &full[s], kb * kBK, col0);
-            else tma_load_2d(sW + s * kSmallStageBytes, map, &full[s], col0, kb * kBK);
+            if (p.b_nk) tma_load_2d(sW + s * kSmallStageBytes, map, &full[s], k, col0);
+            else tma_load_2d(sW + s * kSmallStageBytes, map, &full[s], col0, k);
         };
-        const int first = min(p.stages, kb1 - kb0);
+        const int first = min(p.stages, loads);
         if (lane == 0)
-            for (int i = 0; i < first; ++i) load(i, kb0 + i);
+            for (int i = 0; i < first; ++i) load(i, i);
         __syncwarp();
         if (split) {   // phases 1 and 2, before any wait that the other warps' progress ends
             cluster_wait();
@@ -1027,9 +1035,9 @@ __global__ void __launch_bounds__(kSmallThreads, 2)
         if (lane == 0) {
             int s = 0;
             uint32_t ph = 0;
-            for (int kb = kb0 + first; kb < kb1; ++kb) {
+            for (int i = first; i < loads; ++i) {
                 if (!mbar_wait(&empty[s], ph, status, kDevErrTimeout)) break;
-                load(s, kb);
+                load(s, i);
                 if (++s == p.stages) { s = 0; ph ^= 1u; }
             }
         }
@@ -1044,18 +1052,19 @@ __global__ void __launch_bounds__(kSmallThreads, 2)
             bool ok = mbar_wait(ready, 0, status, kDevErrTimeout);
             int s = 0;
             uint32_t ph = 0;
-            for (int kb = kb0; ok && kb < kb1; ++kb) {
+            for (int i = 0; ok && i < loads; ++i) {
                 if (!mbar_wait(&full[s], ph, status, kDevErrTimeout)) { ok = false; break; }
                 tc_fence_after();
+                const uint32_t d_tmem = tmem_base + (kSwiglu ? (i & 1) * kNT : 0);
                 const uint32_t w_base = smem_u32(sW + s * kSmallStageBytes);
-                const uint32_t q_base = smem_u32(sQ + (size_t)(kb - kb0) * kNT * kBK);
+                const uint32_t q_base = smem_u32(sQ + (size_t)(i / kMats) * kNT * kBK);
 #pragma unroll
                 for (int kk = 0; kk < kBK / 32; ++kk) {
                     // weights [N, K]: K-major rows; [K, N]: MN-major, a K step is 32 rows of 128 bytes
                     const uint64_t wdesc = p.b_nk ? smem_desc_sw128(w_base + kk * 32, 16, 1024)
                                                   : smem_desc_sw128(w_base + kk * 32 * 128, kBK * 128, 1024);
-                    mma_i8_ss(tmem_base, wdesc, smem_desc_sw128(q_base + kk * 32, 16, 1024), p.idesc,
-                              (kb != kb0 || kk != 0) ? 1u : 0u);
+                    mma_i8_ss(d_tmem, wdesc, smem_desc_sw128(q_base + kk * 32, 16, 1024), p.idesc,
+                              (i >= kMats || kk != 0) ? 1u : 0u);
                 }
                 mma_commit(&empty[s]);
                 if (++s == p.stages) { s = 0; ph ^= 1u; }
@@ -1090,20 +1099,6 @@ __global__ void __launch_bounds__(kSmallThreads, 2)
                         d[i].zero();
                         if (t < p.T && k + i * ustep < k1) d[i].load_part(src + k + i * ustep, k1 - k - i * ustep);
                     }
-                }
-                if constexpr (kIn == kInPair) {
-                    In8<T> u[kBatch];
-#pragma unroll
-                    for (int i = 0; i < kBatch; ++i) {
-                        u[i].zero();
-                        if (t >= p.T || k + i * ustep >= k1) continue;
-                        if (whole) u[i].load(src + p.up + k + i * ustep);
-                        else u[i].load_part(src + p.up + k + i * ustep, k1 - k - i * ustep);
-                    }
-#pragma unroll
-                    for (int i = 0; i < kBatch; ++i)
-#pragma unroll
-                        for (int j = 0; j < 8; ++j) d[i].v[j] = u[i].v[j] * silu(d[i].v[j]);
                 }
             };
             if (threadIdx.x - 64 < kNT) s_amax[rank][threadIdx.x - 64] = 0u;
@@ -1193,48 +1188,55 @@ __global__ void __launch_bounds__(kSmallThreads, 2)
         const bool ok = mbar_wait_warp(tfull, 0, status, kDevErrTimeout);
         tc_fence_after();
         const uint32_t taddr = tmem_base + ((uint32_t)(q * 32) << 16) + tok;
-        auto put = [&](int sum, int t, int ch) {   // channel ch of the tile
+        auto put = [&](int sum, int sum1, int t, int ch) {   // channel ch of the tile
             const int col = col0 + ch;
             if (col >= p.N) return;
-            float v = (float)sum * s_tok[t] * __ldg((second ? p.s_ch1 : p.s_ch0) + col);
+            float v = (float)sum * s_tok[t] * __ldg(p.s_ch0 + col);
+            if (kSwiglu) v = (float)sum1 * s_tok[t] * __ldg(p.s_ch1 + col) * silu(v);
             if (p.bias) v += __ldg(p.bias + col);
             if (p.residual) v += load_as_f32(p.residual, t * p.ld_res + col, p.res_type);
-            const int64_t at = t * p.ld_out + col + (second ? p.out1 : 0);
+            const int64_t at = t * p.ld_out + col;
             if (p.out_type == MOE_TYPE_F32) static_cast<float*>(p.out)[at] = v;
             else if (p.out_type == MOE_TYPE_F16) static_cast<__half*>(p.out)[at] = __float2half_rn(v);
             else static_cast<__nv_bfloat16*>(p.out)[at] = __float2bfloat16_rn(v);
         };
         const int wch = 128 / p.split;              // channels of a slice
+        static_assert(kHalfTok == 8, "a thread reads its tokens at once");
+        if (ok && tok < p.T) {                      // the same for the whole warp
+            uint32_t a[kMats][8];
 #pragma unroll
-        for (int g = 0; g < kHalfTok; g += 8) {
-            if (!ok || tok + g >= p.T) break;       // the same for the whole warp
-            uint32_t a[8];
-            tmem_ld_32x32b_x8(taddr + g, a);
+            for (int j = 0; j < kMats; ++j) tmem_ld_32x32b_x8(taddr + j * kNT, a[j]);
             tmem_wait_ld();
             if (!split) {
 #pragma unroll
                 for (int i = 0; i < 8; ++i)
-                    if (tok + g + i < p.T) put((int)a[i], tok + g + i, c);
+                    if (tok + i < p.T) put((int)a[0][i], (int)a[kMats - 1][i], tok + i, c);
             } else {
-                // parts: [source][token / 4][channel of the slice][4 tokens]
+                // parts: [matrix][source][token / 4][channel of the slice][4 tokens]
 #pragma unroll
-                for (int i = 0; i < 8; i += 4) {
-                    if (tok + g + i >= p.T) break;
-                    const uint32_t at = (uint32_t)(((rank * (kNT / 4) + (tok + g + i) / 4) * wch + c % wch) * 16);
-                    st_cluster4(mapa(smem_u32(recv) + at, c / wch), a[i], a[i + 1], a[i + 2], a[i + 3]);
-                }
+                for (int j = 0; j < kMats; ++j)
+#pragma unroll
+                    for (int i = 0; i < 8; i += 4) {
+                        if (tok + i >= p.T) break;
+                        const uint32_t at = (uint32_t)(j * 128 * kNT * 4 +
+                                                       ((rank * (kNT / 4) + (tok + i) / 4) * wch + c % wch) * 16);
+                        st_cluster4(mapa(smem_u32(recv) + at, c / wch), a[j][i], a[j][i + 1], a[j][i + 2], a[j][i + 3]);
+                    }
             }
         }
         if (split) {
             __syncwarp();
             cluster_arrive();   // phase 3: every part has been sent
             cluster_wait();
-            const int* part = reinterpret_cast<const int*>(recv);
+            const int* parts = reinterpret_cast<const int*>(recv);
             for (int i = threadIdx.x - 64; ok && i < wch * p.T; i += kSmallWorkers) {
                 const int t = i / wch, ch = i % wch;
-                int sum = 0;
-                for (int r = 0; r < p.split; ++r) sum += part[((r * (kNT / 4) + t / 4) * wch + ch) * 4 + t % 4];
-                put(sum, t, rank * wch + ch);
+                int sum[kMats] = {};
+                for (int r = 0; r < p.split; ++r)
+#pragma unroll
+                    for (int j = 0; j < kMats; ++j)
+                        sum[j] += parts[j * 128 * kNT + ((r * (kNT / 4) + t / 4) * wch + ch) * 4 + t % 4];
+                put(sum[0], sum[kMats - 1], t, rank * wch + ch);
             }
         }
     }
@@ -1432,9 +1434,9 @@ constexpr int kSmallN = 16;
 constexpr int kSmallStages = 5;
 constexpr size_t kSmallSmem = 112 * 1024;   // two CTAs an SM
 
-template <int kNT, int kIn>
+template <int kIn, bool kSwiglu>
 cudaError_t launch_small_typed(const CUtensorMap (&w)[2], const SmallParams& p, int tiles, size_t smem, cudaStream_t st) {
-    auto kern = small_linear_kernel<kNT, kIn>;
+    auto kern = small_linear_kernel<kSmallN, kIn, kSwiglu>;
     static SmemAttr attr;
     cudaError_t err = ensure_smem(kern, smem, attr);
     if (err != cudaSuccess) return err;
@@ -1446,11 +1448,11 @@ cudaError_t launch_small_typed(const CUtensorMap (&w)[2], const SmallParams& p, 
 // with the most CTAs that are resident at once (two an SM).
 bool plan_small(int64_t T, int K, int N, int mats, int num_sms, int* split, int* stages, size_t* smem) {
     if (T > kSmallTokens) return false;
-    const int kblocks = (K + kBK - 1) / kBK, tiles = (N + 127) / 128 * mats;
+    const int kblocks = (K + kBK - 1) / kBK, tiles = (N + 127) / 128;
     *split = 0;
     for (int s = 1; s <= kMaxSplit && s <= kblocks; s *= 2) {
-        const int blocks = (kblocks + s - 1) / s, st = std::min(kSmallStages, blocks);
-        const size_t need = small_smem<kSmallN>(st, blocks, s);
+        const int blocks = (kblocks + s - 1) / s, st = std::min(kSmallStages, blocks * mats);
+        const size_t need = small_smem<kSmallN>(st, blocks, s, mats);
         if (need > kSmallSmem) continue;
         // clusters of 1, 2, 4 and 8 CTAs of up to half an SM's memory fit 296, 148, 71 and 33 times
         const int at_once = s == 1 ? 2 * num_sms : s == 2 ? num_sms : s == 4 ? num_sms * 71 / 148 : num_sms * 33 / 148;
@@ -1462,10 +1464,10 @@ bool plan_small(int64_t T, int K, int N, int mats, int num_sms, int* split, int*
     return *split != 0;
 }
 
-// A product of few tokens in one launch; x_type: MOE_TYPE_* of x, or -1 for
-// codes.  up != 0: gate and up values.  False where the shape needs the tiles.
-bool try_small(const void* x, int x_type, int64_t ld_x, int64_t up, const LinearParams& l, const Matrix& w0,
-               const Matrix* w1, int num_sms, cudaStream_t st, cudaError_t* err) {
+// A product of few tokens in one launch (w1: gate and up, h written); x_type:
+// MOE_TYPE_* of x, or -1 for codes.  False where the shape needs the tiles.
+bool try_small(const void* x, int x_type, int64_t ld_x, const LinearParams& l, const Matrix& w0, const Matrix* w1,
+               int num_sms, cudaStream_t st, cudaError_t* err) {
     int split, stages;
     size_t smem;
     const int mats = w1 ? 2 : 1;
@@ -1473,7 +1475,6 @@ bool try_small(const void* x, int x_type, int64_t ld_x, int64_t up, const Linear
     SmallParams p{};
     p.x = x;
     p.ld_x = ld_x;
-    p.up = up;
     p.s_tok = l.s_tok;
     p.T = l.T;
     p.K = l.K;
@@ -1481,8 +1482,6 @@ bool try_small(const void* x, int x_type, int64_t ld_x, int64_t up, const Linear
     p.kblocks = (l.K + kBK - 1) / kBK;
     p.split = split;
     p.stages = stages;
-    p.tiles0 = (l.N + 127) / 128;
-    p.out1 = l.out1;
     p.b_nk = l.b_nk;
     p.pdl = l.pdl;
     p.s_ch0 = w0.scale;
@@ -1509,12 +1508,17 @@ bool try_small(const void* x, int x_type, int64_t ld_x, int64_t up, const Linear
         }
     }
     if (mats == 1) w[1] = w[0];
-    const int tiles = p.tiles0 * mats;
-    if (x_type < 0) *err = launch_small_typed<kSmallN, kInCodes>(w, p, tiles, smem, st);
-    else if (up != 0) *err = launch_small_typed<kSmallN, kInPair>(w, p, tiles, smem, st);
-    else if (x_type == MOE_TYPE_F32) *err = launch_small_typed<kSmallN, kInF32>(w, p, tiles, smem, st);
-    else if (x_type == MOE_TYPE_F16) *err = launch_small_typed<kSmallN, kInF16>(w, p, tiles, smem, st);
-    else *err = launch_small_typed<kSmallN, kInBF16>(w, p, tiles, smem, st);
+    const int tiles = (l.N + 127) / 128;
+    if (x_type < 0) *err = launch_small_typed<kInCodes, false>(w, p, tiles, smem, st);
+    else if (x_type == MOE_TYPE_F32)
+        *err = w1 ? launch_small_typed<kInF32, true>(w, p, tiles, smem, st)
+                  : launch_small_typed<kInF32, false>(w, p, tiles, smem, st);
+    else if (x_type == MOE_TYPE_F16)
+        *err = w1 ? launch_small_typed<kInF16, true>(w, p, tiles, smem, st)
+                  : launch_small_typed<kInF16, false>(w, p, tiles, smem, st);
+    else
+        *err = w1 ? launch_small_typed<kInBF16, true>(w, p, tiles, smem, st)
+                  : launch_small_typed<kInBF16, false>(w, p, tiles, smem, st);
     return true;
 }
 
@@ -1599,10 +1603,10 @@ LinearParams out_params(int64_t T, int K, int N, const float* s_tok, const float
 bool fused_swiglu(int64_t T, int64_t f) { return (T + 127) / 128 * ((f + 127) / 128) * 4 >= kRuleSms * 3; }
 
 // Whether the small kernel takes a call (its shared memory depends on K alone).
-bool is_small(int64_t T, int K) {
+bool is_small(int64_t T, int K, int mats = 1) {
     int split, stages;
     size_t smem;
-    return plan_small(T, K, 1, 1, kRuleSms, &split, &stages, &smem);
+    return plan_small(T, K, 1, mats, kRuleSms, &split, &stages, &smem);
 }
 
 size_t linear_scratch(int64_t T, int K) {
@@ -1619,7 +1623,7 @@ SharedScratch shared_scratch(int64_t T, int64_t d, int64_t f) {
     size_t at = 0;
     s.qx = at; at += up256((size_t)T * up16(d));
     s.sx = at; at += up256((size_t)T * sizeof(float));
-    s.h = at;  at += up256((size_t)T * s.ldh * sizeof(float)) * (fused_swiglu(T, f) ? 1 : 2);
+    s.h = at;  at += up256((size_t)T * s.ldh * sizeof(float)) * (fused_swiglu(T, f) || is_small(T, (int)d, 2) ? 1 : 2);
     s.qh = at; at += up256((size_t)T * up16(f));
     s.sh = at; at += up256((size_t)T * sizeof(float));
     s.total = at;
@@ -1683,15 +1687,17 @@ int run_shared_expert(const char* who, const void* x, int x_type, int64_t tokens
     py.res_type = x_type;
     py.vec_res = aligned(residual, 16) && (residual_stride * elem_bytes(x_type)) % 16 == 0;
     cudaError_t e = cudaSuccess;
-    // gate and up: g and u (few tokens, or too few tiles to fuse), or h
-    if (fused || !try_small(x, x_type, row_stride, 0, ph, mg, &mu, num_sms, stream, &e)) {
+    // gate and up: h, or (too few tiles to fuse) g and u
+    const bool small = is_small(tokens, d_model, 2);
+    if (!small || !try_small(x, x_type, row_stride, ph, mg, &mu, num_sms, stream, &e)) {
         ph.pdl = 1;
         e = launch_quantize(x, x_type, tokens, d_model, row_stride, 0, qx, up16(d_model), sx, false, stream);
         if (e == cudaSuccess) e = launch_linear(qx, up16(d_model), ph, mg, &mu, fused, num_sms, stream);
     }
     if (e != cudaSuccess) return cuda_error(who, e);
-    if (fused || !try_small(h, MOE_TYPE_F32, sc.ldh, behind, py, md, nullptr, num_sms, stream, &e)) {
-        e = launch_quantize(h, MOE_TYPE_F32, tokens, d_ff, sc.ldh, fused ? 0 : behind, qh, up16(d_ff), sh, true, stream);
+    const bool pairs = !fused && !small;
+    if (pairs || !try_small(h, MOE_TYPE_F32, sc.ldh, py, md, nullptr, num_sms, stream, &e)) {
+        e = launch_quantize(h, MOE_TYPE_F32, tokens, d_ff, sc.ldh, pairs ? behind : 0, qh, up16(d_ff), sh, true, stream);
         if (e == cudaSuccess) e = launch_linear(qh, up16(d_ff), py, md, nullptr, false, num_sms, stream);
     }
     return e == cudaSuccess ? MOE_OK : cuda_error(who, e);
@@ -1744,7 +1750,7 @@ extern "C" int moe_int8_matmul(const int8_t* q, int64_t q_stride, const float* s
     const LinearParams p = out_params(tokens, K, N, scale, bias, out, out_type, out_stride, w->order, false);
     const Matrix m{w->w, w->row_stride, w->scale};
     cudaError_t e;
-    if (!try_small(q, -1, q_stride, 0, p, m, nullptr, num_sms, stream, &e))
+    if (!try_small(q, -1, q_stride, p, m, nullptr, num_sms, stream, &e))
         e = launch_linear(q, q_stride, p, m, nullptr, false, num_sms, stream);
     return e == cudaSuccess ? MOE_OK : cuda_error(who, e);
 }
@@ -1771,7 +1777,7 @@ extern "C" int moe_int8_linear(const void* x, int x_type, int64_t tokens, int K,
     LinearParams p = out_params(tokens, K, N, s, bias, out, out_type, out_stride, w->order, false);
     const Matrix m{w->w, w->row_stride, w->scale};
     cudaError_t e;
-    if (!try_small(x, x_type, row_stride, 0, p, m, nullptr, num_sms, stream, &e)) {
+    if (!try_small(x, x_type, row_stride, p, m, nullptr, num_sms, stream, &e)) {
         p.pdl = 1;
         e = launch_quantize(x, x_type, tokens, K, row_stride, 0, q, up16(K), s, false, stream);
         if (e == cudaSuccess) e = launch_linear(q, up16(K), p, m, nullptr, false, num_sms, stream);
