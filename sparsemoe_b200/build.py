@@ -1,4 +1,6 @@
-"""Builds libsparsemoe_b200.so (the C-ABI library) in-tree with nvcc for sm_100a.
+"""Builds libsparsemoe_b200.so (the C-ABI library) in-tree with nvcc for sm_100a,
+and _operators.so, the Python entry of the stand-alone operators, with g++
+against torch's headers.
 
 Usage: python sparsemoe_b200/build.py   (loaded by path: the package import needs the built library)
 """
@@ -15,6 +17,8 @@ PKG = Path(__file__).resolve().parent
 CSRC = PKG / "csrc"
 BUILD = PKG / "_build"
 LIB = PKG / "libsparsemoe_b200.so"
+BINDING_SRC = PKG / "binding" / "operators.cpp"
+BINDING = PKG / "_operators.so"
 
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 NVCC_FLAGS = ["-O3", "-lineinfo", "-std=c++17", "-Xcompiler", "-fPIC", "-Xcompiler", "-Wall",
@@ -47,11 +51,35 @@ def _compile(src: Path, extra: list[str]) -> Path:
     return obj
 
 
+def build_binding() -> Path:
+    """The Python entry: no CUDA code, calls the C ABI through addresses it is given."""
+    deps = [BINDING_SRC, PKG.parent / "include" / "sparsemoe_b200.h"]
+    if BINDING.exists() and BINDING.stat().st_mtime >= max(d.stat().st_mtime for d in deps):
+        return BINDING
+    import importlib.util
+    import sysconfig
+    torch = Path(importlib.util.find_spec("torch").origin).parent
+    cuda = Path(nvcc()).resolve().parents[1] / "include"
+    inc = [torch / "include", torch / "include" / "torch" / "csrc" / "api" / "include",
+           Path(sysconfig.get_paths()["include"]), cuda, PKG.parent / "include"]
+    tmp = BINDING.with_suffix(".so.tmp")
+    cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", *(a for i in inc for a in ("-isystem", str(i))),
+           str(BINDING_SRC), "-o", str(tmp), "-L", str(torch / "lib"), "-ltorch_python", "-ltorch", "-ltorch_cpu",
+           "-ltorch_cuda", "-lc10", "-lc10_cuda"]
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        raise RuntimeError(f"g++ failed for {BINDING_SRC.name}:\n{r.stdout}\n{r.stderr}")
+    os.replace(tmp, BINDING)
+    return BINDING
+
+
 def build(verbose: bool = False, extra: list[str] | None = None) -> Path:
     BUILD.mkdir(exist_ok=True)
     extra = extra or []
     with cf.ThreadPoolExecutor(max_workers=min(8, os.cpu_count() or 1)) as ex:
+        binding = ex.submit(build_binding)
         objs = list(ex.map(lambda s: _compile(s, extra), sources()))
+        binding.result()
     newest = max(o.stat().st_mtime for o in objs)
     if not LIB.exists() or LIB.stat().st_mtime < newest:
         tmp = LIB.with_suffix(".so.tmp")
@@ -61,7 +89,7 @@ def build(verbose: bool = False, extra: list[str] | None = None) -> Path:
             raise RuntimeError(f"link failed:\n{r.stdout}\n{r.stderr}")
         os.replace(tmp, LIB)
     if verbose:
-        print(f"built {LIB}")
+        print(f"built {LIB} and {BINDING.name}")
     return LIB
 
 

@@ -12,7 +12,7 @@ import torch
 
 from . import LayerConfig, MoEArgs, check, lib
 from .config import MoeLayerOptions, MoeSharedExpert
-from .operators import Routing, int8_weight, _weight
+from .operators import Routing, int8_weight, weight_struct
 
 
 def _t16(cfg: LayerConfig):
@@ -30,8 +30,12 @@ class SharedExpert:
         self.wg, self.wu, self.wd = (int8_weight(dev(inputs[k])) for k in ("shared_wg", "shared_wu", "shared_wd"))
         self.sg, self.su, self.sd = (dev(inputs[k]) for k in ("shared_sg", "shared_su", "shared_sd"))
         self.d_ff = self.wg.shape[1]
-        if self.wu.shape != (d_model, self.d_ff) or self.wd.shape != (self.d_ff, d_model):
-            raise ValueError(f"shared_wu must be [{d_model}, {self.d_ff}] and shared_wd [{self.d_ff}, {d_model}]")
+        f = self.d_ff
+        for name, t, shape in (("shared_wg", self.wg, (d_model, f)), ("shared_wu", self.wu, (d_model, f)),
+                               ("shared_wd", self.wd, (f, d_model)), ("shared_sg", self.sg, (f,)),
+                               ("shared_su", self.su, (f,)), ("shared_sd", self.sd, (d_model,))):
+            if t.shape != shape or t.dtype != (torch.int8 if len(shape) == 2 else torch.float32):
+                raise ValueError(f"{name} must be {'int8' if len(shape) == 2 else 'f32'} {list(shape)}")
 
     def weights(self) -> tuple:
         return self.wg, self.sg, self.wu, self.su, self.wd, self.sd
@@ -233,11 +237,10 @@ class MoeLayer:
             o.routing = ctypes.pointer(self.routing.struct())
             o.select_bias = None if self.select_bias is None else self.select_bias.data_ptr()
         if self.shared is not None:
-            sh, d, i = self.shared, self.cfg.d_model, self.shared.wg.get_device()
+            sh = self.shared
             o.shared = ctypes.pointer(MoeSharedExpert(
-                _weight(sh.wg, sh.sg, "shared_wg", d, i)[0], _weight(sh.wu, sh.su, "shared_wu", d, i)[0],
-                _weight(sh.wd, sh.sd, "shared_wd", sh.d_ff, i)[0], sh.d_ff, self.shared_out.data_ptr(),
-                self.shared_scratch.data_ptr(), self.shared_scratch.numel()))
+                weight_struct(sh.wg, sh.sg), weight_struct(sh.wu, sh.su), weight_struct(sh.wd, sh.sd), sh.d_ff,
+                self.shared_out.data_ptr(), self.shared_scratch.data_ptr(), self.shared_scratch.numel()))
         return o
 
     def forward(self, stream: torch.cuda.Stream | None = None) -> torch.Tensor:

@@ -121,9 +121,10 @@ def test_int8_weight_layout(shape, order):
     w = a if order == "kn" else a.t().contiguous().t()
     p = sm.int8_weight(w)
     assert torch.equal(p, a)
-    wt, n = sm.operators._weight(p, torch.ones(shape[1]), "w", shape[0], -1)
-    assert n == shape[1] and wt.row_stride % 16 == 0
+    wt = sm.operators.weight_struct(p, torch.ones(shape[1]))
+    assert wt.row_stride % 16 == 0 and wt.w == p.data_ptr()
     if min(shape) > 1:
         assert wt.order == (0 if order == "kn" else 1)
-        with pytest.raises(ValueError, match="int8_weight"):
-            sm.operators._weight(torch.zeros(5, 7, dtype=torch.int8), torch.ones(7), "w", 5, -1)
+        assert wt.row_stride >= (shape[1] if order == "kn" else shape[0])
+    with pytest.raises(ValueError, match="int8"):
+        sm.int8_weight(p.float())
