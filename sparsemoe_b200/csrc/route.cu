@@ -302,34 +302,53 @@ __device__ __forceinline__ float rcp_fast(float x) {   // 1 ulp
 }
 
 // The candidates in lanes 0 .. n-1 (n >= k, or fewer where nothing else is
-// left) ranked by f64 value, equal values by the lower index: lane l gets the
-// l-th.  `top`: largest unmasked logit, where the softmax needs it.
+// left) ranked by value, equal values by the lower index: lane l gets the l-th.
+// f32 values decide where those that follow each other, down to the first behind
+// the k-th, are further apart than their error (logits themselves are exact);
+// else f64 values do.  top, inv_sum: the softmax's statistics; buf: 64 words.
 template <typename T, int NV>
-__device__ __noinline__ int rank_candidates(const RouteParams& p, const T* row, float top, int cand, int n, int* buf,
-                                            int lane) {
+__device__ __noinline__ int rank_candidates(const RouteParams& p, const T* row, float top, float inv_sum, float err2,
+                                            int cand, int n, int* buf, int lane) {
     const float x = lane < n ? to_f32<T>(row[cand]) : 0.0f;
-    double v = x;
-    if (p.bias) {
-        const double b = lane < n ? __ldg(p.bias + cand) : 0.0f;
-        if (p.sigmoid) {
-            v = 1.0 / (1.0 + exp(-(double)x)) + b;
-        } else {
-            float xs[NV];
-            load_row<T, NV>(row, lane * NV, p.E, p.vec != 0, xs);
-            double sum = 0.0;
-#pragma unroll
-            for (int q = 0; q < NV; ++q)
-                if (selectable<T>(xs[q])) sum += xs[q] == top ? 1.0 : exp((double)xs[q] - (double)top);
-            sum = warp_sum(sum);
-            v = (x == top ? 1.0 : exp((double)x - (double)top)) / sum + b;
-        }
-    }
+    const float b = p.bias && lane < n ? __ldg(p.bias + cand) : 0.0f;
+    float f = x;
+    if (p.bias) f = (p.sigmoid ? rcp_fast(1.0f + exp_fast(-x)) : (x == top ? 1.0f : exp_fast(x - top)) * inv_sum) + b;
     int rank = 0;
+    for (int j = 0; j < n; ++j) {
+        const float o = __shfl_sync(kFull, f, j);
+        const int e = __shfl_sync(kFull, cand, j);
+        rank += o > f || (o == f && e < cand) ? 1 : 0;
+    }
+    __syncwarp();
+    if (lane < n) {
+        buf[rank] = cand;
+        buf[32 + rank] = __float_as_int(f);
+    }
+    __syncwarp();
+    if (!p.bias) return lane < n ? buf[lane] : -1;
+    const float hi = __int_as_float(buf[32 + min(lane, n - 1)]), lo = __int_as_float(buf[32 + min(lane + 1, n - 1)]);
+    const bool close = !(hi - lo > err2 + 3e-7f * fmaxf(fabsf(hi), fabsf(lo)));
+    if (!__any_sync(kFull, lane + 1 < n && lane < p.k && close)) return lane < n ? buf[lane] : -1;
+    double v;
+    if (p.sigmoid) {
+        v = 1.0 / (1.0 + exp(-(double)x)) + (double)b;
+    } else {
+        float xs[NV];
+        load_row<T, NV>(row, lane * NV, p.E, p.vec != 0, xs);
+        double sum = 0.0;
+#pragma unroll
+        for (int q = 0; q < NV; ++q)
+            if (selectable<T>(xs[q])) sum += xs[q] == top ? 1.0 : exp((double)xs[q] - (double)top);
+        sum = warp_sum(sum);
+        v = (x == top ? 1.0 : exp((double)x - (double)top)) / sum + (double)b;
+    }
+    rank = 0;
     for (int j = 0; j < n; ++j) {
         const double o = __shfl_sync(kFull, v, j);
         const int e = __shfl_sync(kFull, cand, j);
         rank += o > v || (o == v && e < cand) ? 1 : 0;
     }
+    __syncwarp();
     if (lane < n) buf[rank] = cand;
     __syncwarp();
     return lane < n ? buf[lane] : -1;
@@ -502,7 +521,7 @@ __global__ void __launch_bounds__(kRouteWarps * 32) route_kernel(const __grid_co
             }
             redo = best != 0 && close(last, best);
             if (!redo)
-                my_i = rank_candidates<T, NV>(p, row, top, mine != 0 ? (int)(kIdx - (mine & kIdx)) : -1, n,
+                my_i = rank_candidates<T, NV>(p, row, top, inv_sum, err2, mine != 0 ? (int)(kIdx - (mine & kIdx)) : -1, n,
                                               reinterpret_cast<int*>(sv[warp]), lane);
         }
     }
@@ -745,8 +764,9 @@ __global__ void __launch_bounds__(kRouteWarps * 32) route_many_kernel(const __gr
                 } else {
                     const int count = __shfl_sync(kFull, n, 8 * r), ex = __shfl_sync(kFull, extra, 8 * r);
                     const int c = __shfl_sync(kFull, my_i, 8 * r + (lane & 7));
-                    const float tp = __shfl_sync(kFull, top, 8 * r);
-                    got = rank_candidates<T, NV / 4>(p, rr, tp, lane < count ? c : ex, count + (ex >= 0 ? 1 : 0),
+                    const float tp = __shfl_sync(kFull, top, 8 * r), is = __shfl_sync(kFull, inv_sum, 8 * r);
+                    const float er = __shfl_sync(kFull, err2, 8 * r);
+                    got = rank_candidates<T, NV / 4>(p, rr, tp, is, er, lane < count ? c : ex, count + (ex >= 0 ? 1 : 0),
                                                      reinterpret_cast<int*>(sv[warp]), lane);
                     __syncwarp();
                 }
