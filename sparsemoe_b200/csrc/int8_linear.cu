@@ -1424,12 +1424,13 @@ cudaError_t launch_linear(const int8_t* q, int64_t ldq, LinearParams p, const Ma
     return launch_linear_cfg<128, false, false>(ta, tb, to, p, clusters, st);
 }
 
-// Up to this many tokens small_linear_kernel is used (its MMA has 16 columns).
-// Measured (us in a graph, 7168 x 2048, quantiser included; small kernel, and
-// quantiser + tiles): 1 token 10.9, 11.8; 4 tokens 11.8, 11.8; 8 tokens 13.4,
-// 12.1; 16 tokens 17.5, 14.0.  One launch instead of two costs the host 4.9 us
-// instead of 7.5, which decides at 8.
-constexpr int kSmallTokens = 8;
+// Up to this many tokens small_linear_kernel is used.  Measured (us in a graph;
+// small kernel, then quantiser + tiles): int8_linear 7168 -> 2048 of 1 token 10.2,
+// 11.2, 4 tokens 10.6, 10.6, 8 tokens 11.1, 10.7; 2048 -> 7168 of 4 tokens 9.5, 8.9,
+// 8 tokens 10.0, 8.9 (one launch instead of two costs the host 3.9 us instead of
+// 7.5); codes given, 8 tokens 9.3, 9.8 and 8.3, 8.2; shared expert 7168 / 2048 of 4
+// tokens 21.9, 26.0, 8 tokens 22.6, 26.3, 12 tokens 25.8, 26.7, 16 tokens 27.0, 26.7.
+constexpr int kSmallLinear = 4, kSmallCodes = 8, kSmallShared = 8;
 constexpr int kSmallN = 16;
 constexpr int kSmallStages = 5;
 constexpr size_t kSmallSmem = 112 * 1024;   // two CTAs an SM
@@ -1446,8 +1447,8 @@ cudaError_t launch_small_typed(const CUtensorMap (&w)[2], const SmallParams& p, 
 
 // Whether a call's codes fit beside the weight stages at some split; the split
 // with the most CTAs that are resident at once (two an SM).
-bool plan_small(int64_t T, int K, int N, int mats, int num_sms, int* split, int* stages, size_t* smem) {
-    if (T > kSmallTokens) return false;
+bool plan_small(int64_t T, int limit, int K, int N, int mats, int num_sms, int* split, int* stages, size_t* smem) {
+    if (T > limit) return false;
     const int kblocks = (K + kBK - 1) / kBK, tiles = (N + 127) / 128;
     *split = 0;
     for (int s = 1; s <= kMaxSplit && s <= kblocks; s *= 2) {
@@ -1466,12 +1467,12 @@ bool plan_small(int64_t T, int K, int N, int mats, int num_sms, int* split, int*
 
 // A product of few tokens in one launch (w1: gate and up, h written); x_type:
 // MOE_TYPE_* of x, or -1 for codes.  False where the shape needs the tiles.
-bool try_small(const void* x, int x_type, int64_t ld_x, const LinearParams& l, const Matrix& w0, const Matrix* w1,
+bool try_small(int limit, const void* x, int x_type, int64_t ld_x, const LinearParams& l, const Matrix& w0, const Matrix* w1,
                int num_sms, cudaStream_t st, cudaError_t* err) {
     int split, stages;
     size_t smem;
     const int mats = w1 ? 2 : 1;
-    if (!plan_small(l.T, l.K, l.N, mats, num_sms, &split, &stages, &smem)) return false;
+    if (!plan_small(l.T, limit, l.K, l.N, mats, num_sms, &split, &stages, &smem)) return false;
     SmallParams p{};
     p.x = x;
     p.ld_x = ld_x;
@@ -1603,14 +1604,14 @@ LinearParams out_params(int64_t T, int K, int N, const float* s_tok, const float
 bool fused_swiglu(int64_t T, int64_t f) { return (T + 127) / 128 * ((f + 127) / 128) * 4 >= kRuleSms * 3; }
 
 // Whether the small kernel takes a call (its shared memory depends on K alone).
-bool is_small(int64_t T, int K, int mats = 1) {
+bool is_small(int64_t T, int limit, int K, int mats = 1) {
     int split, stages;
     size_t smem;
-    return plan_small(T, K, 1, mats, kRuleSms, &split, &stages, &smem);
+    return plan_small(T, limit, K, 1, mats, kRuleSms, &split, &stages, &smem);
 }
 
 size_t linear_scratch(int64_t T, int K) {
-    return is_small(T, K) ? 0 : up256((size_t)T * up16(K)) + up256((size_t)T * sizeof(float));
+    return is_small(T, kSmallLinear, K) ? 0 : up256((size_t)T * up16(K)) + up256((size_t)T * sizeof(float));
 }
 
 struct SharedScratch {
@@ -1623,7 +1624,7 @@ SharedScratch shared_scratch(int64_t T, int64_t d, int64_t f) {
     size_t at = 0;
     s.qx = at; at += up256((size_t)T * up16(d));
     s.sx = at; at += up256((size_t)T * sizeof(float));
-    s.h = at;  at += up256((size_t)T * s.ldh * sizeof(float)) * (fused_swiglu(T, f) || is_small(T, (int)d, 2) ? 1 : 2);
+    s.h = at;  at += up256((size_t)T * s.ldh * sizeof(float)) * (fused_swiglu(T, f) || is_small(T, kSmallShared, (int)d, 2) ? 1 : 2);
     s.qh = at; at += up256((size_t)T * up16(f));
     s.sh = at; at += up256((size_t)T * sizeof(float));
     s.total = at;
@@ -1688,15 +1689,15 @@ int run_shared_expert(const char* who, const void* x, int x_type, int64_t tokens
     py.vec_res = aligned(residual, 16) && (residual_stride * elem_bytes(x_type)) % 16 == 0;
     cudaError_t e = cudaSuccess;
     // gate and up: h, or (too few tiles to fuse) g and u
-    const bool small = is_small(tokens, d_model, 2);
-    if (!small || !try_small(x, x_type, row_stride, ph, mg, &mu, num_sms, stream, &e)) {
+    const bool small = is_small(tokens, kSmallShared, d_model, 2);
+    if (!small || !try_small(kSmallShared, x, x_type, row_stride, ph, mg, &mu, num_sms, stream, &e)) {
         ph.pdl = 1;
         e = launch_quantize(x, x_type, tokens, d_model, row_stride, 0, qx, up16(d_model), sx, false, stream);
         if (e == cudaSuccess) e = launch_linear(qx, up16(d_model), ph, mg, &mu, fused, num_sms, stream);
     }
     if (e != cudaSuccess) return cuda_error(who, e);
     const bool pairs = !fused && !small;
-    if (pairs || !try_small(h, MOE_TYPE_F32, sc.ldh, py, md, nullptr, num_sms, stream, &e)) {
+    if (pairs || !try_small(kSmallShared, h, MOE_TYPE_F32, sc.ldh, py, md, nullptr, num_sms, stream, &e)) {
         e = launch_quantize(h, MOE_TYPE_F32, tokens, d_ff, sc.ldh, pairs ? behind : 0, qh, up16(d_ff), sh, true, stream);
         if (e == cudaSuccess) e = launch_linear(qh, up16(d_ff), py, md, nullptr, false, num_sms, stream);
     }
@@ -1750,7 +1751,7 @@ extern "C" int moe_int8_matmul(const int8_t* q, int64_t q_stride, const float* s
     const LinearParams p = out_params(tokens, K, N, scale, bias, out, out_type, out_stride, w->order, false);
     const Matrix m{w->w, w->row_stride, w->scale};
     cudaError_t e;
-    if (!try_small(q, -1, q_stride, p, m, nullptr, num_sms, stream, &e))
+    if (!try_small(kSmallCodes, q, -1, q_stride, p, m, nullptr, num_sms, stream, &e))
         e = launch_linear(q, q_stride, p, m, nullptr, false, num_sms, stream);
     return e == cudaSuccess ? MOE_OK : cuda_error(who, e);
 }
@@ -1777,7 +1778,7 @@ extern "C" int moe_int8_linear(const void* x, int x_type, int64_t tokens, int K,
     LinearParams p = out_params(tokens, K, N, s, bias, out, out_type, out_stride, w->order, false);
     const Matrix m{w->w, w->row_stride, w->scale};
     cudaError_t e;
-    if (!try_small(x, x_type, row_stride, p, m, nullptr, num_sms, stream, &e)) {
+    if (!try_small(kSmallLinear, x, x_type, row_stride, p, m, nullptr, num_sms, stream, &e)) {
         p.pdl = 1;
         e = launch_quantize(x, x_type, tokens, K, row_stride, 0, q, up16(K), s, false, stream);
         if (e == cudaSuccess) e = launch_linear(q, up16(K), p, m, nullptr, false, num_sms, stream);
