@@ -136,56 +136,52 @@ __device__ __forceinline__ void load_row(const T* row, int e0, int E, bool vec, 
     for (int i = 0; i < NV; ++i) x[i] = e0 + i < E ? to_f32<T>(row[e0 + i]) : -INFINITY;
 }
 
-// f64 values of a row's experts lane*NV .. lane*NV + NV - 1: v orders the
-// experts (their logits without a bias), m the members of groups.
-template <typename T, int NV>
-__device__ __forceinline__ void values_f64(const RouteParams& p, const T* row, int lane, double (&v)[NV],
-                                           double (&m)[NV]) {
-    const int e0 = lane * NV;
-    float x[NV];
-    load_row<T, NV>(row, e0, p.E, p.vec != 0, x);
-    double top = -INFINITY, sum = 1.0;
-#pragma unroll
-    for (int q = 0; q < NV; ++q) {
-        v[q] = m[q] = selectable<T>(x[q]) ? (double)x[q] : -INFINITY;
-        top = fmax(top, v[q]);
+// The f64 passes of single rows, rare and therefore small in code and registers
+// (a function that is called takes its registers in every warp of the kernel):
+// values lie in shared memory, lane l looks at experts l, l + 32, ...
+
+// buf[e] = what orders expert e (members: what scores its group), -infinity if masked.
+template <typename T>
+__device__ __forceinline__ void values_f64(const RouteParams& p, const T* row, double* buf, int lane, bool members) {
+    const bool scores = p.bias || (members && p.group_top == 2);
+    double top = -INFINITY, sum = 0.0;
+#pragma unroll 1
+    for (int e = lane; e < p.E; e += 32) {
+        const float x = to_f32<T>(row[e]);
+        const double v = selectable<T>(x) ? (double)x : -INFINITY;
+        top = fmax(top, v);
+        buf[e] = v;
     }
-    if (!p.bias && p.group_top == 1) return;
-    if (p.sigmoid) {
-#pragma unroll
-        for (int q = 0; q < NV; ++q) m[q] = exp(-v[q]);
-#pragma unroll
-        for (int q = 0; q < NV; ++q) m[q] = 1.0 / (1.0 + m[q]);
-    } else {
-        top = warp_max(top);
-        sum = 0.0;
-#pragma unroll
-        for (int q = 0; q < NV; ++q) {
-            m[q] = v[q] == -INFINITY ? 0.0 : v[q] == top ? 1.0 : exp(v[q] - top);
-            sum += m[q];
-        }
-        sum = warp_sum(sum);
+    if (!scores) return;
+    top = warp_max(top);
+#pragma unroll 1
+    for (int e = lane; e < p.E; e += 32) {
+        const double x = buf[e];
+        const double u = p.sigmoid ? exp(-x) : x == top ? 1.0 : exp(x - top);
+        sum += x == -INFINITY ? 0.0 : u;
+        buf[e] = x == -INFINITY ? x : u;
     }
-#pragma unroll
-    for (int q = 0; q < NV; ++q) {
-        m[q] = v[q] == -INFINITY ? -INFINITY : p.sigmoid ? m[q] : m[q] / sum;
+    sum = warp_sum(sum);
+#pragma unroll 1
+    for (int e = lane; e < p.E; e += 32) {
+        const double u = buf[e];
+        if (u == -INFINITY) continue;
+        double v = p.sigmoid ? 1.0 / (1.0 + u) : u / sum;
         if (p.bias) {
-            const float b = e0 + q < p.E ? __ldg(p.bias + e0 + q) : -INFINITY;
-            v[q] = m[q] = b > kMasked ? m[q] + (double)b : -INFINITY;
+            const float b = __ldg(p.bias + e);
+            v = b > kMasked ? v + (double)b : -INFINITY;
         }
+        buf[e] = v;
     }
 }
 
-// Which of up to 32 groups of a row stay, in f64: bit g.  buf: 32 * NV doubles of
-// this warp's shared memory.  Sums of two that agree to 2^-49 are ties
-// (sigmoid(x) + sigmoid(-x) is 1 for every x).
-template <typename T, int NV>
+// Which of up to 32 groups of a row stay: bit g.  buf: E doubles of this warp's
+// shared memory.  Sums of two that agree to 2^-49 are ties (sigmoid(x) +
+// sigmoid(-x) is 1 for every x).
+template <typename T>
 __device__ __noinline__ uint32_t groups_f64(const RouteParams& p, const T* row, double* buf, int lane) {
-    double v[NV], m[NV];
-    values_f64<T, NV>(p, row, lane, v, m);
     __syncwarp();
-#pragma unroll
-    for (int q = 0; q < NV; ++q) buf[lane * NV + q] = m[q];
+    values_f64<T>(p, row, buf, lane, true);
     __syncwarp();
     const bool pair = p.group_top == 2;
     int sub = 32;
@@ -193,7 +189,9 @@ __device__ __noinline__ uint32_t groups_f64(const RouteParams& p, const T* row, 
     const int g = lane / sub;
     double a = -INFINITY, b = -INFINITY;
     if (g < p.G)
+#pragma unroll 1
         for (int i = lane % sub; i < p.per; i += sub) merge2(a, b, buf[g * p.per + i], (double)-INFINITY);
+#pragma unroll 1
     for (int o = sub >> 1; o > 0; o >>= 1) {
         const double c = __shfl_xor_sync(kFull, a, o), d = __shfl_xor_sync(kFull, b, o);
         merge2(a, b, c, d);
@@ -203,6 +201,7 @@ __device__ __noinline__ uint32_t groups_f64(const RouteParams& p, const T* row, 
     if (lane >= p.G) a = -INFINITY;
     const double tie = pair && !isinf(a) ? 0x1p-49 * (1.0 + fabs(a)) : 0.0;
     int rank = 0;
+#pragma unroll 1
     for (int h = 0; h < p.G; ++h) {
         const double other = __shfl_sync(kFull, a, h);
         rank += other > a + tie || (other >= a - tie && h < lane) ? 1 : 0;
@@ -211,79 +210,67 @@ __device__ __noinline__ uint32_t groups_f64(const RouteParams& p, const T* row, 
     return __ballot_sync(kFull, a != -INFINITY && rank < p.kept);
 }
 
-// The whole selection of one row in f64.  Returns the lane's choice (lane l: the
-// l-th) or -1.  buf: 32 * NV doubles of shared memory of this warp.
-template <typename T, int NV>
+// The whole selection of one row.  Returns the lane's choice (lane l: the l-th) or -1.
+template <typename T>
 __device__ __noinline__ int route_row_f64(const RouteParams& p, const T* row, double* buf, int lane) {
-    double v[NV], m[NV];
-    values_f64<T, NV>(p, row, lane, v, m);
-    const int e0 = lane * NV;
-    const bool pair = p.group_top == 2;
-    if (p.G > 1 && p.G <= 32) {
-        const uint32_t stay = groups_f64<T, NV>(p, row, buf, lane);
-#pragma unroll
-        for (int q = 0; q < NV; ++q)
-            if (!(stay >> (min(e0 + q, p.E - 1) / p.per) & 1)) v[q] = -INFINITY;
-    } else if (p.G > 32) {
+    uint32_t keep = kFull;   // lane l, bit i: group l + 32 i
+    if (p.G > 32) {
         __syncwarp();
-#pragma unroll
-        for (int q = 0; q < NV; ++q) buf[e0 + q] = m[q];
+        values_f64<T>(p, row, buf, lane, true);
         __syncwarp();
-        // lane l holds groups l, l + 32, .. (at most NV of them)
-        double gs[NV];
-#pragma unroll
-        for (int i = 0; i < NV; ++i) gs[i] = -INFINITY;
-#pragma unroll
-        for (int i = 0; i < NV; ++i) {
+        const bool pair = p.group_top == 2;
+        double gs[32];
+        const int gn = (p.G + 31) / 32;
+#pragma unroll 1
+        for (int i = 0; i < gn; ++i) {
             const int g = lane + 32 * i;
-            if (g >= p.G) break;
             double a = -INFINITY, b = -INFINITY;
-            for (int j = 0; j < p.per; ++j) merge2(a, b, buf[g * p.per + j], (double)-INFINITY);
+#pragma unroll 1
+            for (int j = 0; g < p.G && j < p.per; ++j) merge2(a, b, buf[g * p.per + j], (double)-INFINITY);
             gs[i] = pair && b != -INFINITY ? a + b : a;
         }
-        uint32_t keep = 0;
+        keep = 0;
         const double tie = pair ? 0x1p-49 : 0.0;
+#pragma unroll 1
         for (int r = 0; r < p.kept; ++r) {
-            double a = gs[0];
-#pragma unroll
-            for (int i = 1; i < NV; ++i) a = fmax(a, gs[i]);
+            double a = -INFINITY;
+            for (int i = 0; i < gn; ++i) a = fmax(a, gs[i]);
             a = warp_max(a);
             if (a == -INFINITY) break;
             const double from = isinf(a) ? a : a - tie * (1.0 + fabs(a));
             uint32_t at = 0xFFFFFFFFu;
-#pragma unroll
-            for (int i = NV - 1; i >= 0; --i)
+            for (int i = gn - 1; i >= 0; --i)
                 if (gs[i] >= from) at = lane + 32 * i;
             at = __reduce_min_sync(kFull, at);
             if ((at & 31) == lane) {
                 keep |= 1u << (at >> 5);
-#pragma unroll
-                for (int i = 0; i < NV; ++i)
-                    if (i == (int)(at >> 5)) gs[i] = -INFINITY;
+                gs[at >> 5] = -INFINITY;
             }
         }
-#pragma unroll
-        for (int q = 0; q < NV; ++q) {
-            const int g = min(e0 + q, p.E - 1) / p.per;
-            if (!((__shfl_sync(kFull, keep, g & 31) >> (g >> 5)) & 1)) v[q] = -INFINITY;
-        }
+    } else if (p.G > 1) {
+        keep = groups_f64<T>(p, row, buf, lane) >> lane & 1;
     }
+    __syncwarp();
+    values_f64<T>(p, row, buf, lane, false);
+    if (p.G > 1)
+#pragma unroll 1
+        for (int e0 = 0; e0 < p.E; e0 += 32) {
+            const int e = e0 + lane, g = min(e, p.E - 1) / p.per;
+            if (!(__shfl_sync(kFull, keep, g & 31) >> (g >> 5) & 1) && e < p.E) buf[e] = -INFINITY;
+        }
     int mine = -1;
+#pragma unroll 1
     for (int l = 0; l < p.k; ++l) {
-        double a = v[0];
-#pragma unroll
-        for (int q = 1; q < NV; ++q) a = fmax(a, v[q]);
+        double a = -INFINITY;
+        for (int e = lane; e < p.E; e += 32) a = fmax(a, buf[e]);
         const double m = warp_max(a);
         if (m == -INFINITY) break;
-        const int wl = __ffs(__ballot_sync(kFull, a == m)) - 1;
-        int at = 0;
-#pragma unroll
-        for (int q = NV - 1; q >= 0; --q) at = v[q] == m ? q : at;
-        at = __shfl_sync(kFull, at, wl);
-        if (lane == l) mine = wl * NV + at;
-#pragma unroll
-        for (int q = 0; q < NV; ++q)
-            if (lane == wl && q == at) v[q] = -INFINITY;
+        uint32_t at = 0xFFFFFFFFu;
+        for (int e = lane; e < p.E; e += 32)
+            if (buf[e] == m && at == 0xFFFFFFFFu) at = e;
+        at = __reduce_min_sync(kFull, at);
+        if ((int)(at & 31) == lane) buf[at] = -INFINITY;
+        if (lane == l) mine = (int)at;
     }
     return mine;
 }
@@ -306,7 +293,7 @@ __device__ __forceinline__ float rcp_fast(float x) {   // 1 ulp
 // f32 values decide where those that follow each other, down to the first behind
 // the k-th, are further apart than their error (logits themselves are exact);
 // else f64 values do.  top, inv_sum: the softmax's statistics; buf: 64 words.
-template <typename T, int NV>
+template <typename T>
 __device__ __noinline__ int rank_candidates(const RouteParams& p, const T* row, float top, float inv_sum, float err2,
                                             int cand, int n, int* buf, int lane) {
     const float x = lane < n ? to_f32<T>(row[cand]) : 0.0f;
@@ -333,12 +320,12 @@ __device__ __noinline__ int rank_candidates(const RouteParams& p, const T* row, 
     if (p.sigmoid) {
         v = 1.0 / (1.0 + exp(-(double)x)) + (double)b;
     } else {
-        float xs[NV];
-        load_row<T, NV>(row, lane * NV, p.E, p.vec != 0, xs);
         double sum = 0.0;
-#pragma unroll
-        for (int q = 0; q < NV; ++q)
-            if (selectable<T>(xs[q])) sum += xs[q] == top ? 1.0 : exp((double)xs[q] - (double)top);
+#pragma unroll 1
+        for (int e = lane; e < p.E; e += 32) {
+            const float o = to_f32<T>(row[e]);
+            if (selectable<T>(o)) sum += o == top ? 1.0 : exp((double)o - (double)top);
+        }
         sum = warp_sum(sum);
         v = (x == top ? 1.0 : exp((double)x - (double)top)) / sum + (double)b;
     }
@@ -466,7 +453,7 @@ __global__ void __launch_bounds__(kRouteWarps * 32) route_kernel(const __grid_co
             }
         }
         if (near && !redo) {
-            const uint32_t mask = groups_f64<T, NV>(p, row, sv[warp], lane);
+            const uint32_t mask = groups_f64<T>(p, row, sv[warp], lane);
             stay = g < p.G && (mask >> g & 1);
         }
         if (p.lanes > 0) {
@@ -521,11 +508,11 @@ __global__ void __launch_bounds__(kRouteWarps * 32) route_kernel(const __grid_co
             }
             redo = best != 0 && close(last, best);
             if (!redo)
-                my_i = rank_candidates<T, NV>(p, row, top, inv_sum, err2, mine != 0 ? (int)(kIdx - (mine & kIdx)) : -1, n,
+                my_i = rank_candidates<T>(p, row, top, inv_sum, err2, mine != 0 ? (int)(kIdx - (mine & kIdx)) : -1, n,
                                               reinterpret_cast<int*>(sv[warp]), lane);
         }
     }
-    if (redo) my_i = route_row_f64<T, NV>(p, row, sv[warp], lane);
+    if (redo) my_i = route_row_f64<T>(p, row, sv[warp], lane);
     if (lane >= p.k) my_i = -1;
 
     const float xs = my_i >= 0 ? to_f32<T>(row[my_i]) : -INFINITY;
@@ -615,38 +602,66 @@ template <int NV> __device__ __forceinline__ void top8(uint32_t (&key)[NV]) {
     }
 }
 
-template <typename T, int NV>
+template <typename T, int NV, bool kWhole>   // kWhole: per == NV
 __global__ void __launch_bounds__(kRouteWarps * 32) route_many_kernel(const __grid_constant__ RouteParams p) {
     constexpr uint32_t kIdx = NV - 1;           // the key bits that hold the place in the lane
-    __shared__ double sv[kRouteWarps][NV / 4 * 32];   // for the whole warp on one row
+    // per warp: the four rows on their way to the lanes' parts, each part padded by
+    // 16 bytes (eight lanes' 16-byte reads fall into different banks); later the
+    // f64 passes' space.  Loading the parts directly touched 32 lines an instruction.
+    constexpr int kRowFloats = 8 * (NV + 4);
+    __shared__ __align__(16) float sx[kRouteWarps][4 * kRowFloats];
+    __shared__ __align__(16) float sb[kRowFloats];    // the bias, as a row
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, sub = lane & 7;
-    const int64_t t = ((int64_t)blockIdx.x * kRouteWarps + warp) * 4 + (lane >> 3);
-    const int64_t tw = ((int64_t)blockIdx.x * kRouteWarps + warp) * 4;
+    const int per = kWhole ? NV : p.E / 8, e0 = sub * per;
+    const float inv_chunks = 4.0f / (float)per;       // chunks of four: of part (c + 1/2) / (per / 4)
+    auto place = [&](int c) { return 4 * c + 4 * (int)(((float)c + 0.5f) * inv_chunks); };
+    if (p.bias) {
+        for (int c = threadIdx.x; c < 2 * per; c += kRouteWarps * 32) {
+            float b[4];
+            load4(p.bias + 4 * c, b);
+            *reinterpret_cast<float4*>(sb + place(c)) = make_float4(b[0], b[1], b[2], b[3]);
+        }
+        __syncthreads();
+    }
+    const int64_t tw = ((int64_t)blockIdx.x * kRouteWarps + warp) * 4, t = tw + (lane >> 3);
     if (tw >= p.T) return;
     const bool live = t < p.T;                  // the last warp's lanes without a token work on its last one
     const T* row = static_cast<const T*>(p.x) + (live ? t : p.T - 1) * p.ld;
-    const int per = p.E / 8, e0 = sub * per;
+    float* const rows = sx[warp] + (lane >> 3) * kRowFloats;
+    double* const wide = reinterpret_cast<double*>(sx[warp]);
     float v[NV];
 #pragma unroll
+    for (int q = 0; q < NV; q += 4)
+        if (q < per) load4(row + 4 * (2 * q + sub), v + q);   // chunks sub, sub + 8, ..: 128 bytes of f32 a row
+#pragma unroll
+    for (int q = 0; q < NV; q += 4)
+        if (q < per) *reinterpret_cast<float4*>(rows + place(2 * q + sub)) = make_float4(v[q], v[q + 1], v[q + 2], v[q + 3]);
+    __syncwarp();
+#pragma unroll
     for (int q = 0; q < NV; q += 4) {
-        if (q < per) {
-            load4(row + e0 + q, v + q);
-        } else {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) v[q + i] = -INFINITY;
-        }
+        float4 x = make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+        if (q < per) x = *reinterpret_cast<const float4*>(rows + sub * (per + 4) + q);
+        v[q] = x.x; v[q + 1] = x.y; v[q + 2] = x.z; v[q + 3] = x.w;
     }
+    __syncwarp();
+    // Rows without masked experts (the whole warp's) skip the tests of every element.
+    float low = INFINITY, sum_all = 0.0f;
 #pragma unroll
-    for (int q = 0; q < NV; ++q) v[q] = selectable<T>(v[q]) ? v[q] : -INFINITY;
+    for (int q = 0; q < NV; ++q)
+        if (q < per) {
+            low = fminf(low, v[q]);
+            sum_all += v[q];
+        }
+    bool clean = __all_sync(kFull, selectable<T>(low) && sum_all == sum_all);
+    if (!clean) {
+#pragma unroll
+        for (int q = 0; q < NV; ++q) v[q] = selectable<T>(v[q]) ? v[q] : -INFINITY;
+    }
 
     const bool pair = p.group_top == 2;
     const bool exact = p.bias == nullptr && sizeof(T) == 2;
     float top = 0.0f, inv_sum = 1.0f;
     float a = -INFINITY, b = -INFINITY;         // the lane's two best members (the group's, where there are eight)
-    auto member = [&](float m) {
-        b = fmaxf(b, fminf(a, m));
-        a = fmaxf(a, m);
-    };
     if (!p.sigmoid && (p.bias || pair || !p.renorm)) {
         top = v[0];
 #pragma unroll
@@ -661,25 +676,47 @@ __global__ void __launch_bounds__(kRouteWarps * 32) route_many_kernel(const __gr
         return p.sigmoid ? rcp_fast(1.0f + exp_fast(-x)) : (x == top ? 1.0f : exp_fast(x - top)) * inv_sum;
     };
     if (p.bias) {
+        low = INFINITY;
+        sum_all = 0.0f;
 #pragma unroll
         for (int q = 0; q < NV; q += 4) {
             if (q >= per) continue;
-            float bias[4];
-            load4(p.bias + e0 + q, bias);
+            const float4 b4 = *reinterpret_cast<const float4*>(sb + sub * (per + 4) + q);
+            const float bias[4] = {b4.x, b4.y, b4.z, b4.w};
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
-                v[q + i] = v[q + i] > -INFINITY && bias[i] > kMasked ? score(v[q + i]) + bias[i] : -INFINITY;
+            for (int i = 0; i < 4; ++i) {
+                if (clean) {
+                    v[q + i] = score(v[q + i]) + bias[i];
+                    low = fminf(low, v[q + i]);
+                    sum_all += v[q + i];
+                } else {
+                    v[q + i] = v[q + i] > -INFINITY && bias[i] > kMasked ? score(v[q + i]) + bias[i] : -INFINITY;
+                }
+            }
+        }
+        if (clean && !__all_sync(kFull, low > 0.1f * kMasked && sum_all == sum_all)) {   // a masking bias
+            clean = false;
+#pragma unroll
+            for (int q = 0; q < NV; ++q)
+                if (q < per && !(__ldg(p.bias + e0 + q) > kMasked)) v[q] = -INFINITY;
         }
     }
     const float err2 = p.sigmoid ? 6e-7f : 4.2e-6f * inv_sum;   // as above
+    uint32_t keep = ~kIdx;
     if (p.G > 1) {
-        if (pair && !p.bias) {
+        if (!pair) {
 #pragma unroll
-            for (int q = 0; q < NV; ++q) member(v[q] == -INFINITY ? v[q] : score(v[q]));
+            for (int q = 0; q < NV; ++q) a = fmaxf(a, v[q]);
         } else {
 #pragma unroll
-            for (int q = 0; q < NV; ++q) member(v[q]);
+            for (int q = 0; q < NV; ++q) {
+                if (q >= per) continue;
+                const float m = p.bias || v[q] == -INFINITY ? v[q] : score(v[q]);
+                b = fmaxf(b, fminf(a, m));
+                a = fmaxf(a, m);
+            }
         }
+        const float least = pair ? b : a;       // of the members that score the group
         if (pair && b != -INFINITY) a += b;
         const uint32_t mine = a != -INFINITY ? order_key(a) : 0u;
         int rank = 0;
@@ -695,38 +732,87 @@ __global__ void __launch_bounds__(kRouteWarps * 32) route_many_kernel(const __gr
             const float lo = key_value(worst), hi = key_value(other);
             near = (p.bias || pair) && !(lo - hi > 2.0f * err2 + 6e-7f * fmaxf(fabsf(lo), fabsf(hi)));
         }
-        const unsigned bad = __ballot_sync(kFull, near);
+        unsigned bad = __ballot_sync(kFull, near);
+        if (bad != 0 && p.sigmoid) {
+            // every lane its group's one or two members in f64, where f32 values tell them from the others
+            const float from = least - (err2 + 3e-7f * fabsf(least));
+            int first = -1, second = -1, count = 0;
+#pragma unroll 4
+            for (int q = 0; q < NV; ++q) {
+                if (q >= per) break;
+                const float x = to_f32<T>(row[e0 + q]);
+                float m = selectable<T>(x) ? rcp_fast(1.0f + exp_fast(-x)) : -INFINITY;
+                if (p.bias) {
+                    const float pb = __ldg(p.bias + e0 + q);
+                    m = pb > kMasked ? m + pb : -INFINITY;
+                }
+                if (m > -INFINITY && m >= from) {
+                    second = count == 1 ? q : second;
+                    first = count == 0 ? q : first;
+                    ++count;
+                }
+            }
+            double sum = 0.0;
+#pragma unroll 1
+            for (int h = 0; h < 2; ++h) {
+                const int q = h == 0 ? first : second;
+                if (q < 0) continue;
+                sum += 1.0 / (1.0 + exp(-(double)to_f32<T>(row[e0 + q])));
+                if (p.bias) sum += (double)__ldg(p.bias + e0 + q);
+            }
+            if (count == 0) sum = -INFINITY;
+            const double tie = pair && count > 0 ? 0x1p-49 * (1.0 + fabs(sum)) : 0.0;
+            int place = 0;
+#pragma unroll 1
+            for (int h = 1; h < 8; ++h) {
+                const double o = __shfl_xor_sync(kFull, sum, h);
+                place += o > sum + tie || (o >= sum - tie && (sub ^ h) < sub) ? 1 : 0;
+            }
+            const bool sure = count <= (pair ? 2 : 1) && least < INFINITY;
+            const unsigned unsure = __ballot_sync(kFull, near && !sure);
+            const bool settled = near && (unsure >> (lane & 24) & 255) == 0;
+            if (settled) stay = count > 0 && place < p.kept;
+            bad = __ballot_sync(kFull, near && !settled);
+        }
         if (bad != 0)
             for (int r = 0; r < 4; ++r) {
                 if ((bad >> (8 * r) & 255) == 0 || tw + r >= p.T) continue;
-                const uint32_t mask = groups_f64<T, NV / 4>(p, static_cast<const T*>(p.x) + (tw + r) * p.ld, sv[warp], lane);
+                const uint32_t mask = groups_f64<T>(p, static_cast<const T*>(p.x) + (tw + r) * p.ld, wide, lane);
                 if (lane >> 3 == r) stay = mask >> sub & 1;
             }
-#pragma unroll
-        for (int q = 0; q < NV; ++q) v[q] = stay ? v[q] : -INFINITY;
+        keep = stay ? ~kIdx : 0u;
     }
 
+    // keys: a lane that does not stay, masked and missing experts keep the place alone (<= kIdx)
     uint32_t key[NV];
 #pragma unroll
-    for (int q = 0; q < NV; ++q) key[q] = v[q] == -INFINITY ? 0u : (order_key(v[q]) & ~kIdx) | (kIdx - q);
+    for (int q = 0; q < NV; ++q) {
+        key[q] = 0;
+        if (q < per) key[q] = (order_key(v[q]) & keep) | (kIdx - q);
+        if (!clean && v[q] == -INFINITY) key[q] = 0;
+    }
     top8<NV>(key);
     // rounds: the largest value, then the lowest lane (in the bits of the place), whose first key is popped
     uint32_t val = 0;                           // lane l: the value bits of the l-th choice
-    int my_i = -1, extra = -1, n = 0;
-    auto best = [&]() { return max8(key[0] != 0 ? (key[0] & ~kIdx) | (7 - sub) : 0u); };
-    auto pop = [&](uint32_t m) {                // the expert of the winner
+    int my_i = -1, extra = -1, n = 0, taken = 0;
+    auto best = [&]() { return max8(key[0] > kIdx ? (key[0] & ~kIdx) | (7 - sub) : 0u); };
+    auto pop = [&](uint32_t m, int last) {      // the expert of the winner; key[0..last) are wanted afterwards
         const int wl = 7 - (int)(m & kIdx);
         const int e = __shfl_sync(kFull, e0 + (int)(kIdx - (key[0] & kIdx)), (lane & 24) | wl);
         if (m != 0 && sub == wl) {
 #pragma unroll
-            for (int q = 0; q < 7; ++q) key[q] = key[q + 1];
-            key[7] = 0;
+            for (int q = 0; q < 7; ++q)
+                if (q < last) key[q] = key[q + 1];
+            if (last >= 7) key[7] = 0;
+            ++taken;
         }
         return e;
     };
-    for (int l = 0; l < p.k; ++l) {             // (no early end: the four tokens go together)
+#pragma unroll
+    for (int l = 0; l < 8; ++l) {               // (the four tokens go together)
+        if (l >= p.k) break;
         const uint32_t m = best();
-        const int e = pop(m);
+        const int e = pop(m, 7);
         n += m != 0 ? 1 : 0;
         if (sub == l && m != 0) {
             val = m & ~kIdx;
@@ -742,17 +828,19 @@ __global__ void __launch_bounds__(kRouteWarps * 32) route_many_kernel(const __gr
         uint32_t next = __shfl_down_sync(kFull, val, 1, 8);
         if (sub == n - 1) next = out & ~kIdx;
         const bool near = sub < n && next != 0 && close(val, next);
-        const unsigned bad = __ballot_sync(kFull, near);
+        // a lane's list ends at its eighth: with one left at most, what follows is not known
+        const bool spent = per > 8 && taken >= 7;
+        const unsigned bad = __ballot_sync(kFull, near || spent);
         if (bad != 0) {
             // the last choice and the first left are close: the latter is a candidate too, if the one behind it is not
             const bool border = near && sub == n - 1;
             const bool grow = (__ballot_sync(kFull, border) >> (lane & 24) & 255) != 0;
-            const int e = pop(grow ? out : 0u);
+            const int e = pop(grow ? out : 0u, 7);
             const uint32_t after = best() & ~kIdx;
-            bool redo = false;                  // of the token: the whole row in f64
+            bool redo = spent;                  // of the token: the whole row in f64
             if (grow) {
                 extra = e;
-                redo = after != 0 && close(out & ~kIdx, after);
+                redo |= after != 0 && close(out & ~kIdx, after);
             }
             const unsigned again = __ballot_sync(kFull, redo);
             for (int r = 0; r < 4; ++r) {
@@ -760,14 +848,14 @@ __global__ void __launch_bounds__(kRouteWarps * 32) route_many_kernel(const __gr
                 const T* rr = static_cast<const T*>(p.x) + (tw + r) * p.ld;
                 int got;
                 if ((again >> (8 * r) & 255) != 0) {
-                    got = route_row_f64<T, NV / 4>(p, rr, sv[warp], lane);
+                    got = route_row_f64<T>(p, rr, wide, lane);
                 } else {
                     const int count = __shfl_sync(kFull, n, 8 * r), ex = __shfl_sync(kFull, extra, 8 * r);
                     const int c = __shfl_sync(kFull, my_i, 8 * r + (lane & 7));
                     const float tp = __shfl_sync(kFull, top, 8 * r), is = __shfl_sync(kFull, inv_sum, 8 * r);
                     const float er = __shfl_sync(kFull, err2, 8 * r);
-                    got = rank_candidates<T, NV / 4>(p, rr, tp, is, er, lane < count ? c : ex, count + (ex >= 0 ? 1 : 0),
-                                                     reinterpret_cast<int*>(sv[warp]), lane);
+                    got = rank_candidates<T>(p, rr, tp, is, er, lane < count ? c : ex, count + (ex >= 0 ? 1 : 0),
+                                                     reinterpret_cast<int*>(wide), lane);
                     __syncwarp();
                 }
                 got = __shfl_sync(kFull, got, sub);
@@ -805,7 +893,8 @@ constexpr int64_t kManyTokens = 4096;
 
 template <typename T, int NV>
 cudaError_t launch_many(const RouteParams& p, cudaStream_t st) {
-    route_many_kernel<T, NV><<<(unsigned)((p.T + 4 * kRouteWarps - 1) / (4 * kRouteWarps)), kRouteWarps * 32, 0, st>>>(p);
+    auto kern = p.E == 8 * NV ? route_many_kernel<T, NV, true> : route_many_kernel<T, NV, false>;
+    kern<<<(unsigned)((p.T + 4 * kRouteWarps - 1) / (4 * kRouteWarps)), kRouteWarps * 32, 0, st>>>(p);
     return cudaGetLastError();
 }
 
@@ -814,7 +903,9 @@ cudaError_t launch_many(const RouteParams& p, cudaStream_t st) {
 template <typename T>
 bool try_many(RouteParams p, cudaStream_t st, cudaError_t* err) {
     const int per = p.E / 8;
+    // (one group kept: every choice comes from one lane, whose list of eight must reach two further)
     if (p.T < kManyTokens || p.E % 32 != 0 || p.E > 256 || p.k > 8 || (p.G != 1 && p.G != 8) ||
+        (p.G == 8 && p.kept == 1 && per > 8 && p.k > 6) ||
         reinterpret_cast<uintptr_t>(p.x) % (4 * sizeof(T)) != 0 || p.ld % 4 != 0 ||
         reinterpret_cast<uintptr_t>(p.bias) % 16 != 0)
         return false;

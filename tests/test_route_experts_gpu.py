@@ -237,6 +237,29 @@ def test_large_batches_equal_small_ones(gpu, E, groups, kept, score, dtype):
     np.testing.assert_allclose(w[rows.cuda()].cpu().double().numpy(), rw, rtol=REL[True], atol=1e-37)
 
 
+@pytest.mark.parametrize("groups, kept", [(1, 1), (8, 1), (8, 2)])
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("k", [5, 6, 7, 8])
+def test_large_batches_with_all_choices_in_one_part(gpu, groups, kept, score, k):
+    """The best experts neighbours of each other, closer than f32 scores tell apart: the border behind the last
+    choice lies within them."""
+    x = logits_of(4200, 256, torch.float32, 21)
+    g = torch.Generator().manual_seed(k)
+    close = (torch.stack([torch.randperm(32, generator=g) for _ in range(4200)]).float() * 2.0 ** -22 + 4.0).cuda()
+    x[:, 64:96] = close                        # one part of 32 holds every choice
+    x[2000:3000, 96:98] = 4.0                  # and ties with it in the next
+    b = (torch.round(torch.randn(256, generator=g) * 2) / 64).cuda()
+    b[64:96] = 0.25
+    for bias in (None, b, torch.zeros(256).cuda()):
+        for top in (1, 2):
+            kw = dict(score=score, bias=bias, groups=groups, kept_groups=kept, group_top=top)
+            idx, w = sm.route_experts(x, k, **kw)
+            parts = [sm.route_experts(x[i: i + 2100], k, **kw) for i in (0, 2100)]
+            assert torch.equal(idx, torch.cat([p[0] for p in parts]))
+            ri, _ = route_ref(x[1995:2005], k, score, bias, groups, kept, top, True, 1.0)
+            np.testing.assert_array_equal(idx[1995:2005].cpu().numpy(), ri)
+
+
 def test_streams_and_graphs(gpu):
     x = logits_of(500, 256, torch.float32, 11)
     kw = dict(score="sigmoid", groups=8, kept_groups=4, group_top=2, bias=torch.zeros(256, device=gpu), scale=2.5)
