@@ -542,11 +542,12 @@ __global__ void __launch_bounds__(kRouteWarps * 32) route_kernel(const __grid_co
 // experts l*per .. l*per + per - 1 (per = E / 8: one group, where there are
 // eight).  Everything that a round costs a warp is then paid for four tokens, and
 // a group's score needs no shuffle.  A lane keeps the eight best of its experts
-// in order (sorting networks of eight, merged); k <= 8.  Rows in which neighbours
-// are too close for f32 are done again by the whole warp.  32768 x 256, sigmoid,
-// bias, 4 of 8 groups: 883 warp instructions a token and 35 us with a warp a
-// token, 300 and 16 us so; below about 4000 tokens the warp a token is faster,
-// its chain of dependent instructions being a third as long.
+// in order (sorting networks of eight, merged); k <= 8.  500 warp instructions a
+// token for the 880 of a warp a token (256 experts, bias, groups), half of them
+// on the half-rate ALU pipe, which bounds both; the chain that a warp runs
+// through is longer.  Measured (us, a warp a token / four a warp): 256 experts in
+// groups 8192 tokens 11.9 / 14.5, 16384 19.4 / 16.5, 32768 32.3 / 26.7; 64 experts 4096
+// tokens 3.2 / 2.9, 16384 7.6 / 4.9, 32768 13.0 / 7.5.
 __device__ __forceinline__ uint32_t max8(uint32_t v) {   // over a token's eight lanes
 #pragma unroll
     for (int o = 4; o > 0; o >>= 1) v = max(v, __shfl_xor_sync(kFull, v, o));
@@ -603,7 +604,7 @@ template <int NV> __device__ __forceinline__ void top8(uint32_t (&key)[NV]) {
 }
 
 template <typename T, int NV, bool kWhole>   // kWhole: per == NV
-__global__ void __launch_bounds__(kRouteWarps * 32) route_many_kernel(const __grid_constant__ RouteParams p) {
+__global__ void __launch_bounds__(kRouteWarps * 32, 7) route_many_kernel(const __grid_constant__ RouteParams p) {
     constexpr uint32_t kIdx = NV - 1;           // the key bits that hold the place in the lane
     // per warp: the four rows on their way to the lanes' parts, each part padded by
     // 16 bytes (eight lanes' 16-byte reads fall into different banks); later the
@@ -888,9 +889,6 @@ __global__ void __launch_bounds__(kRouteWarps * 32) route_many_kernel(const __gr
     }
 }
 
-// Tokens from which four share a warp.
-constexpr int64_t kManyTokens = 4096;
-
 template <typename T, int NV>
 cudaError_t launch_many(const RouteParams& p, cudaStream_t st) {
     auto kern = p.E == 8 * NV ? route_many_kernel<T, NV, true> : route_many_kernel<T, NV, false>;
@@ -904,7 +902,7 @@ template <typename T>
 bool try_many(RouteParams p, cudaStream_t st, cudaError_t* err) {
     const int per = p.E / 8;
     // (one group kept: every choice comes from one lane, whose list of eight must reach two further)
-    if (p.T < kManyTokens || p.E % 32 != 0 || p.E > 256 || p.k > 8 || (p.G != 1 && p.G != 8) ||
+    if (p.T < (per <= 8 ? 4096 : 16384) || p.E % 32 != 0 || p.E > 256 || p.k > 8 || (p.G != 1 && p.G != 8) ||
         (p.G == 8 && p.kept == 1 && per > 8 && p.k > 6) ||
         reinterpret_cast<uintptr_t>(p.x) % (4 * sizeof(T)) != 0 || p.ld % 4 != 0 ||
         reinterpret_cast<uintptr_t>(p.bias) % 16 != 0)
