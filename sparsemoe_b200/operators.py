@@ -15,8 +15,13 @@ import functools
 
 import torch
 
-from . import _operators, check, lib
+from . import _PKG, check, lib
 from .config import MOE_SCORES, MOE_WEIGHT_KN, MOE_WEIGHT_NK, MoeInt8Weight, MoeRouting
+
+try:
+    from . import _operators
+except ImportError as e:
+    raise ImportError(f"{_PKG / '_operators.so'} cannot be loaded ({e}): build it with `python sparsemoe_b200/build.py`") from e
 
 _operators.bind(check, *(ctypes.cast(f, ctypes.c_void_p).value for f in (
     lib.moe_route_experts, lib.moe_int8_quantize_tokens, lib.moe_int8_matmul, lib.moe_int8_linear,
@@ -64,9 +69,9 @@ def route_experts(logits: torch.Tensor, top_k: int, *, score: str = "softmax", b
     Returns (indices int32 [T, top_k], weights f32 [T, top_k]), in descending
     order of the experts' values (score + `bias`, a selection bias [E] f32 that
     leaves the weights alone; without one the logits), equal values by the
-    lower index, as f64 arithmetic on the logits orders them.  Experts masked by a logit
-    that is NaN, -inf, <= -1e20 or f16's lowest value, or by such a bias, are
-    never chosen; slots left empty hold (-1, 0).  `out`: the two contiguous
+    lower index, as f64 arithmetic on the logits orders them.  Experts masked
+    by a logit that is NaN, -inf, <= -1e20 or f16's lowest value, or by such a
+    bias, are never chosen; slots left empty hold (-1, 0).  `out`: the two contiguous
     tensors to write instead.
     """
     spec = _routing(score, groups, kept_groups, group_top, renormalise, scale)
