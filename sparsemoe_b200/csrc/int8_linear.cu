@@ -182,8 +182,8 @@ template <typename T, int TPR, bool kPair>
 __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 8 : 5)
     quantize_tokens_kernel(const T* x, int64_t rows, int K, int64_t ldx, int64_t up, int8_t* q, int64_t ldq,
                            float* scale, int vec) {
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-    asm volatile("griddepcontrol.wait;" ::: "memory");
+    pdl_wait();
+    pdl_trigger();
     constexpr int kRows = 256 / TPR;
     __shared__ uint32_t red[8];
     const int tr = threadIdx.x % TPR;
@@ -263,7 +263,7 @@ struct LinearParams {
     int split;                 // CTAs of a cluster that share a tile's K
     int a_rows;                // rows of the A box
     int b_nk;                  // weights [N, K] (K-contiguous) rather than [K, N]
-    int pdl;                   // launched while its predecessor may still run
+    int ahead;                 // weights may be loaded before the wait
     const float* s_tok;
     const float* s_ch0;        // channel scales (swiglu: gate)
     const float* s_ch1;        // swiglu: up
@@ -296,7 +296,6 @@ struct LinearCfg {
     static constexpr size_t kSmem = 1024 + (size_t)kStages * kStageBytes + kRecvBytes + 256;
 };
 
-__device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ uint32_t cluster_rank() {
     uint32_t r;
     asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
@@ -709,15 +708,17 @@ __global__ void __launch_bounds__(kThreads, 1)
                     if (kBN == 256) load(dst + C::kBBytes / 2, b1, s, kSwiglu ? col : col + 128, k0);
                 }
             };
-            // the weights of the first stages do not depend on the kernel before this one
+            // ahead: the kernel before this one is this call's quantiser, which lets this one start after its own
+            // wait; whoever wrote the weights came before it and has ended
             int ahead = 0;
-            if (p.pdl) {
+            if (p.ahead) {
                 for (int kb = kb0; tile0 < total && kb < kb1 && ahead < C::kStages; ++kb, ++ahead) {
                     expect(ahead);
                     load_b(ahead, tile0 / p.m_tiles, kb);
                 }
-                pdl_wait();
             }
+            pdl_wait();
+            pdl_trigger();
             int s = 0;
             uint32_t ph = 0;
             for (int t = tile0; t < total; t += step) {
@@ -776,7 +777,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
     } else {
         // ---------------- epilogue (warps 2..9) ----------------
-        if (p.pdl) pdl_wait();
+        pdl_wait();
         if (p.split > 1) cluster_wait();
         constexpr int kCols = kOutN / 2;          // output columns of a warp
         const int q = warp & 3, half = (warp - 2) >> 2;
@@ -795,8 +796,8 @@ __global__ void __launch_bounds__(kThreads, 1)
             for (int c = etid; c < kBN; c += kEpiThreads) {
                 const int col = tile_col + (kSwiglu ? c % kOutN : c);
                 const float* src = second || (kSwiglu && c >= kOutN) ? p.s_ch1 : p.s_ch0;
-                scales[c] = col < p.N ? __ldg(src + col) : 0.0f;
-                biases[c] = !kSwiglu && p.bias && col < p.N ? __ldg(p.bias + col) : 0.0f;
+                scales[c] = col < p.N ? src[col] : 0.0f;
+                biases[c] = !kSwiglu && p.bias && col < p.N ? p.bias[col] : 0.0f;
             }
             asm volatile("bar.sync 1, 256;" ::: "memory");
             const float* const sc = scales + half * kCols;
@@ -941,7 +942,7 @@ struct SmallParams {
     const float* s_tok;        // codes given: their scales
     int T, K, N;
     int kblocks, split, stages;
-    int b_nk, pdl, vec_x;
+    int b_nk, ahead, vec_x;
     const float* s_ch0;
     const float* s_ch1;
     const float* bias;
@@ -1013,7 +1014,6 @@ __global__ void __launch_bounds__(kSmallThreads, 2)
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     const uint32_t tmem_base = *tmem_slot;
     const bool split = p.split > 1;
     if (split) cluster_arrive();   // phase 1: every CTA has started
@@ -1031,8 +1031,12 @@ __global__ void __launch_bounds__(kSmallThreads, 2)
             else tma_load_2d(sW + s * kSmallStageBytes, map, &full[s], col0, k);
         };
         const int first = min(p.stages, loads);
-        if (lane == 0)
+        if (lane == 0) {
+            if (!p.ahead) pdl_wait();
             for (int i = 0; i < first; ++i) load(i, i);
+            if (p.ahead) pdl_wait();
+            pdl_trigger();
+        }
         __syncwarp();
         if (split) {   // phases 1 and 2, before any wait that the other warps' progress ends
             cluster_wait();
@@ -1080,7 +1084,7 @@ __global__ void __launch_bounds__(kSmallThreads, 2)
         }
     } else {
         // ---------------- quantiser, then epilogue (warps 2..9) ----------------
-        if (p.pdl) pdl_wait();
+        pdl_wait();
         const int w = warp - 2;
         const int k0 = kb0 * kBK, k1 = min(p.K, kb1 * kBK);
         const T* const x = static_cast<const T*>(p.x);
@@ -1198,9 +1202,9 @@ __global__ void __launch_bounds__(kSmallThreads, 2)
         auto put = [&](int sum, int sum1, int t, int ch) {   // channel ch of the tile
             const int col = col0 + ch;
             if (col >= p.N) return;
-            float v = (float)sum * s_tok[t] * __ldg(p.s_ch0 + col);
-            if (kSwiglu) v = (float)sum1 * s_tok[t] * __ldg(p.s_ch1 + col) * silu(v);
-            if (p.bias) v += __ldg(p.bias + col);
+            float v = (float)sum * s_tok[t] * p.s_ch0[col];
+            if (kSwiglu) v = (float)sum1 * s_tok[t] * p.s_ch1[col] * silu(v);
+            if (p.bias) v += p.bias[col];
             if (p.residual) v += load_as_f32(p.residual, t * p.ld_res + col, p.res_type);
             const int64_t at = t * p.ld_out + col;
             if (p.out_type == MOE_TYPE_F32) static_cast<float*>(p.out)[at] = v;
@@ -1272,8 +1276,8 @@ int64_t up16(int64_t v) { return (v + 15) / 16 * 16; }
 size_t up256(size_t v) { return (v + 255) & ~size_t(255); }
 
 template <typename... P, typename... A>
-cudaError_t launch_ex(void (*kern)(P...), unsigned grid, unsigned threads, size_t smem, int cluster, bool pdl,
-                      cudaStream_t st, A... args) {
+cudaError_t launch_ex(void (*kern)(P...), unsigned grid, unsigned threads, size_t smem, int cluster, cudaStream_t st,
+                      A... args) {
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3(grid);
     cfg.blockDim = dim3(threads);
@@ -1286,11 +1290,9 @@ cudaError_t launch_ex(void (*kern)(P...), unsigned grid, unsigned threads, size_
         at[n].val.clusterDim = {(unsigned)cluster, 1, 1};
         ++n;
     }
-    if (pdl) {
-        at[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-        at[n].val.programmaticStreamSerializationAllowed = 1;
-        ++n;
-    }
+    at[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;   // (see pdl_wait)
+    at[n].val.programmaticStreamSerializationAllowed = 1;
+    ++n;
     cfg.attrs = at;
     cfg.numAttrs = n;
     return cudaLaunchKernelEx(&cfg, kern, P(args)...);
@@ -1298,7 +1300,7 @@ cudaError_t launch_ex(void (*kern)(P...), unsigned grid, unsigned threads, size_
 
 template <typename T, bool kPair>
 cudaError_t launch_quantize_typed(const T* x, int64_t rows, int K, int64_t ldx, int64_t up, int8_t* q, int64_t ldq,
-                                  float* s, bool pdl, cudaStream_t st) {
+                                  float* s, cudaStream_t st) {
     const int vec = aligned(x, 16) && (ldx * (int64_t)sizeof(T)) % 16 == 0;
     // as many threads a row as hold it in registers, four vectors of eight each
     const int tpr = K <= 1024 ? 32 : K <= 2048 ? 64 : K <= 4096 ? 128 : 256;
@@ -1307,23 +1309,22 @@ cudaError_t launch_quantize_typed(const T* x, int64_t rows, int K, int64_t ldx, 
                 : tpr == 64  ? quantize_tokens_kernel<T, 64, kPair>
                 : tpr == 128 ? quantize_tokens_kernel<T, 128, kPair>
                              : quantize_tokens_kernel<T, 256, kPair>;
-    return launch_ex(kern, (unsigned)blocks, 256u, 0, 1, pdl, st, x, rows, K, ldx, up, q, ldq, s, vec);
+    return launch_ex(kern, (unsigned)blocks, 256u, 0, 1, st, x, rows, K, ldx, up, q, ldq, s, vec);
 }
 
 // up != 0: x holds f32 gate values with the up values `up` elements behind.
 cudaError_t launch_quantize(const void* x, int type, int64_t rows, int K, int64_t ldx, int64_t up, int8_t* q,
-                            int64_t ldq, float* s, bool pdl, cudaStream_t st) {
+                            int64_t ldq, float* s, cudaStream_t st) {
     if (up != 0)
-        return launch_quantize_typed<float, true>(static_cast<const float*>(x), rows, K, ldx, up, q, ldq, s, pdl, st);
+        return launch_quantize_typed<float, true>(static_cast<const float*>(x), rows, K, ldx, up, q, ldq, s, st);
     switch (type) {
         case MOE_TYPE_F32:
-            return launch_quantize_typed<float, false>(static_cast<const float*>(x), rows, K, ldx, 0, q, ldq, s, pdl, st);
+            return launch_quantize_typed<float, false>(static_cast<const float*>(x), rows, K, ldx, 0, q, ldq, s, st);
         case MOE_TYPE_F16:
-            return launch_quantize_typed<__half, false>(static_cast<const __half*>(x), rows, K, ldx, 0, q, ldq, s, pdl,
-                                                        st);
+            return launch_quantize_typed<__half, false>(static_cast<const __half*>(x), rows, K, ldx, 0, q, ldq, s, st);
         default:
             return launch_quantize_typed<__nv_bfloat16, false>(static_cast<const __nv_bfloat16*>(x), rows, K, ldx, 0, q,
-                                                               ldq, s, pdl, st);
+                                                               ldq, s, st);
     }
 }
 
@@ -1336,7 +1337,7 @@ cudaError_t launch_linear_cfg(const CUtensorMap& a, const CUtensorMap (&b)[2], c
     const int ctas = kPair ? 2 : p.split;
     cudaError_t err = ensure_smem(kern, smem, attr);
     if (err != cudaSuccess) return err;
-    return launch_ex(kern, (unsigned)(clusters * ctas), (unsigned)kThreads, smem, ctas, p.pdl != 0, st, a, b[0], b[1],
+    return launch_ex(kern, (unsigned)(clusters * ctas), (unsigned)kThreads, smem, ctas, st, a, b[0], b[1],
                      o[0], o[1], p);
 }
 
@@ -1448,7 +1449,7 @@ cudaError_t launch_small_typed(const CUtensorMap (&w)[2], const SmallParams& p, 
     static SmemAttr attr;
     cudaError_t err = ensure_smem(kern, smem, attr);
     if (err != cudaSuccess) return err;
-    return launch_ex(kern, (unsigned)(tiles * p.split), (unsigned)kSmallThreads, smem, p.split, p.pdl != 0, st, w[0], w[1],
+    return launch_ex(kern, (unsigned)(tiles * p.split), (unsigned)kSmallThreads, smem, p.split, st, w[0], w[1],
                      p);
 }
 
@@ -1491,7 +1492,7 @@ bool try_small(int limit, const void* x, int x_type, int64_t ld_x, const LinearP
     p.split = split;
     p.stages = stages;
     p.b_nk = l.b_nk;
-    p.pdl = l.pdl;
+    p.ahead = l.ahead;
     p.s_ch0 = w0.scale;
     p.s_ch1 = w1 ? w1->scale : w0.scale;
     p.bias = l.bias;
@@ -1588,13 +1589,12 @@ int cuda_error(const char* who, cudaError_t e) {
 }
 
 LinearParams out_params(int64_t T, int K, int N, const float* s_tok, const float* bias, void* out, int out_type,
-                        int64_t ldo, int order, bool pdl) {
+                        int64_t ldo, int order) {
     LinearParams p{};
     p.T = (int)T;
     p.K = K;
     p.N = N;
     p.b_nk = order == MOE_WEIGHT_NK;
-    p.pdl = pdl;
     p.s_tok = s_tok;
     p.bias = bias;
     p.out = out;
@@ -1687,9 +1687,10 @@ int run_shared_expert(const char* who, const void* x, int x_type, int64_t tokens
     const int64_t behind = (int64_t)(up256((size_t)tokens * sc.ldh * sizeof(float)) / sizeof(float));
     const Matrix mg{gate->w, gate->row_stride, gate->scale}, mu{up->w, up->row_stride, up->scale},
         md{down->w, down->row_stride, down->scale};
-    LinearParams ph = out_params(tokens, d_model, d_ff, sx, nullptr, h, MOE_TYPE_F32, sc.ldh, gate->order, false);
+    LinearParams ph = out_params(tokens, d_model, d_ff, sx, nullptr, h, MOE_TYPE_F32, sc.ldh, gate->order);
     ph.out1 = behind;
-    LinearParams py = out_params(tokens, d_ff, d_model, sh, nullptr, out, out_type, out_stride, down->order, true);
+    LinearParams py = out_params(tokens, d_ff, d_model, sh, nullptr, out, out_type, out_stride, down->order);
+    py.ahead = 1;
     py.residual = residual;
     py.ld_res = residual_stride;
     py.res_type = x_type;
@@ -1698,14 +1699,14 @@ int run_shared_expert(const char* who, const void* x, int x_type, int64_t tokens
     // gate and up: h, or (too few tiles to fuse) g and u
     const bool small = is_small(tokens, kSmallShared, d_model, 2);
     if (!small || !try_small(kSmallShared, x, x_type, row_stride, ph, mg, &mu, num_sms, stream, &e)) {
-        ph.pdl = 1;
-        e = launch_quantize(x, x_type, tokens, d_model, row_stride, 0, qx, up16(d_model), sx, false, stream);
+        ph.ahead = 1;
+        e = launch_quantize(x, x_type, tokens, d_model, row_stride, 0, qx, up16(d_model), sx, stream);
         if (e == cudaSuccess) e = launch_linear(qx, up16(d_model), ph, mg, &mu, fused, num_sms, stream);
     }
     if (e != cudaSuccess) return cuda_error(who, e);
     const bool pairs = !fused && !small;
     if (pairs || !try_small(kSmallShared, h, MOE_TYPE_F32, sc.ldh, py, md, nullptr, num_sms, stream, &e)) {
-        e = launch_quantize(h, MOE_TYPE_F32, tokens, d_ff, sc.ldh, pairs ? behind : 0, qh, up16(d_ff), sh, true, stream);
+        e = launch_quantize(h, MOE_TYPE_F32, tokens, d_ff, sc.ldh, pairs ? behind : 0, qh, up16(d_ff), sh, stream);
         if (e == cudaSuccess) e = launch_linear(qh, up16(d_ff), py, md, nullptr, false, num_sms, stream);
     }
     return e == cudaSuccess ? MOE_OK : cuda_error(who, e);
@@ -1735,7 +1736,7 @@ extern "C" int moe_int8_quantize_tokens(const void* x, int x_type, int64_t token
     int dev = 0, num_sms = 0;
     rc = current_device(&dev, &num_sms);
     if (rc != MOE_OK) return rc;
-    const cudaError_t e = launch_quantize(x, x_type, tokens, K, row_stride, 0, q, q_stride, scale, false, stream);
+    const cudaError_t e = launch_quantize(x, x_type, tokens, K, row_stride, 0, q, q_stride, scale, stream);
     return e == cudaSuccess ? MOE_OK : cuda_error(who, e);
 }
 
@@ -1755,7 +1756,7 @@ extern "C" int moe_int8_matmul(const int8_t* q, int64_t q_stride, const float* s
     rc = current_device(&dev, &num_sms);
     if (rc != MOE_OK) return rc;
     g_linear_used[dev] = true;
-    const LinearParams p = out_params(tokens, K, N, scale, bias, out, out_type, out_stride, w->order, false);
+    const LinearParams p = out_params(tokens, K, N, scale, bias, out, out_type, out_stride, w->order);
     const Matrix m{w->w, w->row_stride, w->scale};
     cudaError_t e;
     if (!try_small(kSmallCodes, q, -1, q_stride, p, m, nullptr, num_sms, stream, &e))
@@ -1782,12 +1783,12 @@ extern "C" int moe_int8_linear(const void* x, int x_type, int64_t tokens, int K,
     g_linear_used[dev] = true;
     int8_t* q = static_cast<int8_t*>(scratch);   // (null where the small kernel needs none)
     float* s = q ? reinterpret_cast<float*>(q + up256((size_t)tokens * up16(K))) : nullptr;
-    LinearParams p = out_params(tokens, K, N, s, bias, out, out_type, out_stride, w->order, false);
+    LinearParams p = out_params(tokens, K, N, s, bias, out, out_type, out_stride, w->order);
     const Matrix m{w->w, w->row_stride, w->scale};
     cudaError_t e;
     if (!try_small(kSmallLinear, x, x_type, row_stride, p, m, nullptr, num_sms, stream, &e)) {
-        p.pdl = 1;
-        e = launch_quantize(x, x_type, tokens, K, row_stride, 0, q, up16(K), s, false, stream);
+        p.ahead = 1;
+        e = launch_quantize(x, x_type, tokens, K, row_stride, 0, q, up16(K), s, stream);
         if (e == cudaSuccess) e = launch_linear(q, up16(K), p, m, nullptr, false, num_sms, stream);
     }
     return e == cudaSuccess ? MOE_OK : cuda_error(who, e);

@@ -120,13 +120,13 @@ __device__ __forceinline__ void load_row(const T* row, int e0, int E, bool vec, 
         union { T v[NV]; uint4 q[(kBytes + 15) / 16]; uint2 d[(kBytes + 7) / 8]; uint32_t u[(kBytes + 3) / 4]; } r;
         if constexpr (kVec == 16) {
 #pragma unroll
-            for (int i = 0; i < kBytes / 16; ++i) r.q[i] = __ldg(reinterpret_cast<const uint4*>(row + e0) + i);
+            for (int i = 0; i < kBytes / 16; ++i) r.q[i] = reinterpret_cast<const uint4*>(row + e0)[i];
         } else if constexpr (kVec == 8) {
 #pragma unroll
-            for (int i = 0; i < kBytes / 8; ++i) r.d[i] = __ldg(reinterpret_cast<const uint2*>(row + e0) + i);
+            for (int i = 0; i < kBytes / 8; ++i) r.d[i] = reinterpret_cast<const uint2*>(row + e0)[i];
         } else if constexpr (kVec == 4) {
 #pragma unroll
-            for (int i = 0; i < kBytes / 4; ++i) r.u[i] = __ldg(reinterpret_cast<const uint32_t*>(row + e0) + i);
+            for (int i = 0; i < kBytes / 4; ++i) r.u[i] = reinterpret_cast<const uint32_t*>(row + e0)[i];
         }
 #pragma unroll
         for (int i = 0; i < NV; ++i) x[i] = to_f32<T>(r.v[i]);
@@ -168,7 +168,7 @@ __device__ __forceinline__ void values_f64(const RouteParams& p, const T* row, d
         if (u == -INFINITY) continue;
         double v = p.sigmoid ? 1.0 / (1.0 + u) : u / sum;
         if (p.bias) {
-            const float b = __ldg(p.bias + e);
+            const float b = p.bias[e];
             v = b > kMasked ? v + (double)b : -INFINITY;
         }
         buf[e] = v;
@@ -297,7 +297,7 @@ template <typename T>
 __device__ __noinline__ int rank_candidates(const RouteParams& p, const T* row, float top, float inv_sum, float err2,
                                             int cand, int n, int* buf, int lane) {
     const float x = lane < n ? to_f32<T>(row[cand]) : 0.0f;
-    const float b = p.bias && lane < n ? __ldg(p.bias + cand) : 0.0f;
+    const float b = p.bias && lane < n ? p.bias[cand] : 0.0f;
     float f = x;
     if (p.bias) f = (p.sigmoid ? rcp_fast(1.0f + exp_fast(-x)) : (x == top ? 1.0f : exp_fast(x - top)) * inv_sum) + b;
     int rank = 0;
@@ -345,6 +345,8 @@ template <typename T, int NV>
 __global__ void __launch_bounds__(kRouteWarps * 32) route_kernel(const __grid_constant__ RouteParams p) {
     constexpr uint32_t kIdx = 32 * NV - 1;      // the key bits that hold the index
     __shared__ double sv[kRouteWarps][NV * 32];
+    pdl_wait();
+    pdl_trigger();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int64_t t = (int64_t)blockIdx.x * kRouteWarps + warp;
     if (t >= p.T) return;
@@ -566,11 +568,11 @@ __device__ __forceinline__ float sum8(float v) {
 
 // Four consecutive elements (rows allow it: the host checks).
 __device__ __forceinline__ void load4(const float* p, float* x) {
-    const float4 a = __ldg(reinterpret_cast<const float4*>(p));
+    const float4 a = *reinterpret_cast<const float4*>(p);
     x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w;
 }
 template <typename T16> __device__ __forceinline__ void load4(const T16* p, float* x) {
-    const uint2 a = __ldg(reinterpret_cast<const uint2*>(p));
+    const uint2 a = *reinterpret_cast<const uint2*>(p);
     const float2 lo = F16Traits<T16>::unpack2(a.x), hi = F16Traits<T16>::unpack2(a.y);
     x[0] = lo.x; x[1] = lo.y; x[2] = hi.x; x[3] = hi.y;
 }
@@ -613,6 +615,8 @@ __global__ void __launch_bounds__(kRouteWarps * 32, 7) route_many_kernel(const _
     __shared__ __align__(16) float sx[kRouteWarps][4 * kRowFloats];
     __shared__ __align__(16) float sb[kRowFloats];    // the bias, as a row
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, sub = lane & 7;
+    pdl_wait();
+    pdl_trigger();
     const int per = kWhole ? NV : p.E / 8, e0 = sub * per;
     const float inv_chunks = 4.0f / (float)per;       // chunks of four: of part (c + 1/2) / (per / 4)
     auto place = [&](int c) { return 4 * c + 4 * (int)(((float)c + 0.5f) * inv_chunks); };
@@ -699,7 +703,7 @@ __global__ void __launch_bounds__(kRouteWarps * 32, 7) route_many_kernel(const _
             clean = false;
 #pragma unroll
             for (int q = 0; q < NV; ++q)
-                if (q < per && !(__ldg(p.bias + e0 + q) > kMasked)) v[q] = -INFINITY;
+                if (q < per && !(p.bias[e0 + q] > kMasked)) v[q] = -INFINITY;
         }
     }
     const float err2 = p.sigmoid ? 6e-7f : 4.2e-6f * inv_sum;   // as above
@@ -744,7 +748,7 @@ __global__ void __launch_bounds__(kRouteWarps * 32, 7) route_many_kernel(const _
                 const float x = to_f32<T>(row[e0 + q]);
                 float m = selectable<T>(x) ? rcp_fast(1.0f + exp_fast(-x)) : -INFINITY;
                 if (p.bias) {
-                    const float pb = __ldg(p.bias + e0 + q);
+                    const float pb = p.bias[e0 + q];
                     m = pb > kMasked ? m + pb : -INFINITY;
                 }
                 if (m > -INFINITY && m >= from) {
@@ -759,7 +763,7 @@ __global__ void __launch_bounds__(kRouteWarps * 32, 7) route_many_kernel(const _
                 const int q = h == 0 ? first : second;
                 if (q < 0) continue;
                 sum += 1.0 / (1.0 + exp(-(double)to_f32<T>(row[e0 + q])));
-                if (p.bias) sum += (double)__ldg(p.bias + e0 + q);
+                if (p.bias) sum += (double)p.bias[e0 + q];
             }
             if (count == 0) sum = -INFINITY;
             const double tie = pair && count > 0 ? 0x1p-49 * (1.0 + fabs(sum)) : 0.0;
@@ -825,24 +829,45 @@ __global__ void __launch_bounds__(kRouteWarps * 32, 7) route_many_kernel(const _
             const float hi = key_value(x), lo = key_value(y);
             return p.bias ? !(hi - lo > err2 + (NV * 1.2e-7f + 3e-7f) * fmaxf(fabsf(hi), fabsf(lo))) : !(hi > lo);
         };
+        // a list whose eight are all chosen goes on with the best of the lane's others
+        auto refill = [&](bool empty) {
+            if (!__any_sync(kFull, empty)) return;
+            uint32_t used = 0, more = 0;
+            for (int l = 0; l < 9; ++l) {
+                const int q = (l < 8 ? __shfl_sync(kFull, my_i, (lane & 24) | l) : extra) - e0;
+                if (q >= 0 && q < per) used |= 1u << q;
+            }
+#pragma unroll 4
+            for (int q = 0; q < NV; ++q) {
+                if (q >= per) break;
+                const float x = to_f32<T>(row[e0 + q]);
+                float m = selectable<T>(x) ? x : -INFINITY;
+                if (p.bias) {
+                    const float pb = p.bias[e0 + q];
+                    m = m > -INFINITY && pb > kMasked ? score(x) + pb : -INFINITY;
+                }
+                const uint32_t k = m == -INFINITY ? 0u : (order_key(m) & ~kIdx) | (kIdx - q);
+                if (!(used >> q & 1)) more = max(more, k);
+            }
+            if (empty) key[0] = more;
+        };
+        if (per > 8) refill(taken == 8);
         const uint32_t out = best();            // the first that was left
         uint32_t next = __shfl_down_sync(kFull, val, 1, 8);
         if (sub == n - 1) next = out & ~kIdx;
         const bool near = sub < n && next != 0 && close(val, next);
-        // a lane's list ends at its eighth: with one left at most, what follows is not known
-        const bool spent = per > 8 && taken >= 7;
-        const unsigned bad = __ballot_sync(kFull, near || spent);
+        const unsigned bad = __ballot_sync(kFull, near);
         if (bad != 0) {
             // the last choice and the first left are close: the latter is a candidate too, if the one behind it is not
             const bool border = near && sub == n - 1;
             const bool grow = (__ballot_sync(kFull, border) >> (lane & 24) & 255) != 0;
+            const int before = taken;
             const int e = pop(grow ? out : 0u, 7);
+            if (grow) extra = e;
+            if (per > 8) refill(taken > before && taken >= 8);
             const uint32_t after = best() & ~kIdx;
-            bool redo = spent;                  // of the token: the whole row in f64
-            if (grow) {
-                extra = e;
-                redo |= after != 0 && close(out & ~kIdx, after);
-            }
+            // of the token: the whole row in f64
+            const bool redo = grow && after != 0 && close(out & ~kIdx, after);
             const unsigned again = __ballot_sync(kFull, redo);
             for (int r = 0; r < 4; ++r) {
                 if ((bad >> (8 * r) & 255) == 0 || tw + r >= p.T) continue;
@@ -889,11 +914,23 @@ __global__ void __launch_bounds__(kRouteWarps * 32, 7) route_many_kernel(const _
     }
 }
 
+cudaError_t launch_kernel(void (*kern)(RouteParams), int64_t blocks, const RouteParams& p, cudaStream_t st) {
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3((unsigned)blocks);
+    cfg.blockDim = dim3(kRouteWarps * 32);
+    cfg.stream = st;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;   // (see pdl_wait)
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, kern, p);
+}
+
 template <typename T, int NV>
 cudaError_t launch_many(const RouteParams& p, cudaStream_t st) {
     auto kern = p.E == 8 * NV ? route_many_kernel<T, NV, true> : route_many_kernel<T, NV, false>;
-    kern<<<(unsigned)((p.T + 4 * kRouteWarps - 1) / (4 * kRouteWarps)), kRouteWarps * 32, 0, st>>>(p);
-    return cudaGetLastError();
+    return launch_kernel(kern, (p.T + 4 * kRouteWarps - 1) / (4 * kRouteWarps), p, st);
 }
 
 // True (and launched) where the shape fits: 8 parts of a multiple of 4 experts,
@@ -901,9 +938,7 @@ cudaError_t launch_many(const RouteParams& p, cudaStream_t st) {
 template <typename T>
 bool try_many(RouteParams p, cudaStream_t st, cudaError_t* err) {
     const int per = p.E / 8;
-    // (one group kept: every choice comes from one lane, whose list of eight must reach two further)
     if (p.T < (per <= 8 ? 4096 : 16384) || p.E % 32 != 0 || p.E > 256 || p.k > 8 || (p.G != 1 && p.G != 8) ||
-        (p.G == 8 && p.kept == 1 && per > 8 && p.k > 6) ||
         reinterpret_cast<uintptr_t>(p.x) % (4 * sizeof(T)) != 0 || p.ld % 4 != 0 ||
         reinterpret_cast<uintptr_t>(p.bias) % 16 != 0)
         return false;
@@ -921,9 +956,7 @@ cudaError_t launch_nv(RouteParams p, cudaStream_t st) {
     p.vec_bias = reinterpret_cast<uintptr_t>(p.bias) % kVecB == 0;
     const int whole = p.per % NV == 0 ? p.per / NV : 0;
     p.lanes = p.G > 1 && (whole & (whole - 1)) == 0 ? whole : 0;
-    const int64_t blocks = (p.T + kRouteWarps - 1) / kRouteWarps;
-    route_kernel<T, NV><<<(unsigned)blocks, kRouteWarps * 32, 0, st>>>(p);
-    return cudaGetLastError();
+    return launch_kernel(route_kernel<T, NV>, (p.T + kRouteWarps - 1) / kRouteWarps, p, st);
 }
 
 template <typename T>
