@@ -83,8 +83,9 @@ __device__ __forceinline__ void ffma2(float& a0, float& a1, float p0, float p1, 
 // Programmatic dependent launch.  The kernels of the stand-alone operators may
 // start while the kernel before them on the stream still runs.  Each waits for
 // that kernel's end (and so for everything before it) ahead of its first access
-// of memory, and only then lets the kernel behind it start, which thus starts
-// when at most this one is unfinished: all that lies further back has ended.
+// of memory, and only then (or not before its end) lets the kernel behind it
+// start, which thus starts when at most this one is unfinished: all that lies
+// further back has ended.
 __device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void pdl_trigger() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 

@@ -717,8 +717,9 @@ __global__ void __launch_bounds__(kThreads, 1)
                     load_b(ahead, tile0 / p.m_tiles, kb);
                 }
             }
+            // No trigger: the kernel behind is mostly a quantiser, whose CTAs would all settle on the SMs that this
+            // grid leaves idle (the shared expert of 512 tokens took 54.7 us with one here, 50.1 without).
             pdl_wait();
-            pdl_trigger();
             int s = 0;
             uint32_t ph = 0;
             for (int t = tile0; t < total; t += step) {
@@ -1300,10 +1301,13 @@ cudaError_t launch_ex(void (*kern)(P...), unsigned grid, unsigned threads, size_
 
 template <typename T, bool kPair>
 cudaError_t launch_quantize_typed(const T* x, int64_t rows, int K, int64_t ldx, int64_t up, int8_t* q, int64_t ldq,
-                                  float* s, cudaStream_t st) {
+                                  float* s, int num_sms, cudaStream_t st) {
     const int vec = aligned(x, 16) && (ldx * (int64_t)sizeof(T)) % 16 == 0;
-    // as many threads a row as hold it in registers, four vectors of eight each
-    const int tpr = K <= 1024 ? 32 : K <= 2048 ? 64 : K <= 4096 ? 128 : 256;
+    // As many threads a row as hold it in registers, four vectors of eight each; one each for few rows, where the
+    // chain through a row counts and not the CTAs on an SM.  Measured (us, four / one): 64 x 2048 bf16 2.6 / 1.7,
+    // 512 x 2048 2.8 / 2.6, 1024 x 2048 3.4 / 3.9; f32 256 x 2048 2.4 / 1.9, 512 x 2048 2.4 / 3.0.
+    const int span = rows <= (sizeof(T) == 2 || kPair ? 4 : 2) * num_sms ? 256 : 1024;
+    const int tpr = K <= span ? 32 : K <= 2 * span ? 64 : K <= 4 * span ? 128 : 256;
     const int64_t blocks = (rows * tpr + 255) / 256;
     auto kern = tpr == 32    ? quantize_tokens_kernel<T, 32, kPair>
                 : tpr == 64  ? quantize_tokens_kernel<T, 64, kPair>
@@ -1314,17 +1318,17 @@ cudaError_t launch_quantize_typed(const T* x, int64_t rows, int K, int64_t ldx, 
 
 // up != 0: x holds f32 gate values with the up values `up` elements behind.
 cudaError_t launch_quantize(const void* x, int type, int64_t rows, int K, int64_t ldx, int64_t up, int8_t* q,
-                            int64_t ldq, float* s, cudaStream_t st) {
+                            int64_t ldq, float* s, int num_sms, cudaStream_t st) {
     if (up != 0)
-        return launch_quantize_typed<float, true>(static_cast<const float*>(x), rows, K, ldx, up, q, ldq, s, st);
+        return launch_quantize_typed<float, true>(static_cast<const float*>(x), rows, K, ldx, up, q, ldq, s, num_sms, st);
     switch (type) {
         case MOE_TYPE_F32:
-            return launch_quantize_typed<float, false>(static_cast<const float*>(x), rows, K, ldx, 0, q, ldq, s, st);
+            return launch_quantize_typed<float, false>(static_cast<const float*>(x), rows, K, ldx, 0, q, ldq, s, num_sms, st);
         case MOE_TYPE_F16:
-            return launch_quantize_typed<__half, false>(static_cast<const __half*>(x), rows, K, ldx, 0, q, ldq, s, st);
+            return launch_quantize_typed<__half, false>(static_cast<const __half*>(x), rows, K, ldx, 0, q, ldq, s, num_sms, st);
         default:
             return launch_quantize_typed<__nv_bfloat16, false>(static_cast<const __nv_bfloat16*>(x), rows, K, ldx, 0, q,
-                                                               ldq, s, st);
+                                                               ldq, s, num_sms, st);
     }
 }
 
@@ -1700,13 +1704,13 @@ int run_shared_expert(const char* who, const void* x, int x_type, int64_t tokens
     const bool small = is_small(tokens, kSmallShared, d_model, 2);
     if (!small || !try_small(kSmallShared, x, x_type, row_stride, ph, mg, &mu, num_sms, stream, &e)) {
         ph.ahead = 1;
-        e = launch_quantize(x, x_type, tokens, d_model, row_stride, 0, qx, up16(d_model), sx, stream);
+        e = launch_quantize(x, x_type, tokens, d_model, row_stride, 0, qx, up16(d_model), sx, num_sms, stream);
         if (e == cudaSuccess) e = launch_linear(qx, up16(d_model), ph, mg, &mu, fused, num_sms, stream);
     }
     if (e != cudaSuccess) return cuda_error(who, e);
     const bool pairs = !fused && !small;
     if (pairs || !try_small(kSmallShared, h, MOE_TYPE_F32, sc.ldh, py, md, nullptr, num_sms, stream, &e)) {
-        e = launch_quantize(h, MOE_TYPE_F32, tokens, d_ff, sc.ldh, pairs ? behind : 0, qh, up16(d_ff), sh, stream);
+        e = launch_quantize(h, MOE_TYPE_F32, tokens, d_ff, sc.ldh, pairs ? behind : 0, qh, up16(d_ff), sh, num_sms, stream);
         if (e == cudaSuccess) e = launch_linear(qh, up16(d_ff), py, md, nullptr, false, num_sms, stream);
     }
     return e == cudaSuccess ? MOE_OK : cuda_error(who, e);
@@ -1736,7 +1740,7 @@ extern "C" int moe_int8_quantize_tokens(const void* x, int x_type, int64_t token
     int dev = 0, num_sms = 0;
     rc = current_device(&dev, &num_sms);
     if (rc != MOE_OK) return rc;
-    const cudaError_t e = launch_quantize(x, x_type, tokens, K, row_stride, 0, q, q_stride, scale, stream);
+    const cudaError_t e = launch_quantize(x, x_type, tokens, K, row_stride, 0, q, q_stride, scale, num_sms, stream);
     return e == cudaSuccess ? MOE_OK : cuda_error(who, e);
 }
 
@@ -1788,7 +1792,7 @@ extern "C" int moe_int8_linear(const void* x, int x_type, int64_t tokens, int K,
     cudaError_t e;
     if (!try_small(kSmallLinear, x, x_type, row_stride, p, m, nullptr, num_sms, stream, &e)) {
         p.ahead = 1;
-        e = launch_quantize(x, x_type, tokens, K, row_stride, 0, q, up16(K), s, stream);
+        e = launch_quantize(x, x_type, tokens, K, row_stride, 0, q, up16(K), s, num_sms, stream);
         if (e == cudaSuccess) e = launch_linear(q, up16(K), p, m, nullptr, false, num_sms, stream);
     }
     return e == cudaSuccess ? MOE_OK : cuda_error(who, e);
