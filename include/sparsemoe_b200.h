@@ -277,12 +277,12 @@ int moe_int8_matmul(const int8_t* q, int64_t q_stride, const float* scale, int64
                     const MoeInt8Weight* w, int N, const float* bias, void* out, int out_type, int64_t out_stride,
                     cudaStream_t stream);
 // Both in one call: 16-bit or f32 activations times an int8 matrix.  scratch:
-// device, 256-byte aligned, moe_int8_linear_scratch_bytes(tokens, K) -- 0 for a
-// few tokens, then scratch may be null.
+// device, 256-byte aligned, moe_int8_linear_scratch_bytes(tokens, K, N) -- 0 for a
+// few tokens of most shapes, then scratch may be null.
 int moe_int8_linear(const void* x, int x_type, int64_t tokens, int K, int64_t row_stride, const MoeInt8Weight* w,
                     int N, const float* bias, void* out, int out_type, int64_t out_stride, void* scratch,
                     size_t scratch_bytes, cudaStream_t stream);
-size_t moe_int8_linear_scratch_bytes(int64_t tokens, int K);
+size_t moe_int8_linear_scratch_bytes(int64_t tokens, int K, int N);
 // The shared expert of an MoE layer, a SwiGLU FFN that every token takes:
 //   g = linear(x, gate), u = linear(x, up), h = u * g / (1 + exp(-g)) (f32),
 //   out = linear(h, down) + residual,

@@ -103,7 +103,7 @@ def _load() -> ctypes.CDLL:
         "moe_int8_linear": (ctypes.c_int, [_p, ctypes.c_int, ctypes.c_int64, ctypes.c_int, ctypes.c_int64,
                                            ctypes.POINTER(MoeInt8Weight), ctypes.c_int, _p, _p, ctypes.c_int,
                                            ctypes.c_int64, _p, ctypes.c_size_t, _p]),
-        "moe_int8_linear_scratch_bytes": (ctypes.c_size_t, [ctypes.c_int64, ctypes.c_int]),
+        "moe_int8_linear_scratch_bytes": (ctypes.c_size_t, [ctypes.c_int64, ctypes.c_int, ctypes.c_int]),
         "moe_int8_shared_expert": (ctypes.c_int, [_p, ctypes.c_int, ctypes.c_int64, ctypes.c_int, ctypes.c_int64,
                                                   ctypes.POINTER(MoeInt8Weight), ctypes.POINTER(MoeInt8Weight),
                                                   ctypes.POINTER(MoeInt8Weight), ctypes.c_int, _p, ctypes.c_int64, _p,

@@ -268,7 +268,7 @@ PyObject* linear(PyObject*, PyObject* const* a, Py_ssize_t n) {
     int64_t ld;
     Tensor out = output_of(a[5], r.n, N, dtype_of(a[4], x.scalar_type()), dev, &kind, &ld);
     const int K = to_int(r.cols, "x");
-    const size_t bytes = f_linear_scratch(r.n, K);
+    const size_t bytes = f_linear_scratch(r.n, K, N);
     Tensor scratch;
     if (bytes) scratch = fresh({(int64_t)bytes}, at::kByte, dev);
     On on(dev);

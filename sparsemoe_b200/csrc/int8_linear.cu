@@ -381,6 +381,13 @@ __device__ __forceinline__ float load_as_f32(const void* p, int64_t i, int type)
     return __bfloat162float(static_cast<const __nv_bfloat16*>(p)[i]);
 }
 
+// A sum's value, rounded before bias or residual are added: no fused multiply-add
+// in one epilogue that another lacks, so that a token's result is the same bits
+// in any batch.
+__device__ __forceinline__ float dequant(uint32_t sum, float s_tok, float s_ch) {
+    return __fmul_rn((float)(int)sum * s_tok, s_ch);
+}
+
 // Eight consecutive outputs of row t from column n on (those below N) of the first or second matrix.
 __device__ __forceinline__ void emit8(const LinearParams& p, int64_t t, bool second, int n, float (&v)[8]) {
     const int left = p.N - n;
@@ -547,14 +554,14 @@ struct StagedEpilogue {
                 for (int i = 0; i < kU; i += 4) {
                     const int k = j * kU + i;
                     const float4 w = *reinterpret_cast<const float4*>(sc + n + k);
-                    v[i] = (float)(int)a[k] * st * w.x;
-                    v[i + 1] = (float)(int)a[k + 1] * st * w.y;
-                    v[i + 2] = (float)(int)a[k + 2] * st * w.z;
-                    v[i + 3] = (float)(int)a[k + 3] * st * w.w;
+                    v[i] = dequant(a[k], st, w.x);
+                    v[i + 1] = dequant(a[k + 1], st, w.y);
+                    v[i + 2] = dequant(a[k + 2], st, w.z);
+                    v[i + 3] = dequant(a[k + 3], st, w.w);
                     if constexpr (kSwiglu) {
                         const float4 g = *reinterpret_cast<const float4*>(sc + kOutN + n + k);
-                        const float u[4] = {(float)(int)b[k] * st * g.x, (float)(int)b[k + 1] * st * g.y,
-                                            (float)(int)b[k + 2] * st * g.z, (float)(int)b[k + 3] * st * g.w};
+                        const float u[4] = {dequant(b[k], st, g.x), dequant(b[k + 1], st, g.y),
+                                            dequant(b[k + 2], st, g.z), dequant(b[k + 3], st, g.w)};
 #pragma unroll
                         for (int h = 0; h < 4; ++h) v[i + h] = u[h] * silu(v[i + h]);
                     }
@@ -839,8 +846,8 @@ __global__ void __launch_bounds__(kThreads, 1)
                         float v[8];
 #pragma unroll
                         for (int i = 0; i < 8; ++i) {
-                            v[i] = (float)(int)a[h + i] * st * sc[c + h + i];
-                            if (kSwiglu) v[i] = (float)(int)b[h + i] * st * sc[kOutN + c + h + i] * silu(v[i]);
+                            v[i] = dequant(a[h + i], st, sc[c + h + i]);
+                            if (kSwiglu) v[i] = dequant(b[h + i], st, sc[kOutN + c + h + i]) * silu(v[i]);
                             else v[i] += sb[c + h + i];
                         }
                         if (col0 + c + h < p.N) emit8(p, row, second, col0 + c + h, v);
@@ -900,7 +907,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 const float st = p.s_tok[row];
                 float v[8];
 #pragma unroll
-                for (int j = 0; j < 8; ++j) v[j] = (float)sum[j] * st * s_scale[0][c + j] + s_bias[0][c + j];
+                for (int j = 0; j < 8; ++j) v[j] = dequant(sum[j], st, s_scale[0][c + j]) + s_bias[0][c + j];
                 emit8(p, row, second, col0 + c, v);
             }
         }
@@ -925,16 +932,16 @@ __global__ void __launch_bounds__(kThreads, 1)
 // the tokens its columns (N = kNT), so a thread of the epilogue holds one
 // channel's sums of all tokens and consecutive lanes write consecutive columns.
 // A cluster of `split` CTAs shares a tile, each a part of K.  Each CTA asks for
-// its weights at once, reads its part of the tokens twice (amax, which the
-// cluster exchanges through shared memory, then the codes, written where the MMA
-// reads them) and hands the s32 sums of each slice of the channels to the CTA
-// that adds them up.
+// its weights at once, reads the tokens for their amax (short rows whole; of long
+// ones its part, the cluster exchanging what it finds), then its part again for
+// the codes, written where the MMA reads them, and hands the s32 sums of each
+// slice of the channels to the CTA that adds them up.
 // kSwiglu: the tile is 128 features, their gate and up columns are multiplied in
 // turn (two accumulators), and h = up * silu(gate) is written.
-// What bounds it is latency: an empty launch of it takes 4 us, the exchanges of a
-// cluster 2.5, and the MMAs, 128 clocks each whatever their columns, 0.27 us for
-// each block of K; the 14.7 MB of weights of 1 x 7168 x 2048 (10.2 us) are 2.2 us at
-// the HBM's rate.  Kept short for one reason more: a code path that a CTA runs
+// What bounds it is latency: 512 x 2048 takes 4.5 us (3.1 with codes given), an
+// exchange of a cluster about 1, and the MMAs, 128 clocks each whatever their
+// columns, 0.27 us for each block of K; the 14.7 MB of weights of 1 x 7168 x 2048
+// (6.8 us, 8.7 when none of them is in the L2) are 2.2 us at the HBM's rate.  Kept short for one reason more: a code path that a CTA runs
 // once is fetched as slowly as it is long (the quantiser of gate / up pairs, 96
 // times silu in line, cost the down product 17 us).
 struct SmallParams {
@@ -944,6 +951,7 @@ struct SmallParams {
     int T, K, N;
     int kblocks, split, stages;
     int b_nk, ahead, vec_x;
+    int exchange;              // each CTA takes its part's amax and the cluster exchanges them; else every CTA the rows'
     const float* s_ch0;
     const float* s_ch1;
     const float* bias;
@@ -1016,7 +1024,7 @@ __global__ void __launch_bounds__(kSmallThreads, 2)
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem_base = *tmem_slot;
-    const bool split = p.split > 1;
+    const bool split = p.split > 1, exchange = split && kIn != kInCodes && p.exchange;
     if (split) cluster_arrive();   // phase 1: every CTA has started
 
     const int col0 = (int)blockIdx.x / p.split * 128;
@@ -1039,8 +1047,8 @@ __global__ void __launch_bounds__(kSmallThreads, 2)
             pdl_trigger();
         }
         __syncwarp();
-        if (split) {   // phases 1 and 2, before any wait that the other warps' progress ends
-            cluster_wait();
+        if (split) cluster_wait();   // phase 1; and 2, before any wait that the other warps' progress ends
+        if (exchange) {
             cluster_arrive();
             cluster_wait();
         }
@@ -1055,8 +1063,8 @@ __global__ void __launch_bounds__(kSmallThreads, 2)
         }
     } else if (warp == 1) {
         // ---------------- MMA issuer ----------------
-        if (split) {
-            cluster_wait();
+        if (split) cluster_wait();
+        if (exchange) {
             cluster_arrive();
             cluster_wait();
         }
@@ -1095,32 +1103,32 @@ __global__ void __launch_bounds__(kSmallThreads, 2)
             const int tok0 = w / share, tstep = 8 / share;
             const int u0 = (w % share) * 32 + lane, ustep = 32 * share * 8;
             constexpr int kBatch = 4;
-            const bool whole = p.vec_x && (k1 - k0) % 8 == 0;
-            // units k, k + ustep, .. of token t, all asked for before any is used
-            auto fetch = [&](In8<T> (&d)[kBatch], int t, int k) {
+            // units k, k + ustep, .. of token t below `end`, all asked for before any is used
+            auto fetch = [&](In8<T> (&d)[kBatch], int t, int k, int end) {
                 const T* src = x + t * p.ld_x;
-                if (whole) {
+                if (p.vec_x && end % 8 == 0) {
 #pragma unroll
                     for (int i = 0; i < kBatch; ++i) {
                         d[i].zero();
-                        if (t < p.T && k + i * ustep < k1) d[i].load(src + k + i * ustep);
+                        if (t < p.T && k + i * ustep < end) d[i].load(src + k + i * ustep);
                     }
                 } else {
 #pragma unroll
                     for (int i = 0; i < kBatch; ++i) {
                         d[i].zero();
-                        if (t < p.T && k + i * ustep < k1) d[i].load_part(src + k + i * ustep, k1 - k - i * ustep);
+                        if (t < p.T && k + i * ustep < end) d[i].load_part(src + k + i * ustep, end - k - i * ustep);
                     }
                 }
             };
-            if (threadIdx.x - 64 < kNT) s_amax[rank][threadIdx.x - 64] = 0u;
+            const int from = exchange ? k0 : 0, to = exchange ? k1 : p.K, slot = exchange ? rank : 0;   // of the amax
+            if (threadIdx.x - 64 < kNT) s_amax[slot][threadIdx.x - 64] = 0u;
             asm volatile("bar.sync 1, 256;" ::: "memory");
             for (int t = tok0; t < p.T; t += 2 * tstep) {
                 uint32_t m[2] = {0u, 0u};
-                for (int k = k0 + u0 * 8; k - u0 * 8 < k1; k += kBatch * ustep) {
+                for (int k = from + u0 * 8; k - u0 * 8 < to; k += kBatch * ustep) {
                     In8<T> d[2][kBatch];
-                    fetch(d[0], t, k);
-                    fetch(d[1], t + tstep, k);
+                    fetch(d[0], t, k, to);
+                    fetch(d[1], t + tstep, k, to);
 #pragma unroll
                     for (int i = 0; i < kBatch; ++i) {
                         m[0] = max(m[0], d[0][i].amax_bits());
@@ -1130,16 +1138,16 @@ __global__ void __launch_bounds__(kSmallThreads, 2)
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
                     m[h] = __reduce_max_sync(0xffffffffu, m[h]);
-                    if (lane == 0 && t + h * tstep < p.T) atomicMax(&s_amax[rank][t + h * tstep], m[h]);
+                    if (lane == 0 && t + h * tstep < p.T) atomicMax(&s_amax[slot][t + h * tstep], m[h]);
                 }
             }
             asm volatile("bar.sync 1, 256;" ::: "memory");
-            if (split) {
+            if (exchange) {
                 cluster_wait();   // phase 1
                 for (int i = threadIdx.x - 64; i < p.T * p.split; i += kSmallWorkers) {
-                    const int to = i / p.T, t = i % p.T;
-                    if (to != rank)
-                        asm volatile("st.shared::cluster.b32 [%0], %1;" ::"r"(mapa(smem_u32(&s_amax[rank][t]), to)),
+                    const int cta = i / p.T, t = i % p.T;
+                    if (cta != rank)
+                        asm volatile("st.shared::cluster.b32 [%0], %1;" ::"r"(mapa(smem_u32(&s_amax[rank][t]), cta)),
                                      "r"(s_amax[rank][t])
                                      : "memory");
                 }
@@ -1149,12 +1157,13 @@ __global__ void __launch_bounds__(kSmallThreads, 2)
             }
             for (int t = tok0; t < p.T; t += tstep) {
                 uint32_t m = s_amax[0][t];
-                for (int r = 1; r < p.split; ++r) m = max(m, s_amax[r][t]);
+                if (exchange)
+                    for (int r = 1; r < p.split; ++r) m = max(m, s_amax[r][t]);
                 const RowScale rs(m);
                 if (u0 == 0) s_tok[t] = rs.s;
                 for (int k = k0 + u0 * 8; k - u0 * 8 < k1; k += kBatch * ustep) {
                     In8<T> d[kBatch];
-                    fetch(d, t, k);
+                    fetch(d, t, k, k1);
 #pragma unroll
                     for (int i = 0; i < kBatch; ++i) {
                         const int kk = k + i * ustep - k0;
@@ -1169,11 +1178,6 @@ __global__ void __launch_bounds__(kSmallThreads, 2)
                 }
             }
         } else {
-            if (split) {
-                cluster_wait();
-                cluster_arrive();
-                cluster_wait();
-            }
             if (threadIdx.x - 64 < p.T) s_tok[threadIdx.x - 64] = p.s_tok[threadIdx.x - 64];
             const int units = (k1 - k0 + 15) / 16;   // rows start on 16-byte boundaries
             for (int i = threadIdx.x - 64; i < units * p.T; i += kSmallWorkers) {
@@ -1197,14 +1201,15 @@ __global__ void __launch_bounds__(kSmallThreads, 2)
         // a thread: channel c, half of the tokens
         constexpr int kHalfTok = kNT / 2;
         const int q = warp & 3, half = w >> 2, c = q * 32 + lane, tok = half * kHalfTok;
+        if (split && !exchange) cluster_wait();   // phase 1
         const bool ok = mbar_wait_warp(tfull, 0, status, kDevErrTimeout);
         tc_fence_after();
         const uint32_t taddr = tmem_base + ((uint32_t)(q * 32) << 16) + tok;
         auto put = [&](int sum, int sum1, int t, int ch) {   // channel ch of the tile
             const int col = col0 + ch;
             if (col >= p.N) return;
-            float v = (float)sum * s_tok[t] * p.s_ch0[col];
-            if (kSwiglu) v = (float)sum1 * s_tok[t] * p.s_ch1[col] * silu(v);
+            float v = dequant(sum, s_tok[t], p.s_ch0[col]);
+            if (kSwiglu) v = dequant(sum1, s_tok[t], p.s_ch1[col]) * silu(v);
             if (p.bias) v += p.bias[col];
             if (p.residual) v += load_as_f32(p.residual, t * p.ld_res + col, p.res_type);
             const int64_t at = t * p.ld_out + col;
@@ -1436,15 +1441,18 @@ cudaError_t launch_linear(const int8_t* q, int64_t ldq, LinearParams p, const Ma
     return launch_linear_cfg<128, false, false>(ta, tb, to, p, clusters, st);
 }
 
-// Up to this many tokens small_linear_kernel is used.  Measured (us in a graph;
-// small kernel, then quantiser + tiles): int8_linear 7168 -> 2048 of 1 token 10.2,
-// 11.2, 4 tokens 10.6, 10.6, 8 tokens 11.1, 10.7; 2048 -> 7168 of 4 tokens 9.5, 8.9,
-// 8 tokens 10.0, 8.9 (one launch instead of two costs the host 3.9 us instead of
-// 7.5); codes given, 8 tokens 9.3, 9.8 and 8.3, 8.2; shared expert 7168 / 2048 of 4
-// tokens 21.9, 26.0, 8 tokens 22.6, 26.3, 12 tokens 25.8, 26.7, 16 tokens 27.0, 26.7.
-constexpr int kSmallLinear = 4, kSmallCodes = 8, kSmallShared = 8;
+// Up to this many tokens small_linear_kernel is used: with its own quantiser, or
+// on codes (given, or of the quantiser's launch).  Measured (us a call; one launch,
+// quantiser + small kernel, quantiser + tiles): int8_linear 7168 -> 2048 of 1 token
+// 7.3, 8.4, 11.1, 4 tokens 8.2, 8.4, 10.6, 8 tokens 8.9, 8.9, 10.7, 16 tokens 11.0,
+// 9.5, 10.8; 2048 -> 7168 of 8 tokens 8.4, 8.1, 8.9, 16 tokens 10.4, 9.3, 9.2;
+// int8_matmul 7168 -> 2048 of 16 codes 6.7, by tiles 9.5; shared expert 7168 / 2048
+// of 1 token 20.2, 22.0, 22.8, 4 tokens 21.1, 21.5, 22.6, 8 tokens 22.7, 22.6, 22.7,
+// 16 tokens 26.8, 24.4, 23.1.
+constexpr int kSmallLinear = 4, kSmallCodes = 16;   // gate / up: its own quantiser as the linear's
+constexpr int kSmallPairs = 8;                      // gate / up on codes
 constexpr int kSmallN = 16;
-constexpr int kSmallStages = 5;
+constexpr int kSmallStages = 5, kSmallMinStages = 3;
 constexpr size_t kSmallSmem = 112 * 1024;   // two CTAs an SM
 
 template <int kIn, bool kSwiglu>
@@ -1457,19 +1465,22 @@ cudaError_t launch_small_typed(const CUtensorMap (&w)[2], const SmallParams& p, 
                      p);
 }
 
-// Whether a call's codes fit beside the weight stages at some split; the split
-// with the most CTAs that are resident at once (two an SM).
-bool plan_small(int64_t T, int limit, int K, int N, int mats, int num_sms, int* split, int* stages, size_t* smem) {
+// Whether a call's codes fit beside the weight stages at some split with all of
+// its CTAs resident at once (two an SM); the largest such split.  More CTAs are
+// left to the persistent tiles (us, here / there, 1 token: 7168 x 8192 14.1 / 17.7,
+// all at once; 7168 x 14336 26.7 / 25.8, 7168 x 28672 51.3 / 37.1, in rounds).
+bool plan_small(int64_t T, int limit, int K, int N, int mats, int* split, int* stages, size_t* smem) {
     if (T > limit) return false;
     const int kblocks = (K + kBK - 1) / kBK, tiles = (N + 127) / 128;
     *split = 0;
     for (int s = 1; s <= kMaxSplit && s <= kblocks; s *= 2) {
-        const int blocks = (kblocks + s - 1) / s, st = std::min(kSmallStages, blocks * mats);
+        const int blocks = (kblocks + s - 1) / s;
+        int st = std::min(kSmallStages, blocks * mats);
+        while (st > kSmallMinStages && small_smem<kSmallN>(st, blocks, s, mats) > kSmallSmem) --st;
         const size_t need = small_smem<kSmallN>(st, blocks, s, mats);
         if (need > kSmallSmem) continue;
         // clusters of 1, 2, 4 and 8 CTAs of up to half an SM's memory fit 296, 148, 71 and 33 times
-        const int at_once = s == 1 ? 2 * num_sms : s == 2 ? num_sms : s == 4 ? num_sms * 71 / 148 : num_sms * 33 / 148;
-        if (*split != 0 && tiles > at_once) break;
+        if (tiles > (s == 1 ? 2 * kRuleSms : s == 2 ? kRuleSms : s == 4 ? 71 : 33)) break;
         *split = s;
         *stages = st;
         *smem = need;
@@ -1480,11 +1491,11 @@ bool plan_small(int64_t T, int limit, int K, int N, int mats, int num_sms, int* 
 // A product of few tokens in one launch (w1: gate and up, h written); x_type:
 // MOE_TYPE_* of x, or -1 for codes.  False where the shape needs the tiles.
 bool try_small(int limit, const void* x, int x_type, int64_t ld_x, const LinearParams& l, const Matrix& w0, const Matrix* w1,
-               int num_sms, cudaStream_t st, cudaError_t* err) {
+               cudaStream_t st, cudaError_t* err) {
     int split, stages;
     size_t smem;
     const int mats = w1 ? 2 : 1;
-    if (!plan_small(l.T, limit, l.K, l.N, mats, num_sms, &split, &stages, &smem)) return false;
+    if (!plan_small(l.T, limit, l.K, l.N, mats, &split, &stages, &smem)) return false;
     SmallParams p{};
     p.x = x;
     p.ld_x = ld_x;
@@ -1508,6 +1519,8 @@ bool try_small(int limit, const void* x, int x_type, int64_t ld_x, const LinearP
     p.out_type = l.out_type;
     const int size = x_type < 0 ? 1 : elem_bytes(x_type);
     p.vec_x = aligned(x, 16) && (ld_x * size) % 16 == 0;
+    // (us, exchanged / read by each: 1 x 7168 x 2048 7.8 / 7.2, 2 tokens 7.9 / 7.9, 4 tokens 8.1 / 10.0)
+    p.exchange = (int64_t)l.T * l.K * size > 32 * 1024;
     // weights are the A operand (M = 128 channels): MN-major for [K, N]
     p.idesc = idesc_i8(128, kSmallN, false) | (p.b_nk ? 0u : 1u << 15);
     CUtensorMap w[2];
@@ -1522,7 +1535,9 @@ bool try_small(int limit, const void* x, int x_type, int64_t ld_x, const LinearP
     }
     if (mats == 1) w[1] = w[0];
     const int tiles = (l.N + 127) / 128;
-    if (x_type < 0) *err = launch_small_typed<kInCodes, false>(w, p, tiles, smem, st);
+    if (x_type < 0)
+        *err = w1 ? launch_small_typed<kInCodes, true>(w, p, tiles, smem, st)
+                  : launch_small_typed<kInCodes, false>(w, p, tiles, smem, st);
     else if (x_type == MOE_TYPE_F32)
         *err = w1 ? launch_small_typed<kInF32, true>(w, p, tiles, smem, st)
                   : launch_small_typed<kInF32, false>(w, p, tiles, smem, st);
@@ -1614,15 +1629,15 @@ LinearParams out_params(int64_t T, int K, int N, const float* s_tok, const float
 // product's split of K fills.
 bool fused_swiglu(int64_t T, int64_t f) { return (T + 127) / 128 * ((f + 127) / 128) * 4 >= kRuleSms * 3; }
 
-// Whether the small kernel takes a call (its shared memory depends on K alone).
-bool is_small(int64_t T, int limit, int K, int mats = 1) {
+// Whether the small kernel takes a call.
+bool is_small(int64_t T, int limit, int K, int N, int mats = 1) {
     int split, stages;
     size_t smem;
-    return plan_small(T, limit, K, 1, mats, kRuleSms, &split, &stages, &smem);
+    return plan_small(T, limit, K, N, mats, &split, &stages, &smem);
 }
 
-size_t linear_scratch(int64_t T, int K) {
-    return is_small(T, kSmallLinear, K) ? 0 : up256((size_t)T * up16(K)) + up256((size_t)T * sizeof(float));
+size_t linear_scratch(int64_t T, int K, int N) {
+    return is_small(T, kSmallLinear, K, N) ? 0 : up256((size_t)T * up16(K)) + up256((size_t)T * sizeof(float));
 }
 
 struct SharedScratch {
@@ -1635,7 +1650,8 @@ SharedScratch shared_scratch(int64_t T, int64_t d, int64_t f) {
     size_t at = 0;
     s.qx = at; at += up256((size_t)T * up16(d));
     s.sx = at; at += up256((size_t)T * sizeof(float));
-    s.h = at;  at += up256((size_t)T * s.ldh * sizeof(float)) * (fused_swiglu(T, f) || is_small(T, kSmallShared, (int)d, 2) ? 1 : 2);
+    const bool one = fused_swiglu(T, f) || is_small(T, kSmallPairs, (int)d, (int)f, 2);
+    s.h = at;  at += up256((size_t)T * s.ldh * sizeof(float)) * (one ? 1 : 2);
     s.qh = at; at += up256((size_t)T * up16(f));
     s.sh = at; at += up256((size_t)T * sizeof(float));
     s.total = at;
@@ -1701,17 +1717,19 @@ int run_shared_expert(const char* who, const void* x, int x_type, int64_t tokens
     py.vec_res = aligned(residual, 16) && (residual_stride * elem_bytes(x_type)) % 16 == 0;
     cudaError_t e = cudaSuccess;
     // gate and up: h, or (too few tiles to fuse) g and u
-    const bool small = is_small(tokens, kSmallShared, d_model, 2);
-    if (!small || !try_small(kSmallShared, x, x_type, row_stride, ph, mg, &mu, num_sms, stream, &e)) {
+    const bool small = is_small(tokens, kSmallPairs, d_model, d_ff, 2);
+    if (!try_small(kSmallLinear, x, x_type, row_stride, ph, mg, &mu, stream, &e)) {
         ph.ahead = 1;
         e = launch_quantize(x, x_type, tokens, d_model, row_stride, 0, qx, up16(d_model), sx, num_sms, stream);
-        if (e == cudaSuccess) e = launch_linear(qx, up16(d_model), ph, mg, &mu, fused, num_sms, stream);
+        if (e == cudaSuccess && !try_small(kSmallPairs, qx, -1, up16(d_model), ph, mg, &mu, stream, &e))
+            e = launch_linear(qx, up16(d_model), ph, mg, &mu, fused, num_sms, stream);
     }
     if (e != cudaSuccess) return cuda_error(who, e);
     const bool pairs = !fused && !small;
-    if (pairs || !try_small(kSmallShared, h, MOE_TYPE_F32, sc.ldh, py, md, nullptr, num_sms, stream, &e)) {
+    if (pairs || !try_small(kSmallLinear, h, MOE_TYPE_F32, sc.ldh, py, md, nullptr, stream, &e)) {
         e = launch_quantize(h, MOE_TYPE_F32, tokens, d_ff, sc.ldh, pairs ? behind : 0, qh, up16(d_ff), sh, num_sms, stream);
-        if (e == cudaSuccess) e = launch_linear(qh, up16(d_ff), py, md, nullptr, false, num_sms, stream);
+        if (e == cudaSuccess && !try_small(kSmallCodes, qh, -1, up16(d_ff), py, md, nullptr, stream, &e))
+            e = launch_linear(qh, up16(d_ff), py, md, nullptr, false, num_sms, stream);
     }
     return e == cudaSuccess ? MOE_OK : cuda_error(who, e);
 }
@@ -1720,8 +1738,8 @@ int run_shared_expert(const char* who, const void* x, int x_type, int64_t tokens
 
 using namespace moe;
 
-extern "C" size_t moe_int8_linear_scratch_bytes(int64_t tokens, int K) {
-    return tokens < 0 || K < 1 ? 0 : linear_scratch(tokens, K);
+extern "C" size_t moe_int8_linear_scratch_bytes(int64_t tokens, int K, int N) {
+    return tokens < 0 || K < 1 || N < 1 ? 0 : linear_scratch(tokens, K, N);
 }
 
 extern "C" size_t moe_int8_shared_expert_scratch_bytes(int64_t tokens, int d_model, int d_ff) {
@@ -1763,7 +1781,7 @@ extern "C" int moe_int8_matmul(const int8_t* q, int64_t q_stride, const float* s
     const LinearParams p = out_params(tokens, K, N, scale, bias, out, out_type, out_stride, w->order);
     const Matrix m{w->w, w->row_stride, w->scale};
     cudaError_t e;
-    if (!try_small(kSmallCodes, q, -1, q_stride, p, m, nullptr, num_sms, stream, &e))
+    if (!try_small(kSmallCodes, q, -1, q_stride, p, m, nullptr, stream, &e))
         e = launch_linear(q, q_stride, p, m, nullptr, false, num_sms, stream);
     return e == cudaSuccess ? MOE_OK : cuda_error(who, e);
 }
@@ -1779,7 +1797,7 @@ extern "C" int moe_int8_linear(const void* x, int x_type, int64_t tokens, int K,
     if (rc != MOE_OK) return rc;
     if (!aligned(bias, 4)) return bad(who, "bias is not aligned to f32");
     if (tokens == 0) return MOE_OK;
-    rc = check_scratch(who, scratch, scratch_bytes, linear_scratch(tokens, K));
+    rc = check_scratch(who, scratch, scratch_bytes, linear_scratch(tokens, K, N));
     if (rc != MOE_OK) return rc;
     int dev = 0, num_sms = 0;
     rc = current_device(&dev, &num_sms);
@@ -1790,10 +1808,11 @@ extern "C" int moe_int8_linear(const void* x, int x_type, int64_t tokens, int K,
     LinearParams p = out_params(tokens, K, N, s, bias, out, out_type, out_stride, w->order);
     const Matrix m{w->w, w->row_stride, w->scale};
     cudaError_t e;
-    if (!try_small(kSmallLinear, x, x_type, row_stride, p, m, nullptr, num_sms, stream, &e)) {
+    if (!try_small(kSmallLinear, x, x_type, row_stride, p, m, nullptr, stream, &e)) {
         p.ahead = 1;
         e = launch_quantize(x, x_type, tokens, K, row_stride, 0, q, up16(K), s, num_sms, stream);
-        if (e == cudaSuccess) e = launch_linear(q, up16(K), p, m, nullptr, false, num_sms, stream);
+        if (e == cudaSuccess && !try_small(kSmallCodes, q, -1, up16(K), p, m, nullptr, stream, &e))
+            e = launch_linear(q, up16(K), p, m, nullptr, false, num_sms, stream);
     }
     return e == cudaSuccess ? MOE_OK : cuda_error(who, e);
 }

@@ -147,6 +147,23 @@ def test_matmul_takes_codes(gpu):
     assert torch.equal(one, y[:1])
 
 
+@pytest.mark.parametrize("order", ["kn", "nk"])
+@pytest.mark.parametrize("K, N", [(7168, 2048), (2048, 7168), (14336, 400), (1000, 2100), (9001, 4300), (129, 40000)])
+def test_a_few_tokens(gpu, K, N, order):
+    """Every way that few tokens take (rows short and long, K split or not, more tiles than run at once) agrees with
+    the codes' product and, bit for bit, with the rows of a large batch."""
+    g = torch.Generator().manual_seed(K + N)
+    x = tokens(140, K, torch.bfloat16, 11)
+    w, ws = int8_matrix(g, K, N, order, gpu)
+    b = torch.randn(N, generator=g).cuda()
+    whole = sm.int8_linear(x, w, ws, bias=b, out_dtype=torch.float32)
+    check_linear(x[:16], w, ws, b, torch.float32, whole[:16])
+    q, s = sm.quantize_int8_tokens(x)
+    for n in (1, 2, 3, 4, 5, 8, 9, 15, 16, 17):
+        assert torch.equal(sm.int8_linear(x[:n], w, ws, bias=b, out_dtype=torch.float32), whole[:n])
+        assert torch.equal(sm.int8_matmul(q[:n], s[:n], w, ws, bias=b, out_dtype=torch.float32), whole[:n])
+
+
 def test_rows_do_not_depend_on_the_batch(gpu):
     """Exact sums: a token's output is the same bits in any batch, tile or split."""
     g = torch.Generator().manual_seed(6)
@@ -273,6 +290,81 @@ def test_shared_expert(gpu, T, d, f, order):
         if r is not None:                       # the residual may be the output
             z = r.clone()
             assert torch.equal(sm.int8_shared_expert(x, wg, sg, wu, su, wd, sd, residual=z, out=z), y)
+
+
+@pytest.mark.parametrize("d, f", [(2048, 1408), (7168, 600), (300, 9000)])
+def test_shared_expert_of_a_few_tokens(gpu, d, f):
+    gen = torch.Generator().manual_seed(d + f)
+    wg, sg = int8_matrix(gen, d, f, "kn", gpu)
+    wu, su = int8_matrix(gen, d, f, "kn", gpu)
+    wd, sd = int8_matrix(gen, f, d, "kn", gpu)
+    sg, su = sg / math.sqrt(d), su / math.sqrt(d)
+    x = tokens(17, d, torch.bfloat16, 3)
+    for n in (1, 4, 5, 8, 9, 16, 17):
+        y = sm.int8_shared_expert(x[:n], wg, sg, wu, su, wd, sd)
+        ref, tol = shared_ref(x[:n], wg, sg, wu, su, wd, sd, None)
+        tol = tol + half_step(x.dtype) * (1.01 * np.abs(ref) + tol) + tiny(x.dtype)
+        err = np.abs(y.cpu().double().numpy() - ref)
+        assert (err <= tol).all(), f"{n} tokens: worst {np.max(err / tol)} of the tolerance"
+
+
+def test_calls_in_a_row_on_forked_streams(gpu):
+    """Kernels that start early: each call reads what the one before it, or another stream's, has just written, in the
+    order of the streams; eager and captured, the scratch and outputs reused at once."""
+    gen = torch.Generator().manual_seed(8)
+    w, ws = int8_matrix(gen, 1024, 1024, "kn", gpu)
+    w2, ws2 = int8_matrix(gen, 1024, 1024, "nk", gpu)
+    logits_w, logits_s = int8_matrix(gen, 1024, 64, "kn", gpu)
+    side = torch.cuda.Stream()
+
+    def run(x, out):
+        main = torch.cuda.current_stream()
+        a = sm.int8_linear(x, w, ws)
+        for _ in range(3):                      # a chain, each link on what the last has written
+            a = sm.int8_linear(a, w2, ws2, out=out)
+            a = sm.int8_linear(a, w, ws)
+        side.wait_stream(main)
+        with torch.cuda.stream(side):
+            b = sm.int8_linear(a, w2, ws2)
+            b = sm.int8_linear(b, w, ws)
+        c = sm.int8_linear(a, w, ws)
+        main.wait_stream(side)
+        lg = sm.int8_linear(b + c, logits_w, logits_s, out_dtype=torch.float32)
+        idx, wt = sm.route_experts(lg, 6, score="sigmoid")
+        b.record_stream(main)
+        return a, b, c, lg, idx, wt
+
+    for T in (1, 4, 12, 40, 700):
+        x = tokens(T, 1024, torch.bfloat16, T)
+        out = torch.empty(T, 1024, dtype=torch.bfloat16, device=gpu)
+        q = lambda a, m, s: sm.int8_linear(a, m, s)  # noqa: E731
+        steps = [q(x, w, ws)]
+        torch.cuda.synchronize()
+        for _ in range(3):
+            for m, s in ((w2, ws2), (w, ws)):
+                steps.append(q(steps[-1], m, s))
+                torch.cuda.synchronize()        # one at a time
+        a = steps[-1]
+        want = [a, q(q(a, w2, ws2), w, ws), q(a, w, ws)]
+        torch.cuda.synchronize()
+        want.append(sm.int8_linear(want[1] + want[2], logits_w, logits_s, out_dtype=torch.float32))
+        torch.cuda.synchronize()
+        want += sm.route_experts(want[3], 6, score="sigmoid")
+        torch.cuda.synchronize()
+        for _ in range(20):
+            got = run(x, out)
+        torch.cuda.synchronize()
+        assert all(torch.equal(g, h) for g, h in zip(got, want))
+        buf = torch.zeros_like(x)
+        gr = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(gr):
+            got = run(buf, out)
+        for _ in range(5):
+            buf.copy_(x)
+            gr.replay()
+            torch.cuda.synchronize()
+            assert all(torch.equal(g, h) for g, h in zip(got, want))
+            buf.zero_()
 
 
 def test_shared_expert_refusals_and_graph(gpu):

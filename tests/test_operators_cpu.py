@@ -67,10 +67,11 @@ def test_linear_limits():
     assert linear(K=131072, ldx=131072) == sm.MOE_ERR_UNSUPPORTED
     assert linear(T=1 << 31) == sm.MOE_ERR_UNSUPPORTED
     assert linear(T=0, x=None, out=None, scratch=None, n=0) == sm.MOE_OK
-    assert sm.lib.moe_int8_linear_scratch_bytes(50, 100) >= 50 * 112 + 50 * 4
-    assert sm.lib.moe_int8_linear_scratch_bytes(1, 7168) == 0   # a few tokens: one kernel, no scratch
-    assert sm.lib.moe_int8_linear_scratch_bytes(1, 131071) > 0  # whose codes do not fit its shared memory
-    assert sm.lib.moe_int8_linear_scratch_bytes(-1, 100) == 0
+    assert sm.lib.moe_int8_linear_scratch_bytes(50, 100, 64) >= 50 * 112 + 50 * 4
+    assert sm.lib.moe_int8_linear_scratch_bytes(1, 7168, 8192) == 0    # a few tokens: one kernel, no scratch
+    assert sm.lib.moe_int8_linear_scratch_bytes(1, 7168, 65536) > 0    # more CTAs than run at once
+    assert sm.lib.moe_int8_linear_scratch_bytes(1, 131071, 64) > 0  # whose codes do not fit its shared memory
+    assert sm.lib.moe_int8_linear_scratch_bytes(-1, 100, 64) == 0
 
 
 def test_quantize_and_matmul_refusals():
