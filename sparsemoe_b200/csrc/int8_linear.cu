@@ -500,15 +500,24 @@ struct StagedEpilogue {
     // ends inside 16 bytes): consecutive lanes write consecutive columns.
     static __device__ __forceinline__ void store_rows(const LinearParams& p, const uint8_t* stage, int64_t base, int row0,
                                                       int col0, int lane) {
-        const int c = lane % kC;
+        using E = typename std::conditional<kF32, float, uint16_t>::type;
+        constexpr int kStep = 32 / kC, kBatch = 8;   // rows an instruction, instructions at once
+        const int c = lane % kC, first = lane / kC, rows = p.T - row0;
         if (col0 + c >= p.N) return;
         const int unit = c / (kC / 4), in = c % (kC / 4);
-#pragma unroll 4
-        for (int r = lane / kC; r < 32 && row0 + r < p.T; r += 32 / kC) {
-            const uint8_t* src = stage + r * 64 + ((unit ^ ((r >> 1) & 3)) * 16) + in * (64 / kC);
-            const int64_t at = base + (int64_t)(row0 + r) * p.ld_out + col0 + c;
-            if (kF32) static_cast<float*>(p.out)[at] = *reinterpret_cast<const float*>(src);
-            else static_cast<uint16_t*>(p.out)[at] = *reinterpret_cast<const uint16_t*>(src);
+        const uint8_t* src = stage + first * 64 + in * (int)sizeof(E);
+        E* dst = static_cast<E*>(p.out) + base + (int64_t)(row0 + first) * p.ld_out + col0 + c;
+#pragma unroll 1
+        for (int r = 0; r < 32; r += kStep * kBatch) {
+            E v[kBatch];
+#pragma unroll
+            for (int i = 0; i < kBatch; ++i)         // row r + kStep * i + first
+                v[i] = *reinterpret_cast<const E*>(src + (r + kStep * i) * 64 + ((unit ^ ((kStep * i) >> 1 & 3)) * 16));
+#pragma unroll
+            for (int i = 0; i < kBatch; ++i) {
+                if (r + kStep * i + first < rows) *dst = v[i];
+                dst += kStep * p.ld_out;
+            }
         }
     }
 
