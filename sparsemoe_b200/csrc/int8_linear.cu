@@ -757,6 +757,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     } else if (warp == 1) {
         if (lane == 0 && leads) {
             // ---------------- MMA issuer (of a pair, its first CTA's) ----------------
+            pdl_wait();   // the bounds of the waits below count from here
             int s = 0;
             uint32_t ph = 0;
             int acc = 0;
@@ -1078,6 +1079,7 @@ __global__ void __launch_bounds__(kSmallThreads, 2)
             cluster_wait();
         }
         if (lane == 0) {
+            pdl_wait();   // the bounds of the waits below count from here
             bool ok = mbar_wait(ready, 0, status, kDevErrTimeout);
             int s = 0;
             uint32_t ph = 0;
@@ -1468,7 +1470,7 @@ template <int kIn, bool kSwiglu>
 cudaError_t launch_small_typed(const CUtensorMap (&w)[2], const SmallParams& p, int tiles, size_t smem, cudaStream_t st) {
     auto kern = small_linear_kernel<kSmallN, kIn, kSwiglu>;
     static SmemAttr attr;
-    cudaError_t err = ensure_smem(kern, smem, attr);
+    cudaError_t err = ensure_smem(kern, kSmallSmem, attr);   // one limit: threads may call at once
     if (err != cudaSuccess) return err;
     return launch_ex(kern, (unsigned)(tiles * p.split), (unsigned)kSmallThreads, smem, p.split, st, w[0], w[1],
                      p);
@@ -1601,6 +1603,16 @@ int check_out(const char* who, const void* out, int type, int64_t T, int64_t N, 
     return MOE_OK;
 }
 
+// Whether rows of wa bytes sa apart and rows of wb bytes sb apart share memory.
+// Exact for equal strides (two slices of one wider matrix do not).
+bool overlap(const void* a, int64_t sa, int64_t wa, const void* b, int64_t sb, int64_t wb, int64_t T) {
+    const int64_t pa = (int64_t)reinterpret_cast<uintptr_t>(a), pb = (int64_t)reinterpret_cast<uintptr_t>(b);
+    if (pa + (T - 1) * sa + wa <= pb || pb + (T - 1) * sb + wb <= pa) return false;
+    if (T == 1 || sa != sb) return true;
+    const int64_t at = ((pb - pa) % sa + sa) % sa;   // of b's rows in a's
+    return at < wa || at + wb > sa;
+}
+
 int check_scratch(const char* who, const void* scratch, size_t have, size_t need) {
     if (need == 0) return MOE_OK;
     if (!scratch || !aligned(scratch, 256)) return bad(who, "scratch is null or not 256-byte aligned");
@@ -1703,7 +1715,13 @@ int run_shared_expert(const char* who, const void* x, int x_type, int64_t tokens
     if (tokens == 0) return MOE_OK;
     const SharedScratch sc = shared_scratch(tokens, d_model, d_ff);
     rc = check_scratch(who, scratch, scratch_bytes, sc.total);
-    if (rc != MOE_OK || check_only) return rc;
+    if (rc != MOE_OK) return rc;
+    const int in = elem_bytes(x_type), size = elem_bytes(out_type);
+    const bool same = residual == out && x_type == out_type && (tokens == 1 || residual_stride == out_stride);
+    if (residual && !same &&
+        overlap(residual, residual_stride * in, (int64_t)d_model * in, out, out_stride * size, (int64_t)d_model * size, tokens))
+        return bad(who, "the output shares memory with the residual without being it");
+    if (check_only) return MOE_OK;
     int dev = 0, num_sms = 0;
     rc = current_device(&dev, &num_sms);
     if (rc != MOE_OK) return rc;
@@ -1783,6 +1801,9 @@ extern "C" int moe_int8_matmul(const int8_t* q, int64_t q_stride, const float* s
     if (!q || !scale || !aligned(q, 16) || q_stride % 16 != 0 || q_stride < K || !aligned(scale, 4))
         return bad(who, "codes must be rows on 16-byte boundaries (q_stride % 16 == 0, >= K) and scales f32");
     if (!aligned(bias, 4)) return bad(who, "bias is not aligned to f32");
+    const int size = elem_bytes(out_type);
+    if (overlap(q, q_stride, K, out, out_stride * size, (int64_t)N * size, tokens))
+        return bad(who, "the output shares memory with the codes");
     int dev = 0, num_sms = 0;
     rc = current_device(&dev, &num_sms);
     if (rc != MOE_OK) return rc;
@@ -1808,6 +1829,9 @@ extern "C" int moe_int8_linear(const void* x, int x_type, int64_t tokens, int K,
     if (tokens == 0) return MOE_OK;
     rc = check_scratch(who, scratch, scratch_bytes, linear_scratch(tokens, K, N));
     if (rc != MOE_OK) return rc;
+    const int in = elem_bytes(x_type), size = elem_bytes(out_type);
+    if (overlap(x, row_stride * in, (int64_t)K * in, out, out_stride * size, (int64_t)N * size, tokens))
+        return bad(who, "the output shares memory with the activations");
     int dev = 0, num_sms = 0;
     rc = current_device(&dev, &num_sms);
     if (rc != MOE_OK) return rc;

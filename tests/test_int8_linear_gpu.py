@@ -292,6 +292,38 @@ def test_shared_expert(gpu, T, d, f, order):
             assert torch.equal(sm.int8_shared_expert(x, wg, sg, wu, su, wd, sd, residual=z, out=z), y)
 
 
+@pytest.mark.parametrize("K", [96, 4096, 7168])
+def test_broken_rows_among_a_few(gpu, K):
+    x = tokens(16, K, torch.bfloat16, 1)
+    x[0, K - 1], x[1], x[2, 17], x[3, K // 2] = math.inf, 0, math.nan, -math.inf
+    w, ws = int8_matrix(torch.Generator().manual_seed(0), K, 200, "kn", gpu)
+    whole = sm.int8_linear(torch.cat([x, x, x]), w, ws)[:16]
+    q, s = sm.quantize_int8_tokens(x)
+    for n in (1, 4, 5, 16):
+        for y in (sm.int8_linear(x[:n], w, ws), sm.int8_matmul(q[:n], s[:n], w, ws)):
+            bad = [t for t in (0, 2, 3) if t < n]
+            good = [t for t in range(n) if t not in bad]
+            assert torch.isnan(y[bad]).all() and torch.equal(y[good], whole[:n][good])
+            assert n < 2 or (y[1] == 0).all()
+
+
+def test_outputs_beside_and_in_the_inputs(gpu):
+    w, ws = int8_matrix(torch.Generator().manual_seed(0), 256, 256, "kn", gpu)
+    for T in (1, 3, 16, 200):
+        wide = torch.zeros(T, 512, dtype=torch.bfloat16, device=gpu)
+        x = wide[:, :256]
+        x.copy_(tokens(T, 256, torch.bfloat16, T))
+        want = sm.int8_linear(x.clone(), w, ws)
+        assert torch.equal(sm.int8_linear(x, w, ws, out=wide[:, 256:]), want)   # the other half of the rows
+        for bad in (x, wide[:, 128:384]):
+            with pytest.raises(sm.MoeError, match="shares memory"):
+                sm.int8_linear(x, w, ws, out=bad)
+        ref = sm.int8_shared_expert(x, w, ws, w, ws, w, ws, residual=x.clone())
+        with pytest.raises(sm.MoeError, match="shares memory"):
+            sm.int8_shared_expert(x, w, ws, w, ws, w, ws, residual=wide[:, 128:384], out=wide[:, 256:])
+        assert torch.equal(sm.int8_shared_expert(x, w, ws, w, ws, w, ws, residual=x, out=x), ref)
+
+
 @pytest.mark.parametrize("d, f", [(2048, 1408), (7168, 600), (300, 9000)])
 def test_shared_expert_of_a_few_tokens(gpu, d, f):
     gen = torch.Generator().manual_seed(d + f)

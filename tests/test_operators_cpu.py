@@ -74,6 +74,15 @@ def test_linear_limits():
     assert sm.lib.moe_int8_linear_scratch_bytes(-1, 100, 64) == 0
 
 
+@pytest.mark.parametrize("kw", [
+    dict(), dict(out=FAKE + 64), dict(out=FAKE + 128, T=2), dict(out=FAKE - 64), dict(out=FAKE + 100, ldx=100, ldo=100),
+    dict(T=1, out=FAKE + 126), dict(T=1, out=FAKE - 126), dict(ldx=128, ldo=128, out=FAKE + 126),
+    dict(ldx=128, ldo=128, out=FAKE + 130), dict(otyp=0, ldx=256, ldo=128, out=FAKE + 384)])
+def test_outputs_in_the_activations_memory(kw):
+    assert linear(**kw) == sm.MOE_ERR_INVALID_ARG
+    assert b"shares memory" in sm.lib.moe_last_error()
+
+
 def test_quantize_and_matmul_refusals():
     q = lambda x=FAKE, typ=2, T=4, K=64, ldx=64, out=FAKE, ldq=64, s=FAKE: sm.lib.moe_int8_quantize_tokens(  # noqa: E731
         x, typ, T, K, ldx, out, ldq, s, None)
