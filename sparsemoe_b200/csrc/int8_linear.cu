@@ -98,6 +98,17 @@ template <typename T16> struct In8_16 {
 template <> struct In8<__half> : In8_16<__half> {};
 template <> struct In8<__nv_bfloat16> : In8_16<__nv_bfloat16> {};
 
+// Two fused multiply-adds in one instruction.
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+    float2 d;
+    asm("{\n\t.reg .b64 a, b, c, d;\n\t"
+        "mov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tmov.b64 c, {%6, %7};\n\t"
+        "fma.rn.f32x2 d, a, b, c;\n\tmov.b64 {%0, %1}, d;\n\t}"
+        : "=f"(d.x), "=f"(d.y)
+        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+    return d;
+}
+
 // Codes of eight values: round-half-even of the exact x / s.  x * (1/s) is within
 // 127 * 2^-23 of the quotient, so its nearest integer n (which one fma leaves in
 // the low bits of 1.5 * 2^23 + n) is right or the other neighbour of a border.
@@ -116,11 +127,16 @@ __device__ __forceinline__ uint2 quant8(float (&f)[8], float s, float inv, float
 #pragma unroll
         for (int i = 0; i < 8; ++i) f[i] *= pre;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        const float m = fmaf(f[i], inv, kMagic);
-        e[i] = fmaf(kMagic - m, s, f[i]);
-        far = fmaxf(far, fabsf(e[i]));
-        t[i] = __float_as_uint(m);
+    for (int i = 0; i < 8; i += 2) {
+        const float2 x = make_float2(f[i], f[i + 1]);
+        const float2 m = fma2(x, make_float2(inv, inv), make_float2(kMagic, kMagic));
+        const float2 n = fma2(m, make_float2(-1.0f, -1.0f), make_float2(kMagic, kMagic));
+        const float2 d = fma2(n, make_float2(s, s), x);
+        e[i] = d.x;
+        e[i + 1] = d.y;
+        far = fmaxf(far, fmaxf(fabsf(d.x), fabsf(d.y)));
+        t[i] = __float_as_uint(m.x);
+        t[i + 1] = __float_as_uint(m.y);
     }
     const float half = 0.5f * s;
     if (far >= half) {
