@@ -191,11 +191,13 @@ __device__ __forceinline__ float silu(float g) { return g / (1.0f + __expf(-g));
 
 // kPair (T = float): x holds gate values, the up values start `up` elements
 // behind them, and the row that is quantised is up * gate / (1 + exp(-gate)).
-// HBM-bound for many rows: 8192 x 7168 bf16 takes 36.7 us (4.8 TB/s of reads and
-// writes), 8192 x 2048 f32 15.4 us (5.5 TB/s).  The registers are held to 32 a
-// thread (48 for f32), which keeps 2048 (1280) threads' rows in flight on an SM.
+// For many rows instruction issue (four fifths of the slots) and the HBM both
+// count: 8192 x 7168 bf16 takes 34.1 us (5.2 TB/s of reads and writes), 8192 x 2048
+// f32 15.3 (5.5 TB/s).  The registers are held to 32 a thread where 256 share a
+// row (eight blocks an SM; 40 and six took 34.8 us) and to 40 below, where 32
+// spill (8192 x 2048 bf16 12.0 us, 13.3 with 32); to 48 for f32.
 template <typename T, int TPR, bool kPair>
-__global__ void __launch_bounds__(256, sizeof(T) == 2 ? 8 : 5)
+__global__ void __launch_bounds__(256, sizeof(T) == 4 ? 5 : TPR == 256 ? 8 : 6)
     quantize_tokens_kernel(const T* x, int64_t rows, int K, int64_t ldx, int64_t up, int8_t* q, int64_t ldq,
                            float* scale, int vec) {
     pdl_wait();
