@@ -399,6 +399,57 @@ def test_calls_in_a_row_on_forked_streams(gpu):
             buf.zero_()
 
 
+def test_behind_copies_and_fills(gpu):
+    """The kernel before may be none: copies and fills, eager and in a graph."""
+    gen = torch.Generator().manual_seed(9)
+    w, ws = int8_matrix(gen, 512, 512, "kn", gpu)
+    for T in (1, 10, 300):
+        x = tokens(T, 512, torch.bfloat16, T)
+        want, lg = sm.int8_linear(x, w, ws), tokens(T, 64, torch.float32, 1)
+        ridx, rw = sm.route_experts(lg, 4)
+        a, b, lb = torch.empty_like(x), torch.empty_like(x), torch.empty_like(lg)
+
+        def run():
+            b.zero_()
+            a.copy_(x)
+            y = sm.int8_linear(a, w, ws)
+            b.copy_(y)
+            z = sm.int8_matmul(*sm.quantize_int8_tokens(b), w, ws)
+            lb.zero_()
+            lb.copy_(lg)
+            return y, z, *sm.route_experts(lb, 4)
+
+        ref = want, sm.int8_linear(want, w, ws), ridx, rw
+        for _ in range(10):
+            got = run()
+        assert all(torch.equal(g, r) for g, r in zip(got, ref))
+        gr = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(gr):
+            got = run()
+        for _ in range(3):
+            gr.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(g, r) for g, r in zip(got, ref))
+
+
+def test_calls_from_two_threads(gpu):
+    from concurrent.futures import ThreadPoolExecutor
+    gen = torch.Generator().manual_seed(12)
+    w, ws = int8_matrix(gen, 4096, 900, "kn", gpu)
+    xs = [tokens(T, 4096, torch.bfloat16, T) for T in (1, 4, 11, 130)]
+    want = [sm.int8_linear(x, w, ws) for x in xs]
+    torch.cuda.synchronize()
+
+    def work(k):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            out = [sm.int8_linear(xs[(i + k) % 4], w, ws) for i in range(40)]
+            torch.cuda.current_stream().synchronize()
+        return all(torch.equal(y, want[(i + k) % 4]) for i, y in enumerate(out))
+
+    with ThreadPoolExecutor(3) as pool:
+        assert all(pool.map(work, range(3)))
+
+
 def test_shared_expert_refusals_and_graph(gpu):
     gen = torch.Generator().manual_seed(0)
     wg, sg = int8_matrix(gen, 96, 64, "kn", gpu)
