@@ -393,6 +393,18 @@ __device__ __forceinline__ bool mbar_wait_cluster(uint64_t* bar, uint32_t parity
     return ok;
 }
 
+// After a wait that ran out: up to kDrainNs more for what is still in flight (a
+// copy, MMAs), so that none of it arrives in memory that the CTA has left.
+constexpr uint64_t kDrainNs = 1000000;   // 1 ms, where a copy takes microseconds
+__device__ __forceinline__ void mbar_drain(uint64_t* bar, uint32_t parity) {
+    const uint64_t t0 = globaltimer_ns();
+    while (!mbar_try_wait(smem_u32(bar), parity) && globaltimer_ns() - t0 < kDrainNs) {}
+}
+__device__ __forceinline__ void wait_ns(uint64_t ns) {
+    const uint64_t t0 = globaltimer_ns();
+    while (globaltimer_ns() - t0 < ns) __nanosleep(1000);
+}
+
 __device__ __forceinline__ float load_as_f32(const void* p, int64_t i, int type) {
     if (type == MOE_TYPE_F32) return static_cast<const float*>(p)[i];
     if (type == MOE_TYPE_F16) return __half2float(static_cast<const __half*>(p)[i]);
@@ -754,7 +766,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             // No trigger: the kernel behind is mostly a quantiser, whose CTAs would all settle on the SMs that this
             // grid leaves idle (the shared expert of 512 tokens took 54.7 us with one here, 50.1 without).
             pdl_wait();
-            int s = 0;
+            int s = 0, filled = 0;   // filled: stages with a copy that may be in flight
             uint32_t ph = 0;
             for (int t = tile0; t < total; t += step) {
                 const int n = t / p.m_tiles, m = t - n * p.m_tiles;
@@ -768,9 +780,21 @@ __global__ void __launch_bounds__(kThreads, 1)
                     }
                     load(sA + s * C::kABytes, &tmA, s, kb * kBK, token_row(m));
                     if (++s == C::kStages) { s = 0; ph ^= 1u; }
+                    filled = min(filled + 1, C::kStages);
                 }
             }
-        producer_done:;
+            // The last release of each stage arrives in this CTA's memory (of a pair, the first CTA's MMAs arrive in
+            // both): wait for it before the CTA may end.  A stage that was never filled passes, as above.
+            for (int i = 0; i < C::kStages; ++i)
+                if (!mbar_wait(&empty[i], i < s ? ph : ph ^ 1u, status, kDevErrTimeout)) goto producer_done;
+            filled = 0;
+        producer_done:
+            // Given up: the copies in flight land before the CTA ends.  (A pair's second CTA has no barrier of its
+            // own for them; its copies take microseconds.)
+            if (filled > 0) {
+                for (int i = 0; leads && i < filled; ++i) mbar_drain(&full[i], i < s ? ph : ph ^ 1u);
+                if (kPair) wait_ns(kDrainNs);
+            }
         }
     } else if (warp == 1) {
         if (lane == 0 && leads) {
@@ -778,6 +802,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             pdl_wait();   // the bounds of the waits below count from here
             int s = 0;
             uint32_t ph = 0;
+            bool issued = false;
             int acc = 0;
             uint32_t aph = 0;
             for (int t = tile0; t < total; t += step) {
@@ -802,6 +827,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                     }
                     if (kPair) mma_commit2(&empty[s]);
                     else mma_commit(&empty[s]);
+                    issued = true;
                     if (++s == C::kStages) { s = 0; ph ^= 1u; }
                 }
                 if (!ok) break;
@@ -810,6 +836,10 @@ __global__ void __launch_bounds__(kThreads, 1)
                 acc ^= 1;
                 if (acc == 0) aph ^= 1u;
             }
+            // The MMAs issued so far end before the TMEM is freed (of a run that was not given up, the epilogue and
+            // the producers wait for them): their last stage's release.
+            const int last = s > 0 ? s - 1 : C::kStages - 1;
+            if (issued) mbar_drain(&empty[last], s > 0 ? ph : ph ^ 1u);
         }
     } else {
         // ---------------- epilogue (warps 2..9) ----------------
@@ -1083,9 +1113,15 @@ __global__ void __launch_bounds__(kSmallThreads, 2)
         if (lane == 0) {
             int s = 0;
             uint32_t ph = 0;
-            for (int i = first; i < loads; ++i) {
-                if (!mbar_wait(&empty[s], ph, status, kDevErrTimeout)) break;
-                load(s, i);
+            // behind the last load, the last release of each stage: it arrives in this CTA's memory
+            for (int i = first; i < loads + first; ++i) {
+                if (!mbar_wait(&empty[s], ph, status, kDevErrTimeout)) {
+                    // given up: the copies in flight land before the CTA ends
+                    for (int j = max(0, min(i, loads) - p.stages); j < min(i, loads); ++j)
+                        mbar_drain(&full[j % p.stages], (uint32_t)(j / p.stages) & 1u);
+                    break;
+                }
+                if (i < loads) load(s, i);
                 if (++s == p.stages) { s = 0; ph ^= 1u; }
             }
         }
@@ -1099,8 +1135,8 @@ __global__ void __launch_bounds__(kSmallThreads, 2)
         if (lane == 0) {
             pdl_wait();   // the bounds of the waits below count from here
             bool ok = mbar_wait(ready, 0, status, kDevErrTimeout);
-            int s = 0;
-            uint32_t ph = 0;
+            int s = 0, last = -1;
+            uint32_t ph = 0, last_ph = 0;
             for (int i = 0; ok && i < loads; ++i) {
                 if (!mbar_wait(&full[s], ph, status, kDevErrTimeout)) { ok = false; break; }
                 tc_fence_after();
@@ -1116,9 +1152,12 @@ __global__ void __launch_bounds__(kSmallThreads, 2)
                               (i >= kMats || kk != 0) ? 1u : 0u);
                 }
                 mma_commit(&empty[s]);
+                last = s;
+                last_ph = ph;
                 if (++s == p.stages) { s = 0; ph ^= 1u; }
             }
             if (ok) mma_commit(tfull);
+            else if (last >= 0) mbar_drain(&empty[last], last_ph);   // given up: the MMAs end before the TMEM is freed
         }
     } else {
         // ---------------- quantiser, then epilogue (warps 2..9) ----------------
