@@ -371,7 +371,9 @@ int moe_peer_free(void* ptr);
 int moe_memcpy_async(void* dst, const void* src, size_t bytes, cudaStream_t stream);
 
 // Synchronises `stream` and reports a device-side failure (MOE_ERR_TIMEOUT) of
-// the last moe_solve_v2 on this device, MOE_OK otherwise.
+// the last moe_solve_v2 on this device, or of any int8 product on this device
+// since the last call (reported once; the outputs of the call that failed are
+// undefined, those of others are not touched by it), MOE_OK otherwise.
 int moe_check_device_status(cudaStream_t stream);
 
 // Dims used by solve() and by the input builder (inputs/data.h functions).
@@ -404,6 +406,11 @@ void moe_release(void);
 // A following moe_check_device_status(stream) returns MOE_ERR_TIMEOUT; the
 // next layer call clears the word.
 int moe_selftest_wait_timeout(int64_t timeout_ns, cudaStream_t stream);
+// The same for the int8 products: a cluster of two CTAs, the second of which
+// waits for at most timeout_ns on an mbarrier nothing arrives on.  Each CTA
+// then writes 1 into its word of `written` (device int [2]) unless it has been
+// told of the failure.
+int moe_selftest_int8_wait_timeout(int64_t timeout_ns, int* written, cudaStream_t stream);
 
 // Text of the last error recorded on this host thread ("" if none).
 const char* moe_last_error(void);

@@ -38,6 +38,7 @@ def _load() -> ctypes.CDLL:
         "moe_solve_v2": (ctypes.c_int, [ctypes.POINTER(MoEArgs), ctypes.POINTER(MoeDims), _p]),
         "moe_check_device_status": (ctypes.c_int, [_p]),
         "moe_selftest_wait_timeout": (ctypes.c_int, [ctypes.c_int64, _p]),
+        "moe_selftest_int8_wait_timeout": (ctypes.c_int, [ctypes.c_int64, _p, _p]),
         "moe_set_solve_dims": (ctypes.c_int, [ctypes.POINTER(MoeDims)]),
         "moe_get_solve_dims": (ctypes.c_int, [ctypes.POINTER(MoeDims)]),
         "moe_capacity": (ctypes.c_int, [ctypes.c_int, ctypes.c_int, ctypes.c_int, ctypes.c_float]),
@@ -328,7 +329,8 @@ def quantize_per_tensor(w16: np.ndarray, qmax: float = 127.0):
 
 
 from .operators import (  # noqa: E402  (needs `lib` above)
-    Routing, int8_linear, int8_matmul, int8_shared_expert, int8_weight, quantize_int8_tokens, route_experts)
+    Routing, int8_linear, int8_matmul, int8_shared_expert, int8_weight, quantize_int8_tokens, route_experts,
+    sync_check)
 from .layer import MoeLayer  # noqa: E402
 
 __all__ = ["MoEArgs", "MoeDims", "LayerConfig", "MoeLayer", "make_inputs", "capacity", "lib", "check",
@@ -337,4 +339,4 @@ __all__ = ["MoEArgs", "MoeDims", "LayerConfig", "MoeLayer", "make_inputs", "capa
            "DTYPE_W4A16", "quantize_int4_g128", "DTYPE_INT8_CHANNEL", "quantize_int8_channel",
            "DTYPE_NVFP4", "quantize_nvfp4", "DTYPE_INT4_PTX", "DTYPE_FP8", "save_weights", "load_weights", "MoeWeightFile", "MoeWeightArray",
            "Routing", "route_experts", "quantize_int8_tokens", "int8_matmul", "int8_linear", "int8_weight",
-           "int8_shared_expert", "MoeRouting", "MoeInt8Weight", "MoeSharedExpert", "MoeLayerOptions"]
+           "int8_shared_expert", "sync_check", "MoeRouting", "MoeInt8Weight", "MoeSharedExpert", "MoeLayerOptions"]

@@ -28,7 +28,9 @@ namespace {
 
 using namespace sm100;
 
-// Set by a wait that ran out; read and cleared by moe_check_device_status.
+// Report of a wait that ran out, for the host alone: read and cleared by
+// moe_check_device_status.  No kernel reads it, so what one launch reports
+// stops no other.
 __device__ int g_linear_status;
 
 // ---- per-token quantisation --------------------------------------------------------
@@ -386,12 +388,42 @@ __device__ __forceinline__ void tma_load_2d_pair(void* dst, const void* tmap, ui
 __device__ __forceinline__ void arrive_cluster(uint32_t bar) {
     asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }
-// As mbar_wait, for arrivals from the cluster.
-__device__ __forceinline__ bool mbar_wait_cluster(uint64_t* bar, uint32_t parity, int* status, int code) {
-    const bool ok = mbar_wait(bar, parity, status, code);
-    asm volatile("fence.acq_rel.cluster;" ::: "memory");
-    return ok;
-}
+// A CTA's bounded waits.  One that runs out is reported to the host and sets
+// `stop` (shared memory), which ends the waits of the CTA's other roles and, of
+// a pair, the other CTA's.
+struct Waits {
+    uint32_t* stop;
+    uint32_t peer;   // the other CTA's word (0: none)
+    uint64_t limit_ns;
+
+    __device__ __forceinline__ bool operator()(uint64_t* bar, uint32_t parity) const {
+        const uint32_t a = smem_u32(bar);
+        if (mbar_try_wait(a, parity)) return true;
+        const uint64_t t0 = globaltimer_ns();
+        for (uint32_t it = 1;; ++it) {
+            if (mbar_try_wait(a, parity)) return true;
+            if ((it & 15) == 0) {   // (the clock and the word not at every try, as mbar_wait)
+                if (*(volatile uint32_t*)stop != 0) return false;
+                if (globaltimer_ns() - t0 > limit_ns) {
+                    atomicCAS(&g_linear_status, 0, kDevErrTimeout);
+                    *(volatile uint32_t*)stop = 1;
+                    if (peer) asm volatile("st.shared::cluster.b32 [%0], %1;" ::"r"(peer), "r"(1u) : "memory");
+                    return false;
+                }
+            }
+        }
+    }
+    // For roles that go on with warp-collective operations: one answer for the warp.
+    __device__ __forceinline__ bool warp(uint64_t* bar, uint32_t parity) const {
+        return __all_sync(0xffffffffu, (*this)(bar, parity));
+    }
+    // For arrivals from the cluster.
+    __device__ __forceinline__ bool cluster(uint64_t* bar, uint32_t parity) const {
+        const bool ok = (*this)(bar, parity);
+        asm volatile("fence.acq_rel.cluster;" ::: "memory");
+        return ok;
+    }
+};
 
 // After a wait that ran out: up to kDrainNs more for what is still in flight (a
 // copy, MMAs), so that none of it arrives in memory that the CTA has left.
@@ -672,6 +704,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     extern __shared__ uint8_t smem_raw[];
     __shared__ __align__(16) float s_scale[2][kBN];
     __shared__ __align__(16) float s_bias[2][kBN];
+    __shared__ uint32_t s_stop;
 
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     uint8_t* sA = smem;
@@ -685,9 +718,10 @@ __global__ void __launch_bounds__(kThreads, 1)
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int rank = (int)cluster_rank();
-    int* status = &g_linear_status;
+    const Waits wait{&s_stop, kPair ? mapa(smem_u32(&s_stop), rank ^ 1) : 0u, kWaitTimeoutNs};
 
     if (threadIdx.x == 0) {
+        s_stop = 0;
         for (int s = 0; s < C::kStages; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], 1); }
         for (int a = 0; a < 2; ++a) { mbar_init(&tfull[a], 1); mbar_init(&tempty[a], (kPair ? 2 : 1) * kEpiThreads / 32); }
         fence_mbar_init();
@@ -774,7 +808,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                     if (ahead > 0) {
                         --ahead;
                     } else {
-                        if (!mbar_wait(&empty[s], ph ^ 1u, status, kDevErrTimeout)) goto producer_done;
+                        if (!wait(&empty[s], ph ^ 1u)) goto producer_done;
                         expect(s);
                         load_b(s, n, kb);
                     }
@@ -786,7 +820,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             // The last release of each stage arrives in this CTA's memory (of a pair, the first CTA's MMAs arrive in
             // both): wait for it before the CTA may end.  A stage that was never filled passes, as above.
             for (int i = 0; i < C::kStages; ++i)
-                if (!mbar_wait(&empty[i], i < s ? ph : ph ^ 1u, status, kDevErrTimeout)) goto producer_done;
+                if (!wait(&empty[i], i < s ? ph : ph ^ 1u)) goto producer_done;
             filled = 0;
         producer_done:
             // Given up: the copies in flight land before the CTA ends.  (A pair's second CTA has no barrier of its
@@ -806,12 +840,12 @@ __global__ void __launch_bounds__(kThreads, 1)
             int acc = 0;
             uint32_t aph = 0;
             for (int t = tile0; t < total; t += step) {
-                if (!mbar_wait_cluster(&tempty[acc], aph ^ 1u, status, kDevErrTimeout)) break;
+                if (!wait.cluster(&tempty[acc], aph ^ 1u)) break;
                 tc_fence_after();
                 const uint32_t d_tmem = tmem_base + acc * kBN;
                 bool ok = true;
                 for (int kb = kb0; kb < kb1; ++kb) {
-                    if (!mbar_wait(&full[s], ph, status, kDevErrTimeout)) { ok = false; break; }
+                    if (!wait(&full[s], ph)) { ok = false; break; }
                     tc_fence_after();
                     const uint32_t a_base = smem_u32(sA + s * C::kABytes);
                     const uint32_t b_base = smem_u32(sB + s * C::kBBytes);
@@ -874,7 +908,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             const float st = valid ? p.s_tok[row] : 0.0f;
             const uint32_t taddr = tmem_base + ((uint32_t)(q * 32) << 16) + acc * kBN + half * kCols;
             if (p.staged && p.residual) StagedEpilogue<kCols, kOutN, false, false>::prefetch_residual(p, row, col0);
-            if (ok) ok = mbar_wait_warp(&tfull[acc], aph, status, kDevErrTimeout);
+            if (ok) ok = wait.warp(&tfull[acc], aph);
             tc_fence_after();
             if (ok && p.staged) {
                 // TMA stores clip rows at 16-byte units: not for a last tile that ends inside one
@@ -1049,6 +1083,7 @@ __global__ void __launch_bounds__(kSmallThreads, 2)
     extern __shared__ uint8_t smem_raw[];
     __shared__ uint32_t s_amax[kMaxSplit][kNT];   // [source CTA][token]: bits of the largest magnitude
     __shared__ float s_tok[kNT];
+    __shared__ uint32_t s_stop;
 
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     const int rank = p.split > 1 ? (int)cluster_rank() : 0;
@@ -1065,8 +1100,9 @@ __global__ void __launch_bounds__(kSmallThreads, 2)
     uint32_t* const tmem_slot = reinterpret_cast<uint32_t*>(tfull + 1);
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    int* status = &g_linear_status;
+    const Waits wait{&s_stop, 0u, kWaitTimeoutNs};
     if (threadIdx.x == 0) {
+        s_stop = 0;
         for (int s = 0; s < p.stages; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], 1); }
         mbar_init(ready, kSmallWorkers);
         mbar_init(tfull, 1);
@@ -1115,7 +1151,7 @@ __global__ void __launch_bounds__(kSmallThreads, 2)
             uint32_t ph = 0;
             // behind the last load, the last release of each stage: it arrives in this CTA's memory
             for (int i = first; i < loads + first; ++i) {
-                if (!mbar_wait(&empty[s], ph, status, kDevErrTimeout)) {
+                if (!wait(&empty[s], ph)) {
                     // given up: the copies in flight land before the CTA ends
                     for (int j = max(0, min(i, loads) - p.stages); j < min(i, loads); ++j)
                         mbar_drain(&full[j % p.stages], (uint32_t)(j / p.stages) & 1u);
@@ -1134,11 +1170,11 @@ __global__ void __launch_bounds__(kSmallThreads, 2)
         }
         if (lane == 0) {
             pdl_wait();   // the bounds of the waits below count from here
-            bool ok = mbar_wait(ready, 0, status, kDevErrTimeout);
+            bool ok = wait(ready, 0);
             int s = 0, last = -1;
             uint32_t ph = 0, last_ph = 0;
             for (int i = 0; ok && i < loads; ++i) {
-                if (!mbar_wait(&full[s], ph, status, kDevErrTimeout)) { ok = false; break; }
+                if (!wait(&full[s], ph)) { ok = false; break; }
                 tc_fence_after();
                 const uint32_t d_tmem = tmem_base + (kSwiglu ? (i & 1) * kNT : 0);
                 const uint32_t w_base = smem_u32(sW + s * kSmallStageBytes);
@@ -1270,7 +1306,7 @@ __global__ void __launch_bounds__(kSmallThreads, 2)
         constexpr int kHalfTok = kNT / 2;
         const int q = warp & 3, half = w >> 2, c = q * 32 + lane, tok = half * kHalfTok;
         if (split && !exchange) cluster_wait();   // phase 1
-        const bool ok = mbar_wait_warp(tfull, 0, status, kDevErrTimeout);
+        const bool ok = wait.warp(tfull, 0);
         tc_fence_after();
         const uint32_t taddr = tmem_base + ((uint32_t)(q * 32) << 16) + tok;
         auto put = [&](int sum, int sum1, int t, int ch) {   // channel ch of the tile
@@ -1335,6 +1371,30 @@ __global__ void __launch_bounds__(kSmallThreads, 2)
         tc_fence_after();
         tmem_dealloc(tmem_base, kTmemCols);
     }
+}
+
+// ---- self-test of the waits ------------------------------------------------------------
+
+// A cluster of two whose second CTA waits for what nothing completes; then each
+// CTA writes its word, unless it has been told to stop.
+__global__ void __launch_bounds__(32) waits_selftest_kernel(uint64_t limit_ns, int* written) {
+    __shared__ __align__(8) uint64_t bar;
+    __shared__ uint32_t s_stop;
+    const int rank = (int)cluster_rank();
+    if (threadIdx.x == 0) {
+        s_stop = 0;
+        mbar_init(&bar, 1);
+        fence_mbar_init();
+    }
+    __syncwarp();
+    cluster_arrive();
+    cluster_wait();
+    const Waits wait{&s_stop, 0u, limit_ns};
+    if (rank == 1) (void)wait.warp(&bar, 0);
+    __syncwarp();
+    cluster_arrive();
+    cluster_wait();
+    if (threadIdx.x == 0 && s_stop == 0) written[rank] = 1;
 }
 
 // ---- host side -----------------------------------------------------------------------
@@ -1821,6 +1881,27 @@ int run_shared_expert(const char* who, const void* x, int x_type, int64_t tokens
 }  // namespace moe
 
 using namespace moe;
+
+extern "C" int moe_selftest_int8_wait_timeout(int64_t timeout_ns, int* written, cudaStream_t stream) {
+    const char* who = "moe_selftest_int8_wait_timeout";
+    if (timeout_ns <= 0 || timeout_ns > 10000000000ll) return bad(who, "timeout_ns must be in (0, 10 s]");
+    if (!written || !aligned(written, 4)) return bad(who, "written is null or not aligned to int");
+    int dev = 0, num_sms = 0;
+    const int rc = current_device(&dev, &num_sms);
+    if (rc != MOE_OK) return rc;
+    g_linear_used[dev] = true;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(2);
+    cfg.blockDim = dim3(32);
+    cfg.stream = stream;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim = {2, 1, 1};
+    cfg.attrs = at;
+    cfg.numAttrs = 1;
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, waits_selftest_kernel, (uint64_t)timeout_ns, written);
+    return e == cudaSuccess ? MOE_OK : cuda_error(who, e);
+}
 
 extern "C" size_t moe_int8_linear_scratch_bytes(int64_t tokens, int K, int N) {
     return tokens < 0 || K < 1 || N < 1 ? 0 : linear_scratch(tokens, K, N);

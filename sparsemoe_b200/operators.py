@@ -5,7 +5,9 @@ Every call runs on torch's current stream of the tensors' device, allocates its
 outputs and scratch from torch's allocator (so calls may overlap on several
 streams and be captured into CUDA graphs), does not synchronise, and has no
 gradient: the library serves models, it does not train them.  Wrong arguments
-raise ValueError, failures of the library MoeError.
+raise ValueError, failures of the library MoeError.  The waits inside the int8
+products are bounded: a product that gives up returns like any other, its
+outputs undefined, and the next sync_check() raises.
 """
 from __future__ import annotations
 
@@ -26,6 +28,14 @@ except ImportError as e:
 _operators.bind(check, *(ctypes.cast(f, ctypes.c_void_p).value for f in (
     lib.moe_route_experts, lib.moe_int8_quantize_tokens, lib.moe_int8_matmul, lib.moe_int8_linear,
     lib.moe_int8_linear_scratch_bytes, lib.moe_int8_shared_expert, lib.moe_int8_shared_expert_scratch_bytes)))
+
+
+def sync_check(device: torch.device | str | int | None = None) -> None:
+    """Waits for torch's current stream on `device` (default: the current one) and raises MoeError if a wait inside
+    an int8 product has run out on that device since the last check, on any stream (reported once; other calls'
+    outputs are not affected), or in the last layer call there."""
+    with torch.cuda.device(device):
+        check(lib.moe_check_device_status(ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)))
 
 
 # ---- routing ---------------------------------------------------------------------

@@ -49,3 +49,26 @@ def test_fused_gate_and_up_of_every_number_of_blocks(gpu):
         assert all(torch.equal(z, y[0]) for z in y[1:])
         assert torch.equal(y[0][:300], part), K
     sm.check(sm.lib.moe_check_device_status(torch.cuda.current_stream().cuda_stream))
+
+
+def test_a_wait_that_ran_out_stops_no_other_call(gpu):
+    """A cluster whose wait runs out after 50 ms leaves a report for the host: products behind it, of every kind of
+    tile, are not touched by it, and the report comes once."""
+    gen = torch.Generator(device=gpu).manual_seed(2)
+    sm.sync_check()
+    cases = []
+    for T, K, N in ((3, 7168, 600), (16, 900, 600), (130, 131071, 300), (700, 2048, 2000), (16384, 1024, 4097)):
+        q, w, s, ws = codes(gen, T, K, N, gpu)
+        cases.append((q, s, w, ws, sm.int8_matmul(q, s, w, ws, out_dtype=torch.float32)))
+    sm.sync_check()
+    written = torch.zeros(2, dtype=torch.int32, device=gpu)
+    sm.check(sm.lib.moe_selftest_int8_wait_timeout(50_000_000, written.data_ptr(),
+                                                   torch.cuda.current_stream().cuda_stream))
+    got = [sm.int8_matmul(q, s, w, ws, out_dtype=torch.float32) for q, s, w, ws, _ in cases]
+    with pytest.raises(sm.MoeError, match="int8 product"):
+        sm.sync_check()
+    assert all(torch.equal(y, c[-1]) for y, c in zip(got, cases))
+    sm.sync_check(gpu)
+    y = sm.int8_matmul(*cases[0][:4], out_dtype=torch.float32)
+    sm.sync_check("cuda:0")
+    assert torch.equal(y, cases[0][-1])
