@@ -369,12 +369,12 @@ __device__ __forceinline__ void mma_i8_ss2(uint32_t d_tmem, uint64_t a_desc, uin
         "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
         : "memory");
 }
-// Arrives on this barrier of both CTAs when the tcgen05 operations issued so far are done.
-__device__ __forceinline__ void mma_commit2(uint64_t* bar) {
+// Arrives on this barrier of the CTAs in `ctas` (both) when the tcgen05 operations issued so far are done.
+__device__ __forceinline__ void mma_commit2(uint64_t* bar, uint16_t ctas = 3) {
     asm volatile(
         "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(
             smem_u32(bar)),
-        "h"((uint16_t)3)
+        "h"(ctas)
         : "memory");
 }
 // A load into this CTA whose bytes count on a barrier of either CTA of the pair.
@@ -397,11 +397,14 @@ struct Waits {
     uint64_t limit_ns;
 
     __device__ __forceinline__ bool operator()(uint64_t* bar, uint32_t parity) const {
-        const uint32_t a = smem_u32(bar);
-        if (mbar_try_wait(a, parity)) return true;
+        return mbar_try_wait(smem_u32(bar), parity) || longer(smem_u32(bar), parity, stop, peer, limit_ns);
+    }
+    // The tries behind the first, not in line: most waits end in the first one, which may last.
+    static __device__ __noinline__ bool longer(uint32_t bar, uint32_t parity, uint32_t* stop, uint32_t peer,
+                                               uint64_t limit_ns) {
         const uint64_t t0 = globaltimer_ns();
         for (uint32_t it = 1;; ++it) {
-            if (mbar_try_wait(a, parity)) return true;
+            if (mbar_try_wait(bar, parity)) return true;
             if ((it & 15) == 0) {   // (the clock and the word not at every try, as mbar_wait)
                 if (*(volatile uint32_t*)stop != 0) return false;
                 if (globaltimer_ns() - t0 > limit_ns) {
@@ -425,16 +428,20 @@ struct Waits {
     }
 };
 
-// After a wait that ran out: up to kDrainNs more for what is still in flight (a
-// copy, MMAs), so that none of it arrives in memory that the CTA has left.
-constexpr uint64_t kDrainNs = 1000000;   // 1 ms, where a copy takes microseconds
-__device__ __forceinline__ void mbar_drain(uint64_t* bar, uint32_t parity) {
-    const uint64_t t0 = globaltimer_ns();
-    while (!mbar_try_wait(smem_u32(bar), parity) && globaltimer_ns() - t0 < kDrainNs) {}
-}
-__device__ __forceinline__ void wait_ns(uint64_t ns) {
-    const uint64_t t0 = globaltimer_ns();
-    while (globaltimer_ns() - t0 < ns) __nanosleep(1000);
+// After a wait that ran out, by the thread that issues the MMAs: up to 1 ms each
+// for the copies that may be in flight (the next one of each stage; a copy takes
+// microseconds) and for the MMAs issued so far, so that none of them reaches
+// memory that the CTA has left.  (The producers run at most that far ahead.)
+constexpr uint64_t kDrainNs = 1000000;
+template <bool kPair> __device__ __noinline__ void drain(uint64_t* full, int s, uint32_t ph, int stages, uint64_t* bail) {
+    if (kPair) mma_commit2(bail, 1);
+    else mma_commit(bail);
+    for (int i = 0; i <= stages; ++i) {
+        const uint32_t bar = smem_u32(i < stages ? &full[s] : bail), parity = i < stages ? ph : 0;
+        const uint64_t t0 = globaltimer_ns();
+        while (!mbar_try_wait(bar, parity) && globaltimer_ns() - t0 < kDrainNs) {}
+        if (++s == stages) { s = 0; ph ^= 1u; }
+    }
 }
 
 __device__ __forceinline__ float load_as_f32(const void* p, int64_t i, int type) {
@@ -714,7 +721,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     uint64_t* empty = full + C::kStages;
     uint64_t* tfull = empty + C::kStages;
     uint64_t* tempty = tfull + 2;
-    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(tempty + 2);
+    uint64_t* bail = tempty + 2;   // of MMAs that were given up
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bail + 1);
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int rank = (int)cluster_rank();
@@ -724,6 +732,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         s_stop = 0;
         for (int s = 0; s < C::kStages; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], 1); }
         for (int a = 0; a < 2; ++a) { mbar_init(&tfull[a], 1); mbar_init(&tempty[a], (kPair ? 2 : 1) * kEpiThreads / 32); }
+        mbar_init(bail, 1);
         fence_mbar_init();
         tma_prefetch_desc(&tmA);
         tma_prefetch_desc(&tmB0);
@@ -800,7 +809,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             // No trigger: the kernel behind is mostly a quantiser, whose CTAs would all settle on the SMs that this
             // grid leaves idle (the shared expert of 512 tokens took 54.7 us with one here, 50.1 without).
             pdl_wait();
-            int s = 0, filled = 0;   // filled: stages with a copy that may be in flight
+            int s = 0;
             uint32_t ph = 0;
             for (int t = tile0; t < total; t += step) {
                 const int n = t / p.m_tiles, m = t - n * p.m_tiles;
@@ -814,21 +823,9 @@ __global__ void __launch_bounds__(kThreads, 1)
                     }
                     load(sA + s * C::kABytes, &tmA, s, kb * kBK, token_row(m));
                     if (++s == C::kStages) { s = 0; ph ^= 1u; }
-                    filled = min(filled + 1, C::kStages);
                 }
             }
-            // The last release of each stage arrives in this CTA's memory (of a pair, the first CTA's MMAs arrive in
-            // both): wait for it before the CTA may end.  A stage that was never filled passes, as above.
-            for (int i = 0; i < C::kStages; ++i)
-                if (!wait(&empty[i], i < s ? ph : ph ^ 1u)) goto producer_done;
-            filled = 0;
-        producer_done:
-            // Given up: the copies in flight land before the CTA ends.  (A pair's second CTA has no barrier of its
-            // own for them; its copies take microseconds.)
-            if (filled > 0) {
-                for (int i = 0; leads && i < filled; ++i) mbar_drain(&full[i], i < s ? ph : ph ^ 1u);
-                if (kPair) wait_ns(kDrainNs);
-            }
+        producer_done:;
         }
     } else if (warp == 1) {
         if (lane == 0 && leads) {
@@ -836,11 +833,14 @@ __global__ void __launch_bounds__(kThreads, 1)
             pdl_wait();   // the bounds of the waits below count from here
             int s = 0;
             uint32_t ph = 0;
-            bool issued = false;
+            bool gave_up = false;
+            // blocks yet to come; a stage is released only for a fill that comes and waits for it, so that no release
+            // (of a pair's MMAs, one in the other CTA's memory) can arrive behind the CTA's end
+            int64_t left = (int64_t)(total - tile0 + step - 1) / step * (kb1 - kb0);
             int acc = 0;
             uint32_t aph = 0;
             for (int t = tile0; t < total; t += step) {
-                if (!wait.cluster(&tempty[acc], aph ^ 1u)) break;
+                if (!wait.cluster(&tempty[acc], aph ^ 1u)) { gave_up = true; break; }
                 tc_fence_after();
                 const uint32_t d_tmem = tmem_base + acc * kBN;
                 bool ok = true;
@@ -859,21 +859,20 @@ __global__ void __launch_bounds__(kThreads, 1)
                         if (kPair) mma_i8_ss2(d_tmem, adesc, bdesc, p.idesc, (kb != kb0 || kk != 0) ? 1u : 0u);
                         else mma_i8_ss(d_tmem, adesc, bdesc, p.idesc, (kb != kb0 || kk != 0) ? 1u : 0u);
                     }
-                    if (kPair) mma_commit2(&empty[s]);
-                    else mma_commit(&empty[s]);
-                    issued = true;
+                    if (left-- > C::kStages) {
+                        if (kPair) mma_commit2(&empty[s]);
+                        else mma_commit(&empty[s]);
+                    }
                     if (++s == C::kStages) { s = 0; ph ^= 1u; }
                 }
-                if (!ok) break;
+                gave_up = !ok;
+                if (gave_up) break;
                 if (kPair) mma_commit2(&tfull[acc]);
                 else mma_commit(&tfull[acc]);
                 acc ^= 1;
                 if (acc == 0) aph ^= 1u;
             }
-            // The MMAs issued so far end before the TMEM is freed (of a run that was not given up, the epilogue and
-            // the producers wait for them): their last stage's release.
-            const int last = s > 0 ? s - 1 : C::kStages - 1;
-            if (issued) mbar_drain(&empty[last], s > 0 ? ph : ph ^ 1u);
+            if (gave_up) drain<kPair>(full, s, ph, C::kStages, bail);
         }
     } else {
         // ---------------- epilogue (warps 2..9) ----------------
@@ -1097,7 +1096,8 @@ __global__ void __launch_bounds__(kSmallThreads, 2)
     uint64_t* const empty = full + 8;
     uint64_t* const ready = empty + 8;   // the codes are written
     uint64_t* const tfull = ready + 1;
-    uint32_t* const tmem_slot = reinterpret_cast<uint32_t*>(tfull + 1);
+    uint64_t* const bail = tfull + 1;    // of MMAs that were given up
+    uint32_t* const tmem_slot = reinterpret_cast<uint32_t*>(bail + 1);
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const Waits wait{&s_stop, 0u, kWaitTimeoutNs};
@@ -1106,6 +1106,7 @@ __global__ void __launch_bounds__(kSmallThreads, 2)
         for (int s = 0; s < p.stages; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], 1); }
         mbar_init(ready, kSmallWorkers);
         mbar_init(tfull, 1);
+        mbar_init(bail, 1);
         fence_mbar_init();
         tma_prefetch_desc(&tmW0);
         tma_prefetch_desc(&tmW1);
@@ -1149,15 +1150,9 @@ __global__ void __launch_bounds__(kSmallThreads, 2)
         if (lane == 0) {
             int s = 0;
             uint32_t ph = 0;
-            // behind the last load, the last release of each stage: it arrives in this CTA's memory
-            for (int i = first; i < loads + first; ++i) {
-                if (!wait(&empty[s], ph)) {
-                    // given up: the copies in flight land before the CTA ends
-                    for (int j = max(0, min(i, loads) - p.stages); j < min(i, loads); ++j)
-                        mbar_drain(&full[j % p.stages], (uint32_t)(j / p.stages) & 1u);
-                    break;
-                }
-                if (i < loads) load(s, i);
+            for (int i = first; i < loads; ++i) {
+                if (!wait(&empty[s], ph)) break;
+                load(s, i);
                 if (++s == p.stages) { s = 0; ph ^= 1u; }
             }
         }
@@ -1171,8 +1166,8 @@ __global__ void __launch_bounds__(kSmallThreads, 2)
         if (lane == 0) {
             pdl_wait();   // the bounds of the waits below count from here
             bool ok = wait(ready, 0);
-            int s = 0, last = -1;
-            uint32_t ph = 0, last_ph = 0;
+            int s = 0;
+            uint32_t ph = 0;
             for (int i = 0; ok && i < loads; ++i) {
                 if (!wait(&full[s], ph)) { ok = false; break; }
                 tc_fence_after();
@@ -1187,13 +1182,11 @@ __global__ void __launch_bounds__(kSmallThreads, 2)
                     mma_i8_ss(d_tmem, wdesc, smem_desc_sw128(q_base + kk * 32, 16, 1024), p.idesc,
                               (i >= kMats || kk != 0) ? 1u : 0u);
                 }
-                mma_commit(&empty[s]);
-                last = s;
-                last_ph = ph;
+                if (i + p.stages < loads) mma_commit(&empty[s]);   // (as the tiles: only for a load that waits for it)
                 if (++s == p.stages) { s = 0; ph ^= 1u; }
             }
             if (ok) mma_commit(tfull);
-            else if (last >= 0) mbar_drain(&empty[last], last_ph);   // given up: the MMAs end before the TMEM is freed
+            else drain<false>(full, s, ph, p.stages, bail);
         }
     } else {
         // ---------------- quantiser, then epilogue (warps 2..9) ----------------
