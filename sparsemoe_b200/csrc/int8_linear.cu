@@ -420,6 +420,14 @@ struct Waits {
     __device__ __forceinline__ bool warp(uint64_t* bar, uint32_t parity) const {
         return __all_sync(0xffffffffu, (*this)(bar, parity));
     }
+    // Tells the other CTAs of a cluster of `ctas` that this one has given up, ahead of the cluster barrier behind
+    // which their sums take its parts (all of them have started: an earlier phase of the barrier is behind).  The
+    // epilogue's warps call it: where another role gives up, theirs is the wait that runs out or is ended.
+    static __device__ __noinline__ void tell(uint32_t stop, int ctas) {
+        for (int r = 0; r < ctas; ++r)
+            asm volatile("st.shared::cluster.b32 [%0], %1;" ::"r"(mapa(stop, r)), "r"(1u) : "memory");
+    }
+    __device__ __forceinline__ bool stopped() const { return *(volatile uint32_t*)stop != 0; }
     // For arrivals from the cluster.
     __device__ __forceinline__ bool cluster(uint64_t* bar, uint32_t parity) const {
         const bool ok = (*this)(bar, parity);
@@ -971,6 +979,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             acc ^= 1;
             if (acc == 0) aph ^= 1u;
         }
+        if (p.split > 1 && !ok) Waits::tell(smem_u32(&s_stop), p.split);
         if (lane == 0) bulk_wait_read<0>();   // the staged chunks are read before the CTA's memory goes
     }
     if (p.split > 1) {
@@ -984,6 +993,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             const int col0 = (second ? n - p.n0_tiles : n) * kOutN;
             // this CTA's 128 / split columns: consecutive lanes take consecutive units of a row
             const int units = kBN / 8 / p.split, rows = min(kBM, p.T - m * kBM);
+            const bool all = !wait.stopped();   // else a part is missing
             for (int i = threadIdx.x - 64; i >= 0 && i < units * rows; i += kEpiThreads) {
                 const int u = i % units, r = i / units, c = (rank * units + u) * 8;
                 if (col0 + c >= p.N) continue;
@@ -999,7 +1009,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 float v[8];
 #pragma unroll
                 for (int j = 0; j < 8; ++j) v[j] = dequant(sum[j], st, s_scale[0][c + j]) + s_bias[0][c + j];
-                emit8(p, row, second, col0 + c, v);
+                if (all) emit8(p, row, second, col0 + c, v);
             }
         }
     }
@@ -1339,18 +1349,20 @@ __global__ void __launch_bounds__(kSmallThreads, 2)
             }
         }
         if (split) {
+            if (!ok) Waits::tell(smem_u32(&s_stop), p.split);
             __syncwarp();
             cluster_arrive();   // phase 3: every part has been sent
             cluster_wait();
             const int* parts = reinterpret_cast<const int*>(recv);
-            for (int i = threadIdx.x - 64; ok && i < wch * p.T; i += kSmallWorkers) {
+            const bool all = !wait.stopped();   // else a part is missing
+            for (int i = threadIdx.x - 64; i < wch * p.T; i += kSmallWorkers) {
                 const int t = i / wch, ch = i % wch;
                 int sum[kMats] = {};
                 for (int r = 0; r < p.split; ++r)
 #pragma unroll
                     for (int j = 0; j < kMats; ++j)
                         sum[j] += parts[j * 128 * kNT + ((r * (kNT / 4) + t / 4) * wch + ch) * 4 + t % 4];
-                put(sum[0], sum[kMats - 1], t, rank * wch + ch);
+                if (all) put(sum[0], sum[kMats - 1], t, rank * wch + ch);
             }
         }
     }
@@ -1383,11 +1395,11 @@ __global__ void __launch_bounds__(32) waits_selftest_kernel(uint64_t limit_ns, i
     cluster_arrive();
     cluster_wait();
     const Waits wait{&s_stop, 0u, limit_ns};
-    if (rank == 1) (void)wait.warp(&bar, 0);
+    if (rank == 1 && !wait.warp(&bar, 0)) Waits::tell(smem_u32(&s_stop), 2);
     __syncwarp();
     cluster_arrive();
     cluster_wait();
-    if (threadIdx.x == 0 && s_stop == 0) written[rank] = 1;
+    if (threadIdx.x == 0 && !wait.stopped()) written[rank] = 1;
 }
 
 // ---- host side -----------------------------------------------------------------------

@@ -72,3 +72,13 @@ def test_a_wait_that_ran_out_stops_no_other_call(gpu):
     y = sm.int8_matmul(*cases[0][:4], out_dtype=torch.float32)
     sm.sync_check("cuda:0")
     assert torch.equal(y, cases[0][-1])
+
+
+def test_no_cta_of_a_cluster_writes_behind_a_wait_that_ran_out(gpu):
+    """The CTA that sums up the parts of a cluster learns that another one has given up."""
+    written = torch.zeros(2, dtype=torch.int32, device=gpu)
+    sm.check(sm.lib.moe_selftest_int8_wait_timeout(20_000_000, written.data_ptr(),
+                                                   torch.cuda.current_stream().cuda_stream))
+    with pytest.raises(sm.MoeError, match="int8 product"):
+        sm.sync_check()
+    assert written.tolist() == [0, 0]
