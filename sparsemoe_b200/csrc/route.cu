@@ -341,6 +341,15 @@ __device__ __noinline__ int rank_candidates(const RouteParams& p, const T* row, 
     return lane < n ? buf[lane] : -1;
 }
 
+// What a group's score, a or the sum of its two best members a and b, may be off
+// by in f32: err2 for the members' scores, 2^-24 each for the members (of their
+// own sizes, which biases of both signs leave in a small sum), the sum, and the
+// addition of this slack to it.
+__device__ __forceinline__ float group_slack(float a, float b, float err2) {
+    const float size = fabsf(a) + (b == -INFINITY ? 0.0f : fabsf(b));
+    return size < INFINITY ? err2 + 2.5e-7f * size : 0.0f;
+}
+
 template <typename T, int NV>
 __global__ void __launch_bounds__(kRouteWarps * 32) route_kernel(const __grid_constant__ RouteParams p) {
     constexpr uint32_t kIdx = 32 * NV - 1;      // the key bits that hold the index
@@ -432,27 +441,23 @@ __global__ void __launch_bounds__(kRouteWarps * 32) route_kernel(const __grid_co
             __syncwarp();
         }
         bool near = false;
+        const float slack = scored ? group_slack(a, b, err2) : 0.0f;
         if (pair && b != -INFINITY) a += b;
         if (g >= p.G) a = -INFINITY;
         const uint32_t gk = a != -INFINITY ? (order_key(a) & ~31u) | (31 - g) : 0u;
-        uint32_t cur = gk, last = 0;
+        uint32_t cur = gk;
         for (int r = 0; r < p.kept; ++r) {
             const uint32_t best = __reduce_max_sync(kFull, cur);
             if (best == 0) break;
-            last = best;
             if (cur == best) cur = 0;
         }
         bool stay = gk != 0 && cur == 0;
         const uint32_t out = __reduce_max_sync(kFull, cur);
         if (out != 0 && (scored || !exact)) {
-            // close with the index in the low bits: the scores themselves decide
-            const float lo = key_value(last & ~31u), hi = key_value(out & ~31u);
-            if (!(lo - hi > 1.2e-5f * fmaxf(fabsf(lo), fabsf(hi)) + 2.0f * err2)) {
-                const float worst = key_value(__reduce_min_sync(kFull, stay ? order_key(a) : 0xFFFFFFFFu));
-                const float other = key_value(__reduce_max_sync(kFull, stay || gk == 0 ? 0u : order_key(a)));
-                near = scored ? !(worst - other > 2.0f * err2 + 6e-7f * fmaxf(fabsf(worst), fabsf(other)))
-                              : !(worst > other);
-            }
+            // close with the index in the low bits: the scores themselves, as far off as they may be, decide
+            const float worst = key_value(__reduce_min_sync(kFull, stay ? order_key(a - slack) : 0xFFFFFFFFu));
+            const float other = key_value(__reduce_max_sync(kFull, stay || gk == 0 ? 0u : order_key(a + slack)));
+            near = !(worst > other);
         }
         if (near && !redo) {
             const uint32_t mask = groups_f64<T>(p, row, sv[warp], lane);
@@ -722,6 +727,7 @@ __global__ void __launch_bounds__(kRouteWarps * 32, 7) route_many_kernel(const _
             }
         }
         const float least = pair ? b : a;       // of the members that score the group
+        const float slack = group_slack(a, b, err2);
         if (pair && b != -INFINITY) a += b;
         const uint32_t mine = a != -INFINITY ? order_key(a) : 0u;
         int rank = 0;
@@ -732,11 +738,9 @@ __global__ void __launch_bounds__(kRouteWarps * 32, 7) route_many_kernel(const _
             rank += other > mine || (other == mine && (sub ^ h) < sub) ? 1 : 0;
         }
         bool stay = mine != 0 && rank < p.kept;
-        const uint32_t worst = ~max8(stay ? ~mine : 0u), other = max8(stay ? 0u : mine);
-        if (other != 0) {
-            const float lo = key_value(worst), hi = key_value(other);
-            near = (p.bias || pair) && !(lo - hi > 2.0f * err2 + 6e-7f * fmaxf(fabsf(lo), fabsf(hi)));
-        }
+        const uint32_t worst = ~max8(stay ? ~order_key(a - slack) : 0u);
+        const uint32_t other = max8(stay || mine == 0 ? 0u : order_key(a + slack));
+        near = other != 0 && (p.bias || pair) && !(key_value(worst) > key_value(other));
         unsigned bad = __ballot_sync(kFull, near);
         if (bad != 0 && p.sigmoid) {
             // every lane its group's one or two members in f64, where f32 values tell them from the others
