@@ -245,7 +245,7 @@ typedef struct MoeRouting {
 // (device f32 [num_experts]; it moves the choice, never the weight), or
 // without a bias its logit.  Order: value descending, equal values by the
 // lower index, as f64 arithmetic on the logits orders them (group sums that
-// agree to 2^-49 are equal).  Weights: the scores of the chosen,
+// agree to 2^-49 of the values and biases they are summed from are equal).  Weights: the scores of the chosen,
 // renormalised if asked, times scale.  An expert is masked by a logit that is
 // NaN, -infinity, <= -1e20 or f16's lowest value, or by such a bias; slots
 // that no expert fills hold index -1 and weight 0.  Writes indices and weights

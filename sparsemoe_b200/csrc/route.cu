@@ -19,8 +19,8 @@
 // of the order are closer than both, the candidates (the chosen and what is that
 // close behind them) are ranked again, one a lane, by their f64 values; where the
 // last kept and the first left group are, the whole row is selected in f64, and
-// group sums that agree to 2^-49 are ties (sigmoid(x) + sigmoid(-x) is 1 for every
-// x).  16-bit logits without a bias give up only zeros and need neither.
+// group sums that agree to 2^-49 of what they are summed from are ties (sigmoid(x) +
+// sigmoid(-x) is 1 for every x).  16-bit logits without a bias give up only zeros and need neither.
 //
 // One warp per token, lane l holding experts l*NV .. l*NV + NV - 1.  Each lane
 // sorts its keys once; a round of the selection is one redux.sync over the
@@ -175,9 +175,43 @@ __device__ __forceinline__ void values_f64(const RouteParams& p, const T* row, d
     }
 }
 
+// Group sums of two are equal where they agree to 2^-49 of what they are summed
+// from, the members' values and biases: sigmoid(x) + sigmoid(-x) is 1 for every x,
+// which f64 leaves within a few 2^-53 of their sizes, while the order of scores of
+// any size stands.  a, b: the two best members, bias: the largest magnitude of
+// theirs.
+__device__ __forceinline__ double group_tie(bool pair, double a, double b, float bias) {
+    if (!pair || isinf(a)) return 0.0;
+    return 0x1p-49 * (fabs(a) + (b == -INFINITY ? 0.0 : fabs(b)) + 2.0 * fabs((double)bias));
+}
+
+// Best members a, b of group g and the largest bias of theirs, from lanes lane % sub
+// of sub that share it (all get them).
+__device__ __forceinline__ void group_best(const RouteParams& p, const double* buf, int g, int first, int sub, double& a,
+                                           double& b, float& bias) {
+    a = b = -INFINITY;
+    bias = 0.0f;
+    if (g < p.G)
+#pragma unroll 1
+        for (int i = first; i < p.per; i += sub) merge2(a, b, buf[g * p.per + i], (double)-INFINITY);
+#pragma unroll 1
+    for (int o = sub >> 1; o > 0; o >>= 1) {
+        const double c = __shfl_xor_sync(kFull, a, o), d = __shfl_xor_sync(kFull, b, o);
+        merge2(a, b, c, d);
+    }
+    if (p.bias == nullptr || p.group_top != 2) return;
+    if (g < p.G)
+#pragma unroll 1
+        for (int i = first; i < p.per; i += sub) {
+            const double v = buf[g * p.per + i];
+            if (v >= b && v != -INFINITY) bias = fmaxf(bias, fabsf(p.bias[g * p.per + i]));
+        }
+#pragma unroll 1
+    for (int o = sub >> 1; o > 0; o >>= 1) bias = fmaxf(bias, __shfl_xor_sync(kFull, bias, o));
+}
+
 // Which of up to 32 groups of a row stay: bit g.  buf: E doubles of this warp's
-// shared memory.  Sums of two that agree to 2^-49 are ties (sigmoid(x) +
-// sigmoid(-x) is 1 for every x).
+// shared memory.  Chosen one by one: the lowest of those that equal the largest.
 template <typename T>
 __device__ __noinline__ uint32_t groups_f64(const RouteParams& p, const T* row, double* buf, int lane) {
     __syncwarp();
@@ -186,28 +220,26 @@ __device__ __noinline__ uint32_t groups_f64(const RouteParams& p, const T* row, 
     const bool pair = p.group_top == 2;
     int sub = 32;
     while (32 / sub < p.G) sub >>= 1;
-    const int g = lane / sub;
-    double a = -INFINITY, b = -INFINITY;
-    if (g < p.G)
-#pragma unroll 1
-        for (int i = lane % sub; i < p.per; i += sub) merge2(a, b, buf[g * p.per + i], (double)-INFINITY);
-#pragma unroll 1
-    for (int o = sub >> 1; o > 0; o >>= 1) {
-        const double c = __shfl_xor_sync(kFull, a, o), d = __shfl_xor_sync(kFull, b, o);
-        merge2(a, b, c, d);
-    }
+    double a, b;
+    float bias;
+    group_best(p, buf, lane / sub, lane % sub, sub, a, b, bias);
+    double tie = group_tie(pair, a, b, bias);
     if (pair && b != -INFINITY) a += b;
     a = __shfl_sync(kFull, a, (lane * sub) & 31);   // lane g: group g
+    tie = __shfl_sync(kFull, tie, (lane * sub) & 31);
     if (lane >= p.G) a = -INFINITY;
-    const double tie = pair && !isinf(a) ? 0x1p-49 * (1.0 + fabs(a)) : 0.0;
-    int rank = 0;
+    uint32_t stay = 0;
 #pragma unroll 1
-    for (int h = 0; h < p.G; ++h) {
-        const double other = __shfl_sync(kFull, a, h);
-        rank += other > a + tie || (other >= a - tie && h < lane) ? 1 : 0;
+    for (int r = 0; r < p.kept; ++r) {
+        const double m = warp_max(a);
+        if (m == -INFINITY) break;
+        const double from = -warp_max(a == m ? tie - a : -INFINITY);
+        const uint32_t at = __reduce_min_sync(kFull, a != -INFINITY && a + tie >= from ? lane : 32);
+        stay |= 1u << at;
+        if (lane == (int)at) a = -INFINITY;
     }
     __syncwarp();
-    return __ballot_sync(kFull, a != -INFINITY && rank < p.kept);
+    return stay;
 }
 
 // The whole selection of one row.  Returns the lane's choice (lane l: the l-th) or -1.
@@ -219,28 +251,30 @@ __device__ __noinline__ int route_row_f64(const RouteParams& p, const T* row, do
         values_f64<T>(p, row, buf, lane, true);
         __syncwarp();
         const bool pair = p.group_top == 2;
-        double gs[32];
+        double gs[32], ties[32];
         const int gn = (p.G + 31) / 32;
 #pragma unroll 1
         for (int i = 0; i < gn; ++i) {
-            const int g = lane + 32 * i;
-            double a = -INFINITY, b = -INFINITY;
-#pragma unroll 1
-            for (int j = 0; g < p.G && j < p.per; ++j) merge2(a, b, buf[g * p.per + j], (double)-INFINITY);
+            double a, b;
+            float bias;
+            group_best(p, buf, lane + 32 * i, 0, 1, a, b, bias);
+            ties[i] = group_tie(pair, a, b, bias);
             gs[i] = pair && b != -INFINITY ? a + b : a;
         }
         keep = 0;
-        const double tie = pair ? 0x1p-49 : 0.0;
 #pragma unroll 1
         for (int r = 0; r < p.kept; ++r) {
             double a = -INFINITY;
             for (int i = 0; i < gn; ++i) a = fmax(a, gs[i]);
-            a = warp_max(a);
-            if (a == -INFINITY) break;
-            const double from = isinf(a) ? a : a - tie * (1.0 + fabs(a));
+            const double m = warp_max(a);
+            if (m == -INFINITY) break;
+            double from = -INFINITY;
+            for (int i = 0; i < gn; ++i)
+                if (gs[i] == m) from = fmax(from, ties[i] - m);
+            from = -warp_max(from);
             uint32_t at = 0xFFFFFFFFu;
             for (int i = gn - 1; i >= 0; --i)
-                if (gs[i] >= from) at = lane + 32 * i;
+                if (gs[i] != -INFINITY && gs[i] + ties[i] >= from) at = lane + 32 * i;
             at = __reduce_min_sync(kFull, at);
             if ((at & 31) == lane) {
                 keep |= 1u << (at >> 5);
@@ -565,6 +599,11 @@ __device__ __forceinline__ float fmax8(float v) {
     for (int o = 4; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(kFull, v, o));
     return v;
 }
+__device__ __forceinline__ double fmax8(double v) {
+#pragma unroll 1
+    for (int o = 4; o > 0; o >>= 1) v = fmax(v, __shfl_xor_sync(kFull, v, o));
+    return v;
+}
 __device__ __forceinline__ float sum8(float v) {
 #pragma unroll
     for (int o = 4; o > 0; o >>= 1) v += __shfl_xor_sync(kFull, v, o);
@@ -761,26 +800,38 @@ __global__ void __launch_bounds__(kRouteWarps * 32, 7) route_many_kernel(const _
                     ++count;
                 }
             }
-            double sum = 0.0;
+            double m1 = -INFINITY, m2 = -INFINITY;
+            float bias = 0.0f;
 #pragma unroll 1
             for (int h = 0; h < 2; ++h) {
                 const int q = h == 0 ? first : second;
                 if (q < 0) continue;
-                sum += 1.0 / (1.0 + exp(-(double)to_f32<T>(row[e0 + q])));
-                if (p.bias) sum += (double)p.bias[e0 + q];
+                double m = 1.0 / (1.0 + exp(-(double)to_f32<T>(row[e0 + q])));
+                if (p.bias) {
+                    m += (double)p.bias[e0 + q];
+                    bias = fmaxf(bias, fabsf(p.bias[e0 + q]));
+                }
+                m2 = m1;
+                m1 = m;
             }
-            if (count == 0) sum = -INFINITY;
-            const double tie = pair && count > 0 ? 0x1p-49 * (1.0 + fabs(sum)) : 0.0;
-            int place = 0;
+            const double tie = group_tie(pair, m1, m2, bias);
+            double sum = m2 == -INFINITY ? m1 : m1 + m2;
+            // as groups_f64, in the token's eight lanes
+            bool among = false;
 #pragma unroll 1
-            for (int h = 1; h < 8; ++h) {
-                const double o = __shfl_xor_sync(kFull, sum, h);
-                place += o > sum + tie || (o >= sum - tie && (sub ^ h) < sub) ? 1 : 0;
+            for (int r = 0; r < p.kept; ++r) {
+                const double m = fmax8(sum);
+                const double from = -fmax8(sum == m ? tie - sum : -INFINITY);
+                const uint32_t equal = sum != -INFINITY && sum + tie >= from ? 8 - sub : 0;
+                if (max8(equal) == equal && equal != 0) {
+                    among = true;
+                    sum = -INFINITY;
+                }
             }
             const bool sure = count <= (pair ? 2 : 1) && least < INFINITY;
             const unsigned unsure = __ballot_sync(kFull, near && !sure);
             const bool settled = near && (unsure >> (lane & 24) & 255) == 0;
-            if (settled) stay = count > 0 && place < p.kept;
+            if (settled) stay = among;
             bad = __ballot_sync(kFull, near && !settled);
         }
         if (bad != 0)

@@ -62,3 +62,59 @@ def test_biases_that_cancel_in_a_group(gpu, size, E, T, score):
     check(x, b.flatten().cuda(), score, 8, 4, 2, 4)
     check(x, (b.flatten() + 0.1 * torch.randn(E, generator=g)).cuda(), score, 8, 3, 2, 4)
     check(x, b.flatten().cuda(), score, 8, 4, 1, 4)
+
+
+# (experts, groups, tokens): groups of whole lanes, groups inside lanes and across them, more than 32 groups, groups of one
+SHAPES = [(256, 8, 17000), (64, 8, 6000), (32, 8, 6000), (160, 8, 17000), (256, 4, 3000), (244, 4, 3000), (96, 32, 3000),
+          (288, 36, 1000), (1024, 64, 300), (8, 8, 3000)]
+
+
+@pytest.mark.parametrize("E, groups, T", SHAPES)
+@pytest.mark.parametrize("mean", [-30.0, -40.0, -300.0])
+def test_small_sigmoids(gpu, E, groups, T, mean):
+    """Scores far below one, whose sums differ by far less than 2^-49."""
+    g = torch.Generator().manual_seed(E)
+    x = (1.6 * torch.randn(T, E, generator=g) + mean).cuda()
+    zero = torch.zeros(E, device=gpu)
+    for kept in sorted({1, groups // 2, groups - 1} - {0}):
+        k = min(8, kept * (E // groups))
+        check(x, None, "sigmoid", groups, kept, 2, k)
+    check(x, zero, "sigmoid", groups, 1, 2, 1)
+    check(x, (1e-14 * torch.randn(E, generator=g)).cuda(), "sigmoid", groups, 1, 2, 1)
+
+
+@pytest.mark.parametrize("E, groups, T", SHAPES)
+@pytest.mark.parametrize("spread", [16.0, 80.0])
+def test_softmax_of_wide_logits(gpu, E, groups, T, spread):
+    g = torch.Generator().manual_seed(E)
+    x = (spread * torch.randn(T, E, generator=g)).cuda()
+    for kept in sorted({1, groups // 2, groups - 1} - {0}):
+        k = min(8, kept * (E // groups))
+        check(x, None, "softmax", groups, kept, 2, k)
+    check(x, torch.zeros(E, device=gpu), "softmax", groups, 1, 2, 1)
+
+
+@pytest.mark.parametrize("E, groups, T", [(32, 8, 4200), (64, 16, 50), (320, 40, 50)])
+def test_sums_each_equal_to_the_next(gpu, E, groups, T):
+    """Group sums 1 + 3 j 2^-50 in any order: neighbours are equal, others are not.  As many groups stay as are asked for."""
+    x = torch.zeros(T, E, device=gpu)
+    for seed in range(6):
+        order = torch.randperm(groups, generator=torch.Generator().manual_seed(seed))
+        b = torch.full((groups, E // groups), -1.0)
+        b[:, 0] = 0.0
+        b[:, 1] = 3.0 * order * 2.0 ** -50
+        b = b[:, torch.randperm(E // groups, generator=torch.Generator().manual_seed(seed))].flatten().cuda()
+        for kept in (1, 2, 5, groups - 1):
+            check(x, b, "sigmoid", groups, kept, 2, min(2 * kept, 8), parts=40)
+
+
+@pytest.mark.parametrize("E, groups, T", SHAPES[:-1])
+def test_mirrored_sigmoids_are_equal(gpu, E, groups, T):
+    """sigmoid(x) + sigmoid(-x) is one for every x: the first groups stay."""
+    g = torch.Generator().manual_seed(E)
+    half = 5.0 * torch.rand(T, groups, 1, generator=g) + 0.1
+    x = torch.cat([half, -half, torch.full((T, groups, E // groups - 2), -7.0)], 2).reshape(T, E).cuda()
+    kept = groups // 2
+    want = chosen(x.double().cpu().numpy(), None, "sigmoid", groups, kept, 2, kept)
+    assert (want // (E // groups) < kept).all()
+    check(x, None, "sigmoid", groups, kept, 2, min(kept, 8))
