@@ -431,9 +431,14 @@ __global__ void __launch_bounds__(kRouteWarps * 32) route_kernel(const __grid_co
 #pragma unroll
         for (int q = 0; q < NV; ++q) v[q] = v[q] > -INFINITY && b[q] > kMasked ? s[q] + b[q] : -INFINITY;
     }
-    // Twice the error of a score: the sigmoid's is at most 0.65 2^-23 (of exp,
-    // times s (1 - s)) + 2^-24 + 2^-23 (of 1 + e and rcp), the softmax's at most
-    // 17 2^-23 of its largest score (the sum's relative error times s).
+    // Bound of the error in a difference of two scores, in units of 2^-23.  The
+    // sigmoid's error is at most 0.65 (of exp, times s (1 - s)) + 0.5 + 1 (of 1 + e
+    // and rcp), 5 units for two.  The softmax's is in units of its largest score
+    // 35: the sum's relative error, 18 (36 additions of half a unit) + 7 (of its
+    // exps, 2 + 1.2 d for a logit d below the largest: weighted by e^-d over 1024
+    // experts their mean is at most 7) + 0.5 (1 / sum), is one factor of the whole
+    // row and counts once; the two scores' own exps add at most 2 each (e^-d (2 +
+    // 1.2 d) falls with d), their products half each.  30.5 in all.
     const float err2 = p.sigmoid ? 6e-7f : 4.2e-6f * inv_sum;
 
     bool redo = false;                          // the whole row in f64

@@ -118,3 +118,19 @@ def test_mirrored_sigmoids_are_equal(gpu, E, groups, T):
     want = chosen(x.double().cpu().numpy(), None, "sigmoid", groups, kept, 2, kept)
     assert (want // (E // groups) < kept).all()
     check(x, None, "sigmoid", groups, kept, 2, min(kept, 8))
+
+
+@pytest.mark.parametrize("E, part, T", [(1024, 32, 200), (1024, 32, 3), (256, 32, 17000), (512, 16, 100)])
+def test_sums_that_round_one_way(gpu, E, part, T):
+    """Softmax sums of 1 + 2^-24 + 2^-24 + .., every addition of a lane rounded up by nearly half a step, and biases
+    that leave values of the size of that error."""
+    x = torch.full((E // part, part), -16.6353)     # exp: 2^-24 (1 + 2^-12)
+    x[:, 0] = 0.0
+    x[: E // part // 2, 1] = -16.0
+    x = x.flatten().repeat(T, 1)
+    s = torch.softmax(x[0].double(), 0)
+    for seed in range(4):
+        g = torch.Generator().manual_seed(seed)
+        b = (-s + 40 * 2.0 ** -23 * s.max() * torch.randn(E, generator=g, dtype=torch.float64)).float()
+        for kept, groups, top in ((1, 1, 1), (3, 8, 1), (3, 8, 2)):
+            check(x.cuda(), b.cuda(), "softmax", groups, kept, top, 8)
