@@ -267,7 +267,8 @@ typedef struct MoeInt8Weight {
 // Per-token quantiser: scale[t] = max |x_t| * f32(1/127) in f32 (1 where that is 0),
 // q = round-half-even(x / scale) of the exact quotient.  A row with a NaN or
 // an infinity gets a NaN scale (and so NaN outputs).  q: [tokens, q_stride],
-// q_stride a multiple of 16; bytes behind K are left as they are.
+// q_stride a multiple of 16; bytes behind K are left as they are.  x, q and
+// scale must not share memory.
 int moe_int8_quantize_tokens(const void* x, int x_type, int64_t tokens, int K, int64_t row_stride, int8_t* q,
                              int64_t q_stride, float* scale, cudaStream_t stream);
 // out[t, n] = (sum_k q[t, k] w[k, n]) * scale[t] * w->scale[n] + bias[n]

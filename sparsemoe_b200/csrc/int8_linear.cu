@@ -1725,14 +1725,22 @@ int check_out(const char* who, const void* out, int type, int64_t T, int64_t N, 
     return MOE_OK;
 }
 
-// Whether rows of wa bytes sa apart and rows of wb bytes sb apart share memory.
-// Exact for equal strides (two slices of one wider matrix do not).
-bool overlap(const void* a, int64_t sa, int64_t wa, const void* b, int64_t sb, int64_t wb, int64_t T) {
-    const int64_t pa = (int64_t)reinterpret_cast<uintptr_t>(a), pb = (int64_t)reinterpret_cast<uintptr_t>(b);
-    if (pa + (T - 1) * sa + wa <= pb || pb + (T - 1) * sb + wb <= pa) return false;
-    if (T == 1 || sa != sb) return true;
-    const int64_t at = ((pb - pa) % sa + sa) % sa;   // of b's rows in a's
-    return at < wa || at + wb > sa;
+// Rows of `width` bytes, `stride` bytes apart.
+struct Span {
+    const void* p;
+    int64_t stride, width, rows;
+};
+Span vector_span(const void* p, int64_t bytes) { return {p, 0, bytes, 1}; }
+// Whether two share memory.  Exact for single rows and equal strides (two
+// slices of one wider matrix do not); else where their address ranges meet.
+bool overlap(const Span& a, const Span& b) {
+    if (!a.p || !b.p || a.rows < 1 || b.rows < 1) return false;
+    const int64_t pa = (int64_t)reinterpret_cast<uintptr_t>(a.p), pb = (int64_t)reinterpret_cast<uintptr_t>(b.p);
+    if (pa + (a.rows - 1) * a.stride + a.width <= pb || pb + (b.rows - 1) * b.stride + b.width <= pa) return false;
+    if (a.rows == 1 && b.rows > 1) return overlap(b, a);
+    if (a.rows == 1 || (b.rows > 1 && a.stride != b.stride)) return true;
+    const int64_t at = ((pb - pa) % a.stride + a.stride) % a.stride;   // of b's rows in a's
+    return at < a.width || at + b.width > a.stride;
 }
 
 int check_scratch(const char* who, const void* scratch, size_t have, size_t need) {
@@ -1841,7 +1849,8 @@ int run_shared_expert(const char* who, const void* x, int x_type, int64_t tokens
     const int in = elem_bytes(x_type), size = elem_bytes(out_type);
     const bool same = residual == out && x_type == out_type && (tokens == 1 || residual_stride == out_stride);
     if (residual && !same &&
-        overlap(residual, residual_stride * in, (int64_t)d_model * in, out, out_stride * size, (int64_t)d_model * size, tokens))
+        overlap({residual, residual_stride * in, (int64_t)d_model * in, tokens},
+                {out, out_stride * size, (int64_t)d_model * size, tokens}))
         return bad(who, "the output shares memory with the residual without being it");
     if (check_only) return MOE_OK;
     int dev = 0, num_sms = 0;
@@ -1925,6 +1934,11 @@ extern "C" int moe_int8_quantize_tokens(const void* x, int x_type, int64_t token
     if (tokens == 0) return MOE_OK;
     if (!q || !scale || !aligned(q, 16) || q_stride % 16 != 0 || q_stride < K || !aligned(scale, 4))
         return bad(who, "codes must be rows on 16-byte boundaries (q_stride % 16 == 0, >= K) and scales f32");
+    const int in = elem_bytes(x_type);
+    const Span rows{x, row_stride * in, (int64_t)K * in, tokens}, codes{q, q_stride, K, tokens},
+        scales = vector_span(scale, tokens * 4);
+    if (overlap(rows, codes) || overlap(rows, scales) || overlap(codes, scales))
+        return bad(who, "an output shares memory with the activations or the other output");
     int dev = 0, num_sms = 0;
     rc = current_device(&dev, &num_sms);
     if (rc != MOE_OK) return rc;
@@ -1945,7 +1959,7 @@ extern "C" int moe_int8_matmul(const int8_t* q, int64_t q_stride, const float* s
         return bad(who, "codes must be rows on 16-byte boundaries (q_stride % 16 == 0, >= K) and scales f32");
     if (!aligned(bias, 4)) return bad(who, "bias is not aligned to f32");
     const int size = elem_bytes(out_type);
-    if (overlap(q, q_stride, K, out, out_stride * size, (int64_t)N * size, tokens))
+    if (overlap({q, q_stride, K, tokens}, {out, out_stride * size, (int64_t)N * size, tokens}))
         return bad(who, "the output shares memory with the codes");
     int dev = 0, num_sms = 0;
     rc = current_device(&dev, &num_sms);
@@ -1973,7 +1987,7 @@ extern "C" int moe_int8_linear(const void* x, int x_type, int64_t tokens, int K,
     rc = check_scratch(who, scratch, scratch_bytes, linear_scratch(tokens, K, N));
     if (rc != MOE_OK) return rc;
     const int in = elem_bytes(x_type), size = elem_bytes(out_type);
-    if (overlap(x, row_stride * in, (int64_t)K * in, out, out_stride * size, (int64_t)N * size, tokens))
+    if (overlap({x, row_stride * in, (int64_t)K * in, tokens}, {out, out_stride * size, (int64_t)N * size, tokens}))
         return bad(who, "the output shares memory with the activations");
     int dev = 0, num_sms = 0;
     rc = current_device(&dev, &num_sms);

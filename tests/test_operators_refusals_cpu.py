@@ -12,3 +12,15 @@ def test_int8_selftest_refusals():
     for ns, written in ((0, FAKE), (-5, FAKE), (10_000_000_001, FAKE), (50_000_000, None), (50_000_000, FAKE + 2)):
         assert sm.lib.moe_selftest_int8_wait_timeout(ns, written, None) == sm.MOE_ERR_INVALID_ARG
         assert b"selftest" in sm.lib.moe_last_error()
+
+
+@pytest.mark.parametrize("kw", [
+    dict(), dict(q=FAKE + 496), dict(q=FAKE - 192), dict(ldx=128, q=FAKE + 112), dict(typ=0, q=FAKE + 512, ldq=256),
+    dict(q=FAKE + 4096, s=FAKE + 4096 + 60), dict(q=FAKE + 4096, s=FAKE + 508), dict(q=FAKE + 4096, s=FAKE - 12),
+    dict(T=1, q=FAKE + 112), dict(ldx=128, ldq=256, q=FAKE + 64)])
+def test_codes_and_scales_in_the_activations_memory(kw):
+    """Rows of other blocks are still read where the first codes are written."""
+    a = dict(typ=2, T=4, K=64, ldx=64, q=FAKE, ldq=64, s=FAKE + (1 << 16))
+    a.update(kw)
+    rc = sm.lib.moe_int8_quantize_tokens(FAKE, a["typ"], a["T"], a["K"], a["ldx"], a["q"], a["ldq"], a["s"], None)
+    assert rc == sm.MOE_ERR_INVALID_ARG and b"shares memory" in sm.lib.moe_last_error()
