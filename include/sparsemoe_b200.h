@@ -249,7 +249,8 @@ typedef struct MoeRouting {
 // renormalised if asked, times scale.  An expert is masked by a logit that is
 // NaN, -infinity, <= -1e20 or f16's lowest value, or by such a bias; slots
 // that no expert fills hold index -1 and weight 0.  Writes indices and weights
-// [tokens, top_k]; num_experts <= 1024, top_k <= 32.
+// [tokens, top_k]; num_experts <= 1024, top_k <= 32.  The outputs must share no
+// memory with the logits, the bias or each other.
 int moe_route_experts(const void* logits, int logits_type, int64_t tokens, int num_experts, int64_t row_stride,
                       int top_k, const MoeRouting* routing, const float* select_bias, int* indices, float* weights,
                       cudaStream_t stream);

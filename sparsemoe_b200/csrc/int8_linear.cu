@@ -1725,24 +1725,6 @@ int check_out(const char* who, const void* out, int type, int64_t T, int64_t N, 
     return MOE_OK;
 }
 
-// Rows of `width` bytes, `stride` bytes apart.
-struct Span {
-    const void* p;
-    int64_t stride, width, rows;
-};
-Span vector_span(const void* p, int64_t bytes) { return {p, 0, bytes, 1}; }
-// Whether two share memory.  Exact for single rows and equal strides (two
-// slices of one wider matrix do not); else where their address ranges meet.
-bool overlap(const Span& a, const Span& b) {
-    if (!a.p || !b.p || a.rows < 1 || b.rows < 1) return false;
-    const int64_t pa = (int64_t)reinterpret_cast<uintptr_t>(a.p), pb = (int64_t)reinterpret_cast<uintptr_t>(b.p);
-    if (pa + (a.rows - 1) * a.stride + a.width <= pb || pb + (b.rows - 1) * b.stride + b.width <= pa) return false;
-    if (a.rows == 1 && b.rows > 1) return overlap(b, a);
-    if (a.rows == 1 || (b.rows > 1 && a.stride != b.stride)) return true;
-    const int64_t at = ((pb - pa) % a.stride + a.stride) % a.stride;   // of b's rows in a's
-    return at < a.width || at + b.width > a.stride;
-}
-
 int check_scratch(const char* who, const void* scratch, size_t have, size_t need) {
     if (need == 0) return MOE_OK;
     if (!scratch || !aligned(scratch, 256)) return bad(who, "scratch is null or not 256-byte aligned");

@@ -190,6 +190,24 @@ int check_routing(const MoeRouting* r, int E, int k);
 cudaError_t launch_route(const void* logits, int type, int64_t T, int E, int64_t ld, int k, const MoeRouting& r,
                          const float* bias, int* idx, float* w, cudaStream_t st);
 
+// Rows of `width` bytes, `stride` bytes apart.
+struct Span {
+    const void* p;
+    int64_t stride, width, rows;
+};
+inline Span vector_span(const void* p, int64_t bytes) { return {p, 0, bytes, 1}; }
+// Whether two share memory.  Exact for single rows and equal strides (two
+// slices of one wider matrix do not); else where their address ranges meet.
+inline bool overlap(const Span& a, const Span& b) {
+    if (!a.p || !b.p || a.rows < 1 || b.rows < 1) return false;
+    const int64_t pa = (int64_t)reinterpret_cast<uintptr_t>(a.p), pb = (int64_t)reinterpret_cast<uintptr_t>(b.p);
+    if (pa + (a.rows - 1) * a.stride + a.width <= pb || pb + (b.rows - 1) * b.stride + b.width <= pa) return false;
+    if (a.rows == 1 && b.rows > 1) return overlap(b, a);
+    if (a.rows == 1 || (b.rows > 1 && a.stride != b.stride)) return true;
+    const int64_t at = ((pb - pa) % a.stride + a.stride) % a.stride;   // of b's rows in a's
+    return at < a.width || at + b.width > a.stride;
+}
+
 // int8_linear.cu: checks and (unless check_only) enqueues the shared expert of T rows.
 int run_shared_expert(const char* who, const void* x, int x_type, int64_t tokens, int d_model, int64_t row_stride,
                       const MoeInt8Weight* gate, const MoeInt8Weight* up, const MoeInt8Weight* down, int d_ff,

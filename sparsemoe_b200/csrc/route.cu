@@ -1125,6 +1125,13 @@ extern "C" int moe_route_experts(const void* logits, int logits_type, int64_t to
         set_error("moe_route_experts: a buffer is not aligned to its type");
         return MOE_ERR_INVALID_ARG;
     }
+    const Span rows{logits, row_stride * size, (int64_t)num_experts * size, tokens};
+    const Span outs[2] = {vector_span(indices, tokens * top_k * 4), vector_span(weights, tokens * top_k * 4)};
+    for (const Span& o : outs)
+        if (overlap(rows, o) || overlap(vector_span(select_bias, num_experts * 4), o) || overlap(outs[0], outs[1])) {
+            set_error("moe_route_experts: an output shares memory with the logits, the bias or the other output");
+            return MOE_ERR_INVALID_ARG;
+        }
     int dev = 0, num_sms = 0;
     rc = current_device(&dev, &num_sms);
     if (rc != MOE_OK) return rc;

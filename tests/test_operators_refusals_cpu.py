@@ -24,3 +24,15 @@ def test_codes_and_scales_in_the_activations_memory(kw):
     a.update(kw)
     rc = sm.lib.moe_int8_quantize_tokens(FAKE, a["typ"], a["T"], a["K"], a["ldx"], a["q"], a["ldq"], a["s"], None)
     assert rc == sm.MOE_ERR_INVALID_ARG and b"shares memory" in sm.lib.moe_last_error()
+
+
+@pytest.mark.parametrize("kw", [
+    dict(idx=FAKE), dict(w=FAKE), dict(idx=FAKE + 1020), dict(w=FAKE - 92), dict(idx=FAKE + (1 << 16)),
+    dict(w=FAKE + (1 << 17) - 92), dict(ld=80, idx=FAKE + 200), dict(bias=FAKE + (1 << 17) + 92),
+    dict(bias=FAKE + (1 << 16) - 252), dict(typ=1, w=FAKE + 508), dict(T=1, w=FAKE + 252)])
+def test_routes_in_the_logits_memory(kw):
+    a = dict(typ=0, T=4, ld=64, bias=None, idx=FAKE + (1 << 17), w=FAKE + (1 << 16))
+    a.update(kw)
+    r = sm.MoeRouting(0, 1, 1, 1, 1, 1.0)
+    rc = sm.lib.moe_route_experts(FAKE, a["typ"], a["T"], 64, a["ld"], 6, ctypes.byref(r), a["bias"], a["idx"], a["w"], None)
+    assert rc == sm.MOE_ERR_INVALID_ARG and b"shares memory" in sm.lib.moe_last_error()
