@@ -274,14 +274,14 @@ int moe_int8_quantize_tokens(const void* x, int x_type, int64_t tokens, int K, i
                              int64_t q_stride, float* scale, cudaStream_t stream);
 // out[t, n] = (sum_k q[t, k] w[k, n]) * scale[t] * w->scale[n] + bias[n]
 // (bias: device f32 [N] or null), s32 sums, f32 after them, rounded once to
-// out_type.  K <= 131071.  The output must not share memory with the codes.
+// out_type.  K <= 131071.  The output must not share memory with an input.
 int moe_int8_matmul(const int8_t* q, int64_t q_stride, const float* scale, int64_t tokens, int K,
                     const MoeInt8Weight* w, int N, const float* bias, void* out, int out_type, int64_t out_stride,
                     cudaStream_t stream);
 // Both in one call: 16-bit or f32 activations times an int8 matrix.  scratch:
 // device, 256-byte aligned, moe_int8_linear_scratch_bytes(tokens, K, N) -- 0 for a
-// few tokens of most shapes, then scratch may be null.  The output must not
-// share memory with x.
+// few tokens of most shapes, then scratch may be null.  The output and the
+// scratch must not share memory with an input or each other.
 int moe_int8_linear(const void* x, int x_type, int64_t tokens, int K, int64_t row_stride, const MoeInt8Weight* w,
                     int N, const float* bias, void* out, int out_type, int64_t out_stride, void* scratch,
                     size_t scratch_bytes, cudaStream_t stream);
@@ -291,8 +291,8 @@ size_t moe_int8_linear_scratch_bytes(int64_t tokens, int K, int N);
 //   out = linear(h, down) + residual,
 // with x and h quantised per token.  residual: [tokens, d_model] of x_type, or
 // null; it may be `out` itself when the types are the same (but not overlap it
-// otherwise).  gate and up have
-// one order.
+// otherwise).  The output may lie in the memory of x, which has been read by
+// then, but of no other input and not of the scratch.  gate and up have one order.
 int moe_int8_shared_expert(const void* x, int x_type, int64_t tokens, int d_model, int64_t row_stride,
                            const MoeInt8Weight* gate, const MoeInt8Weight* up, const MoeInt8Weight* down, int d_ff,
                            const void* residual, int64_t residual_stride, void* out, int out_type, int64_t out_stride,

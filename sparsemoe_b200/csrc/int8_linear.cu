@@ -1735,6 +1735,16 @@ int check_scratch(const char* who, const void* scratch, size_t have, size_t need
     return MOE_OK;
 }
 
+// An output in the memory of what other blocks still read: a matrix, its scales, the bias or the scratch.
+int check_apart(const char* who, const Span& out, const MoeInt8Weight& w, int64_t K, int64_t N, const float* bias,
+                const void* scratch, size_t scratch_bytes) {
+    const Span m{w.w, w.row_stride, w.order == MOE_WEIGHT_KN ? N : K, w.order == MOE_WEIGHT_KN ? K : N};
+    if (overlap(out, m) || overlap(out, vector_span(w.scale, N * 4)) || overlap(out, vector_span(bias, N * 4)))
+        return bad(who, "the output shares memory with a weight matrix, its scales or the bias");
+    if (overlap(out, vector_span(scratch, (int64_t)scratch_bytes))) return bad(who, "the output shares memory with the scratch");
+    return MOE_OK;
+}
+
 int cuda_error(const char* who, cudaError_t e) {
     set_error("%s: %s", who, cudaGetErrorString(e));
     return MOE_ERR_CUDA;
@@ -1830,10 +1840,15 @@ int run_shared_expert(const char* who, const void* x, int x_type, int64_t tokens
     if (rc != MOE_OK) return rc;
     const int in = elem_bytes(x_type), size = elem_bytes(out_type);
     const bool same = residual == out && x_type == out_type && (tokens == 1 || residual_stride == out_stride);
-    if (residual && !same &&
-        overlap({residual, residual_stride * in, (int64_t)d_model * in, tokens},
-                {out, out_stride * size, (int64_t)d_model * size, tokens}))
-        return bad(who, "the output shares memory with the residual without being it");
+    const Span rows{out, out_stride * size, (int64_t)d_model * size, tokens},
+        act{x, row_stride * in, (int64_t)d_model * in, tokens}, res{residual, residual_stride * in, (int64_t)d_model * in, tokens},
+        temp = vector_span(scratch, (int64_t)sc.total);
+    if (!same && overlap(res, rows)) return bad(who, "the output shares memory with the residual without being it");
+    if (overlap(act, temp) || overlap(res, temp)) return bad(who, "the scratch shares memory with the activations or the residual");
+    rc = check_apart(who, rows, *gate, d_model, d_ff, nullptr, scratch, sc.total);
+    if (rc == MOE_OK) rc = check_apart(who, rows, *up, d_model, d_ff, nullptr, nullptr, 0);
+    if (rc == MOE_OK) rc = check_apart(who, rows, *down, d_ff, d_model, nullptr, nullptr, 0);
+    if (rc != MOE_OK) return rc;
     if (check_only) return MOE_OK;
     int dev = 0, num_sms = 0;
     rc = current_device(&dev, &num_sms);
@@ -1941,8 +1956,11 @@ extern "C" int moe_int8_matmul(const int8_t* q, int64_t q_stride, const float* s
         return bad(who, "codes must be rows on 16-byte boundaries (q_stride % 16 == 0, >= K) and scales f32");
     if (!aligned(bias, 4)) return bad(who, "bias is not aligned to f32");
     const int size = elem_bytes(out_type);
-    if (overlap({q, q_stride, K, tokens}, {out, out_stride * size, (int64_t)N * size, tokens}))
-        return bad(who, "the output shares memory with the codes");
+    const Span rows{out, out_stride * size, (int64_t)N * size, tokens};
+    if (overlap({q, q_stride, K, tokens}, rows) || overlap(vector_span(scale, tokens * 4), rows))
+        return bad(who, "the output shares memory with the codes or their scales");
+    rc = check_apart(who, rows, *w, K, N, bias, nullptr, 0);
+    if (rc != MOE_OK) return rc;
     int dev = 0, num_sms = 0;
     rc = current_device(&dev, &num_sms);
     if (rc != MOE_OK) return rc;
@@ -1966,11 +1984,15 @@ extern "C" int moe_int8_linear(const void* x, int x_type, int64_t tokens, int K,
     if (rc != MOE_OK) return rc;
     if (!aligned(bias, 4)) return bad(who, "bias is not aligned to f32");
     if (tokens == 0) return MOE_OK;
-    rc = check_scratch(who, scratch, scratch_bytes, linear_scratch(tokens, K, N));
+    const size_t need = linear_scratch(tokens, K, N);
+    rc = check_scratch(who, scratch, scratch_bytes, need);
     if (rc != MOE_OK) return rc;
     const int in = elem_bytes(x_type), size = elem_bytes(out_type);
-    if (overlap({x, row_stride * in, (int64_t)K * in, tokens}, {out, out_stride * size, (int64_t)N * size, tokens}))
-        return bad(who, "the output shares memory with the activations");
+    const Span rows{out, out_stride * size, (int64_t)N * size, tokens}, act{x, row_stride * in, (int64_t)K * in, tokens};
+    if (overlap(act, rows)) return bad(who, "the output shares memory with the activations");
+    if (overlap(act, vector_span(scratch, (int64_t)need))) return bad(who, "the scratch shares memory with the activations");
+    rc = check_apart(who, rows, *w, K, N, bias, scratch, need);
+    if (rc != MOE_OK) return rc;
     int dev = 0, num_sms = 0;
     rc = current_device(&dev, &num_sms);
     if (rc != MOE_OK) return rc;

@@ -133,7 +133,7 @@ def int8_linear(x: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, *, bias
     """x [T, K] (f32, f16, bf16) times the int8 matrix w [K, N] with f32 scales
     w_scale [N], the tokens quantised on the fly (quantize_int8_tokens, then
     int8_matmul); the output has x's type unless out_dtype or out says otherwise;
-    out must not share memory with x."""
+    out must share memory with no input."""
     return _operators.linear(x, w, w_scale, bias, out_dtype, out)
 
 

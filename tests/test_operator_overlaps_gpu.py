@@ -43,3 +43,39 @@ def test_routes_beside_the_logits(gpu, T):
     for out in ((inside.view(torch.int32), w), (i, inside), (i, i.view(torch.float32))):
         with pytest.raises(sm.MoeError, match="shares memory"):
             sm.route_experts(y, 6, bias=b, out=out)
+
+
+@pytest.mark.parametrize("T", [1, 6, 12, 300])
+def test_products_in_one_allocation(gpu, T):
+    """Everything a call reads and writes in one buffer, side by side; one element into a neighbour is refused."""
+    K = N = 128
+    x = torch.randn(T, K, device=gpu).bfloat16()
+    w = torch.randint(-127, 128, (K, N), dtype=torch.int8, device=gpu)
+    s, b = torch.rand(N, device=gpu) * 0.01, torch.randn(N, device=gpu)
+    want, plain = sm.int8_linear(x, w, s, bias=b), sm.int8_shared_expert(x, w, s, w, s, w, s)
+    flat = torch.zeros(2 * T * K * 2 + K * N + 2 * N * 4 + 64, dtype=torch.uint8, device=gpu)
+    at = 0
+
+    def place(t):
+        nonlocal at
+        v = flat[at: at + t.numel() * t.element_size()].view(t.dtype).view(t.shape)
+        at += v.numel() * v.element_size()
+        return v.copy_(t)
+
+    fx, fw, fs, fo, fb = place(x), place(w), place(s), place(torch.zeros_like(x)), place(b)
+    assert torch.equal(sm.int8_linear(fx, fw, fs, bias=fb, out=fo), want)
+    q, sq = sm.quantize_int8_tokens(fx)
+    assert torch.equal(sm.int8_matmul(q, sq, fw, fs, bias=fb, out=fo), want)
+    assert torch.equal(sm.int8_shared_expert(fx, fw, fs, fw, fs, fw, fs, out=fo), plain)
+    half = flat.view(torch.bfloat16)
+    first = (fo.data_ptr() - flat.data_ptr()) // 2
+    for off in (-1, 1):                          # into the scales before it, the bias behind it
+        out = half[first + off: first + off + T * N].view(T, N)
+        for call in (lambda: sm.int8_linear(fx, fw, fs, bias=fb, out=out),
+                     lambda: sm.int8_matmul(q, sq, fw, fs, bias=fb, out=out)):
+            with pytest.raises(sm.MoeError, match="shares memory"):
+                call()
+    with pytest.raises(sm.MoeError, match="shares memory"):
+        sm.int8_shared_expert(fx, fw, fs, fw, fs, fw, fs, out=half[first - 1: first - 1 + T * N].view(T, N))
+    # the activations' own memory: they have been read by the time the output is written
+    assert torch.equal(sm.int8_shared_expert(fx, fw, fs, fw, fs, fw, fs, out=fx), plain)

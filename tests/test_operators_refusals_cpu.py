@@ -36,3 +36,43 @@ def test_routes_in_the_logits_memory(kw):
     r = sm.MoeRouting(0, 1, 1, 1, 1, 1.0)
     rc = sm.lib.moe_route_experts(FAKE, a["typ"], a["T"], 64, a["ld"], 6, ctypes.byref(r), a["bias"], a["idx"], a["w"], None)
     assert rc == sm.MOE_ERR_INVALID_ARG and b"shares memory" in sm.lib.moe_last_error()
+
+
+FAR = [FAKE + (i << 20) for i in range(1, 12)]   # memory apart
+
+
+def apart(order=0, **kw):
+    a = dict(x=FAR[0], out=FAR[1], scratch=FAR[2], w=FAR[3], ws=FAR[4], bias=FAR[5], s=FAR[6])
+    a.update(kw)
+    return a, sm.MoeInt8Weight(a["w"], 64, a["ws"], order)
+
+
+@pytest.mark.parametrize("kw", [
+    dict(out=FAR[3]), dict(out=FAR[3] + 63 * 64), dict(out=FAR[3] + 63 * 64, order=1), dict(out=FAR[4] + 252),
+    dict(out=FAR[5] - 32 * 128 + 2), dict(out=FAR[2]), dict(out=FAR[2] + 32 * 64), dict(x=FAR[2]),
+    dict(x=FAR[2] - 32 * 128 + 2)])
+def test_linear_outputs_in_an_inputs_memory(kw):
+    a, w = apart(**kw)
+    rc = sm.lib.moe_int8_linear(a["x"], 2, 32, 64, 64, ctypes.byref(w), 64, a["bias"], a["out"], 2, 64, a["scratch"],
+                                1 << 18, None)
+    assert rc == sm.MOE_ERR_INVALID_ARG and b"shares memory" in sm.lib.moe_last_error()
+
+
+@pytest.mark.parametrize("kw", [dict(out=FAR[6]), dict(out=FAR[6] + 124), dict(out=FAR[3] + 64), dict(out=FAR[4]),
+                                dict(out=FAR[5] + 252), dict(out=FAR[0] + 31 * 64 + 62)])
+def test_matmul_outputs_in_an_inputs_memory(kw):
+    a, w = apart(**kw)
+    rc = sm.lib.moe_int8_matmul(a["x"], 64, a["s"], 32, 64, ctypes.byref(w), 64, a["bias"], a["out"], 2, 64, None)
+    assert rc == sm.MOE_ERR_INVALID_ARG and b"shares memory" in sm.lib.moe_last_error()
+
+
+@pytest.mark.parametrize("kw", [dict(out=FAR[2]), dict(out=FAR[3]), dict(out=FAR[4]), dict(out=FAR[7]), dict(out=FAR[8] + 252),
+                                dict(out=FAR[9] + 64), dict(x=FAR[2] + 64), dict(res=FAR[2]), dict(res=FAR[1] + 2),
+                                dict(res=FAR[1], ldr=72)])
+def test_shared_expert_outputs_in_an_inputs_memory(kw):
+    ldr = kw.pop("ldr", 64)
+    a, gate = apart(**kw)
+    up, down = sm.MoeInt8Weight(FAR[7], 64, FAR[8], 0), sm.MoeInt8Weight(FAR[9], 64, FAR[10], 0)
+    rc = sm.lib.moe_int8_shared_expert(a["x"], 2, 32, 64, 64, ctypes.byref(gate), ctypes.byref(up), ctypes.byref(down), 64,
+                                       a.get("res"), ldr, a["out"], 2, 64, a["scratch"], 1 << 18, None)
+    assert rc == sm.MOE_ERR_INVALID_ARG and b"shares memory" in sm.lib.moe_last_error()
