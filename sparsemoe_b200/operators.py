@@ -20,14 +20,26 @@ import torch
 from . import _PKG, check, lib
 from .config import MOE_SCORES, MOE_WEIGHT_KN, MOE_WEIGHT_NK, MoeInt8Weight, MoeRouting
 
+
+class _Missing:
+    """In the place of a native entry that cannot be loaded: the layer and the C API's mirror work without it, an
+    operator's call raises."""
+
+    def __init__(self, reason: ImportError):
+        self._reason = reason
+
+    def __getattr__(self, name):
+        raise ImportError(f"{_PKG / '_operators.so'}, the entry of the stand-alone operators, cannot be loaded "
+                          f"({self._reason}): build it with `python sparsemoe_b200/build.py`") from self._reason
+
+
 try:
     from . import _operators
+    _operators.bind(check, *(ctypes.cast(f, ctypes.c_void_p).value for f in (
+        lib.moe_route_experts, lib.moe_int8_quantize_tokens, lib.moe_int8_matmul, lib.moe_int8_linear,
+        lib.moe_int8_linear_scratch_bytes, lib.moe_int8_shared_expert, lib.moe_int8_shared_expert_scratch_bytes)))
 except ImportError as e:
-    raise ImportError(f"{_PKG / '_operators.so'} cannot be loaded ({e}): build it with `python sparsemoe_b200/build.py`") from e
-
-_operators.bind(check, *(ctypes.cast(f, ctypes.c_void_p).value for f in (
-    lib.moe_route_experts, lib.moe_int8_quantize_tokens, lib.moe_int8_matmul, lib.moe_int8_linear,
-    lib.moe_int8_linear_scratch_bytes, lib.moe_int8_shared_expert, lib.moe_int8_shared_expert_scratch_bytes)))
+    _operators = _Missing(e)
 
 
 def sync_check(device: torch.device | str | int | None = None) -> None:
