@@ -51,12 +51,22 @@ def _compile(src: Path, extra: list[str]) -> Path:
     return obj
 
 
-def build_binding() -> Path:
-    """The Python entry: no CUDA code, calls the C ABI through addresses it is given."""
-    deps = [BINDING_SRC, PKG.parent / "include" / "sparsemoe_b200.h"]
-    if BINDING.exists() and BINDING.stat().st_mtime >= max(d.stat().st_mtime for d in deps):
-        return BINDING
+def binding_stamp() -> str:
+    """What the binding's binary depends on besides its sources: the torch and the Python it was built against."""
+    import importlib.metadata
+    return f"torch {importlib.metadata.version('torch')}, python {sys.version_info[0]}.{sys.version_info[1]}"
+
+
+def build_binding() -> Path | None:
+    """The Python entry: no CUDA code, calls the C ABI through addresses it is given.  None where there is no torch."""
     import importlib.util
+    if importlib.util.find_spec("torch") is None:
+        return None
+    deps = [BINDING_SRC, PKG.parent / "include" / "sparsemoe_b200.h"]
+    stamp = BUILD / (BINDING.name + ".stamp")
+    if BINDING.exists() and BINDING.stat().st_mtime >= max(d.stat().st_mtime for d in deps) and \
+            stamp.exists() and stamp.read_text() == binding_stamp():
+        return BINDING
     import sysconfig
     torch = Path(importlib.util.find_spec("torch").origin).parent
     cuda = Path(nvcc()).resolve().parents[1] / "include"
@@ -70,6 +80,7 @@ def build_binding() -> Path:
     if r.returncode != 0:
         raise RuntimeError(f"g++ failed for {BINDING_SRC.name}:\n{r.stdout}\n{r.stderr}")
     os.replace(tmp, BINDING)
+    stamp.write_text(binding_stamp())
     return BINDING
 
 
@@ -79,7 +90,6 @@ def build(verbose: bool = False, extra: list[str] | None = None) -> Path:
     with cf.ThreadPoolExecutor(max_workers=min(8, os.cpu_count() or 1)) as ex:
         binding = ex.submit(build_binding)
         objs = list(ex.map(lambda s: _compile(s, extra), sources()))
-        binding.result()
     newest = max(o.stat().st_mtime for o in objs)
     if not LIB.exists() or LIB.stat().st_mtime < newest:
         tmp = LIB.with_suffix(".so.tmp")
@@ -88,8 +98,9 @@ def build(verbose: bool = False, extra: list[str] | None = None) -> Path:
         if r.returncode != 0:
             raise RuntimeError(f"link failed:\n{r.stdout}\n{r.stderr}")
         os.replace(tmp, LIB)
+    entry = binding.result()   # (the library stands without it)
     if verbose:
-        print(f"built {LIB} and {BINDING.name}")
+        print(f"built {LIB}" + (f" and {entry.name}" if entry else "; no torch, so no Python entry of the operators"))
     return LIB
 
 
