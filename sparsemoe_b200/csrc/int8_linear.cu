@@ -390,18 +390,24 @@ __device__ __forceinline__ void arrive_cluster(uint32_t bar) {
 }
 // A CTA's bounded waits.  One that runs out is reported to the host and sets
 // `stop` (shared memory), which ends the waits of the CTA's other roles and, of
-// a pair, the other CTA's.
-struct Waits {
+// a pair, the other CTA's.  Most waits end in their first try, which may last;
+// the others are in line in the small kernel (1 x 7168 x 2048 7.37 us, 7.47 with
+// a call) and a call in the tiles (512 x 2048 x 7168 15.12, 15.35 in line).
+template <bool kInline> struct Waits {
     uint32_t* stop;
     uint32_t peer;   // the other CTA's word (0: none)
     uint64_t limit_ns;
 
     __device__ __forceinline__ bool operator()(uint64_t* bar, uint32_t parity) const {
-        return mbar_try_wait(smem_u32(bar), parity) || longer(smem_u32(bar), parity, stop, peer, limit_ns);
+        if (mbar_try_wait(smem_u32(bar), parity)) return true;
+        return kInline ? tries(smem_u32(bar), parity, stop, peer, limit_ns) : called(smem_u32(bar), parity, stop, peer, limit_ns);
     }
-    // The tries behind the first, not in line: most waits end in the first one, which may last.
-    static __device__ __noinline__ bool longer(uint32_t bar, uint32_t parity, uint32_t* stop, uint32_t peer,
+    static __device__ __noinline__ bool called(uint32_t bar, uint32_t parity, uint32_t* stop, uint32_t peer,
                                                uint64_t limit_ns) {
+        return tries(bar, parity, stop, peer, limit_ns);
+    }
+    static __device__ __forceinline__ bool tries(uint32_t bar, uint32_t parity, uint32_t* stop, uint32_t peer,
+                                                 uint64_t limit_ns) {
         const uint64_t t0 = globaltimer_ns();
         for (uint32_t it = 1;; ++it) {
             if (mbar_try_wait(bar, parity)) return true;
@@ -420,13 +426,6 @@ struct Waits {
     __device__ __forceinline__ bool warp(uint64_t* bar, uint32_t parity) const {
         return __all_sync(0xffffffffu, (*this)(bar, parity));
     }
-    // Tells the other CTAs of a cluster of `ctas` that this one has given up, ahead of the cluster barrier behind
-    // which their sums take its parts (all of them have started: an earlier phase of the barrier is behind).  The
-    // epilogue's warps call it: where another role gives up, theirs is the wait that runs out or is ended.
-    static __device__ __noinline__ void tell(uint32_t stop, int ctas) {
-        for (int r = 0; r < ctas; ++r)
-            asm volatile("st.shared::cluster.b32 [%0], %1;" ::"r"(mapa(stop, r)), "r"(1u) : "memory");
-    }
     __device__ __forceinline__ bool stopped() const { return *(volatile uint32_t*)stop != 0; }
     // For arrivals from the cluster.
     __device__ __forceinline__ bool cluster(uint64_t* bar, uint32_t parity) const {
@@ -435,6 +434,15 @@ struct Waits {
         return ok;
     }
 };
+
+// Tells the CTAs of a cluster of `ctas` that this one has given up, ahead of the
+// cluster barrier behind which their sums take its parts (all of them have
+// started: an earlier phase of the barrier is behind).  The epilogue's warps call
+// it: where another role gives up, theirs is the wait that runs out or is ended.
+__device__ __noinline__ void tell_cluster(uint32_t stop, int ctas) {
+    for (int r = 0; r < ctas; ++r)
+        asm volatile("st.shared::cluster.b32 [%0], %1;" ::"r"(mapa(stop, r)), "r"(1u) : "memory");
+}
 
 // After a wait that ran out, by the thread that issues the MMAs: up to 1 ms each
 // for the copies that may be in flight (the next one of each stage; a copy takes
@@ -734,7 +742,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int rank = (int)cluster_rank();
-    const Waits wait{&s_stop, kPair ? mapa(smem_u32(&s_stop), rank ^ 1) : 0u, kWaitTimeoutNs};
+    const Waits<false> wait{&s_stop, kPair ? mapa(smem_u32(&s_stop), rank ^ 1) : 0u, kWaitTimeoutNs};
 
     if (threadIdx.x == 0) {
         s_stop = 0;
@@ -979,7 +987,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             acc ^= 1;
             if (acc == 0) aph ^= 1u;
         }
-        if (p.split > 1 && !ok) Waits::tell(smem_u32(&s_stop), p.split);
+        if (p.split > 1 && !ok) tell_cluster(smem_u32(&s_stop), p.split);
         if (lane == 0) bulk_wait_read<0>();   // the staged chunks are read before the CTA's memory goes
     }
     if (p.split > 1) {
@@ -1110,7 +1118,7 @@ __global__ void __launch_bounds__(kSmallThreads, 2)
     uint32_t* const tmem_slot = reinterpret_cast<uint32_t*>(bail + 1);
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const Waits wait{&s_stop, 0u, kWaitTimeoutNs};
+    const Waits<true> wait{&s_stop, 0u, kWaitTimeoutNs};
     if (threadIdx.x == 0) {
         s_stop = 0;
         for (int s = 0; s < p.stages; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], 1); }
@@ -1349,7 +1357,7 @@ __global__ void __launch_bounds__(kSmallThreads, 2)
             }
         }
         if (split) {
-            if (!ok) Waits::tell(smem_u32(&s_stop), p.split);
+            if (!ok) tell_cluster(smem_u32(&s_stop), p.split);
             __syncwarp();
             cluster_arrive();   // phase 3: every part has been sent
             cluster_wait();
@@ -1394,8 +1402,8 @@ __global__ void __launch_bounds__(32) waits_selftest_kernel(uint64_t limit_ns, i
     __syncwarp();
     cluster_arrive();
     cluster_wait();
-    const Waits wait{&s_stop, 0u, limit_ns};
-    if (rank == 1 && !wait.warp(&bar, 0)) Waits::tell(smem_u32(&s_stop), 2);
+    const Waits<true> wait{&s_stop, 0u, limit_ns};
+    if (rank == 1 && !wait.warp(&bar, 0)) tell_cluster(smem_u32(&s_stop), 2);
     __syncwarp();
     cluster_arrive();
     cluster_wait();
