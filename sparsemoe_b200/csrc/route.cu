@@ -8,7 +8,7 @@
 //         the sum of its two largest v (no bias: s); the `kept` best stay;
 //   the k largest v of the kept groups, equal values by the lower index;
 //   w_l = s / sum over the chosen of s (renormalised; where every chosen
-//         sigmoid underflows, exp(x - max) in its place, its limit) or s, times scale.
+//         sigmoid is tiny, exp(x - max) in its place, its limit) or s, times scale.
 // Masked experts (NaN, logits <= -1e20 or f16's lowest value, a bias that is
 // NaN or <= -1e20) are never chosen; slots that stay empty hold (-1, 0).
 //
@@ -322,6 +322,16 @@ __device__ __forceinline__ float rcp_fast(float x) {   // 1 ulp
     return r;
 }
 
+// 1 / (1 + exp(-x)), its small values (exp(x) / (1 + exp(x))) down to the subnormal ones.
+__device__ __forceinline__ float sigmoid(float x) {
+    const float t = expf(-fabsf(x)), r = rcp_fast(1.0f + t);
+    return x < 0.0f ? t * r : r;
+}
+// Up to this sum of sigmoids exp(x - max) stands for them: sigmoid(x) is exp(x)
+// (1 - exp(x) + ..), off by less than 2^-26, and no score that counts beside the
+// largest underflows.
+constexpr float kSmallSum = 0x1p-26f;
+
 // The candidates in lanes 0 .. n-1 (n >= k, or fewer where nothing else is
 // left) ranked by value, equal values by the lower index: lane l gets the l-th.
 // f32 values decide where those that follow each other, down to the first behind
@@ -564,14 +574,14 @@ __global__ void __launch_bounds__(kRouteWarps * 32) route_kernel(const __grid_co
     const float xs = my_i >= 0 ? to_f32<T>(row[my_i]) : -INFINITY;
     float e = 0.0f;
     if (p.sigmoid) {
-        e = rcp_fast(1.0f + expf(-xs));
+        e = sigmoid(xs);
     } else if (!p.renorm) {
         e = my_i < 0 ? 0.0f : (xs == top ? 1.0f : expf(xs - top)) * inv_sum;
     }
     if (p.renorm) {
         float sum = 0.0f;
         if (p.sigmoid) sum = warp_sum(e);
-        if (!(sum > 1e-30f)) {   // softmax, or sigmoids so small that only their ratios, exp of the differences, are left
+        if (!(sum > kSmallSum)) {   // softmax, or sigmoids so small that their ratios are exp of the differences
             const float mx = warp_max(xs);
             e = my_i < 0 ? 0.0f : xs == mx ? 1.0f : expf(xs - mx);
             sum = warp_sum(e);
@@ -953,15 +963,15 @@ __global__ void __launch_bounds__(kRouteWarps * 32, 7) route_many_kernel(const _
 
     const float xs = my_i >= 0 ? to_f32<T>(row[my_i]) : -INFINITY;
     float e = 0.0f;
-    if (p.sigmoid) e = rcp_fast(1.0f + expf(-xs));
+    if (p.sigmoid) e = sigmoid(xs);
     else if (!p.renorm) e = my_i < 0 ? 0.0f : (xs == top ? 1.0f : expf(xs - top)) * inv_sum;
     if (p.renorm) {
         float sum = p.sigmoid ? sum8(e) : 0.0f;
-        if (!__all_sync(kFull, sum > 1e-30f)) {   // as above; a token whose sum stands keeps it
+        if (!__all_sync(kFull, sum > kSmallSum)) {   // as above; a token whose sum stands keeps it
             const float mx = fmax8(xs);
             const float f = my_i < 0 ? 0.0f : xs == mx ? 1.0f : expf(xs - mx);
             const float g = sum8(f);
-            if (!(sum > 1e-30f)) {
+            if (!(sum > kSmallSum)) {
                 e = f;
                 sum = g;
             }
