@@ -1050,9 +1050,10 @@ __global__ void __launch_bounds__(kThreads, 1)
 // What bounds it is latency: 512 x 2048 takes 4.5 us (3.1 with codes given), an
 // exchange of a cluster about 1, and the MMAs, 128 clocks each whatever their
 // columns, 0.27 us for each block of K; the 14.7 MB of weights of 1 x 7168 x 2048
-// (6.8 us, 8.7 when none of them is in the L2) are 2.2 us at the HBM's rate.  Kept short for one reason more: a code path that a CTA runs
-// once is fetched as slowly as it is long (the quantiser of gate / up pairs, 96
-// times silu in line, cost the down product 17 us).
+// (6.8 us, 8.7 when none of them is in the L2) are 2.2 us at the HBM's rate.
+// Kept short for one reason more: a code path that a CTA runs once is fetched as
+// slowly as it is long (the quantiser of gate / up pairs, 96 times silu in line,
+// cost the down product 17 us).
 struct SmallParams {
     const void* x;             // tokens, rows ld_x elements apart
     int64_t ld_x;
@@ -1502,7 +1503,9 @@ cudaError_t launch_linear_cfg(const CUtensorMap& a, const CUtensorMap (&b)[2], c
 // 128x7168x2048 22.5, 22.2, 20.3 / 16.3 / 13.6 / 22.5; 512x7168x2048 22.8, 22.8,
 // 20.9 / 17.6 / 28.7 / 59; 512x2048x7168 12.5, 12.1, 16.0 / 41.6 / 75.6 / 155;
 // 1024x2048x2048 12.1, 11.7, 10.8 / 22.4 / 44.5 / 92; 2048x7168x2048 25.0, 26.6,
-// 39.4 / 66 / 109 / 205; 8192x7168x4096 159, 201, 270 / 455 / 791 / 1577.
+// 39.4 / 66 / 109 / 205; 8192x7168x4096 159, 201, 270 / 455 / 791 / 1577.  The
+// estimate leaves out the epilogue, which a CTA's only tile does not hide: at
+// 512x2048x7168 it puts the pair 1 % ahead of 128 x 256, which measured 3 % faster.
 struct Tiles {
     bool wide, pair;
     int split;
@@ -1610,6 +1613,8 @@ cudaError_t launch_small_typed(const CUtensorMap (&w)[2], const SmallParams& p, 
 // its CTAs resident at once (two an SM); the largest such split.  More CTAs are
 // left to the persistent tiles (us, here / there, 1 token: 7168 x 8192 14.1 / 17.7,
 // all at once; 7168 x 14336 26.7 / 25.8, 7168 x 28672 51.3 / 37.1, in rounds).
+// The counts are a whole B200's: the scratch sizes follow the choice and are asked
+// for without a device.  With fewer SMs the CTAs run in rounds, slower.
 bool plan_small(int64_t T, int limit, int K, int N, int mats, int* split, int* stages, size_t* smem) {
     if (T > limit) return false;
     const int kblocks = (K + kBK - 1) / kBK, tiles = (N + 127) / 128;
